@@ -16,29 +16,29 @@ IGNORE = -100
 def listed():
     return [
         # the norm in front of every layer while one token at a time is generated: latency
-        {"name": "norm, one token", "op": "norm", "dtype": "bf16", "params": "bf16", "rows": 1, "cols": 4096},
+        {"name": "norm: one token", "op": "norm", "dtype": "bf16", "params": "bf16", "rows": 1, "cols": 4096},
         # a batch of 256 images of 197 patches, 12 heads of 64
-        {"name": "norm, image patches", "op": "norm", "dtype": "bf16", "params": "bf16", "rows": 256 * 197, "cols": 768},
+        {"name": "norm: image patches", "op": "norm", "dtype": "bf16", "params": "bf16", "rows": 256 * 197, "cols": 768},
         # odd row length: no row but the first starts on a 16-byte boundary
-        {"name": "norm, odd rows", "op": "norm", "dtype": "f32", "params": "f32", "rows": 4099, "cols": 1001},
+        {"name": "norm: odd rows", "op": "norm", "dtype": "f32", "params": "f32", "rows": 4099, "cols": 1001},
         # the backward pass over a batch of eight sequences of 2048 tokens
-        {"name": "norm gradient, long rows", "op": "norm_grad", "dtype": "bf16", "params": "bf16", "rows": 8 * 2048, "cols": 4096},
+        {"name": "norm gradient: long rows", "op": "norm_grad", "dtype": "bf16", "params": "bf16", "rows": 8 * 2048, "cols": 4096},
         # the patches again, float16 activations and float32 parameters (mixed-precision training)
-        {"name": "norm gradient, image patches", "op": "norm_grad", "dtype": "fp16", "params": "f32", "rows": 256 * 197, "cols": 768},
+        {"name": "norm gradient: image patches", "op": "norm_grad", "dtype": "fp16", "params": "f32", "rows": 256 * 197, "cols": 768},
         # one image: a small batch, where the reduction over rows is the latency
-        {"name": "norm gradient, one image", "op": "norm_grad", "dtype": "f32", "params": "f32", "rows": 197, "cols": 768},
+        {"name": "norm gradient: one image", "op": "norm_grad", "dtype": "f32", "params": "f32", "rows": 197, "cols": 768},
         # scoring one token against the whole vocabulary: reading the weights is the work
-        {"name": "loss, one token", "op": "loss", "dtype": "bf16", "tokens": 1, "hidden": 4096, "vocab": 131072, "ignored": 0.0},
+        {"name": "loss: one token", "op": "loss", "dtype": "bf16", "tokens": 1, "hidden": 4096, "vocab": 131072, "ignored": 0.0},
         # an evaluation batch, no extent a multiple of a tile
-        {"name": "loss, ragged", "op": "loss", "dtype": "fp16", "tokens": 4095, "hidden": 768, "vocab": 50257, "ignored": 0.1},
+        {"name": "loss: ragged", "op": "loss", "dtype": "fp16", "tokens": 4095, "hidden": 768, "vocab": 50257, "ignored": 0.1},
         # full precision, a small model
-        {"name": "loss, float32", "op": "loss", "dtype": "f32", "tokens": 512, "hidden": 1024, "vocab": 14336, "ignored": 0.0},
+        {"name": "loss: float32", "op": "loss", "dtype": "f32", "tokens": 512, "hidden": 1024, "vocab": 14336, "ignored": 0.0},
         # a training step's largest product
-        {"name": "loss gradient, large", "op": "loss_grad", "dtype": "bf16", "tokens": 8192, "hidden": 4096, "vocab": 131072, "ignored": 0.02},
+        {"name": "loss gradient: large", "op": "loss_grad", "dtype": "bf16", "tokens": 8192, "hidden": 4096, "vocab": 131072, "ignored": 0.02},
         # a padded batch: a third of the tokens carry no target
-        {"name": "loss gradient, ragged", "op": "loss_grad", "dtype": "fp16", "tokens": 1021, "hidden": 768, "vocab": 50257, "ignored": 0.33},
+        {"name": "loss gradient: ragged", "op": "loss_grad", "dtype": "fp16", "tokens": 1021, "hidden": 768, "vocab": 50257, "ignored": 0.33},
         # adapting to a handful of tokens: the weights' gradient is the traffic
-        {"name": "loss gradient, few tokens", "op": "loss_grad", "dtype": "bf16", "tokens": 4, "hidden": 4096, "vocab": 32000, "ignored": 0.0},
+        {"name": "loss gradient: few tokens", "op": "loss_grad", "dtype": "bf16", "tokens": 4, "hidden": 4096, "vocab": 32000, "ignored": 0.0},
     ]
 
 
