@@ -395,6 +395,28 @@ tn_status tn_reduce_stats(const tn_tensor_t* src, tn_tensor_t* max_out, tn_tenso
 tn_status tn_argsum_fixed_scratch(const tn_tensor_t* src, tn_tensor_t* dst, tn_stream_t stream,
                                   uint8_t axis);
 
+/* ------------------------------------------------------------------ normalisation ---- */
+
+/* No counterpart in the reference (its users write a mean, a subtraction, a product, a mean, an rsqrt and
+ * two broadcasts). Layer normalisation over the last axis in one pass over x:
+ *   mean = sum(x) / C,  rstd = 1 / sqrt(sum((x - mean)^2) / C + eps),  y = (x - mean) * rstd * weight + bias
+ * x: float16, bfloat16, float32 or float64, any strides; y: dense, x's dtype and shape (it may be x itself where x is
+ * dense). weight and bias: contiguous vectors of x's dtype, or float32 beside 16-bit x; either may be NULL. mean
+ * and rstd, float32 (float64 for float64 x) and one value per row, may be NULL; the backward pass reads them.
+ * Everything is computed in float32 (float64 for float64) and rounded once. A tensor without rows is
+ * accepted; an empty last axis is refused with TN_ERROR. */
+tn_status tn_layer_norm(const tn_tensor_t* x, const tn_tensor_t* weight, const tn_tensor_t* bias, tn_tensor_t* y,
+                        tn_tensor_t* mean, tn_tensor_t* rstd, tn_stream_t stream, double eps);
+/* Its gradient, from the statistics of the forward pass. With z = (x - mean) * rstd and g = dy * weight:
+ *   dx = rstd * (g - sum(g) / C - z * sum(g * z) / C),  dweight = sum over rows of dy * z,  dbias = sum over rows of dy
+ * dx is dense and may be dy or x where that one is dense. dweight and dbias have the parameters' dtype and
+ * may be NULL; weight is NULL where the forward pass had none. The sums over rows are added in an
+ * order that depends on the sizes only, so the same call gives the same bits. Without rows the
+ * parameters' gradients are zero. */
+tn_status tn_layer_norm_grad(const tn_tensor_t* dy, const tn_tensor_t* x, const tn_tensor_t* mean, const tn_tensor_t* rstd,
+                             const tn_tensor_t* weight, tn_tensor_t* dx, tn_tensor_t* dweight, tn_tensor_t* dbias,
+                             tn_stream_t stream);
+
 /* ------------------------------------------------------------------ utilities -------- */
 
 /* reference: cuda::cpy, src/cuda/cpy.cu:55-69 — strided -> strided copy (slice assignment). */

@@ -139,6 +139,8 @@ PROTOTYPES = {
     "tn_view_as_polar": [_TP, _TP, _TP, StreamT],
     "tn_reduce_stats": [_TP, _TP, _TP, _TP, StreamT, C.c_uint8],
     "tn_argsum_fixed_scratch": [_TP, _TP, StreamT, C.c_uint8],
+    "tn_layer_norm": [_TP, _TP, _TP, _TP, _TP, _TP, StreamT, C.c_double],
+    "tn_layer_norm_grad": [_TP, _TP, _TP, _TP, _TP, _TP, _TP, _TP, StreamT],
     "tn_cpy": [_TP, _TP, StreamT],
     "tn_allclose": [_TP, _TP, StreamT, C.c_double, C.c_double, C.POINTER(C.c_int)],
     "tn_device_errors": [C.POINTER(C.c_uint)],

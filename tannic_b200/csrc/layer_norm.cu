@@ -1,0 +1,661 @@
+// Layer normalisation over the last axis, forward and backward.
+//
+//   mu = mean(x)   r = 1 / sqrt(mean((x - mu)^2) + eps)   y = (x - mu) r w + b
+//   z = (x - mu) r,  g = dy w:   dx = r (g - mean(g) - z mean(g z)),  dw = sum_rows dy z,  db = sum_rows dy
+//
+// Both passes are bound by HBM: the forward pass has to move x once in and y once out, the backward
+// pass x and dy in and dx out, so a row is read once into registers (as it is stored: 16 bytes of a
+// 16-bit type cost four registers) and everything else happens there. The mean is subtracted before
+// the squares are summed (no E[x^2] - mu^2 cancellation); sums are float32 (float64 for float64).
+//
+// A row belongs to a group of TPR threads, each of which holds EPT elements: a warp up to 1024
+// columns (no barrier, four rows per thread block), 128 threads up to 2048, and so on to 512 for 16384. Longer rows are
+// read again from L2 by a looping kernel.
+//
+// The parameters' gradients are sums over all rows. The thread blocks of the backward kernel are
+// resident for the whole pass and walk the rows with the grid's stride; a thread sees the same columns
+// in every row, so it keeps its columns' two sums in registers and the block writes ONE partial
+// row at its end. A second kernel adds the partial rows (a few hundred) in a fixed order: no
+// atomics, the same bits on every run.
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace tnb {
+namespace {
+
+struct NormArgs {
+    const void* x;
+    const void* dy;       // backward only
+    const void* weight;   // may be null
+    const void* bias;     // may be null
+    void* y;              // y, or dx
+    void* mean;           // float32 (float64 for float64 rows); the forward pass may leave them out
+    void* rstd;
+    void* partial;        // backward: [blocks][2][cols]
+    int64_t rows, x_pitch, dy_pitch;
+    int cols;
+    double eps;
+};
+
+template <typename T> struct stat_of { using type = float; };
+template <> struct stat_of<double> { using type = double; };
+
+// VEC consecutive elements moved by loads of up to 16 bytes.
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC < 16 ? sizeof(T) * VEC : 16) Pack {
+    T v[VEC];
+};
+
+template <typename S>
+__device__ __forceinline__ S warp_sum(S v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+
+// Sum over a group of TPR threads. `slot` is the shared memory of this reduction ([TPR / 32] values); two
+// consecutive reductions use different slots, so one barrier each is enough: a slot is written
+// again only after a barrier that every reader of its old contents has passed.
+template <typename S, int TPR>
+__device__ __forceinline__ S group_sum(S v, S* slot) {
+    v = warp_sum(v);
+    if constexpr (TPR > 32) {
+        if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = slot[0];
+#pragma unroll
+        for (int w = 1; w < TPR / 32; ++w) v += slot[w];
+    }
+    return v;
+}
+
+template <int TPR> constexpr int kBlock = TPR < 128 ? 128 : TPR;
+
+template <typename T, typename P, int VEC, int EPT, int TPR>
+__global__ void __launch_bounds__(kBlock<TPR>) norm_forward(const NormArgs a) {
+    using S = typename stat_of<T>::type;
+    constexpr int ITEMS = EPT / VEC, GROUPS = kBlock<TPR> / TPR;
+    __shared__ S slots[2][TPR / 32];
+    const int t = threadIdx.x % TPR, vecs = a.cols / VEC;
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + threadIdx.x / TPR; row < a.rows; row += static_cast<int64_t>(gridDim.x) * GROUPS) {
+        const Pack<T, VEC>* x = reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.x) + row * a.x_pitch);
+        Pack<T, VEC> raw[ITEMS];
+        S sum = 0;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (i * TPR + t < vecs) raw[i] = x[i * TPR + t];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (i * TPR + t < vecs) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) sum += to_compute<S>(raw[i].v[j]);
+            }
+        const S mean = group_sum<S, TPR>(sum, slots[0]) / static_cast<S>(a.cols);
+        S square = 0;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (i * TPR + t < vecs) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const S c = to_compute<S>(raw[i].v[j]) - mean;
+                    square += c * c;
+                }
+            }
+        const S rstd = S(1) / sqrt(group_sum<S, TPR>(square, slots[1]) / static_cast<S>(a.cols) + static_cast<S>(a.eps));
+        if (t == 0) {
+            if (a.mean) static_cast<S*>(a.mean)[row] = mean;
+            if (a.rstd) static_cast<S*>(a.rstd)[row] = rstd;
+        }
+        Pack<T, VEC>* y = reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.y) + row * a.cols);
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int at = i * TPR + t;
+            if (at < vecs) {
+                Pack<P, VEC> w, b;
+                if (a.weight) w = static_cast<const Pack<P, VEC>*>(a.weight)[at];
+                if (a.bias) b = static_cast<const Pack<P, VEC>*>(a.bias)[at];
+                Pack<T, VEC> out;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    S v = (to_compute<S>(raw[i].v[j]) - mean) * rstd;
+                    if (a.weight) v *= to_compute<S>(w.v[j]);
+                    if (a.bias) v += to_compute<S>(b.v[j]);
+                    out.v[j] = from_compute<T, S>(v);
+                }
+                y[at] = out;
+            }
+        }
+    }
+}
+
+template <typename T, typename P, int VEC, int EPT, int TPR>
+__global__ void __launch_bounds__(kBlock<TPR>) norm_backward(const NormArgs a) {
+    using S = typename stat_of<T>::type;
+    constexpr int ITEMS = EPT / VEC, GROUPS = kBlock<TPR> / TPR;
+    // 32 elements in each of 512 threads leave room for the two sums of a column but not for the row as well:
+    // the second half of the work then reads x, dy and w again, from L1 and L2
+    constexpr bool KEEP = EPT * TPR <= 8192;
+    __shared__ S slots[2][2][TPR / 32];
+    extern __shared__ uint8_t dynamic[];
+    const int t = threadIdx.x % TPR, group = threadIdx.x / TPR, vecs = a.cols / VEC;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * GROUPS;
+    S dw[EPT], db[EPT];
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) dw[e] = db[e] = 0;
+    Pack<P, VEC> w[KEEP ? ITEMS : 1];
+    if (KEEP && a.weight) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (i * TPR + t < vecs) w[i] = static_cast<const Pack<P, VEC>*>(a.weight)[i * TPR + t];
+    }
+    int parity = 0;
+    // with TPR > 32 a block has one group, so the block's threads leave this loop together
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group; row < a.rows; row += step, parity ^= 1) {
+        const Pack<T, VEC>* x = reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.x) + row * a.x_pitch);
+        const Pack<T, VEC>* dy = reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dy) + row * a.dy_pitch);
+        const S mean = static_cast<const S*>(a.mean)[row], rstd = static_cast<const S*>(a.rstd)[row];
+        Pack<T, VEC> rx[KEEP ? ITEMS : 1], rd[KEEP ? ITEMS : 1];
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (i * TPR + t < vecs) {
+                    rx[i] = x[i * TPR + t];
+                    rd[i] = dy[i * TPR + t];
+                }
+        }
+        auto fetch = [&](int i) {
+            if constexpr (!KEEP) {
+                rx[0] = x[i * TPR + t];
+                rd[0] = dy[i * TPR + t];
+                if (a.weight) w[0] = static_cast<const Pack<P, VEC>*>(a.weight)[i * TPR + t];
+            }
+            return KEEP ? i : 0;
+        };
+        S sum_g = 0, sum_gz = 0;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (i * TPR + t < vecs) {
+                const int k = fetch(i);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const S z = (to_compute<S>(rx[k].v[j]) - mean) * rstd, d = to_compute<S>(rd[k].v[j]);
+                    const S g = a.weight ? d * to_compute<S>(w[k].v[j]) : d;
+                    sum_g += g;
+                    sum_gz += g * z;
+                    dw[i * VEC + j] += d * z;
+                    db[i * VEC + j] += d;
+                }
+            }
+        sum_g = warp_sum(sum_g);
+        sum_gz = warp_sum(sum_gz);
+        if constexpr (TPR > 32) {
+            if ((threadIdx.x & 31) == 0) {
+                slots[parity][0][threadIdx.x >> 5] = sum_g;
+                slots[parity][1][threadIdx.x >> 5] = sum_gz;
+            }
+            __syncthreads();  // the other parity's slots are written only after every thread passed this
+            sum_g = slots[parity][0][0];
+            sum_gz = slots[parity][1][0];
+#pragma unroll
+            for (int q = 1; q < TPR / 32; ++q) {
+                sum_g += slots[parity][0][q];
+                sum_gz += slots[parity][1][q];
+            }
+        }
+        const S mean_g = sum_g / static_cast<S>(a.cols), mean_gz = sum_gz / static_cast<S>(a.cols);
+        Pack<T, VEC>* dx = reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.y) + row * a.cols);
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (i * TPR + t < vecs) {
+                const int k = fetch(i);
+                Pack<T, VEC> out;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const S z = (to_compute<S>(rx[k].v[j]) - mean) * rstd, d = to_compute<S>(rd[k].v[j]);
+                    const S g = a.weight ? d * to_compute<S>(w[k].v[j]) : d;
+                    out.v[j] = from_compute<T, S>((g - mean_g - z * mean_gz) * rstd);
+                }
+                dx[i * TPR + t] = out;
+            }
+    }
+    if (a.partial == nullptr) return;  // uniform: no parameter gradients wanted
+    S* mine = static_cast<S*>(a.partial) + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
+    if constexpr (GROUPS == 1) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (i * TPR + t < vecs) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    mine[(i * TPR + t) * VEC + j] = dw[i * VEC + j];
+                    mine[a.cols + (i * TPR + t) * VEC + j] = db[i * VEC + j];
+                }
+            }
+    } else {
+        // the block's groups add up in shared memory, one after the other
+        S* all = reinterpret_cast<S*>(dynamic);
+        for (int k = 0; k < GROUPS; ++k) {
+            if (group == k) {
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i)
+                    if (i * TPR + t < vecs) {
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) {
+                            const int c = (i * TPR + t) * VEC + j;
+                            all[c] = k ? all[c] + dw[i * VEC + j] : dw[i * VEC + j];
+                            all[a.cols + c] = k ? all[a.cols + c] + db[i * VEC + j] : db[i * VEC + j];
+                        }
+                    }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < 2 * a.cols; c += kBlock<TPR>) mine[c] = all[c];
+    }
+}
+
+// Rows longer than the registers of 512 threads hold: the row is read three times, from L2 after the first.
+constexpr int kLong = 1024;
+
+template <typename T, typename P>
+__global__ void __launch_bounds__(kLong) norm_forward_long(const NormArgs a) {
+    using S = typename stat_of<T>::type;
+    __shared__ S slots[2][kLong / 32];
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + row * a.x_pitch;
+        S sum = 0;
+        for (int c = threadIdx.x; c < a.cols; c += kLong) sum += to_compute<S>(x[c]);
+        const S mean = group_sum<S, kLong>(sum, slots[0]) / static_cast<S>(a.cols);
+        S square = 0;
+        for (int c = threadIdx.x; c < a.cols; c += kLong) {
+            const S d = to_compute<S>(x[c]) - mean;
+            square += d * d;
+        }
+        const S rstd = S(1) / sqrt(group_sum<S, kLong>(square, slots[1]) / static_cast<S>(a.cols) + static_cast<S>(a.eps));
+        if (threadIdx.x == 0) {
+            if (a.mean) static_cast<S*>(a.mean)[row] = mean;
+            if (a.rstd) static_cast<S*>(a.rstd)[row] = rstd;
+        }
+        T* y = static_cast<T*>(a.y) + row * a.cols;
+        for (int c = threadIdx.x; c < a.cols; c += kLong) {
+            S v = (to_compute<S>(x[c]) - mean) * rstd;
+            if (a.weight) v *= to_compute<S>(static_cast<const P*>(a.weight)[c]);
+            if (a.bias) v += to_compute<S>(static_cast<const P*>(a.bias)[c]);
+            y[c] = from_compute<T, S>(v);
+        }
+    }
+}
+
+template <typename T, typename P>
+__global__ void __launch_bounds__(kLong) norm_backward_long(const NormArgs a) {
+    using S = typename stat_of<T>::type;
+    __shared__ S slots[2][kLong / 32];
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + row * a.x_pitch;
+        const T* dy = static_cast<const T*>(a.dy) + row * a.dy_pitch;
+        const S mean = static_cast<const S*>(a.mean)[row], rstd = static_cast<const S*>(a.rstd)[row];
+        S sum_g = 0, sum_gz = 0;
+        for (int c = threadIdx.x; c < a.cols; c += kLong) {
+            const S z = (to_compute<S>(x[c]) - mean) * rstd;
+            S g = to_compute<S>(dy[c]);
+            if (a.weight) g *= to_compute<S>(static_cast<const P*>(a.weight)[c]);
+            sum_g += g;
+            sum_gz += g * z;
+        }
+        const S mean_g = group_sum<S, kLong>(sum_g, slots[0]) / static_cast<S>(a.cols);
+        const S mean_gz = group_sum<S, kLong>(sum_gz, slots[1]) / static_cast<S>(a.cols);
+        T* dx = static_cast<T*>(a.y) + row * a.cols;
+        for (int c = threadIdx.x; c < a.cols; c += kLong) {
+            const S z = (to_compute<S>(x[c]) - mean) * rstd;
+            S g = to_compute<S>(dy[c]);
+            if (a.weight) g *= to_compute<S>(static_cast<const P*>(a.weight)[c]);
+            dx[c] = from_compute<T, S>((g - mean_g - z * mean_gz) * rstd);
+        }
+    }
+}
+
+// The parameters' gradients of such rows: blockIdx.y takes every gridDim.y-th row, a thread one column.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_columns_long(const NormArgs a) {
+    using S = typename stat_of<T>::type;
+    S* mine = static_cast<S*>(a.partial) + static_cast<int64_t>(blockIdx.y) * 2 * a.cols;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (c >= a.cols) return;
+    S dw = 0, db = 0;
+#pragma unroll 4
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        const S mean = static_cast<const S*>(a.mean)[row], rstd = static_cast<const S*>(a.rstd)[row];
+        const S d = to_compute<S>(static_cast<const T*>(a.dy)[row * a.dy_pitch + c]);
+        dw += d * ((to_compute<S>(static_cast<const T*>(a.x)[row * a.x_pitch + c]) - mean) * rstd);
+        db += d;
+    }
+    mine[c] = dw;
+    mine[a.cols + c] = db;
+}
+
+// Adds the partial rows, in an order that depends on their number only: 32 columns per block, 32 threads a column.
+template <typename S, typename P>
+__global__ void __launch_bounds__(1024) norm_parameters(const S* __restrict__ partial, int blocks, int cols, P* __restrict__ dweight, P* __restrict__ dbias) {
+    __shared__ S part[32][33];
+    const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
+    // columns [0, cols) are the weight's, [cols, 2 cols) the bias's
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+    const int64_t all = static_cast<int64_t>(cols) * 2;
+    S sum = 0;
+    if (c < all) {
+#pragma unroll 4
+        for (int b = k; b < blocks; b += 32) sum += partial[static_cast<int64_t>(b) * all + c];
+    }
+    part[k][lane] = sum;
+    __syncthreads();
+    sum = warp_sum(part[lane][k]);  // thread (lane, k): partial sum `lane` of column k
+    const int64_t out = static_cast<int64_t>(blockIdx.x) * 32 + k;
+    if (lane == 0 && out < all) {
+        if (out < cols) {
+            if (dweight) dweight[out] = from_compute<P, S>(sum);
+        } else if (dbias) {
+            dbias[out - cols] = from_compute<P, S>(sum);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host ---------------
+int64_t rows_grid(int64_t rows, int groups) { return std::min<int64_t>(ceil_div(rows, groups), int64_t(1) << 30); }
+
+struct Launch {
+    NormArgs args;
+    cudaStream_t stream;
+    bool backward;
+    void* dweight = nullptr;  // backward: parameter gradients, either may be null
+    void* dbias = nullptr;
+};
+
+// Allocates the partial rows of a backward pass with `blocks` thread blocks.
+template <typename S>
+tn_status alloc_partial(Launch& l, int64_t blocks) {
+    l.args.partial = nullptr;
+    if (!l.dweight && !l.dbias) return TN_SUCCESS;
+    return scratch_alloc(&l.args.partial, sizeof(S) * 2 * static_cast<size_t>(blocks) * static_cast<size_t>(l.args.cols), l.stream);
+}
+
+template <typename S, typename P>
+tn_status finish_partial(Launch& l, int64_t blocks) {
+    if (!l.args.partial) return TN_SUCCESS;
+    norm_parameters<S, P><<<(unsigned)ceil_div(2 * (int64_t)l.args.cols, 32), 1024, 0, l.stream>>>(
+        static_cast<const S*>(l.args.partial), (int)blocks, l.args.cols, static_cast<P*>(l.dweight), static_cast<P*>(l.dbias));
+    return after_launch("norm_parameters");
+}
+
+template <typename T, typename P, int VEC, int EPT, int TPR>
+tn_status launch_rows(Launch& l) {
+    using S = typename stat_of<T>::type;
+    constexpr int GROUPS = kBlock<TPR> / TPR;
+    if (!l.backward) {
+        norm_forward<T, P, VEC, EPT, TPR><<<(unsigned)rows_grid(l.args.rows, GROUPS), kBlock<TPR>, 0, l.stream>>>(l.args);
+        return after_launch("norm_forward");
+    }
+    const size_t smem = GROUPS > 1 ? sizeof(S) * 2 * (size_t)l.args.cols : 0;
+    // one resident wave: every block walks rows until the pass ends, then writes its partial row
+    static std::atomic<int> resident{0};
+    int per_sm = resident.load(std::memory_order_relaxed);
+    if (per_sm == 0) {
+        TN_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, norm_backward<T, P, VEC, EPT, TPR>, kBlock<TPR>, GROUPS > 1 ? sizeof(S) * 2 * EPT * TPR : 0));
+        if (per_sm < 1) per_sm = 1;
+        resident.store(per_sm, std::memory_order_relaxed);
+    }
+    const int64_t blocks = std::min<int64_t>(ceil_div(l.args.rows, GROUPS), (int64_t)sm_count() * per_sm);
+    TN_TRY(alloc_partial<S>(l, blocks));
+    norm_backward<T, P, VEC, EPT, TPR><<<(unsigned)blocks, kBlock<TPR>, smem, l.stream>>>(l.args);
+    tn_status st = after_launch("norm_backward");
+    if (st == TN_SUCCESS) st = finish_partial<S, P>(l, blocks);
+    if (l.args.partial) {
+        const tn_status freed = scratch_free(l.args.partial, l.stream);
+        if (st == TN_SUCCESS) st = freed;
+    }
+    return st;
+}
+
+template <typename T, typename P>
+tn_status launch_long(Launch& l) {
+    using S = typename stat_of<T>::type;
+    if (!l.backward) {
+        norm_forward_long<T, P><<<(unsigned)rows_grid(l.args.rows, 1), kLong, 0, l.stream>>>(l.args);
+        return after_launch("norm_forward_long");
+    }
+    // the columns first: dx may take the place of dy or x
+    const int64_t across = ceil_div(l.args.cols, 256);
+    const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(l.args.rows, 1024), ceil_div((int64_t)sm_count() * 8, across)));
+    TN_TRY(alloc_partial<S>(l, blocks));
+    tn_status st = TN_SUCCESS;
+    if (l.args.partial) {
+        norm_columns_long<T><<<dim3((unsigned)across, (unsigned)blocks), 256, 0, l.stream>>>(l.args);
+        st = after_launch("norm_columns_long");
+        if (st == TN_SUCCESS) st = finish_partial<S, P>(l, blocks);
+        const tn_status freed = scratch_free(l.args.partial, l.stream);
+        if (st == TN_SUCCESS) st = freed;
+    }
+    if (st != TN_SUCCESS) return st;
+    norm_backward_long<T, P><<<(unsigned)rows_grid(l.args.rows, 1), kLong, 0, l.stream>>>(l.args);
+    return after_launch("norm_backward_long");
+}
+
+template <typename T, typename P, int VEC>
+tn_status launch_sized(Launch& l) {
+    const int c = l.args.cols;
+    if (c <= 256) return launch_rows<T, P, VEC, 8, 32>(l);
+    if (c <= 512) return launch_rows<T, P, VEC, 16, 32>(l);
+    if constexpr (std::is_same<T, double>::value) {  // twice the registers an element
+        if (c <= 2048) return launch_rows<T, P, VEC, 16, 128>(l);
+    } else {
+        if (c <= 1024) return launch_rows<T, P, VEC, 32, 32>(l);
+        if (c <= 2048) return launch_rows<T, P, VEC, 16, 128>(l);
+        if (c <= 4096) return launch_rows<T, P, VEC, 16, 256>(l);
+        if (c <= 8192) return launch_rows<T, P, VEC, 16, 512>(l);
+        if (c <= 16384) return launch_rows<T, P, VEC, 32, 512>(l);
+    }
+    return launch_long<T, P>(l);
+}
+
+template <typename T, typename P>
+tn_status launch_typed(Launch& l) {
+    constexpr int VEC = 16 / sizeof(T);
+    const NormArgs& a = l.args;
+    // 16-byte accesses need every row of every operand to start on a 16-byte boundary
+    auto fits = [](const void* p, int64_t pitch_bytes) { return ((reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(pitch_bytes)) & 15) == 0; };
+    bool wide = a.cols % VEC == 0 && fits(a.x, a.x_pitch * (int64_t)sizeof(T)) && fits(a.y, a.cols * (int64_t)sizeof(T)) && fits(a.weight, 0) && fits(a.bias, 0);
+    if (l.backward) wide = wide && fits(a.dy, a.dy_pitch * (int64_t)sizeof(T));
+    return wide ? launch_sized<T, P, VEC>(l) : launch_sized<T, P, 1>(l);
+}
+
+tn_status launch_any(Launch& l, int dtype, int param_dtype) {
+    const bool wide_params = param_dtype == TN_FLOAT32;
+    switch (dtype) {
+        case TN_FLOAT16: return wide_params ? launch_typed<__half, float>(l) : launch_typed<__half, __half>(l);
+        case TN_BFLOAT16: return wide_params ? launch_typed<__nv_bfloat16, float>(l) : launch_typed<__nv_bfloat16, __nv_bfloat16>(l);
+        case TN_FLOAT32: return launch_typed<float, float>(l);
+        default: return launch_typed<double, double>(l);
+    }
+}
+
+bool dense(const tn_tensor_t* t) {
+    int64_t expect = 1;
+    for (int d = t->rank - 1; d >= 0; --d) {
+        if (t->shape.sizes[d] != 1 && t->strides.sizes[d] != expect) return false;
+        expect *= (int64_t)t->shape.sizes[d];
+    }
+    return true;
+}
+
+// An operand whose rows can be read in place: the last axis contiguous and all rows one pitch apart
+// (any pitch, 0 for a broadcast row). Otherwise the view is copied dense into scratch memory first.
+struct Rows {
+    const void* base = nullptr;
+    int64_t pitch = 0;
+    void* scratch = nullptr;
+};
+tn_status rows_of(const tn_tensor_t* t, Rows* out, tn_stream_t stream) {
+    const int last = t->rank - 1;
+    out->base = t->address;
+    out->pitch = (int64_t)t->shape.sizes[last];
+    bool one = t->shape.sizes[last] == 1 || t->strides.sizes[last] == 1;
+    int64_t expect = 0;
+    bool any = false;
+    for (int d = last - 1; one && d >= 0; --d) {
+        if (t->shape.sizes[d] == 1) continue;
+        if (!any) out->pitch = t->strides.sizes[d];
+        else one = t->strides.sizes[d] == expect;
+        any = true;
+        expect = t->strides.sizes[d] * (int64_t)t->shape.sizes[d];
+    }
+    if (one) return TN_SUCCESS;
+    tn_tensor_t copy = *t;
+    int64_t run = 1;
+    for (int d = last; d >= 0; --d) {
+        copy.strides.sizes[d] = run;
+        run *= (int64_t)t->shape.sizes[d];
+    }
+    copy.layout = TN_CONTIGUOUS;
+    TN_TRY(scratch_alloc(&out->scratch, t->size * (size_t)dtype_bytes(t->dtype), as_cuda(stream)));
+    copy.address = out->scratch;
+    out->base = out->scratch;
+    out->pitch = (int64_t)t->shape.sizes[last];
+    return tn_cpy(t, &copy, stream);
+}
+tn_status release(Rows* r, cudaStream_t s, tn_status st) {
+    if (!r->scratch) return st;
+    const tn_status freed = scratch_free(r->scratch, s);
+    r->scratch = nullptr;
+    return st == TN_SUCCESS ? freed : st;
+}
+
+tn_status check_rows(const tn_tensor_t* x, const char* op) {
+    if (!x) return fail(TN_ERROR, "%s: null tensor", op);
+    if (x->rank < 1) return fail(TN_ERROR, "%s: the input needs an axis to normalise over", op);
+    if (!is_float(x->dtype)) return fail(TN_UNSUPPORTED_DTYPE, "%s: dtype %d unsupported", op, (int)x->dtype);
+    if (x->environment.kind != TN_DEVICE) return fail(TN_INCOMPATIBLE_DEVICES, "%s: device entry point called with a host tensor (no CPU fallback)", op);
+    const size_t cols = x->shape.sizes[x->rank - 1];
+    if (cols == 0) return fail(TN_ERROR, "%s: the last axis is empty", op);
+    if (cols > (size_t(1) << 30)) return fail(TN_ERROR, "%s: %zu columns, at most 2^30", op, cols);
+    return TN_SUCCESS;
+}
+tn_status same_device(const tn_tensor_t* x, const tn_tensor_t* t, const char* op) {
+    if (t->environment.kind != TN_DEVICE || t->environment.resource.device.id != x->environment.resource.device.id)
+        return fail(TN_INCOMPATIBLE_DEVICES, "%s: operands must live on one device", op);
+    return TN_SUCCESS;
+}
+tn_status check_like(const tn_tensor_t* x, const tn_tensor_t* t, bool result, const char* op, const char* what) {
+    if (!t) return fail(TN_ERROR, "%s: null %s", op, what);
+    if (t->dtype != x->dtype) return fail(TN_UNSUPPORTED_DTYPE, "%s: %s has dtype %d, the input %d", op, what, (int)t->dtype, (int)x->dtype);
+    bool same = t->rank == x->rank;
+    for (int d = 0; same && d < x->rank; ++d) same = t->shape.sizes[d] == x->shape.sizes[d];
+    if (!same) return fail(TN_ERROR, "%s: %s must have the input's shape", op, what);
+    if (result && !dense(t)) return fail(TN_ERROR, "%s: %s must be dense", op, what);
+    return same_device(x, t, op);
+}
+tn_status check_stat(const tn_tensor_t* x, const tn_tensor_t* t, const char* op, const char* what) {
+    const tn_dtype want = x->dtype == TN_FLOAT64 ? TN_FLOAT64 : TN_FLOAT32;
+    if (t->dtype != want) return fail(TN_UNSUPPORTED_DTYPE, "%s: %s has dtype %d, expected %d", op, what, (int)t->dtype, (int)want);
+    const size_t rows = x->size / x->shape.sizes[x->rank - 1];
+    if (t->size != rows) return fail(TN_ERROR, "%s: %s has %zu elements, the input has %zu rows", op, what, t->size, rows);
+    if (!dense(t)) return fail(TN_ERROR, "%s: %s must be dense", op, what);
+    return same_device(x, t, op);
+}
+// A parameter row (or its gradient): [columns], contiguous, of the input's dtype or float32 beside 16-bit rows.
+tn_status check_param(const tn_tensor_t* x, const tn_tensor_t* t, const char* op, const char* what) {
+    if (t->dtype != x->dtype && !(is_half(x->dtype) && t->dtype == TN_FLOAT32))
+        return fail(TN_UNSUPPORTED_DTYPE, "%s: %s has dtype %d beside an input of dtype %d", op, what, (int)t->dtype, (int)x->dtype);
+    if (t->rank != 1 || t->shape.sizes[0] != x->shape.sizes[x->rank - 1]) return fail(TN_ERROR, "%s: %s must be a vector as long as the last axis", op, what);
+    if (!dense(t)) return fail(TN_ERROR, "%s: %s must be contiguous", op, what);
+    return same_device(x, t, op);
+}
+
+}  // namespace
+}  // namespace tnb
+
+using namespace tnb;
+
+extern "C" {
+
+tn_status tn_layer_norm(const tn_tensor_t* x, const tn_tensor_t* weight, const tn_tensor_t* bias, tn_tensor_t* y, tn_tensor_t* mean, tn_tensor_t* rstd,
+                        tn_stream_t stream, double eps) {
+    const char* op = "layer_norm";
+    TN_TRY(check_rows(x, op));
+    TN_TRY(check_like(x, y, true, op, "the result"));
+    if (weight) TN_TRY(check_param(x, weight, op, "weight"));
+    if (bias) TN_TRY(check_param(x, bias, op, "bias"));
+    if (weight && bias && weight->dtype != bias->dtype) return fail(TN_UNSUPPORTED_DTYPE, "layer_norm: weight and bias must share a dtype");
+    if (mean) TN_TRY(check_stat(x, mean, op, "mean"));
+    if (rstd) TN_TRY(check_stat(x, rstd, op, "rstd"));
+    if (!(eps >= 0.0)) return fail(TN_ERROR, "layer_norm: eps must not be negative");
+    TN_TRY(use_device_of(x));
+    if (x->size == 0) return TN_SUCCESS;
+    Rows rows;
+    tn_status st = rows_of(x, &rows, stream);
+    if (st == TN_SUCCESS) {
+        Launch l = {};
+        l.stream = as_cuda(stream);
+        l.backward = false;
+        NormArgs& a = l.args;
+        a.x = rows.base;
+        a.x_pitch = rows.pitch;
+        a.weight = weight ? weight->address : nullptr;
+        a.bias = bias ? bias->address : nullptr;
+        a.y = y->address;
+        a.mean = mean ? mean->address : nullptr;
+        a.rstd = rstd ? rstd->address : nullptr;
+        a.cols = (int)x->shape.sizes[x->rank - 1];
+        a.rows = (int64_t)x->size / a.cols;
+        a.eps = eps;
+        st = launch_any(l, x->dtype, weight ? weight->dtype : bias ? bias->dtype : x->dtype);
+    }
+    return release(&rows, as_cuda(stream), st);
+}
+
+tn_status tn_layer_norm_grad(const tn_tensor_t* dy, const tn_tensor_t* x, const tn_tensor_t* mean, const tn_tensor_t* rstd, const tn_tensor_t* weight,
+                             tn_tensor_t* dx, tn_tensor_t* dweight, tn_tensor_t* dbias, tn_stream_t stream) {
+    const char* op = "layer_norm_grad";
+    TN_TRY(check_rows(x, op));
+    TN_TRY(check_like(x, dy, false, op, "the result's gradient"));
+    TN_TRY(check_like(x, dx, true, op, "the input's gradient"));
+    if (!mean || !rstd) return fail(TN_ERROR, "layer_norm_grad: null statistics");
+    TN_TRY(check_stat(x, mean, op, "mean"));
+    TN_TRY(check_stat(x, rstd, op, "rstd"));
+    if (weight) TN_TRY(check_param(x, weight, op, "weight"));
+    if (dweight) TN_TRY(check_param(x, dweight, op, "the weight's gradient"));
+    if (dbias) TN_TRY(check_param(x, dbias, op, "the bias's gradient"));
+    const int param = weight ? weight->dtype : dweight ? dweight->dtype : dbias ? dbias->dtype : x->dtype;
+    if ((dweight && (int)dweight->dtype != param) || (dbias && (int)dbias->dtype != param))
+        return fail(TN_UNSUPPORTED_DTYPE, "layer_norm_grad: the parameters and their gradients must share a dtype");
+    TN_TRY(use_device_of(x));
+    cudaStream_t s = as_cuda(stream);
+    if (x->size == 0) {  // no rows: the sums over them are zero
+        for (tn_tensor_t* t : {dweight, dbias})
+            if (t) TN_CUDA(cudaMemsetAsync(t->address, 0, t->size * (size_t)dtype_bytes(t->dtype), s));
+        return TN_SUCCESS;
+    }
+    Rows rx, rd;
+    tn_status st = rows_of(x, &rx, stream);
+    if (st == TN_SUCCESS) st = rows_of(dy, &rd, stream);
+    if (st == TN_SUCCESS) {
+        Launch l = {};
+        l.stream = s;
+        l.backward = true;
+        l.dweight = dweight ? dweight->address : nullptr;
+        l.dbias = dbias ? dbias->address : nullptr;
+        NormArgs& a = l.args;
+        a.x = rx.base;
+        a.x_pitch = rx.pitch;
+        a.dy = rd.base;
+        a.dy_pitch = rd.pitch;
+        a.weight = weight ? weight->address : nullptr;
+        a.y = dx->address;
+        a.mean = mean->address;
+        a.rstd = rstd->address;
+        a.cols = (int)x->shape.sizes[x->rank - 1];
+        a.rows = (int64_t)x->size / a.cols;
+        st = launch_any(l, x->dtype, param);
+    }
+    st = release(&rd, s, st);
+    return release(&rx, s, st);
+}
+
+}  // extern "C"

@@ -467,6 +467,39 @@ def reduce_stats(x: torch.Tensor, axis=-1, keepdim=False):
     return mx, sm, am
 
 
+def _ref(t: torch.Tensor | None):
+    """A record to pass by reference, or a null pointer."""
+    return None if t is None else C.byref(desc(t))
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5, stats: bool = False,
+               out: torch.Tensor | None = None):
+    """(x - mean) * rstd * weight + bias over the last axis (tn_layer_norm). `weight` and `bias`: vectors of x's dtype,
+    or float32 beside 16-bit x. With `stats`, (y, mean, rstd): the statistics `layer_norm_grad` needs, one per row.
+    `out` (optional) is a preallocated dense result; it may be x itself where x is dense."""
+    if x.dim() == 0:
+        raise ValueError("cannot normalise a rank-0 tensor")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if stats:
+        mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float64 if x.dtype == torch.float64 else torch.float32, device=x.device) for _ in range(2))
+    A.check(A.lib().tn_layer_norm(_ref(x), _ref(weight), _ref(bias), _ref(out), _ref(mean), _ref(rstd), current_stream(x), eps))
+    return (out, mean, rstd) if stats else out
+
+
+def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None = None, bias: bool = True):
+    """(dx, dweight, dbias) of `layer_norm` from its result's gradient and its statistics (tn_layer_norm_grad). Without
+    `weight` the normalisation has no parameters and dweight and dbias are None; `bias=False`: it has no bias."""
+    if x.dim() == 0:
+        raise ValueError("cannot normalise a rank-0 tensor")
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dweight = torch.empty(weight.shape, dtype=weight.dtype, device=x.device) if weight is not None else None
+    dbias = torch.empty(weight.shape, dtype=weight.dtype, device=x.device) if weight is not None and bias else None
+    A.check(A.lib().tn_layer_norm_grad(_ref(dy), _ref(x), _ref(mean), _ref(rstd), _ref(weight), _ref(dx), _ref(dweight), _ref(dbias), current_stream(x)))
+    return dx, dweight, dbias
+
+
 def allclose(a: torch.Tensor, b: torch.Tensor, rtol: float = 1e-5, atol: float = 1e-8) -> bool:
     """include/tannic/comparisons.hpp:128 defaults."""
     da, db = desc(a), desc(b)
