@@ -141,6 +141,8 @@ PROTOTYPES = {
     "tn_argsum_fixed_scratch": [_TP, _TP, StreamT, C.c_uint8],
     "tn_layer_norm": [_TP, _TP, _TP, _TP, _TP, _TP, StreamT, C.c_double],
     "tn_layer_norm_grad": [_TP, _TP, _TP, _TP, _TP, _TP, _TP, _TP, StreamT],
+    "tn_linear_cross_entropy": [_TP, _TP, _TP, _TP, _TP, StreamT, C.c_int64],
+    "tn_linear_cross_entropy_grad": [_TP, _TP, _TP, _TP, _TP, _TP, _TP, StreamT, C.c_int64],
     "tn_cpy": [_TP, _TP, StreamT],
     "tn_allclose": [_TP, _TP, StreamT, C.c_double, C.c_double, C.POINTER(C.c_int)],
     "tn_device_errors": [C.POINTER(C.c_uint)],

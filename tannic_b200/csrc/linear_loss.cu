@@ -1,0 +1,1090 @@
+// Softmax cross entropy of a linear layer over a large vocabulary, and its gradient, without the logits.
+//
+//   l = h W^T    lse = log sum_v exp(l_v)    loss = lse - l_target
+//   d = (exp(l - lse) - onehot(target)) grad      dh = d W      dW = d^T h
+//
+// The products carry all the work (2 N H V for the loss, 6 N H V for the gradient, N tokens, H hidden, V
+// vocabulary) and run on the tensor cores (tcgen05, fp32 accumulation in tensor memory); the [N, V] logits
+// exist only as 128 x 256 tiles of tensor memory:
+//
+//   loss       The epilogue of the product keeps, per row and per half of a tile, the running maximum m and
+//              s = sum exp(l - m), and picks the target's logit out of its registers. A small kernel joins the halves
+//              of a row: lse = M + log sum s exp(m - M).
+//   gradient   The vocabulary is cut into pieces. For each piece the product is formed again (the same
+//              instructions in the same order, so the same logits) and its epilogue writes d, rounded to the operands' type, into a
+//              workspace of at most about half a GiB; two more products read it, dW's piece = d^T h and
+//              dh += d W's piece, the latter in float32 in memory. Forming the logits again costs
+//              2 N H V operations and saves writing, keeping and reading 4 N V bytes.
+//
+// Tokens without a target (ignore_index) take no part in the gradient: the rows of the others are
+// gathered in front, and the products stop at the last one. Their number stays on the device.
+//
+// float32 operands are written as three bfloat16 parts (24 significand bits), and a product as the six
+// products of parts that matter; a 64-wide block of K is six passes over those parts. bfloat16 and float16 are one part.
+//
+// d is rounded to the operands' 16-bit type because the tensor cores take operands of one type. It is
+// scaled by a power of two first, so that the largest upstream gradient lands at 2^14: float16 would lose the small
+// probabilities otherwise (grad = 1/N and p = 1/V are below its smallest number). The results are
+// scaled back, exactly, in float32.
+//
+// Kernel layout as in gemm_tc.cu: warp 0 TMA producer, warp 1 MMA issuer, warps 2..9 epilogue, persistent
+// thread blocks of a 128 x 256 tile, 64-wide K blocks in four stages, two accumulators so that the
+// epilogue of a tile runs under the products of the next. Bounded waits throughout.
+#include <algorithm>
+
+#include "tc_common.cuh"
+
+namespace tnb {
+
+static __device__ unsigned int g_loss_aborts = 0;
+
+tn_status loss_abort_count(unsigned int* count) {
+    TN_CUDA(cudaMemcpyFromSymbol(count, g_loss_aborts, sizeof(unsigned int)));
+    return TN_SUCCESS;
+}
+
+namespace {
+
+constexpr int STAGES = 4;
+constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpilogueWarps;
+constexpr uint32_t kBoxBytes = 2048;                       // 32 rows x 64 bytes
+constexpr uint32_t kWarpBytes = 2 * kBoxBytes;             // two boxes per warp, or 32 rows x 80 bytes
+constexpr uint32_t kSmemBytes = 1024 + STAGES * STAGE_BYTES + kEpilogueWarps * kWarpBytes + 256;
+static_assert(kSmemBytes <= 232448, "exceeds the shared memory of an SM");
+
+// A row of the gradient's products: a token with a target, or (target kNoRow) nothing.
+struct alignas(16) RowInfo {
+    float lse;
+    float grad;   // upstream gradient times the scale of d
+    int target;
+    int unused;
+};
+constexpr int kNoRow = -1;
+
+// Passes over the parts of a float32 operand pair, largest product first.
+__constant__ int kPartA[6] = {0, 0, 1, 0, 1, 2};
+__constant__ int kPartB[6] = {0, 1, 0, 2, 1, 0};
+
+enum { EPI_STATS = 0, EPI_D = 1, EPI_SUM = 2, EPI_RESULT = 3 };
+// How the number of tokens that count bounds a product: not at all, its rows, or its K extent.
+enum { COUNT_NONE = 0, COUNT_ROWS = 1, COUNT_K = 2 };
+
+struct LossArgs {
+    int64_t M, N;            // rows and columns of the result
+    int n_tiles;
+    int m_tiles;
+    int k_blocks;            // 64-wide blocks of K, all splits together
+    int splits, split_blocks;
+    int terms;               // 1, or 6 for float32 operands
+    int is_bf16;
+    const int* count;        // tokens with a target
+    int count_is;
+    int64_t vocab0;          // first vocabulary entry of this piece
+    // EPI_STATS
+    const void* targets;
+    int wide_targets;        // int64, else int32
+    float2* halves;          // [2 * column tiles of all pieces][M]: maximum, sum of exponentials
+    int64_t first_half;
+    float* target_logit;     // [M]
+    // EPI_D
+    const RowInfo* rows;
+    // EPI_SUM: add to what is there
+    int add;
+    // EPI_RESULT
+    void* d;
+    int64_t ldd;
+    const float* scale;
+    int tma_store;
+};
+
+__device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
+        ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+
+// Hands 32 rows x 64 bytes (a lane's row in `w`) to TMA, which clips the box at the tensor's edges.
+struct BoxStore {
+    uint8_t* stage;
+    const CUtensorMap* map;
+    int lane, flip;
+    __device__ __forceinline__ void put(const uint32_t (&w)[16], int c0, int c1, int c2, bool add) {
+        uint8_t* buf = stage + (flip & 1) * kBoxBytes;
+        flip ^= 1;
+        if (lane == 0) bulk_wait_read_1();  // the box that used this buffer two boxes ago has left it
+        __syncwarp();
+        const int x = (lane >> 1) & 3;      // 64-byte swizzle
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ x) << 4)) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            if (add) tma_add_3d(map, smem_u32(buf), c0, c1, c2);
+            else tma_store_3d(map, smem_u32(buf), c0, c1, c2);
+            bulk_commit();
+        }
+    }
+};
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// x = p0 + p1 + p2, each part a bfloat16 (whose exponent range is float32's). An infinity or NaN stays in p0.
+__device__ __forceinline__ void three_parts(float x, float& p0, float& p1, float& p2) {
+    p0 = __bfloat162float(__float2bfloat16_rn(x));
+    if (isinf(p0) && !isinf(x)) p0 = copysignf(__uint_as_float(0x7F7F0000u), x);  // rounded up past the largest number
+    const float r = isfinite(x) ? x - p0 : 0.0f;
+    p1 = __bfloat162float(__float2bfloat16_rn(r));
+    p2 = r - p1;  // at most 8 significand bits are left; rounded when it is packed
+}
+
+// Calls body(values, chunk) for this warp's 32-column chunks of an accumulator; the next chunk's load runs under the body.
+template <typename Body>
+__device__ __forceinline__ void drain(uint32_t taddr, int first, int chunks, Body&& body) {
+    uint32_t va[32], vb[32];
+    int c = first;
+    if (c >= chunks) return;
+    tmem_load_issue(taddr + c * 32, va);
+    while (true) {
+        tmem_load_wait(va);
+        if (c + 2 < chunks) tmem_load_issue(taddr + (c + 2) * 32, vb);
+        body(va, c);
+        c += 2;
+        if (c >= chunks) break;
+        tmem_load_wait(vb);
+        if (c + 2 < chunks) tmem_load_issue(taddr + (c + 2) * 32, va);
+        body(vb, c);
+        c += 2;
+        if (c >= chunks) break;
+    }
+}
+
+// Running maximum and sum of exponentials of the valid ones among 32 logits.
+__device__ __forceinline__ void online_softmax(const uint32_t (&v)[32], int ncols, float& m, float& s) {
+    float top = -INFINITY;
+    if (ncols == 32) {  // warp-uniform
+#pragma unroll
+        for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(v[j]));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (j < ncols) top = fmaxf(top, __uint_as_float(v[j]));
+    }
+    const float now = fmaxf(m, top);
+    const float base = now == -INFINITY ? 0.0f : now;  // nothing but -inf so far: the sum stays 0
+    s *= __expf(m - base);
+    float s0 = 0.0f, s1 = 0.0f;
+    if (ncols == 32) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+            s0 += __expf(__uint_as_float(v[j]) - base);
+            s1 += __expf(__uint_as_float(v[j + 1]) - base);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (j < ncols) s0 += __expf(__uint_as_float(v[j]) - base);
+    }
+    s += s0 + s1;
+    m = now;
+}
+
+// A_M: A is stored [K, M] (M contiguous), else [M, K]. B_N: B is stored [K, N], else [N, K]. T: operand type (bfloat16 parts
+// for float32). OUT: result type of EPI_RESULT. PARTS: parts of d that EPI_D writes.
+template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS>
+__global__ void __launch_bounds__(kThreads, 1)
+loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_d, const LossArgs g) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;  // swizzled tiles need 1024-byte alignment
+    uint8_t* base_ptr = smem_raw + (base - raw);
+    uint8_t* staging_ptr = base_ptr + STAGES * STAGE_BYTES;
+    const uint32_t bars = base + STAGES * STAGE_BYTES + kEpilogueWarps * kWarpBytes;
+    // barriers of 8 bytes: full[STAGES], empty[STAGES], accumulator full[2], accumulator empty[2]
+    const uint32_t full0 = bars, empty0 = bars + 8 * STAGES, accf0 = bars + 16 * STAGES, acce0 = accf0 + 16;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(staging_ptr + kEpilogueWarps * kWarpBytes + 16 * STAGES + 32);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // the tokens that count bound the rows or the K extent
+    int m_tiles = g.m_tiles, k_blocks = g.k_blocks;
+    if (g.count_is != COUNT_NONE) {
+        const int count = *g.count;
+        if (g.count_is == COUNT_ROWS) m_tiles = (count + BM - 1) / BM;
+        else k_blocks = (count + BK - 1) / BK;
+    }
+    const uint32_t per_split = static_cast<uint32_t>(m_tiles) * static_cast<uint32_t>(g.n_tiles);
+    const uint32_t total = per_split * static_cast<uint32_t>(g.splits);
+    // K blocks [first, first + n) of split z
+    auto split_range = [&](int z, int& first, int& n) {
+        first = z * g.split_blocks;
+        n = min(k_blocks - first, g.split_blocks);
+    };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(accf0 + 8 * b, 1);
+            mbar_init(acce0 + 8 * b, kEpilogueWarps);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer ----
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
+                int z, mt, nt, first, blocks;
+                tile_coords(t, m_tiles, g.n_tiles, z, mt, nt);
+                split_range(z, first, blocks);
+                for (int kb = first; ok && kb < first + blocks; ++kb) {
+                    for (int term = 0; term < g.terms; ++term, ++it) {
+                        const int s = it % STAGES;
+                        if (!mbar_wait(empty0 + 8 * s, ((it / STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                        const uint32_t sa = base + s * STAGE_BYTES, sb = sa + A_BYTES, bar = full0 + 8 * s;
+                        const int pa = g.terms > 1 ? kPartA[term] : 0, pb = g.terms > 1 ? kPartB[term] : 0;
+                        mbar_expect_tx(bar, STAGE_BYTES);
+                        if constexpr (A_M) {
+#pragma unroll
+                            for (int c = 0; c < BM / 64; ++c) tma_load_3d(sa + c * (64 * BK * 2), &map_a, bar, mt * BM + c * 64, kb * BK, pa);
+                        } else {
+                            tma_load_3d(sa, &map_a, bar, kb * BK, mt * BM, pa);
+                        }
+                        if constexpr (B_N) {
+#pragma unroll
+                            for (int c = 0; c < BN / 64; ++c) tma_load_3d(sb + c * (64 * BK * 2), &map_b, bar, nt * BN + c * 64, kb * BK, pb);
+                        } else {
+                            tma_load_3d(sb, &map_b, bar, kb * BK, nt * BN, pb);
+                        }
+                    }
+                }
+            }
+            if (!ok) {
+                // transactions that were already issued land before the shared memory goes away
+                for (int spin = 0; spin < 4096; ++spin) __nanosleep(64);
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer ------
+        if (lane == 0) {
+            // D = F32 (bits 4-5), A and B format (7-9, 10-12: 0 = F16, 1 = BF16), A and B stored with M / N contiguous (15, 16),
+            // N >> 3 (17-22), M >> 4 (24-28)
+            const uint32_t fmt = g.is_bf16 ? 1u : 0u;
+            const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((A_M ? 1u : 0u) << 15) | ((B_N ? 1u : 0u) << 16) |
+                                   (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>(BM >> 4) << 24);
+            uint32_t it = 0, local = 0;
+            bool ok = true;
+            for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x, ++local) {
+                int z, mt, nt, first, blocks;
+                tile_coords(t, m_tiles, g.n_tiles, z, mt, nt);
+                split_range(z, first, blocks);
+                if (blocks <= 0) continue;
+                const int buf = local & 1;
+                if (!mbar_wait(acce0 + 8 * buf, ((local >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t acc = tmem_base + buf * BN;
+                const int steps = blocks * g.terms;
+                for (int i = 0; i < steps; ++i, ++it) {
+                    const int s = it % STAGES;
+                    if (!mbar_wait(full0 + 8 * s, (it / STAGES) & 1, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t sa = base + s * STAGE_BYTES, sb = sa + A_BYTES;
+#pragma unroll
+                    for (int k = 0; k < BK / UMMA_K; ++k) {
+                        // K contiguous: 32 bytes further along the swizzled row; else 16 rows of 128 bytes further, 64-wide boxes 8 KiB apart
+                        const uint64_t da = A_M ? smem_desc(sa + k * UMMA_K * 128, 64 * BK * 2, 1024) : smem_desc(sa + k * UMMA_K * 2, 16, 1024);
+                        const uint64_t db = B_N ? smem_desc(sb + k * UMMA_K * 128, 64 * BK * 2, 1024) : smem_desc(sb + k * UMMA_K * 2, 16, 1024);
+                        umma_f16(acc, da, db, idesc, (i > 0 || k > 0) ? 1u : 0u);
+                    }
+                    umma_commit(empty0 + 8 * s);  // frees the stage once these MMAs have read it
+                }
+                if (ok) umma_commit(accf0 + 8 * buf);
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ epilogue --------
+        const int ew = warp - 2;
+        const int quarter = warp & 3;  // tensor-memory lanes [32 * quarter, 32 * quarter + 32)
+        const int half = ew >> 2;      // this warp takes the chunks half, half + 2, ...
+        BoxStore box = {staging_ptr + ew * kWarpBytes, &map_d, lane, 0};
+        const float scale = EPI == EPI_RESULT ? *g.scale : 1.0f;
+        uint32_t local = 0;
+        bool ok = true;
+        for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x, ++local) {
+            int z, mt, nt, first, blocks;
+            tile_coords(t, m_tiles, g.n_tiles, z, mt, nt);
+            split_range(z, first, blocks);
+            const int buf = local & 1;
+            const int64_t row0 = static_cast<int64_t>(mt) * BM + quarter * 32, row = row0 + lane;
+            const int64_t col0 = static_cast<int64_t>(nt) * BN;
+            const int rows = static_cast<int>(max(int64_t(0), min(int64_t(32), g.M - row0)));
+            const int cols = static_cast<int>(min(int64_t(BN), g.N - col0)), chunks = (cols + 31) >> 5;
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN;
+            const bool empty = blocks <= 0;  // no token counts: the product is zero and nothing was accumulated
+            if (!empty) {
+                if (!mbar_wait(accf0 + 8 * buf, (local >> 1) & 1, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+            }
+            if constexpr (EPI == EPI_STATS) {
+                // where this row's target lies within the piece (anywhere outside when it has none here)
+                int64_t target = -1;
+                if (lane < rows) {
+                    target = g.wide_targets ? static_cast<const int64_t*>(g.targets)[row] : static_cast<const int32_t*>(g.targets)[row];
+                    target -= g.vocab0 + col0;
+                }
+                const int at = target >= 0 && target < cols ? static_cast<int>(target) : -1;
+                float m = -INFINITY, s = 0.0f, hit = 0.0f;
+                if (rows > 0) {  // warp-uniform
+                    drain(taddr, half, chunks, [&](uint32_t (&v)[32], int c) {
+                        online_softmax(v, min(32, cols - c * 32), m, s);
+                        if (at >= c * 32 && at < c * 32 + 32) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (at == c * 32 + j) hit = __uint_as_float(v[j]);
+                        }
+                    });
+                }
+                if (lane < rows) {
+                    g.halves[(g.first_half + 2 * nt + half) * g.M + row] = make_float2(m, s);
+                    if (at >= 0 && ((at >> 5) & 1) == half) g.target_logit[row] = hit;
+                }
+            } else if constexpr (EPI == EPI_D) {
+                RowInfo info = {0.0f, 0.0f, kNoRow, 0};
+                if (lane < rows) info = g.rows[row];
+                const int64_t rel = info.target >= 0 ? info.target - g.vocab0 - col0 : -1;
+                const int at = rel >= 0 && rel < cols ? static_cast<int>(rel) : -1;
+                if (rows > 0) {
+                    drain(taddr, half, chunks, [&](uint32_t (&v)[32], int c) {
+                        float d[32];
+                        if (info.target == kNoRow) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) d[j] = 0.0f;  // whatever the logits are
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) d[j] = __expf(__uint_as_float(v[j]) - info.lse) * info.grad;
+                            if (at >= c * 32 && at < c * 32 + 32) {
+                                // p - 1 without cancellation: the gradient of a token that is almost certain
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (at == c * 32 + j) d[j] = expm1f(__uint_as_float(v[j]) - info.lse) * info.grad;
+                            }
+                        }
+                        uint32_t w[16];
+                        const int x = static_cast<int>(col0) + c * 32, y = static_cast<int>(row0);
+                        if constexpr (PARTS == 1) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) w[j] = pack2<T>(d[2 * j], d[2 * j + 1]);
+                            box.put(w, x, y, 0, false);
+                        } else {
+                            // the first part goes out; what it leaves stays in d for the next
+#pragma unroll
+                            for (int p = 0; p < PARTS; ++p) {
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) {
+                                    float lo, hi, unused0, unused1;
+                                    three_parts(d[2 * j], lo, unused0, unused1);
+                                    three_parts(d[2 * j + 1], hi, unused0, unused1);
+                                    w[j] = pack2<T>(lo, hi);
+                                    d[2 * j] = isfinite(d[2 * j]) ? d[2 * j] - lo : 0.0f;
+                                    d[2 * j + 1] = isfinite(d[2 * j + 1]) ? d[2 * j + 1] - hi : 0.0f;
+                                }
+                                box.put(w, x, y, p, false);
+                            }
+                        }
+                    });
+                }
+            } else if constexpr (EPI == EPI_SUM) {
+                if (rows > 0) {
+                    drain(taddr, half, chunks, [&](uint32_t (&v)[32], int c) {
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            uint32_t w[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) w[j] = v[q * 16 + j];
+                            const int x = static_cast<int>(col0) + c * 32 + q * 16;
+                            if (x < g.N) box.put(w, x, static_cast<int>(row0), z, g.add != 0);
+                        }
+                    });
+                }
+            } else {
+                auto store = [&](uint32_t (&v)[32], int c) {
+                    constexpr bool F32 = std::is_same<OUT, float>::value;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = empty ? 0u : __float_as_uint(__uint_as_float(v[j]) * scale);
+                    if (g.tma_store) {
+#pragma unroll
+                        for (int q = 0; q < (F32 ? 2 : 1); ++q) {
+                            uint32_t w[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                if constexpr (F32) w[j] = v[q * 16 + j];
+                                else w[j] = pack2<OUT>(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                            }
+                            const int x = static_cast<int>(col0) + c * 32 + q * 16;
+                            if (x < g.N) box.put(w, x, static_cast<int>(row0), 0, false);
+                        }
+                    } else {
+                        // any alignment: through shared memory so that a store instruction runs along a row
+                        float* mine = reinterpret_cast<float*>(box.stage);
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            __syncwarp();
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) mine[lane * 17 + j] = __uint_as_float(v[q * 16 + j]);
+                            __syncwarp();
+                            const int64_t col = col0 + c * 32 + q * 16 + (lane & 15);
+                            if (col < g.N)
+                                for (int r = lane >> 4; r < rows; r += 2)
+                                    static_cast<OUT*>(g.d)[(row0 + r) * g.ldd + col] = from_compute<OUT, float>(mine[r * 17 + (lane & 15)]);
+                        }
+                    }
+                };
+                if (rows > 0) {
+                    if (!empty) {
+                        drain(taddr, half, chunks, store);
+                    } else {
+                        uint32_t v[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = 0u;
+                        for (int c = half; c < chunks; c += 2) store(v, c);
+                    }
+                }
+            }
+            // this warp has finished reading the accumulator
+            if (!empty) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acce0 + 8 * buf);
+            }
+        }
+        if (lane == 0) bulk_wait_all();  // shared memory stays valid until the last box has left
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    }
+    if (threadIdx.x == 0 && *abort_flag) atomicAdd(&g_loss_aborts, 1u);
+}
+
+// Joins the halves of a row: 32 rows per block, `halves` of them spread over 32 threads each.
+__global__ void __launch_bounds__(1024) loss_join(const float2* __restrict__ halves, int64_t n_halves, int64_t rows, const float* __restrict__ target_logit,
+                                                  const void* targets, int wide, int64_t ignore, int64_t vocab, float* __restrict__ loss, float* __restrict__ lse) {
+    __shared__ float2 part[32][33];
+    const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+    float m = -INFINITY, s = 0.0f;
+    auto join = [&](float2 p) {
+        const float now = fmaxf(m, p.x), base = now == -INFINITY ? 0.0f : now;
+        s = s * __expf(m - base) + p.y * __expf(p.x - base);
+        m = now;
+    };
+    if (row < rows) {
+#pragma unroll 4
+        for (int64_t i = k; i < n_halves; i += 32) join(halves[i * rows + row]);
+    }
+    part[k][lane] = make_float2(m, s);
+    __syncthreads();
+    // thread (lane, k): part `lane` of row k
+    const float2 mine = part[lane][k];
+    float top = mine.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = mine.y * __expf(mine.x - base);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    const int64_t out = static_cast<int64_t>(blockIdx.x) * 32 + k;
+    if (lane == 0 && out < rows) {
+        const float z = top + logf(sum);
+        const int64_t target = wide ? static_cast<const int64_t*>(targets)[out] : static_cast<const int32_t*>(targets)[out];
+        if (lse) lse[out] = z;
+        if (loss) loss[out] = target == ignore ? 0.0f : target < 0 || target >= vocab ? NAN : z - target_logit[out];
+    }
+}
+
+// The rows of the gradient's products. Token i goes to row slot[i] where it has a target; the others fill the
+// rows behind (slot[i] = -1 - row), as rows of nothing. Every block counts all targets for itself (they lie
+// in L2), so there is no order between blocks to wait for.
+__global__ void __launch_bounds__(256) loss_rows(const void* targets, int wide, int64_t n, const float* __restrict__ grad, const float* __restrict__ lse, int64_t ignore,
+                                                 int64_t vocab, int per_block, RowInfo* __restrict__ info, int* __restrict__ slot, int* __restrict__ count,
+                                                 float* __restrict__ scale) {
+    __shared__ int ints[3][8];
+    __shared__ float tops[8];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int64_t n0 = static_cast<int64_t>(blockIdx.x) * per_block;
+    auto target_of = [&](int64_t i) { return wide ? static_cast<const int64_t*>(targets)[i] : static_cast<int64_t>(static_cast<const int32_t*>(targets)[i]); };
+    int before = 0, all = 0;
+    float top = 0.0f;
+    for (int64_t i = tid; i < n; i += 256) {
+        if (target_of(i) == ignore) continue;
+        ++all;
+        before += i < n0;
+        const float a = fabsf(grad[i]);
+        if (isfinite(a)) top = fmaxf(top, a);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
+        all += __shfl_xor_sync(0xFFFFFFFFu, all, o);
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    }
+    const int64_t mine = n0 + tid;
+    const bool here = tid < per_block && mine < n;
+    const int64_t target = here ? target_of(mine) : 0;
+    const bool counts = here && target != ignore;
+    const unsigned votes = __ballot_sync(0xFFFFFFFFu, counts);
+    if (lane == 0) {
+        ints[0][warp] = before;
+        ints[1][warp] = all;
+        ints[2][warp] = __popc(votes);
+        tops[warp] = top;
+    }
+    __syncthreads();
+    before = all = 0;
+    top = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        before += ints[0][w] + (w < warp ? ints[2][w] : 0);
+        all += ints[1][w];
+        top = fmaxf(top, tops[w]);
+    }
+    before += __popc(votes & ((1u << lane) - 1u));
+    // the power of two that brings the largest upstream gradient below 2^14
+    int exponent = 0;
+    if (top > 0.0f) frexpf(top, &exponent);
+    const int shift = top > 0.0f ? max(-100, min(100, 14 - exponent)) : 0;
+    if (here) {
+        const int row = counts ? before : all + static_cast<int>(mine - before);
+        slot[mine] = counts ? row : -1 - row;
+        RowInfo r = {0.0f, 0.0f, kNoRow, 0};
+        if (counts) {
+            r.lse = lse[mine];
+            const bool inside = target >= 0 && target < vocab;
+            r.grad = inside ? ldexpf(grad[mine], shift) : NAN;  // a target outside the vocabulary has no gradient
+            r.target = inside ? static_cast<int>(target) : -2;
+        }
+        info[row] = r;
+    }
+    if (blockIdx.x == 0 && tid == 0) {
+        *count = all;
+        *scale = ldexpf(1.0f, -shift);
+    }
+}
+
+// Rows of an operand as the products read them: a multiple of 8 elements long (zeros behind the last), 16-byte aligned, in
+// order, or row r at slot[r] (zeros where that is negative: row -1 - slot[r]); float32 as three parts of bfloat16.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_rows(const T* __restrict__ src, int64_t pitch, int64_t rows, int64_t cols, int64_t padded, uint16_t* __restrict__ dst,
+                                                 int64_t part_stride, const int* __restrict__ slot, int vectors) {
+    const int64_t groups = padded / 8, n = rows * groups;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t r = i / groups, c = (i - r * groups) * 8;
+        int64_t to = r;
+        bool zero = false;
+        if (slot) {
+            const int at = slot[r];
+            zero = at < 0;
+            to = zero ? -1 - at : at;
+        }
+        alignas(16) T x[8];
+        if (!zero && vectors && c + 8 <= cols) {
+#pragma unroll
+            for (int q = 0; q < static_cast<int>(sizeof(T)) / 2; ++q) reinterpret_cast<uint4*>(x)[q] = reinterpret_cast<const uint4*>(src + r * pitch + c)[q];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = !zero && c + j < cols ? src[r * pitch + c + j] : T(0);
+        }
+        uint16_t* out = dst + to * padded + c;
+        if constexpr (std::is_same<T, float>::value) {
+            uint32_t w[3][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float lo[3], hi[3];
+                three_parts(x[2 * j], lo[0], lo[1], lo[2]);
+                three_parts(x[2 * j + 1], hi[0], hi[1], hi[2]);
+#pragma unroll
+                for (int p = 0; p < 3; ++p) w[p][j] = pack2<__nv_bfloat16>(lo[p], hi[p]);
+            }
+#pragma unroll
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4*>(out + p * part_stride) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+        } else {
+            *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(x);
+        }
+    }
+}
+
+// dh: the float32 sums of the splits, added in order, scaled back, and put where the tokens stand.
+template <typename T>
+__global__ void __launch_bounds__(256) loss_dhidden(const float* __restrict__ sums, int splits, int64_t rows, int64_t cols, int64_t padded, const int* __restrict__ slot,
+                                                    const float* __restrict__ scale, T* __restrict__ out) {
+    const float by = *scale;
+    const int64_t n = rows * cols;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t r = i / cols, c = i - r * cols;
+        const int at = slot[r];
+        float v = 0.0f;
+        if (at >= 0)
+            for (int z = 0; z < splits; ++z) v += sums[(z * rows + at) * padded + c];
+        out[i] = from_compute<T, float>(at >= 0 ? v * by : 0.0f);
+    }
+}
+
+// ------------------------------------------------------------------ host ---------------
+// Memory of one call, all of it released together.
+struct Scratch {
+    cudaStream_t stream;
+    void* held[16];
+    int n = 0;
+    explicit Scratch(cudaStream_t s) : stream(s) {}
+    template <typename P>
+    tn_status take(P** out, size_t bytes) {
+        if (n == 16) return fail(TN_ERROR, "linear_cross_entropy: too many workspaces");
+        void* p = nullptr;
+        TN_TRY(scratch_alloc(&p, bytes, stream));
+        held[n++] = p;
+        *out = static_cast<P*>(p);
+        return TN_SUCCESS;
+    }
+    tn_status release(tn_status st) {
+        while (n > 0) {
+            const tn_status freed = scratch_free(held[--n], stream);
+            if (st == TN_SUCCESS) st = freed;
+        }
+        return st;
+    }
+};
+
+bool is_dense(const tn_tensor_t* t) {
+    int64_t expect = 1;
+    for (int d = t->rank - 1; d >= 0; --d) {
+        if (t->shape.sizes[d] != 1 && t->strides.sizes[d] != expect) return false;
+        expect *= (int64_t)t->shape.sizes[d];
+    }
+    return true;
+}
+
+// Address of a dense tensor with t's elements: t itself or a copy.
+tn_status densely(const tn_tensor_t* t, const void** out, Scratch& mem, tn_stream_t stream) {
+    *out = t->address;
+    if (is_dense(t)) return TN_SUCCESS;
+    tn_tensor_t copy = *t;
+    int64_t run = 1;
+    for (int d = t->rank - 1; d >= 0; --d) {
+        copy.strides.sizes[d] = run;
+        run *= (int64_t)t->shape.sizes[d];
+    }
+    copy.layout = TN_CONTIGUOUS;
+    TN_TRY(mem.take(&copy.address, t->size * (size_t)dtype_bytes(t->dtype)));
+    *out = copy.address;
+    return tn_cpy(t, &copy, stream);
+}
+
+// A matrix of rows, read in place where its last axis is contiguous and its rows are one pitch apart.
+struct RowsIn {
+    const void* base;
+    int64_t pitch;
+};
+tn_status rows_in(const tn_tensor_t* t, RowsIn* out, Scratch& mem, tn_stream_t stream) {
+    const int last = t->rank - 1;
+    const int64_t cols = (int64_t)t->shape.sizes[last];
+    out->pitch = cols;
+    bool one = cols == 1 || t->strides.sizes[last] == 1, any = false;
+    int64_t expect = 0;
+    for (int d = last - 1; one && d >= 0; --d) {
+        if (t->shape.sizes[d] == 1) continue;
+        if (!any) out->pitch = t->strides.sizes[d];
+        else one = t->strides.sizes[d] == expect;
+        any = true;
+        expect = t->strides.sizes[d] * (int64_t)t->shape.sizes[d];
+    }
+    out->base = t->address;
+    if (one) return TN_SUCCESS;
+    out->pitch = cols;
+    return densely(t, &out->base, mem, stream);
+}
+
+// An operand in the form the tensor maps address.
+struct Operand {
+    const void* ptr = nullptr;
+    int64_t pitch = 0, part_stride = 0;
+    int parts = 1;
+};
+
+struct Problem {
+    int dtype;
+    bool bf16;
+    int parts, terms;
+    int64_t tokens, hidden, vocab, padded;
+    cudaStream_t stream;
+};
+
+bool in_place(const Problem& p, const RowsIn& r, int64_t rows) {
+    return p.parts == 1 && mult8(r.pitch) && r.pitch >= p.hidden && aligned16(r.base) && rows > 0;
+}
+
+// Writes `rows` rows into `to` (room for parts * rows * padded elements).
+tn_status pack(const Problem& p, const RowsIn& r, int64_t first, int64_t rows, uint16_t* to, const int* slot) {
+    const int64_t size = p.parts == 1 ? 2 : 4;
+    const uint8_t* src = static_cast<const uint8_t*>(r.base) + first * r.pitch * size;
+    const int vectors = aligned16(src) && (r.pitch * size) % 16 == 0;
+    const int64_t work = rows * (p.padded / 8);
+    const int grid = (int)std::min<int64_t>(ceil_div(work, 256), (int64_t)sm_count() * 16);
+    if (p.parts == 1)
+        pack_rows<uint16_t><<<grid, 256, 0, p.stream>>>(reinterpret_cast<const uint16_t*>(src), r.pitch, rows, p.hidden, p.padded, to, 0, slot, vectors);
+    else
+        pack_rows<float><<<grid, 256, 0, p.stream>>>(reinterpret_cast<const float*>(src), r.pitch, rows, p.hidden, p.padded, to, rows * p.padded, slot, vectors);
+    return after_launch("pack_rows");
+}
+
+// The weights' rows [first, first + rows): in place, or packed into `room`.
+tn_status weight_piece(const Problem& p, const RowsIn& w, int64_t first, int64_t rows, uint16_t* room, Operand* out) {
+    out->parts = p.parts;
+    if (!room) {
+        out->ptr = static_cast<const uint16_t*>(w.base) + first * w.pitch;
+        out->pitch = w.pitch;
+        return TN_SUCCESS;
+    }
+    out->ptr = room;
+    out->pitch = p.padded;
+    out->part_stride = rows * p.padded;
+    return pack(p, w, first, rows, room, nullptr);
+}
+
+// Tensor map over an operand: (inner, rows, part).
+tn_status operand_map(CUtensorMap* map, const Operand& o, bool bf16, int64_t inner, int64_t rows, int box_inner, int box_rows) {
+    return make_map(map, o.ptr, bf16, inner, rows, o.parts, o.pitch, o.part_stride, box_inner, box_rows);
+}
+
+template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS>
+tn_status launch_one(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d, const LossArgs& g, cudaStream_t stream) {
+    static thread_local int attr_device = -1;  // the opt-in shared-memory size belongs to kernel and device
+    int dev = 0;
+    TN_CUDA(cudaGetDevice(&dev));
+    if (attr_device != dev) {
+        TN_CUDA(cudaFuncSetAttribute(loss_gemm<A_M, B_N, EPI, T, OUT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+        attr_device = dev;
+    }
+    const int64_t total = (int64_t)g.m_tiles * g.n_tiles * g.splits;
+    if (total >= (int64_t(1) << 31)) return fail(TN_ERROR, "linear_cross_entropy: %lld tiles are too many", (long long)total);
+    const int64_t sms = sm_count() - sm_margin();
+    loss_gemm<A_M, B_N, EPI, T, OUT, PARTS><<<(unsigned)std::min(total, sms), kThreads, kSmemBytes, stream>>>(a, b, d, g);
+    return after_launch("loss_gemm");
+}
+
+LossArgs gemm_args(const Problem& p, int64_t m, int64_t n, int64_t k) {
+    LossArgs g = {};
+    g.M = m;
+    g.N = n;
+    g.m_tiles = (int)ceil_div(m, BM);
+    g.n_tiles = (int)ceil_div(n, BN);
+    g.k_blocks = (int)ceil_div(k, BK);
+    g.splits = 1;
+    g.split_blocks = g.k_blocks;
+    g.terms = p.terms;
+    g.is_bf16 = p.bf16;
+    return g;
+}
+
+// Vocabulary entries per piece: `bytes_each` is the workspace that one of them takes.
+// Half a GiB is 4 ms of products at the least; below 4096 entries the traffic of dh's float32 sums would show.
+int64_t piece_entries(int64_t vocab, int64_t bytes_each) {
+    if (bytes_each <= 0) return vocab;
+    const int64_t fits = ((int64_t(512) << 20) / bytes_each) & ~int64_t(255);
+    return std::min(vocab, std::max<int64_t>(fits, 4096));
+}
+
+tn_status check_problem(const char* op, const tn_tensor_t* hidden, const tn_tensor_t* weight, const tn_tensor_t* targets) {
+    if (!hidden || !weight || !targets) return fail(TN_ERROR, "%s: null tensor", op);
+    if (hidden->rank < 1) return fail(TN_ERROR, "%s: the hidden states need a last axis", op);
+    if (!is_half(hidden->dtype) && hidden->dtype != TN_FLOAT32) return fail(TN_UNSUPPORTED_DTYPE, "%s: dtype %d unsupported (float16, bfloat16, float32)", op, (int)hidden->dtype);
+    if (weight->dtype != hidden->dtype) return fail(TN_UNSUPPORTED_DTYPE, "%s: hidden states of dtype %d and weights of dtype %d", op, (int)hidden->dtype, (int)weight->dtype);
+    if (targets->dtype != TN_INT32 && targets->dtype != TN_INT64) return fail(TN_UNSUPPORTED_DTYPE, "%s: targets of dtype %d, expected int32 or int64", op, (int)targets->dtype);
+    for (const tn_tensor_t* t : {hidden, weight, targets})
+        if (t->environment.kind != TN_DEVICE || hidden->environment.kind != TN_DEVICE || t->environment.resource.device.id != hidden->environment.resource.device.id)
+            return fail(TN_INCOMPATIBLE_DEVICES, "%s: operands must live on one device (no CPU fallback)", op);
+    if (weight->rank != 2) return fail(TN_ERROR, "%s: the weights must be a matrix [vocabulary, hidden]", op);
+    const size_t h = hidden->shape.sizes[hidden->rank - 1];
+    if (weight->shape.sizes[1] != h) return fail(TN_ERROR, "%s: hidden states of %zu and weights of %zu columns", op, h, (size_t)weight->shape.sizes[1]);
+    if (h == 0 || weight->shape.sizes[0] == 0) return fail(TN_ERROR, "%s: an empty hidden axis or vocabulary", op);
+    const size_t limit = (size_t(1) << 31) - 512;
+    if (h > limit || weight->shape.sizes[0] > limit || hidden->size / h > limit) return fail(TN_ERROR, "%s: an extent of 2^31 or more", op);
+    bool same = targets->rank == hidden->rank - 1;
+    for (int d = 0; same && d < targets->rank; ++d) same = targets->shape.sizes[d] == hidden->shape.sizes[d];
+    if (!same) return fail(TN_ERROR, "%s: the targets must have the hidden states' leading shape", op);
+    return TN_SUCCESS;
+}
+tn_status check_tokens(const char* op, const tn_tensor_t* targets, const tn_tensor_t* t, bool result, const char* what) {
+    if (t->dtype != TN_FLOAT32) return fail(TN_UNSUPPORTED_DTYPE, "%s: %s has dtype %d, expected float32", op, what, (int)t->dtype);
+    bool same = t->rank == targets->rank;
+    for (int d = 0; same && d < t->rank; ++d) same = t->shape.sizes[d] == targets->shape.sizes[d];
+    if (!same) return fail(TN_ERROR, "%s: %s must have the targets' shape", op, what);
+    if (result && !is_dense(t)) return fail(TN_ERROR, "%s: %s must be dense", op, what);
+    if (t->environment.kind != TN_DEVICE || t->environment.resource.device.id != targets->environment.resource.device.id)
+        return fail(TN_INCOMPATIBLE_DEVICES, "%s: operands must live on one device", op);
+    return TN_SUCCESS;
+}
+tn_status check_result(const char* op, const tn_tensor_t* like, const tn_tensor_t* t, const char* what) {
+    if (t->dtype != like->dtype) return fail(TN_UNSUPPORTED_DTYPE, "%s: %s has dtype %d, expected %d", op, what, (int)t->dtype, (int)like->dtype);
+    bool same = t->rank == like->rank;
+    for (int d = 0; same && d < t->rank; ++d) same = t->shape.sizes[d] == like->shape.sizes[d];
+    if (!same) return fail(TN_ERROR, "%s: %s has the wrong shape", op, what);
+    if (!is_dense(t)) return fail(TN_ERROR, "%s: %s must be dense", op, what);
+    if (t->environment.kind != TN_DEVICE || t->environment.resource.device.id != like->environment.resource.device.id)
+        return fail(TN_INCOMPATIBLE_DEVICES, "%s: operands must live on one device", op);
+    return TN_SUCCESS;
+}
+
+Problem make_problem(const tn_tensor_t* hidden, const tn_tensor_t* weight, tn_stream_t stream) {
+    Problem p;
+    p.dtype = hidden->dtype;
+    p.bf16 = hidden->dtype != TN_FLOAT16;
+    p.parts = hidden->dtype == TN_FLOAT32 ? 3 : 1;
+    p.terms = p.parts == 3 ? 6 : 1;
+    p.hidden = (int64_t)hidden->shape.sizes[hidden->rank - 1];
+    p.tokens = (int64_t)hidden->size / p.hidden;
+    p.vocab = (int64_t)weight->shape.sizes[0];
+    p.padded = (p.hidden + 7) & ~int64_t(7);
+    p.stream = as_cuda(stream);
+    return p;
+}
+
+tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const tn_tensor_t* targets, tn_tensor_t* loss, tn_tensor_t* lse, tn_stream_t stream,
+                   int64_t ignore, Scratch& mem) {
+    const Problem p = make_problem(hidden, weight, stream);
+    RowsIn h, w;
+    const void* t = nullptr;
+    TN_TRY(rows_in(hidden, &h, mem, stream));
+    TN_TRY(rows_in(weight, &w, mem, stream));
+    TN_TRY(densely(targets, &t, mem, stream));
+    Operand a;
+    a.parts = p.parts;
+    if (in_place(p, h, p.tokens)) {
+        a.ptr = h.base;
+        a.pitch = h.pitch;
+    } else {
+        uint16_t* room = nullptr;
+        TN_TRY(mem.take(&room, (size_t)p.parts * p.tokens * p.padded * 2));
+        TN_TRY(pack(p, h, 0, p.tokens, room, nullptr));
+        a.ptr = room;
+        a.pitch = p.padded;
+        a.part_stride = p.tokens * p.padded;
+    }
+    const bool packed = !in_place(p, w, p.vocab);
+    const int64_t piece = piece_entries(p.vocab, packed ? p.padded * 2 * p.parts : 0);
+    uint16_t* room = nullptr;
+    if (packed) TN_TRY(mem.take(&room, (size_t)p.parts * piece * p.padded * 2));
+    int64_t tiles = 0;
+    for (int64_t v0 = 0; v0 < p.vocab; v0 += piece) tiles += ceil_div(std::min(piece, p.vocab - v0), BN);
+    float2* halves = nullptr;
+    float* target_logit = nullptr;
+    TN_TRY(mem.take(&halves, sizeof(float2) * 2 * (size_t)tiles * p.tokens));
+    TN_TRY(mem.take(&target_logit, sizeof(float) * p.tokens));
+    CUtensorMap map_a, map_b;
+    TN_TRY(operand_map(&map_a, a, p.bf16, p.hidden, p.tokens, BK, BM));
+    int64_t first_half = 0;
+    for (int64_t v0 = 0; v0 < p.vocab; v0 += piece) {
+        const int64_t n = std::min(piece, p.vocab - v0);
+        Operand b;
+        TN_TRY(weight_piece(p, w, v0, n, room, &b));
+        TN_TRY(operand_map(&map_b, b, p.bf16, p.hidden, n, BK, BN));
+        LossArgs g = gemm_args(p, p.tokens, n, p.hidden);
+        g.vocab0 = v0;
+        g.targets = t;
+        g.wide_targets = targets->dtype == TN_INT64;
+        g.halves = halves;
+        g.first_half = first_half;
+        g.target_logit = target_logit;
+        TN_TRY((launch_one<false, false, EPI_STATS, __half, float, 1>(map_a, map_b, map_a, g, p.stream)));
+        first_half += 2 * (int64_t)g.n_tiles;
+    }
+    loss_join<<<(unsigned)ceil_div(p.tokens, 32), 1024, 0, p.stream>>>(halves, first_half, p.tokens, target_logit, t, targets->dtype == TN_INT64, ignore, p.vocab,
+                                                                      loss ? static_cast<float*>(loss->address) : nullptr, lse ? static_cast<float*>(lse->address) : nullptr);
+    return after_launch("loss_join");
+}
+
+template <typename T, typename OUT, int PARTS>
+tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_tensor_t* weight, const tn_tensor_t* targets, const tn_tensor_t* lse, tn_tensor_t* dhidden,
+                   tn_tensor_t* dweight, tn_stream_t stream, int64_t ignore, Scratch& mem) {
+    const Problem p = make_problem(hidden, weight, stream);
+    RowsIn h, w;
+    const void *t = nullptr, *up = nullptr, *z = nullptr;
+    TN_TRY(rows_in(hidden, &h, mem, stream));
+    TN_TRY(rows_in(weight, &w, mem, stream));
+    TN_TRY(densely(targets, &t, mem, stream));
+    TN_TRY(densely(grad, &up, mem, stream));
+    TN_TRY(densely(lse, &z, mem, stream));
+    RowInfo* info = nullptr;
+    int *slot = nullptr, *count = nullptr;
+    TN_TRY(mem.take(&info, sizeof(RowInfo) * p.tokens));
+    TN_TRY(mem.take(&slot, sizeof(int) * p.tokens));
+    TN_TRY(mem.take(&count, 2 * sizeof(int)));
+    float* scale = reinterpret_cast<float*>(count + 1);
+    const int per_block = (int)std::min<int64_t>(256, std::max<int64_t>(8, ceil_div(p.tokens, 1024)));
+    loss_rows<<<(unsigned)ceil_div(p.tokens, per_block), 256, 0, p.stream>>>(t, targets->dtype == TN_INT64, p.tokens, static_cast<const float*>(up), static_cast<const float*>(z),
+                                                                            ignore, p.vocab, per_block, info, slot, count, scale);
+    TN_TRY(after_launch("loss_rows"));
+    uint16_t* gathered = nullptr;
+    TN_TRY(mem.take(&gathered, (size_t)p.parts * p.tokens * p.padded * 2));
+    TN_TRY(pack(p, h, 0, p.tokens, gathered, slot));
+    Operand a;
+    a.ptr = gathered;
+    a.pitch = p.padded;
+    a.part_stride = p.tokens * p.padded;
+    a.parts = p.parts;
+
+    const bool packed = !in_place(p, w, p.vocab);
+    const int64_t piece = piece_entries(p.vocab, (p.tokens + (packed ? p.padded : 0)) * 2 * p.parts);
+    uint16_t *room = nullptr, *d = nullptr;
+    if (packed) TN_TRY(mem.take(&room, (size_t)p.parts * piece * p.padded * 2));
+    const int64_t d_pitch = (piece + 7) & ~int64_t(7);
+    TN_TRY(mem.take(&d, (size_t)p.parts * p.tokens * d_pitch * 2));
+    Operand dd;
+    dd.ptr = d;
+    dd.pitch = d_pitch;
+    dd.part_stride = p.tokens * d_pitch;
+    dd.parts = p.parts;
+
+    // dh has few tiles when there are few tokens: K (the vocabulary) is split until every SM has a tile, each
+    // split with at least four blocks, and the splits' sums are added in order afterwards
+    float* sums = nullptr;
+    int splits = 1;
+    const int64_t sms = sm_count() - sm_margin();
+    if (dhidden) {
+        const int64_t tiles = ceil_div(p.tokens, BM) * ceil_div(p.hidden, BN);
+        splits = (int)std::max<int64_t>(1, std::min(sms / tiles, ceil_div(piece, BK) / 4));
+        TN_TRY(mem.take(&sums, sizeof(float) * (size_t)splits * p.tokens * p.padded));
+    }
+
+    CUtensorMap rows_a, rows_b, map;
+    TN_TRY(operand_map(&rows_a, a, p.bf16, p.hidden, p.tokens, BK, BM));   // h as [tokens, hidden], K = hidden
+    TN_TRY(operand_map(&rows_b, a, p.bf16, p.hidden, p.tokens, 64, BK));   // h as B of dW, K = tokens
+    for (int64_t v0 = 0; v0 < p.vocab; v0 += piece) {
+        const int64_t n = std::min(piece, p.vocab - v0);
+        Operand b;
+        TN_TRY(weight_piece(p, w, v0, n, room, &b));
+        {   // d of this piece
+            CUtensorMap map_d;
+            TN_TRY(operand_map(&map, b, p.bf16, p.hidden, n, BK, BN));
+            const cuuint64_t dims[3] = {(cuuint64_t)n, (cuuint64_t)p.tokens, (cuuint64_t)p.parts};
+            const cuuint64_t strides[2] = {(cuuint64_t)d_pitch * 2, (cuuint64_t)dd.part_stride * 2};
+            const cuuint32_t box[3] = {32, 32, 1};
+            TN_TRY(encode_as(&map_d, d, p.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_SWIZZLE_64B, 3, dims, strides, box));
+            LossArgs g = gemm_args(p, p.tokens, n, p.hidden);
+            g.vocab0 = v0;
+            g.count = count;
+            g.count_is = COUNT_ROWS;
+            g.rows = info;
+            TN_TRY((launch_one<false, false, EPI_D, T, float, PARTS>(rows_a, map, map_d, g, p.stream)));
+        }
+        if (dhidden) {
+            CUtensorMap map_d, map_w;
+            TN_TRY(operand_map(&map, dd, p.bf16, n, p.tokens, BK, BM));
+            TN_TRY(operand_map(&map_w, b, p.bf16, p.hidden, n, 64, BK));
+            TN_TRY(make_result_map(&map_d, sums, true, false, p.padded, p.tokens, splits, p.padded, p.tokens * p.padded));
+            LossArgs g = gemm_args(p, p.tokens, p.padded, n);
+            g.count = count;
+            g.count_is = COUNT_ROWS;
+            // the last piece may be shorter: every split that has been written keeps at least one block or none
+            g.split_blocks = (int)ceil_div(g.k_blocks, splits);
+            g.splits = (int)ceil_div(g.k_blocks, g.split_blocks);
+            g.add = v0 > 0;
+            if (v0 == 0) splits = g.splits;
+            TN_TRY((launch_one<false, true, EPI_SUM, T, float, 1>(map, map_w, map_d, g, p.stream)));
+        }
+        if (dweight) {
+            CUtensorMap map_d;
+            TN_TRY(operand_map(&map, dd, p.bf16, n, p.tokens, 64, BK));
+            OUT* to = static_cast<OUT*>(dweight->address) + v0 * p.hidden;
+            LossArgs g = gemm_args(p, n, p.hidden, p.tokens);
+            g.count = count;
+            g.count_is = COUNT_K;
+            g.scale = scale;
+            g.d = to;
+            g.ldd = p.hidden;
+            constexpr bool F32 = std::is_same<OUT, float>::value;
+            g.tma_store = can_tma_store(to, p.hidden, p.hidden * 8, BN, F32);
+            map_d = map;  // placeholder when the result does not leave through TMA
+            if (g.tma_store) TN_TRY(make_result_map(&map_d, to, F32, p.bf16, p.hidden, n, 1, p.hidden, 0));
+            TN_TRY((launch_one<true, true, EPI_RESULT, T, OUT, 1>(map, rows_b, map_d, g, p.stream)));
+        }
+    }
+    if (dhidden) {
+        const int grid = (int)std::min<int64_t>(ceil_div(p.tokens * p.hidden, 256), sms * 16);
+        loss_dhidden<OUT><<<grid, 256, 0, p.stream>>>(sums, splits, p.tokens, p.hidden, p.padded, slot, scale, static_cast<OUT*>(dhidden->address));
+        TN_TRY(after_launch("loss_dhidden"));
+    }
+    return TN_SUCCESS;
+}
+
+}  // namespace
+}  // namespace tnb
+
+using namespace tnb;
+
+extern "C" {
+
+tn_status tn_linear_cross_entropy(const tn_tensor_t* hidden, const tn_tensor_t* weight, const tn_tensor_t* targets, tn_tensor_t* loss, tn_tensor_t* lse,
+                                  tn_stream_t stream, int64_t ignore_index) {
+    const char* op = "linear_cross_entropy";
+    TN_TRY(check_problem(op, hidden, weight, targets));
+    if (!loss && !lse) return fail(TN_ERROR, "linear_cross_entropy: no output requested");
+    if (loss) TN_TRY(check_tokens(op, targets, loss, true, "the loss"));
+    if (lse) TN_TRY(check_tokens(op, targets, lse, true, "lse"));
+    TN_TRY(use_device_of(hidden));
+    if (hidden->size == 0) return TN_SUCCESS;
+    Scratch mem(as_cuda(stream));
+    return mem.release(run_loss(hidden, weight, targets, loss, lse, stream, ignore_index, mem));
+}
+
+tn_status tn_linear_cross_entropy_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_tensor_t* weight, const tn_tensor_t* targets, const tn_tensor_t* lse,
+                                       tn_tensor_t* dhidden, tn_tensor_t* dweight, tn_stream_t stream, int64_t ignore_index) {
+    const char* op = "linear_cross_entropy_grad";
+    TN_TRY(check_problem(op, hidden, weight, targets));
+    if (!grad || !lse) return fail(TN_ERROR, "%s: null tensor", op);
+    TN_TRY(check_tokens(op, targets, grad, false, "the loss's gradient"));
+    TN_TRY(check_tokens(op, targets, lse, false, "lse"));
+    if (!dhidden && !dweight) return fail(TN_ERROR, "%s: no output requested", op);
+    if (dhidden) TN_TRY(check_result(op, hidden, dhidden, "the hidden states' gradient"));
+    if (dweight) TN_TRY(check_result(op, weight, dweight, "the weights' gradient"));
+    TN_TRY(use_device_of(hidden));
+    if (hidden->size == 0) {  // no tokens: the sum over them is zero
+        if (dweight) TN_CUDA(cudaMemsetAsync(dweight->address, 0, dweight->size * (size_t)dtype_bytes(dweight->dtype), as_cuda(stream)));
+        return TN_SUCCESS;
+    }
+    Scratch mem(as_cuda(stream));
+    tn_status st;
+    switch (hidden->dtype) {
+        case TN_FLOAT16: st = run_grad<__half, __half, 1>(grad, hidden, weight, targets, lse, dhidden, dweight, stream, ignore_index, mem); break;
+        case TN_BFLOAT16: st = run_grad<__nv_bfloat16, __nv_bfloat16, 1>(grad, hidden, weight, targets, lse, dhidden, dweight, stream, ignore_index, mem); break;
+        default: st = run_grad<__nv_bfloat16, float, 3>(grad, hidden, weight, targets, lse, dhidden, dweight, stream, ignore_index, mem); break;
+    }
+    return mem.release(st);
+}
+
+}  // extern "C"

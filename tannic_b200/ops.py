@@ -500,6 +500,27 @@ def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd:
     return dx, dweight, dbias
 
 
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100):
+    """(loss, lse): the softmax cross entropy of the logits hidden . weight^T with `targets`, one float32 per token, and
+    the logits' log-sum-exp, which `linear_cross_entropy_grad` reads (tn_linear_cross_entropy). The logits are not
+    written. Tokens whose target is `ignore_index` have loss 0."""
+    loss, lse = (torch.empty(targets.shape, dtype=torch.float32, device=hidden.device) for _ in range(2))
+    A.check(A.lib().tn_linear_cross_entropy(_ref(hidden), _ref(weight), _ref(targets), _ref(loss), _ref(lse), current_stream(hidden), ignore_index))
+    return loss, lse
+
+
+def linear_cross_entropy_grad(grad: torch.Tensor, hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor,
+                              ignore_index: int = -100, dhidden: bool = True, dweight: bool = True):
+    """(dhidden, dweight) of `linear_cross_entropy` from `grad`, the gradient of every token's loss (for the mean over the
+    tokens that count: 1 / their number, expanded), and its lse (tn_linear_cross_entropy_grad). `dhidden=False` or
+    `dweight=False` leaves that one out (None): a frozen trunk, a frozen head."""
+    dh = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if dhidden else None
+    dw = torch.empty(weight.shape, dtype=weight.dtype, device=hidden.device) if dweight else None
+    A.check(A.lib().tn_linear_cross_entropy_grad(_ref(grad), _ref(hidden), _ref(weight), _ref(targets), _ref(lse), _ref(dh), _ref(dw),
+                                                 current_stream(hidden), ignore_index))
+    return dh, dw
+
+
 def allclose(a: torch.Tensor, b: torch.Tensor, rtol: float = 1e-5, atol: float = 1e-8) -> bool:
     """include/tannic/comparisons.hpp:128 defaults."""
     da, db = desc(a), desc(b)
