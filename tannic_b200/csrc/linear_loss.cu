@@ -23,13 +23,20 @@
 // products of parts that matter; a 64-wide block of K is six passes over those parts. bfloat16 and float16 are one part.
 //
 // d is rounded to the operands' 16-bit type because the tensor cores take operands of one type. It is
-// scaled by a power of two first, so that the largest upstream gradient lands at 2^14: float16 would lose the small
-// probabilities otherwise (grad = 1/N and p = 1/V are below its smallest number). The results are
-// scaled back, exactly, in float32.
+// divided by the largest upstream gradient and multiplied by 2^14 first: float16 would lose the small
+// probabilities otherwise (grad = 1/N and p = 1/V are below its smallest number), and where all tokens weigh the same, the usual
+// mean, their weight is not rounded at all (1/N rounded to bfloat16 would be off by up to 2^-9 in every term
+// alike). The results are multiplied back in float32.
 //
-// Kernel layout as in gemm_tc.cu: warp 0 TMA producer, warp 1 MMA issuer, warps 2..9 epilogue, persistent
+// Kernel layout: warp 0 TMA producer, warp 1 MMA issuer, warp 2 tensor memory, warps 4..11 epilogue, persistent
 // thread blocks of a 128 x 256 tile, 64-wide K blocks in four stages, two accumulators so that the
 // epilogue of a tile runs under the products of the next. Bounded waits throughout.
+//
+// The tensor cores cut off, rather than round, what falls below an accumulator's last place: a sum of K / 16 steps is low by up to
+// K / 16 half units, always towards zero (loss of 8192-wide float32 rows: 2e-6 relative, against 2e-7 of a float32
+// sum). Where the result is float32 or the sum is long (PROMOTE) an accumulator takes only `period` blocks and the epilogue warps
+// add it, in float32, to sums in their registers (128 a thread); its double hides that under the next blocks' products.
+// The register split that takes is 40 a thread for warps 0..3 and 232 for the others, of 384 x 168 at launch.
 #include <algorithm>
 
 #include "tc_common.cuh"
@@ -46,8 +53,8 @@ tn_status loss_abort_count(unsigned int* count) {
 namespace {
 
 constexpr int STAGES = 4;
-constexpr int kEpilogueWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpilogueWarps;
+constexpr int kEpilogueWarps = 8;                          // warps 4..11
+constexpr int kThreads = 128 + 32 * kEpilogueWarps;
 constexpr uint32_t kBoxBytes = 2048;                       // 32 rows x 64 bytes
 constexpr uint32_t kWarpBytes = 2 * kBoxBytes;             // two boxes per warp, or 32 rows x 80 bytes
 constexpr uint32_t kSmemBytes = 1024 + STAGES * STAGE_BYTES + kEpilogueWarps * kWarpBytes + 256;
@@ -56,11 +63,14 @@ static_assert(kSmemBytes <= 232448, "exceeds the shared memory of an SM");
 // A row of the gradient's products: a token with a target, or (target kNoRow) nothing.
 struct alignas(16) RowInfo {
     float lse;
-    float grad;   // upstream gradient times the scale of d
+    float grad;   // upstream gradient over the largest, times 2^14
     int target;
     int unused;
 };
 constexpr int kNoRow = -1;
+constexpr int kPeriod = 16;       // 64-wide blocks an accumulator takes before it is added up in registers
+constexpr float kTop = 16384.0f;  // where the largest |grad| lands in d: float16 ends at 65504
+__device__ __forceinline__ float unscale(float v, float largest) { return v * (1.0f / kTop) * largest; }
 
 // Passes over the parts of a float32 operand pair, largest product first.
 __constant__ int kPartA[6] = {0, 0, 1, 0, 1, 2};
@@ -77,6 +87,7 @@ struct LossArgs {
     int k_blocks;            // 64-wide blocks of K, all splits together
     int splits, split_blocks;
     int terms;               // 1, or 6 for float32 operands
+    int period;              // PROMOTE: passes over a 64-wide block that one accumulator takes
     int is_bf16;
     const int* count;        // tokens with a target
     int count_is;
@@ -200,7 +211,7 @@ __device__ __forceinline__ void online_softmax(const uint32_t (&v)[32], int ncol
 
 // A_M: A is stored [K, M] (M contiguous), else [M, K]. B_N: B is stored [K, N], else [N, K]. T: operand type (bfloat16 parts
 // for float32). OUT: result type of EPI_RESULT. PARTS: parts of d that EPI_D writes.
-template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS>
+template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS, bool PROMOTE>
 __global__ void __launch_bounds__(kThreads, 1)
 loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_d, const LossArgs g) {
     extern __shared__ uint8_t smem_raw[];
@@ -251,103 +262,157 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
-    if (warp == 0) {
-        // ------------------------------------------------------------ TMA producer ----
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool ok = true;
-            for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
-                int z, mt, nt, first, blocks;
-                tile_coords(t, m_tiles, g.n_tiles, z, mt, nt);
-                split_range(z, first, blocks);
-                for (int kb = first; ok && kb < first + blocks; ++kb) {
-                    for (int term = 0; term < g.terms; ++term, ++it) {
-                        const int s = it % STAGES;
-                        if (!mbar_wait(empty0 + 8 * s, ((it / STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
-                        const uint32_t sa = base + s * STAGE_BYTES, sb = sa + A_BYTES, bar = full0 + 8 * s;
-                        const int pa = g.terms > 1 ? kPartA[term] : 0, pb = g.terms > 1 ? kPartB[term] : 0;
-                        mbar_expect_tx(bar, STAGE_BYTES);
-                        if constexpr (A_M) {
+    // all four warps of a group take part, so this comes before the roles
+    if (warp < 4) {
+        if constexpr (PROMOTE) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 0) {
+            // ------------------------------------------------------------ TMA producer ----
+            if (lane == 0) {
+                uint32_t it = 0;
+                bool ok = true;
+                for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
+                    int z, mt, nt, first, blocks;
+                    tile_coords(t, m_tiles, g.n_tiles, z, mt, nt);
+                    split_range(z, first, blocks);
+                    for (int kb = first; ok && kb < first + blocks; ++kb) {
+                        for (int term = 0; term < g.terms; ++term, ++it) {
+                            const int s = it % STAGES;
+                            if (!mbar_wait(empty0 + 8 * s, ((it / STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                            const uint32_t sa = base + s * STAGE_BYTES, sb = sa + A_BYTES, bar = full0 + 8 * s;
+                            const int pa = g.terms > 1 ? kPartA[term] : 0, pb = g.terms > 1 ? kPartB[term] : 0;
+                            mbar_expect_tx(bar, STAGE_BYTES);
+                            if constexpr (A_M) {
 #pragma unroll
-                            for (int c = 0; c < BM / 64; ++c) tma_load_3d(sa + c * (64 * BK * 2), &map_a, bar, mt * BM + c * 64, kb * BK, pa);
-                        } else {
-                            tma_load_3d(sa, &map_a, bar, kb * BK, mt * BM, pa);
-                        }
-                        if constexpr (B_N) {
+                                for (int c = 0; c < BM / 64; ++c) tma_load_3d(sa + c * (64 * BK * 2), &map_a, bar, mt * BM + c * 64, kb * BK, pa);
+                            } else {
+                                tma_load_3d(sa, &map_a, bar, kb * BK, mt * BM, pa);
+                            }
+                            if constexpr (B_N) {
 #pragma unroll
-                            for (int c = 0; c < BN / 64; ++c) tma_load_3d(sb + c * (64 * BK * 2), &map_b, bar, nt * BN + c * 64, kb * BK, pb);
-                        } else {
-                            tma_load_3d(sb, &map_b, bar, kb * BK, nt * BN, pb);
+                                for (int c = 0; c < BN / 64; ++c) tma_load_3d(sb + c * (64 * BK * 2), &map_b, bar, nt * BN + c * 64, kb * BK, pb);
+                            } else {
+                                tma_load_3d(sb, &map_b, bar, kb * BK, nt * BN, pb);
+                            }
                         }
                     }
                 }
-            }
-            if (!ok) {
-                // transactions that were already issued land before the shared memory goes away
-                for (int spin = 0; spin < 4096; ++spin) __nanosleep(64);
-            }
-        }
-    } else if (warp == 1) {
-        // ------------------------------------------------------------ MMA issuer ------
-        if (lane == 0) {
-            // D = F32 (bits 4-5), A and B format (7-9, 10-12: 0 = F16, 1 = BF16), A and B stored with M / N contiguous (15, 16),
-            // N >> 3 (17-22), M >> 4 (24-28)
-            const uint32_t fmt = g.is_bf16 ? 1u : 0u;
-            const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((A_M ? 1u : 0u) << 15) | ((B_N ? 1u : 0u) << 16) |
-                                   (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>(BM >> 4) << 24);
-            uint32_t it = 0, local = 0;
-            bool ok = true;
-            for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x, ++local) {
-                int z, mt, nt, first, blocks;
-                tile_coords(t, m_tiles, g.n_tiles, z, mt, nt);
-                split_range(z, first, blocks);
-                if (blocks <= 0) continue;
-                const int buf = local & 1;
-                if (!mbar_wait(acce0 + 8 * buf, ((local >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
-                tc_fence_after();
-                const uint32_t acc = tmem_base + buf * BN;
-                const int steps = blocks * g.terms;
-                for (int i = 0; i < steps; ++i, ++it) {
-                    const int s = it % STAGES;
-                    if (!mbar_wait(full0 + 8 * s, (it / STAGES) & 1, abort_flag)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint32_t sa = base + s * STAGE_BYTES, sb = sa + A_BYTES;
-#pragma unroll
-                    for (int k = 0; k < BK / UMMA_K; ++k) {
-                        // K contiguous: 32 bytes further along the swizzled row; else 16 rows of 128 bytes further, 64-wide boxes 8 KiB apart
-                        const uint64_t da = A_M ? smem_desc(sa + k * UMMA_K * 128, 64 * BK * 2, 1024) : smem_desc(sa + k * UMMA_K * 2, 16, 1024);
-                        const uint64_t db = B_N ? smem_desc(sb + k * UMMA_K * 128, 64 * BK * 2, 1024) : smem_desc(sb + k * UMMA_K * 2, 16, 1024);
-                        umma_f16(acc, da, db, idesc, (i > 0 || k > 0) ? 1u : 0u);
-                    }
-                    umma_commit(empty0 + 8 * s);  // frees the stage once these MMAs have read it
+                if (!ok) {
+                    // transactions that were already issued land before the shared memory goes away
+                    for (int spin = 0; spin < 4096; ++spin) __nanosleep(64);
                 }
-                if (ok) umma_commit(accf0 + 8 * buf);
+            }
+        } else if (warp == 1) {
+            // ------------------------------------------------------------ MMA issuer ------
+            if (lane == 0) {
+                // D = F32 (bits 4-5), A and B format (7-9, 10-12: 0 = F16, 1 = BF16), A and B stored with M / N contiguous (15, 16),
+                // N >> 3 (17-22), M >> 4 (24-28)
+                const uint32_t fmt = g.is_bf16 ? 1u : 0u;
+                const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((A_M ? 1u : 0u) << 15) | ((B_N ? 1u : 0u) << 16) |
+                                       (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>(BM >> 4) << 24);
+                uint32_t it = 0, local = 0;
+                bool ok = true;
+                for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
+                    int z, mt, nt, first, blocks;
+                    tile_coords(t, m_tiles, g.n_tiles, z, mt, nt);
+                    split_range(z, first, blocks);
+                    const int steps = blocks * g.terms;
+                    const int period = PROMOTE ? g.period : steps;
+                    for (int i0 = 0; ok && i0 < steps; i0 += period, ++local) {
+                        const int buf = local & 1;
+                        if (!mbar_wait(acce0 + 8 * buf, ((local >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint32_t acc = tmem_base + buf * BN;
+                        const int i1 = min(steps, i0 + period);
+                        for (int i = i0; i < i1; ++i, ++it) {
+                            const int s = it % STAGES;
+                            if (!mbar_wait(full0 + 8 * s, (it / STAGES) & 1, abort_flag)) { ok = false; break; }
+                            tc_fence_after();
+                            const uint32_t sa = base + s * STAGE_BYTES, sb = sa + A_BYTES;
+#pragma unroll
+                            for (int k = 0; k < BK / UMMA_K; ++k) {
+                                // K contiguous: 32 bytes further along the swizzled row; else 16 rows of 128 bytes further, 64-wide boxes 8 KiB apart
+                                const uint64_t da = A_M ? smem_desc(sa + k * UMMA_K * 128, 64 * BK * 2, 1024) : smem_desc(sa + k * UMMA_K * 2, 16, 1024);
+                                const uint64_t db = B_N ? smem_desc(sb + k * UMMA_K * 128, 64 * BK * 2, 1024) : smem_desc(sb + k * UMMA_K * 2, 16, 1024);
+                                umma_f16(acc, da, db, idesc, (i > i0 || k > 0) ? 1u : 0u);
+                            }
+                            umma_commit(empty0 + 8 * s);  // frees the stage once these MMAs have read it
+                        }
+                        if (ok) umma_commit(accf0 + 8 * buf);
+                    }
+                }
             }
         }
     } else {
         // ------------------------------------------------------------ epilogue --------
-        const int ew = warp - 2;
+        if constexpr (PROMOTE) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        const int ew = warp - 4;
         const int quarter = warp & 3;  // tensor-memory lanes [32 * quarter, 32 * quarter + 32)
         const int half = ew >> 2;      // this warp takes the chunks half, half + 2, ...
         BoxStore box = {staging_ptr + ew * kWarpBytes, &map_d, lane, 0};
         const float scale = EPI == EPI_RESULT ? *g.scale : 1.0f;
         uint32_t local = 0;
         bool ok = true;
-        for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x, ++local) {
+        for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
             int z, mt, nt, first, blocks;
             tile_coords(t, m_tiles, g.n_tiles, z, mt, nt);
             split_range(z, first, blocks);
-            const int buf = local & 1;
             const int64_t row0 = static_cast<int64_t>(mt) * BM + quarter * 32, row = row0 + lane;
             const int64_t col0 = static_cast<int64_t>(nt) * BN;
             const int rows = static_cast<int>(max(int64_t(0), min(int64_t(32), g.M - row0)));
             const int cols = static_cast<int>(min(int64_t(BN), g.N - col0)), chunks = (cols + 31) >> 5;
-            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN;
+            const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
             const bool empty = blocks <= 0;  // no token counts: the product is zero and nothing was accumulated
-            if (!empty) {
+            uint32_t taddr = lanes;
+            float sums[PROMOTE ? BN / 64 : 1][32];
+            if constexpr (PROMOTE) {
+#pragma unroll
+                for (int i = 0; i < BN / 64; ++i)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) sums[i][j] = 0.0f;
+                const int steps = blocks * g.terms;
+                for (int i0 = 0; i0 < steps; i0 += g.period, ++local) {
+                    const int buf = local & 1;
+                    if (!mbar_wait(accf0 + 8 * buf, (local >> 1) & 1, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                    if (rows > 0) {  // warp-uniform
+#pragma unroll
+                        for (int i = 0; i < BN / 64; ++i) {
+                            if (half + 2 * i < chunks) {
+                                uint32_t v[32];
+                                tmem_load_issue(lanes + buf * BN + (half + 2 * i) * 32, v);
+                                tmem_load_wait(v);
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) sums[i][j] += __uint_as_float(v[j]);
+                            }
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(acce0 + 8 * buf);
+                }
+                if (!ok) break;
+            } else if (!empty) {
+                const int buf = local & 1;
                 if (!mbar_wait(accf0 + 8 * buf, (local >> 1) & 1, abort_flag)) { ok = false; break; }
                 tc_fence_after();
+                taddr = lanes + buf * BN;
             }
+            // body(values, chunk) for every 32-column chunk of this warp
+            auto each = [&](auto&& body) {
+                if constexpr (PROMOTE) {
+#pragma unroll
+                    for (int i = 0; i < BN / 64; ++i) {
+                        if (half + 2 * i < chunks) {
+                            uint32_t v[32];
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sums[i][j]);
+                            body(v, half + 2 * i);
+                        }
+                    }
+                } else {
+                    drain(taddr, half, chunks, body);
+                }
+            };
             if constexpr (EPI == EPI_STATS) {
                 // where this row's target lies within the piece (anywhere outside when it has none here)
                 int64_t target = -1;
@@ -358,7 +423,7 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 const int at = target >= 0 && target < cols ? static_cast<int>(target) : -1;
                 float m = -INFINITY, s = 0.0f, hit = 0.0f;
                 if (rows > 0) {  // warp-uniform
-                    drain(taddr, half, chunks, [&](uint32_t (&v)[32], int c) {
+                    each([&](uint32_t (&v)[32], int c) {
                         online_softmax(v, min(32, cols - c * 32), m, s);
                         if (at >= c * 32 && at < c * 32 + 32) {
 #pragma unroll
@@ -377,7 +442,7 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 const int64_t rel = info.target >= 0 ? info.target - g.vocab0 - col0 : -1;
                 const int at = rel >= 0 && rel < cols ? static_cast<int>(rel) : -1;
                 if (rows > 0) {
-                    drain(taddr, half, chunks, [&](uint32_t (&v)[32], int c) {
+                    each([&](uint32_t (&v)[32], int c) {
                         float d[32];
                         if (info.target == kNoRow) {
 #pragma unroll
@@ -418,7 +483,7 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 }
             } else if constexpr (EPI == EPI_SUM) {
                 if (rows > 0) {
-                    drain(taddr, half, chunks, [&](uint32_t (&v)[32], int c) {
+                    each([&](uint32_t (&v)[32], int c) {
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
                             uint32_t w[16];
@@ -433,7 +498,7 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 auto store = [&](uint32_t (&v)[32], int c) {
                     constexpr bool F32 = std::is_same<OUT, float>::value;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = empty ? 0u : __float_as_uint(__uint_as_float(v[j]) * scale);
+                    for (int j = 0; j < 32; ++j) v[j] = empty ? 0u : __float_as_uint(unscale(__uint_as_float(v[j]), scale));
                     if (g.tma_store) {
 #pragma unroll
                         for (int q = 0; q < (F32 ? 2 : 1); ++q) {
@@ -463,8 +528,8 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     }
                 };
                 if (rows > 0) {
-                    if (!empty) {
-                        drain(taddr, half, chunks, store);
+                    if (PROMOTE || !empty) {
+                        each(store);
                     } else {
                         uint32_t v[32];
 #pragma unroll
@@ -473,11 +538,13 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     }
                 }
             }
-            // this warp has finished reading the accumulator
-            if (!empty) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(acce0 + 8 * buf);
+            if constexpr (!PROMOTE) {
+                if (!empty) {  // this warp has finished reading the accumulator
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(acce0 + 8 * (local & 1));
+                    ++local;
+                }
             }
         }
         if (lane == 0) bulk_wait_all();  // shared memory stays valid until the last box has left
@@ -492,36 +559,61 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     if (threadIdx.x == 0 && *abort_flag) atomicAdd(&g_loss_aborts, 1u);
 }
 
-// Joins the halves of a row: 32 rows per block, `halves` of them spread over 32 threads each.
+// Joins the halves of a row: R rows per block (32, or 1 when there are few), the halves of a row spread over 1024 / R threads. A
+// thread takes eight at a time, so that eight loads are in flight and one maximum serves eight exponentials.
+template <int R>
 __global__ void __launch_bounds__(1024) loss_join(const float2* __restrict__ halves, int64_t n_halves, int64_t rows, const float* __restrict__ target_logit,
                                                   const void* targets, int wide, int64_t ignore, int64_t vocab, float* __restrict__ loss, float* __restrict__ lse) {
     __shared__ float2 part[32][33];
-    const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+    constexpr int STEP = 1024 / R;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * R + threadIdx.x % R;
     float m = -INFINITY, s = 0.0f;
-    auto join = [&](float2 p) {
-        const float now = fmaxf(m, p.x), base = now == -INFINITY ? 0.0f : now;
-        s = s * __expf(m - base) + p.y * __expf(p.x - base);
-        m = now;
-    };
     if (row < rows) {
-#pragma unroll 4
-        for (int64_t i = k; i < n_halves; i += 32) join(halves[i * rows + row]);
+        for (int64_t i0 = threadIdx.x / R; i0 < n_halves; i0 += 8 * STEP) {
+            float2 p[8];
+            float top = m;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                p[q] = i0 + q * STEP < n_halves ? halves[(i0 + q * STEP) * rows + row] : make_float2(-INFINITY, 0.0f);
+                top = fmaxf(top, p[q].x);
+            }
+            const float base = top == -INFINITY ? 0.0f : top;
+            s *= __expf(m - base);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) s += p[q].y * __expf(p[q].x - base);
+            m = top;
+        }
     }
-    part[k][lane] = make_float2(m, s);
-    __syncthreads();
-    // thread (lane, k): part `lane` of row k
-    const float2 mine = part[lane][k];
-    float top = mine.x;
+    auto across = [&](float& top, float& sum) {  // over the lanes of a warp
+        float all = top;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    const float base = top == -INFINITY ? 0.0f : top;
-    float sum = mine.y * __expf(mine.x - base);
+        for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
+        sum *= __expf(top - (all == -INFINITY ? 0.0f : all));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    const int64_t out = static_cast<int64_t>(blockIdx.x) * 32 + k;
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        top = all;
+    };
+    int64_t out;
+    if constexpr (R == 32) {
+        part[warp][lane] = make_float2(m, s);
+        __syncthreads();
+        m = part[lane][warp].x;  // lane: which share of the halves, warp: which row
+        s = part[lane][warp].y;
+        across(m, s);
+        out = static_cast<int64_t>(blockIdx.x) * 32 + warp;
+    } else {
+        across(m, s);
+        if (lane == 0) part[0][warp] = make_float2(m, s);
+        __syncthreads();
+        if (warp > 0) return;
+        m = part[0][lane].x;
+        s = part[0][lane].y;
+        across(m, s);
+        out = blockIdx.x;
+    }
     if (lane == 0 && out < rows) {
-        const float z = top + logf(sum);
+        const float z = m + logf(s);
         const int64_t target = wide ? static_cast<const int64_t*>(targets)[out] : static_cast<const int32_t*>(targets)[out];
         if (lse) lse[out] = z;
         if (loss) loss[out] = target == ignore ? 0.0f : target < 0 || target >= vocab ? NAN : z - target_logit[out];
@@ -575,10 +667,7 @@ __global__ void __launch_bounds__(256) loss_rows(const void* targets, int wide, 
         top = fmaxf(top, tops[w]);
     }
     before += __popc(votes & ((1u << lane) - 1u));
-    // the power of two that brings the largest upstream gradient below 2^14
-    int exponent = 0;
-    if (top > 0.0f) frexpf(top, &exponent);
-    const int shift = top > 0.0f ? max(-100, min(100, 14 - exponent)) : 0;
+    if (top == 0.0f) top = 1.0f;
     if (here) {
         const int row = counts ? before : all + static_cast<int>(mine - before);
         slot[mine] = counts ? row : -1 - row;
@@ -586,14 +675,14 @@ __global__ void __launch_bounds__(256) loss_rows(const void* targets, int wide, 
         if (counts) {
             r.lse = lse[mine];
             const bool inside = target >= 0 && target < vocab;
-            r.grad = inside ? ldexpf(grad[mine], shift) : NAN;  // a target outside the vocabulary has no gradient
+            r.grad = inside ? grad[mine] / top * kTop : NAN;  // a target outside the vocabulary has no gradient
             r.target = inside ? static_cast<int>(target) : -2;
         }
         info[row] = r;
     }
     if (blockIdx.x == 0 && tid == 0) {
         *count = all;
-        *scale = ldexpf(1.0f, -shift);
+        *scale = top;
     }
 }
 
@@ -639,19 +728,34 @@ __global__ void __launch_bounds__(256) pack_rows(const T* __restrict__ src, int6
     }
 }
 
-// dh: the float32 sums of the splits, added in order, scaled back, and put where the tokens stand.
-template <typename T>
+// dh: the float32 sums of the splits, added in order, scaled back, and put where the tokens stand. VEC: 4 where the rows of the
+// result start on boundaries of four elements, else 1.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(256) loss_dhidden(const float* __restrict__ sums, int splits, int64_t rows, int64_t cols, int64_t padded, const int* __restrict__ slot,
                                                     const float* __restrict__ scale, T* __restrict__ out) {
+    struct alignas(sizeof(T) * VEC) Result { T v[VEC]; };
+    struct alignas(sizeof(float) * VEC) Sums { float v[VEC]; };
     const float by = *scale;
-    const int64_t n = rows * cols;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t r = i / cols, c = i - r * cols;
+    const int64_t groups = cols / VEC;
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
         const int at = slot[r];
-        float v = 0.0f;
-        if (at >= 0)
-            for (int z = 0; z < splits; ++z) v += sums[(z * rows + at) * padded + c];
-        out[i] = from_compute<T, float>(at >= 0 ? v * by : 0.0f);
+        for (int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; c < groups; c += static_cast<int64_t>(gridDim.x) * 256) {
+            Sums total;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) total.v[j] = 0.0f;
+            if (at >= 0) {
+#pragma unroll 4
+                for (int z = 0; z < splits; ++z) {
+                    const Sums one = *reinterpret_cast<const Sums*>(sums + (z * rows + at) * padded + c * VEC);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) total.v[j] += one.v[j];
+                }
+            }
+            Result res;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) res.v[j] = from_compute<T, float>(at >= 0 ? unscale(total.v[j], by) : 0.0f);
+            *reinterpret_cast<Result*>(out + r * cols + c * VEC) = res;
+        }
     }
 }
 
@@ -781,19 +885,19 @@ tn_status operand_map(CUtensorMap* map, const Operand& o, bool bf16, int64_t inn
     return make_map(map, o.ptr, bf16, inner, rows, o.parts, o.pitch, o.part_stride, box_inner, box_rows);
 }
 
-template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS>
+template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS, bool PROMOTE>
 tn_status launch_one(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d, const LossArgs& g, cudaStream_t stream) {
     static thread_local int attr_device = -1;  // the opt-in shared-memory size belongs to kernel and device
     int dev = 0;
     TN_CUDA(cudaGetDevice(&dev));
     if (attr_device != dev) {
-        TN_CUDA(cudaFuncSetAttribute(loss_gemm<A_M, B_N, EPI, T, OUT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+        TN_CUDA(cudaFuncSetAttribute(loss_gemm<A_M, B_N, EPI, T, OUT, PARTS, PROMOTE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
         attr_device = dev;
     }
     const int64_t total = (int64_t)g.m_tiles * g.n_tiles * g.splits;
     if (total >= (int64_t(1) << 31)) return fail(TN_ERROR, "linear_cross_entropy: %lld tiles are too many", (long long)total);
     const int64_t sms = sm_count() - sm_margin();
-    loss_gemm<A_M, B_N, EPI, T, OUT, PARTS><<<(unsigned)std::min(total, sms), kThreads, kSmemBytes, stream>>>(a, b, d, g);
+    loss_gemm<A_M, B_N, EPI, T, OUT, PARTS, PROMOTE><<<(unsigned)std::min(total, sms), kThreads, kSmemBytes, stream>>>(a, b, d, g);
     return after_launch("loss_gemm");
 }
 
@@ -807,6 +911,7 @@ LossArgs gemm_args(const Problem& p, int64_t m, int64_t n, int64_t k) {
     g.splits = 1;
     g.split_blocks = g.k_blocks;
     g.terms = p.terms;
+    g.period = kPeriod;
     g.is_bf16 = p.bf16;
     return g;
 }
@@ -920,11 +1025,13 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
         g.halves = halves;
         g.first_half = first_half;
         g.target_logit = target_logit;
-        TN_TRY((launch_one<false, false, EPI_STATS, __half, float, 1>(map_a, map_b, map_a, g, p.stream)));
+        TN_TRY((launch_one<false, false, EPI_STATS, __half, float, 1, true>(map_a, map_b, map_a, g, p.stream)));
         first_half += 2 * (int64_t)g.n_tiles;
     }
-    loss_join<<<(unsigned)ceil_div(p.tokens, 32), 1024, 0, p.stream>>>(halves, first_half, p.tokens, target_logit, t, targets->dtype == TN_INT64, ignore, p.vocab,
-                                                                      loss ? static_cast<float*>(loss->address) : nullptr, lse ? static_cast<float*>(lse->address) : nullptr);
+    const bool few = p.tokens <= 2 * sm_count();  // a block per row fills the GPU at most once
+    (few ? loss_join<1> : loss_join<32>)<<<(unsigned)ceil_div(p.tokens, few ? 1 : 32), 1024, 0, p.stream>>>(
+        halves, first_half, p.tokens, target_logit, t, targets->dtype == TN_INT64, ignore, p.vocab, loss ? static_cast<float*>(loss->address) : nullptr,
+        lse ? static_cast<float*>(lse->address) : nullptr);
     return after_launch("loss_join");
 }
 
@@ -1000,7 +1107,7 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
             g.count = count;
             g.count_is = COUNT_ROWS;
             g.rows = info;
-            TN_TRY((launch_one<false, false, EPI_D, T, float, PARTS>(rows_a, map, map_d, g, p.stream)));
+            TN_TRY((launch_one<false, false, EPI_D, T, float, PARTS, PARTS == 3>(rows_a, map, map_d, g, p.stream)));
         }
         if (dhidden) {
             CUtensorMap map_d, map_w;
@@ -1015,7 +1122,7 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
             g.splits = (int)ceil_div(g.k_blocks, g.split_blocks);
             g.add = v0 > 0;
             if (v0 == 0) splits = g.splits;
-            TN_TRY((launch_one<false, true, EPI_SUM, T, float, 1>(map, map_w, map_d, g, p.stream)));
+            TN_TRY((launch_one<false, true, EPI_SUM, T, float, 1, true>(map, map_w, map_d, g, p.stream)));
         }
         if (dweight) {
             CUtensorMap map_d;
@@ -1031,12 +1138,14 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
             g.tma_store = can_tma_store(to, p.hidden, p.hidden * 8, BN, F32);
             map_d = map;  // placeholder when the result does not leave through TMA
             if (g.tma_store) TN_TRY(make_result_map(&map_d, to, F32, p.bf16, p.hidden, n, 1, p.hidden, 0));
-            TN_TRY((launch_one<true, true, EPI_RESULT, T, OUT, 1>(map, rows_b, map_d, g, p.stream)));
+            TN_TRY((launch_one<true, true, EPI_RESULT, T, OUT, 1, PARTS == 3>(map, rows_b, map_d, g, p.stream)));
         }
     }
     if (dhidden) {
-        const int grid = (int)std::min<int64_t>(ceil_div(p.tokens * p.hidden, 256), sms * 16);
-        loss_dhidden<OUT><<<grid, 256, 0, p.stream>>>(sums, splits, p.tokens, p.hidden, p.padded, slot, scale, static_cast<OUT*>(dhidden->address));
+        OUT* to = static_cast<OUT*>(dhidden->address);
+        const bool wide = p.hidden % 4 == 0 && (reinterpret_cast<uintptr_t>(to) & (4 * sizeof(OUT) - 1)) == 0;
+        const dim3 grid((unsigned)std::min<int64_t>(ceil_div(p.hidden, wide ? 1024 : 256), 1024), (unsigned)std::min<int64_t>(p.tokens, 65535));
+        (wide ? loss_dhidden<OUT, 4> : loss_dhidden<OUT, 1>)<<<grid, 256, 0, p.stream>>>(sums, splits, p.tokens, p.hidden, p.padded, slot, scale, to);
         TN_TRY(after_launch("loss_dhidden"));
     }
     return TN_SUCCESS;

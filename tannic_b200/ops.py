@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import builtins as _b
 import ctypes as C
+import functools
 from typing import Sequence
 
 import torch
@@ -28,18 +29,32 @@ TORCH_TO_TN = {
 TN_TO_TORCH = {v: k for k, v in TORCH_TO_TN.items()}
 
 
+@functools.lru_cache(maxsize=4096)
+def _geometry(shape, strides, dtype, device: int) -> bytes:
+    """A device record without its address. Small calls are paced by the host, and filling a record field by field costs
+    more than launching a kernel, so the last few thousand geometries are kept."""
+    if dtype not in TORCH_TO_TN:
+        raise A.TannicError(A.UNSUPPORTED_DTYPE, f"torch dtype {dtype} has no Tannic equivalent")
+    record = bytes(A.make_tensor(0, tuple(shape), tuple(strides), TORCH_TO_TN[dtype], device))
+    return record[A.TensorT.address.offset + A.TensorT.address.size:]
+
+
 def desc(t: torch.Tensor) -> A.TensorT:
     """tn_tensor_t over a torch tensor's storage (CUDA -> DEVICE environment, CPU -> HOST)."""
+    if t.is_cuda:
+        return A.TensorT.from_buffer_copy(t.data_ptr().to_bytes(8, "little") + _geometry(t.shape, t.stride(), t.dtype, t.get_device()))
     if t.dtype not in TORCH_TO_TN:
         raise A.TannicError(A.UNSUPPORTED_DTYPE, f"torch dtype {t.dtype} has no Tannic equivalent")
-    device = t.device.index if t.is_cuda else None
-    if t.is_cuda and device is None:
-        device = torch.cuda.current_device()
-    return A.make_tensor(t.data_ptr(), tuple(t.shape), tuple(t.stride()), TORCH_TO_TN[t.dtype], device,
-                         pinned=(not t.is_cuda) and t.is_pinned())
+    return A.make_tensor(t.data_ptr(), tuple(t.shape), tuple(t.stride()), TORCH_TO_TN[t.dtype], None, pinned=t.is_pinned())
+
+
+# torch's own shortcut past the Stream object, where this torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def current_stream(t: torch.Tensor) -> A.StreamT:
+    if _raw_stream is not None and t.is_cuda:
+        return A.StreamT(_raw_stream(t.get_device()))
     return A.StreamT(torch.cuda.current_stream(t.device).cuda_stream)
 
 
@@ -480,10 +495,11 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     if x.dim() == 0:
         raise ValueError("cannot normalise a rank-0 tensor")
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(x.shape)
     mean = rstd = None
     if stats:
-        mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float64 if x.dtype == torch.float64 else torch.float32, device=x.device) for _ in range(2))
+        wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+        mean, rstd = x.new_empty(x.shape[:-1], dtype=wide), x.new_empty(x.shape[:-1], dtype=wide)
     A.check(A.lib().tn_layer_norm(_ref(x), _ref(weight), _ref(bias), _ref(out), _ref(mean), _ref(rstd), current_stream(x), eps))
     return (out, mean, rstd) if stats else out
 
@@ -493,9 +509,9 @@ def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd:
     `weight` the normalisation has no parameters and dweight and dbias are None; `bias=False`: it has no bias."""
     if x.dim() == 0:
         raise ValueError("cannot normalise a rank-0 tensor")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dweight = torch.empty(weight.shape, dtype=weight.dtype, device=x.device) if weight is not None else None
-    dbias = torch.empty(weight.shape, dtype=weight.dtype, device=x.device) if weight is not None and bias else None
+    dx = x.new_empty(x.shape)
+    dweight = weight.new_empty(weight.shape) if weight is not None else None
+    dbias = weight.new_empty(weight.shape) if weight is not None and bias else None
     A.check(A.lib().tn_layer_norm_grad(_ref(dy), _ref(x), _ref(mean), _ref(rstd), _ref(weight), _ref(dx), _ref(dweight), _ref(dbias), current_stream(x)))
     return dx, dweight, dbias
 
@@ -504,7 +520,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     """(loss, lse): the softmax cross entropy of the logits hidden . weight^T with `targets`, one float32 per token, and
     the logits' log-sum-exp, which `linear_cross_entropy_grad` reads (tn_linear_cross_entropy). The logits are not
     written. Tokens whose target is `ignore_index` have loss 0."""
-    loss, lse = (torch.empty(targets.shape, dtype=torch.float32, device=hidden.device) for _ in range(2))
+    loss, lse = hidden.new_empty(targets.shape, dtype=torch.float32), hidden.new_empty(targets.shape, dtype=torch.float32)
     A.check(A.lib().tn_linear_cross_entropy(_ref(hidden), _ref(weight), _ref(targets), _ref(loss), _ref(lse), current_stream(hidden), ignore_index))
     return loss, lse
 
@@ -514,8 +530,8 @@ def linear_cross_entropy_grad(grad: torch.Tensor, hidden: torch.Tensor, weight: 
     """(dhidden, dweight) of `linear_cross_entropy` from `grad`, the gradient of every token's loss (for the mean over the
     tokens that count: 1 / their number, expanded), and its lse (tn_linear_cross_entropy_grad). `dhidden=False` or
     `dweight=False` leaves that one out (None): a frozen trunk, a frozen head."""
-    dh = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if dhidden else None
-    dw = torch.empty(weight.shape, dtype=weight.dtype, device=hidden.device) if dweight else None
+    dh = hidden.new_empty(hidden.shape) if dhidden else None
+    dw = weight.new_empty(weight.shape) if dweight else None
     A.check(A.lib().tn_linear_cross_entropy_grad(_ref(grad), _ref(hidden), _ref(weight), _ref(targets), _ref(lse), _ref(dh), _ref(dw),
                                                  current_stream(hidden), ignore_index))
     return dh, dw
