@@ -8,14 +8,17 @@
 // 16-bit type cost four registers) and everything else happens there. The mean is subtracted before
 // the squares are summed (no E[x^2] - mu^2 cancellation); sums are float32 (float64 for float64).
 //
-// A row belongs to a group of TPR threads, each of which holds EPT elements: a warp up to 1024
-// columns (no barrier, four rows per thread block), 128 threads up to 2048, and so on to 512 for 16384. Longer rows are
-// read again from L2 by a looping kernel.
+// A row belongs to a warp while its lanes can hold it (32 elements each, 24 for 768 columns), beyond that to a thread block of
+// up to 512 threads: few threads with many elements each keep the shuffles down. What is in flight must not depend
+// on registers then, so the rows come through a ring in shared memory (cp.async, 16 bytes): a thread copies the
+// vectors that it reads itself, two or three rows ahead, and waits for nobody else's. Rows that are not
+// aligned to 16 bytes go element by element (VEC = 1; 16-bit ones without the ring, whose copies start at four bytes); rows
+// longer than 16384 elements are read again from L2 by a looping kernel.
 //
 // The parameters' gradients are sums over all rows. The thread blocks of the backward kernel are
 // resident for the whole pass and walk the rows with the grid's stride; a thread sees the same columns
-// in every row, so it keeps its columns' two sums in registers and the block writes ONE partial
-// row at its end. A second kernel adds the partial rows (a few hundred) in a fixed order: no
+// in every row, so it keeps its columns' two sums in registers, the warps of a block add theirs up in shared memory, and the
+// block writes ONE partial row at its end. A second kernel adds the partial rows (a few hundred) in a fixed order: no
 // atomics, the same bits on every run.
 #include <algorithm>
 
@@ -70,186 +73,306 @@ __device__ __forceinline__ S group_sum(S v, S* slot) {
     return v;
 }
 
-template <int TPR> constexpr int kBlock = TPR < 128 ? 128 : TPR;
+constexpr int kMost = 512;       // threads of a block that holds one row
+constexpr int kRowWarps = 4;     // warps of a block whose warps hold a row each
 
-template <typename T, typename P, int VEC, int EPT, int TPR>
-__global__ void __launch_bounds__(kBlock<TPR>) norm_forward(const NormArgs a) {
+// Sums of NV values over the threads that share a row: the warp, or (BLOCK) the thread block. `slots`: shared memory, NV values for each
+// warp. Two consecutive reductions use different slots, so one barrier each is enough: a slot is written again only
+// after a barrier that every reader of its old contents has passed.
+template <typename S, int NV, bool BLOCK>
+__device__ __forceinline__ void row_sums(S (&v)[NV], S* slots) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) v[k] += __shfl_xor_sync(0xFFFFFFFFu, v[k], o);
+    }
+    if constexpr (BLOCK) {
+        if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) slots[(threadIdx.x >> 5) * NV + k] = v[k];
+        }
+        __syncthreads();
+        const int warps = blockDim.x >> 5;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) v[k] = slots[k];
+        for (int w = 1; w < warps; ++w) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) v[k] += slots[w * NV + k];
+        }
+    }
+}
+
+__device__ __forceinline__ float inverse_root(float v) { return rsqrtf(v); }
+__device__ __forceinline__ double inverse_root(double v) { return 1.0 / sqrt(v); }
+
+// Where a thread stands: lane `t` of the `threads` that share row `first`, then every `step`-th.
+template <bool BLOCK>
+struct Place {
+    int threads, t;
+    int64_t first, step;
+    __device__ __forceinline__ Place() {
+        if constexpr (BLOCK) {
+            threads = blockDim.x;
+            t = threadIdx.x;
+            first = blockIdx.x;
+            step = gridDim.x;
+        } else {
+            threads = 32;
+            t = threadIdx.x & 31;
+            first = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+            step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+        }
+    }
+};
+
+// N operands' vectors of the next DEPTH - 1 rows, on their way into shared memory: [slot][operand][item][thread].
+template <typename T, int VEC, int ITEMS, int N, int DEPTH>
+struct Ring {
+    static constexpr bool kAsync = sizeof(T) * VEC >= 4;  // cp.async copies 4, 8 or 16 bytes
+    Pack<T, VEC>* mine;   // this thread's place in the first slot
+    int pitch;            // threads of the block
+    int slot = 0;
+    __device__ __forceinline__ Ring(uint8_t* smem) : mine(reinterpret_cast<Pack<T, VEC>*>(smem) + threadIdx.x), pitch(blockDim.x) {}
+    __device__ __forceinline__ Pack<T, VEC>* at(int s, int operand, int item) const { return mine + ((s * N + operand) * ITEMS + item) * pitch; }
+    __device__ __forceinline__ void copy(int s, int operand, int item, const Pack<T, VEC>* from) const {
+        constexpr int bytes = sizeof(Pack<T, VEC>);
+        const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(at(s, operand, item)));
+        if constexpr (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+        else if constexpr (kAsync) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(bytes) : "memory");
+    }
+    __device__ __forceinline__ static void commit() {
+        if constexpr (kAsync) asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    // until the oldest of DEPTH groups has arrived
+    __device__ __forceinline__ static void wait() {
+        if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+    }
+    __device__ __forceinline__ void next() { slot = slot + 1 == DEPTH ? 0 : slot + 1; }
+};
+
+template <typename T, typename P, int VEC, int ITEMS, int DEPTH, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_forward(const NormArgs a) {
     using S = typename stat_of<T>::type;
-    constexpr int ITEMS = EPT / VEC, GROUPS = kBlock<TPR> / TPR;
-    __shared__ S slots[2][TPR / 32];
-    const int t = threadIdx.x % TPR, vecs = a.cols / VEC;
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + threadIdx.x / TPR; row < a.rows; row += static_cast<int64_t>(gridDim.x) * GROUPS) {
-        const Pack<T, VEC>* x = reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.x) + row * a.x_pitch);
-        Pack<T, VEC> raw[ITEMS];
-        S sum = 0;
+    using In = Ring<T, VEC, ITEMS, 1, DEPTH>;
+    __shared__ S slots[2][BLOCK ? kMost / 32 : 1];
+    extern __shared__ __align__(16) uint8_t dynamic[];
+    const Place<BLOCK> at;
+    In ring(dynamic);
+    const int vecs = a.cols / VEC;
+    const S share = S(1) / static_cast<S>(a.cols);
+    auto inside = [&](int i) { return i * at.threads + at.t < vecs; };
+    auto x_at = [&](int64_t r, int i) { return reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.x) + r * a.x_pitch) + (i * at.threads + at.t); };
+    auto fetch = [&](int64_t r, int slot) {
+        if constexpr (In::kAsync) {
+            if (r < a.rows) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (i * TPR + t < vecs) raw[i] = x[i * TPR + t];
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (i * TPR + t < vecs) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) sum += to_compute<S>(raw[i].v[j]);
+                for (int i = 0; i < ITEMS; ++i)
+                    if (inside(i)) ring.copy(slot, 0, i, x_at(r, i));
             }
-        const S mean = group_sum<S, TPR>(sum, slots[0]) / static_cast<S>(a.cols);
-        S square = 0;
+            In::commit();
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d) fetch(at.first + d * at.step, d);
+    for (int64_t row = at.first; row < a.rows; row += at.step) {
+        // the slot before this row's is the one that was read last
+        fetch(row + (DEPTH - 1) * at.step, ring.slot == 0 ? DEPTH - 1 : ring.slot - 1);
+        In::wait();
+        S v[ITEMS * VEC], sum[1] = {0};
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            Pack<T, VEC> p;
+            if (inside(i)) p = In::kAsync ? *ring.at(ring.slot, 0, i) : *x_at(row, i);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[i * VEC + j] = inside(i) ? to_compute<S>(p.v[j]) : S(0);
+        }
+#pragma unroll
+        for (int e = 0; e < ITEMS * VEC; ++e) sum[0] += v[e];
+        row_sums<S, 1, BLOCK>(sum, slots[0]);
+        const S mean = sum[0] * share;
+        sum[0] = 0;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
-            if (i * TPR + t < vecs) {
+            if (inside(i)) {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const S c = to_compute<S>(raw[i].v[j]) - mean;
-                    square += c * c;
+                    v[i * VEC + j] -= mean;
+                    sum[0] += v[i * VEC + j] * v[i * VEC + j];
                 }
             }
-        const S rstd = S(1) / sqrt(group_sum<S, TPR>(square, slots[1]) / static_cast<S>(a.cols) + static_cast<S>(a.eps));
-        if (t == 0) {
+        row_sums<S, 1, BLOCK>(sum, slots[1]);
+        const S rstd = inverse_root(sum[0] * share + static_cast<S>(a.eps));
+        if (at.t == 0) {
             if (a.mean) static_cast<S*>(a.mean)[row] = mean;
             if (a.rstd) static_cast<S*>(a.rstd)[row] = rstd;
         }
         Pack<T, VEC>* y = reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.y) + row * a.cols);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            const int at = i * TPR + t;
-            if (at < vecs) {
-                Pack<P, VEC> w, b;
-                if (a.weight) w = static_cast<const Pack<P, VEC>*>(a.weight)[at];
-                if (a.bias) b = static_cast<const Pack<P, VEC>*>(a.bias)[at];
+            const int c = i * at.threads + at.t;
+            if (inside(i)) {
                 Pack<T, VEC> out;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    S v = (to_compute<S>(raw[i].v[j]) - mean) * rstd;
-                    if (a.weight) v *= to_compute<S>(w.v[j]);
-                    if (a.bias) v += to_compute<S>(b.v[j]);
-                    out.v[j] = from_compute<T, S>(v);
+                for (int j = 0; j < VEC; ++j) v[i * VEC + j] *= rstd;
+                if (a.weight) {
+                    const Pack<P, VEC> p = static_cast<const Pack<P, VEC>*>(a.weight)[c];
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) v[i * VEC + j] *= to_compute<S>(p.v[j]);
                 }
-                y[at] = out;
+                if (a.bias) {
+                    const Pack<P, VEC> p = static_cast<const Pack<P, VEC>*>(a.bias)[c];
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) v[i * VEC + j] += to_compute<S>(p.v[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) out.v[j] = from_compute<T, S>(v[i * VEC + j]);
+                y[c] = out;
             }
         }
+        ring.next();
     }
 }
 
-template <typename T, typename P, int VEC, int EPT, int TPR>
-__global__ void __launch_bounds__(kBlock<TPR>) norm_backward(const NormArgs a) {
+// KEEP: z and g stay in registers between the two halves of the work; else (32 elements in each of 512 threads) they are formed again.
+template <typename T, typename P, int VEC, int ITEMS, int DEPTH, bool BLOCK, bool KEEP>
+__global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_backward(const NormArgs a) {
     using S = typename stat_of<T>::type;
-    constexpr int ITEMS = EPT / VEC, GROUPS = kBlock<TPR> / TPR;
-    // 32 elements in each of 512 threads leave room for the two sums of a column but not for the row as well:
-    // the second half of the work then reads x, dy and w again, from L1 and L2
-    constexpr bool KEEP = EPT * TPR <= 8192;
-    __shared__ S slots[2][2][TPR / 32];
-    extern __shared__ uint8_t dynamic[];
-    const int t = threadIdx.x % TPR, group = threadIdx.x / TPR, vecs = a.cols / VEC;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * GROUPS;
-    S dw[EPT], db[EPT];
+    using In = Ring<T, VEC, ITEMS, 2, DEPTH>;
+    constexpr int E = VEC * ITEMS;
+    __shared__ S slots[2][BLOCK ? kMost / 32 * 2 : 1];
+    extern __shared__ __align__(16) uint8_t dynamic[];
+    const Place<BLOCK> at;
+    In ring(dynamic);
+    const int vecs = a.cols / VEC;
+    const S share = S(1) / static_cast<S>(a.cols);
+    S dw[E], db[E];
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) dw[e] = db[e] = 0;
-    Pack<P, VEC> w[KEEP ? ITEMS : 1];
-    if (KEEP && a.weight) {
+    for (int e = 0; e < E; ++e) dw[e] = db[e] = 0;
+    auto inside = [&](int i) { return i * at.threads + at.t < vecs; };
+    auto weight_at = [&](int i) {
+        Pack<P, VEC> p;
+        if (a.weight) {
+            p = static_cast<const Pack<P, VEC>*>(a.weight)[i * at.threads + at.t];
+        } else {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (i * TPR + t < vecs) w[i] = static_cast<const Pack<P, VEC>*>(a.weight)[i * TPR + t];
-    }
-    int parity = 0;
-    // with TPR > 32 a block has one group, so the block's threads leave this loop together
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group; row < a.rows; row += step, parity ^= 1) {
-        const Pack<T, VEC>* x = reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.x) + row * a.x_pitch);
-        const Pack<T, VEC>* dy = reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dy) + row * a.dy_pitch);
-        const S mean = static_cast<const S*>(a.mean)[row], rstd = static_cast<const S*>(a.rstd)[row];
-        Pack<T, VEC> rx[KEEP ? ITEMS : 1], rd[KEEP ? ITEMS : 1];
-        if constexpr (KEEP) {
-#pragma unroll
-            for (int i = 0; i < ITEMS; ++i)
-                if (i * TPR + t < vecs) {
-                    rx[i] = x[i * TPR + t];
-                    rd[i] = dy[i * TPR + t];
-                }
+            for (int j = 0; j < VEC; ++j) p.v[j] = from_compute<P, S>(S(1));
         }
-        auto fetch = [&](int i) {
-            if constexpr (!KEEP) {
-                rx[0] = x[i * TPR + t];
-                rd[0] = dy[i * TPR + t];
-                if (a.weight) w[0] = static_cast<const Pack<P, VEC>*>(a.weight)[i * TPR + t];
+        return p;
+    };
+    auto x_at = [&](int64_t r, int i) { return reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.x) + r * a.x_pitch) + (i * at.threads + at.t); };
+    auto dy_at = [&](int64_t r, int i) { return reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dy) + r * a.dy_pitch) + (i * at.threads + at.t); };
+    auto fetch = [&](int64_t r, int slot) {
+        if constexpr (In::kAsync) {
+            if (r < a.rows) {
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i)
+                    if (inside(i)) {
+                        ring.copy(slot, 0, i, x_at(r, i));
+                        ring.copy(slot, 1, i, dy_at(r, i));
+                    }
             }
-            return KEEP ? i : 0;
-        };
-        S sum_g = 0, sum_gz = 0;
+            In::commit();
+        }
+    };
+    auto load = [&](int64_t r, int i, Pack<T, VEC>& px, Pack<T, VEC>& pd) {
+        px = In::kAsync ? *ring.at(ring.slot, 0, i) : *x_at(r, i);
+        pd = In::kAsync ? *ring.at(ring.slot, 1, i) : *dy_at(r, i);
+    };
+    Pack<P, VEC> w[KEEP ? ITEMS : 1];
+    if constexpr (KEEP) {
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
-            if (i * TPR + t < vecs) {
-                const int k = fetch(i);
+            if (inside(i)) w[i] = weight_at(i);
+    }
+    S mean = 0, rstd = 0;
+    auto statistics = [&](int64_t r) {
+        if (r < a.rows) {
+            mean = static_cast<const S*>(a.mean)[r];
+            rstd = static_cast<const S*>(a.rstd)[r];
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d) fetch(at.first + d * at.step, d);
+    statistics(at.first);
+    int parity = 0;
+    for (int64_t row = at.first; row < a.rows; row += at.step, parity ^= 1) {
+        fetch(row + (DEPTH - 1) * at.step, ring.slot == 0 ? DEPTH - 1 : ring.slot - 1);
+        const S mu = mean, rs = rstd;
+        statistics(row + at.step);
+        In::wait();
+        S z[KEEP ? E : 1], g[KEEP ? E : 1];
+        S sums[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (inside(i)) {
+                Pack<T, VEC> px, pd;
+                load(row, i, px, pd);
+                const Pack<P, VEC> pw = KEEP ? w[KEEP ? i : 0] : weight_at(i);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const S z = (to_compute<S>(rx[k].v[j]) - mean) * rstd, d = to_compute<S>(rd[k].v[j]);
-                    const S g = a.weight ? d * to_compute<S>(w[k].v[j]) : d;
-                    sum_g += g;
-                    sum_gz += g * z;
-                    dw[i * VEC + j] += d * z;
-                    db[i * VEC + j] += d;
+                    const int e = i * VEC + j;
+                    const S zz = (to_compute<S>(px.v[j]) - mu) * rs, d = to_compute<S>(pd.v[j]), gg = d * to_compute<S>(pw.v[j]);
+                    sums[0] += gg;
+                    sums[1] += gg * zz;
+                    dw[e] += d * zz;
+                    db[e] += d;
+                    if constexpr (KEEP) {
+                        z[e] = zz;
+                        g[e] = gg;
+                    }
                 }
             }
-        sum_g = warp_sum(sum_g);
-        sum_gz = warp_sum(sum_gz);
-        if constexpr (TPR > 32) {
-            if ((threadIdx.x & 31) == 0) {
-                slots[parity][0][threadIdx.x >> 5] = sum_g;
-                slots[parity][1][threadIdx.x >> 5] = sum_gz;
-            }
-            __syncthreads();  // the other parity's slots are written only after every thread passed this
-            sum_g = slots[parity][0][0];
-            sum_gz = slots[parity][1][0];
-#pragma unroll
-            for (int q = 1; q < TPR / 32; ++q) {
-                sum_g += slots[parity][0][q];
-                sum_gz += slots[parity][1][q];
-            }
-        }
-        const S mean_g = sum_g / static_cast<S>(a.cols), mean_gz = sum_gz / static_cast<S>(a.cols);
+        row_sums<S, 2, BLOCK>(sums, slots[parity]);
+        const S mean_g = sums[0] * share, mean_gz = sums[1] * share;
         Pack<T, VEC>* dx = reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.y) + row * a.cols);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
-            if (i * TPR + t < vecs) {
-                const int k = fetch(i);
-                Pack<T, VEC> out;
+            if (inside(i)) {
+                Pack<T, VEC> px, pd, out;
+                Pack<P, VEC> pw;
+                if constexpr (!KEEP) {
+                    load(row, i, px, pd);
+                    pw = weight_at(i);
+                }
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const S z = (to_compute<S>(rx[k].v[j]) - mean) * rstd, d = to_compute<S>(rd[k].v[j]);
-                    const S g = a.weight ? d * to_compute<S>(w[k].v[j]) : d;
-                    out.v[j] = from_compute<T, S>((g - mean_g - z * mean_gz) * rstd);
+                    const int e = i * VEC + j;
+                    S zz, gg;
+                    if constexpr (KEEP) {
+                        zz = z[e];
+                        gg = g[e];
+                    } else {
+                        zz = (to_compute<S>(px.v[j]) - mu) * rs;
+                        gg = to_compute<S>(pd.v[j]) * to_compute<S>(pw.v[j]);
+                    }
+                    out.v[j] = from_compute<T, S>((gg - mean_g - zz * mean_gz) * rs);
                 }
-                dx[i * TPR + t] = out;
+                dx[i * at.threads + at.t] = out;
             }
+        ring.next();
     }
     if (a.partial == nullptr) return;  // uniform: no parameter gradients wanted
     S* mine = static_cast<S*>(a.partial) + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
-    if constexpr (GROUPS == 1) {
+    S* all = BLOCK ? mine : reinterpret_cast<S*>(dynamic);
+    // a block that holds one row has its sums; the warps of the others add theirs up one after the other, where the ring was
+    for (int k = 0; k < (BLOCK ? 1 : static_cast<int>(blockDim.x >> 5)); ++k) {
+        if (!BLOCK) __syncthreads();
+        if (BLOCK || static_cast<int>(threadIdx.x >> 5) == k) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (i * TPR + t < vecs) {
+            for (int i = 0; i < ITEMS; ++i)
+                if (inside(i)) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    mine[(i * TPR + t) * VEC + j] = dw[i * VEC + j];
-                    mine[a.cols + (i * TPR + t) * VEC + j] = db[i * VEC + j];
-                }
-            }
-    } else {
-        // the block's groups add up in shared memory, one after the other
-        S* all = reinterpret_cast<S*>(dynamic);
-        for (int k = 0; k < GROUPS; ++k) {
-            if (group == k) {
-#pragma unroll
-                for (int i = 0; i < ITEMS; ++i)
-                    if (i * TPR + t < vecs) {
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) {
-                            const int c = (i * TPR + t) * VEC + j;
-                            all[c] = k ? all[c] + dw[i * VEC + j] : dw[i * VEC + j];
-                            all[a.cols + c] = k ? all[a.cols + c] + db[i * VEC + j] : db[i * VEC + j];
-                        }
+                    for (int j = 0; j < VEC; ++j) {
+                        const int c = (i * at.threads + at.t) * VEC + j, e = i * VEC + j;
+                        all[c] = k ? all[c] + dw[e] : dw[e];
+                        all[a.cols + c] = k ? all[a.cols + c] + db[e] : db[e];
                     }
-            }
-            __syncthreads();
+                }
         }
-        for (int c = threadIdx.x; c < 2 * a.cols; c += kBlock<TPR>) mine[c] = all[c];
+    }
+    if (!BLOCK) {
+        __syncthreads();
+        for (int c = threadIdx.x; c < 2 * a.cols; c += blockDim.x) mine[c] = all[c];
     }
 }
 
@@ -385,30 +508,61 @@ tn_status finish_partial(Launch& l, int64_t blocks) {
     return after_launch("norm_parameters");
 }
 
-template <typename T, typename P, int VEC, int EPT, int TPR>
-tn_status launch_rows(Launch& l) {
+// Thread blocks of a kernel that are on the GPU at once; lets the kernel have that much shared memory. The answer to the last
+// question (device, threads, shared memory) is kept in `last`, one per kernel and thread.
+struct Resident {
+    int device = -1, threads = 0;
+    size_t smem = 0;
+    int64_t blocks = 0;
+};
+template <typename K>
+tn_status resident_blocks(K kernel, int threads, size_t smem, Resident& last) {
+    int device = 0, per_sm = 0;
+    TN_CUDA(cudaGetDevice(&device));
+    if (last.device == device && last.threads == threads && last.smem == smem) return TN_SUCCESS;
+    // 48 KiB need no permission, but the kernels' static shared memory counts as well
+    if (smem > 40 * 1024) TN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    TN_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
+    last = {device, threads, smem, (int64_t)sm_count() * std::max(per_sm, 1)};
+    return TN_SUCCESS;
+}
+
+template <typename T, int VEC, int ITEMS, bool BLOCK>
+int block_threads(int cols) {
+    return BLOCK ? (int)(ceil_div(ceil_div(cols / VEC, ITEMS), 32) * 32) : 32 * kRowWarps;
+}
+
+template <typename T, typename P, int VEC, int ITEMS, bool BLOCK>
+tn_status launch_forward(Launch& l) {
+    constexpr int DEPTH = 3;
+    const NormArgs& a = l.args;
+    const int threads = block_threads<T, VEC, ITEMS, BLOCK>(a.cols);
+    const size_t smem = Ring<T, VEC, ITEMS, 1, DEPTH>::kAsync ? sizeof(T) * VEC * ITEMS * DEPTH * (size_t)threads : 0;
+    static thread_local Resident resident;
+    TN_TRY(resident_blocks(norm_forward<T, P, VEC, ITEMS, DEPTH, BLOCK>, threads, smem, resident));
+    const int64_t blocks = std::min(resident.blocks, ceil_div(a.rows, BLOCK ? 1 : kRowWarps));
+    norm_forward<T, P, VEC, ITEMS, DEPTH, BLOCK><<<(unsigned)blocks, threads, smem, l.stream>>>(a);
+    return after_launch("norm_forward");
+}
+
+template <typename T, typename P, int VEC, int ITEMS, bool BLOCK, bool KEEP>
+tn_status launch_backward(Launch& l) {
     using S = typename stat_of<T>::type;
-    constexpr int GROUPS = kBlock<TPR> / TPR;
-    if (!l.backward) {
-        norm_forward<T, P, VEC, EPT, TPR><<<(unsigned)rows_grid(l.args.rows, GROUPS), kBlock<TPR>, 0, l.stream>>>(l.args);
-        return after_launch("norm_forward");
-    }
-    const size_t smem = GROUPS > 1 ? sizeof(S) * 2 * (size_t)l.args.cols : 0;
+    constexpr int DEPTH = !KEEP && sizeof(T) == 4 ? 1 : 3;  // one row of 16384 float32 twice is 128 KiB
+    NormArgs& a = l.args;
+    const int threads = block_threads<T, VEC, ITEMS, BLOCK>(a.cols);
+    size_t smem = Ring<T, VEC, ITEMS, 2, DEPTH>::kAsync ? sizeof(T) * VEC * ITEMS * 2 * DEPTH * (size_t)threads : 0;
+    if (!BLOCK) smem = std::max(smem, sizeof(S) * 2 * (size_t)a.cols);
     // one resident wave: every block walks rows until the pass ends, then writes its partial row
-    static std::atomic<int> resident{0};
-    int per_sm = resident.load(std::memory_order_relaxed);
-    if (per_sm == 0) {
-        TN_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, norm_backward<T, P, VEC, EPT, TPR>, kBlock<TPR>, GROUPS > 1 ? sizeof(S) * 2 * EPT * TPR : 0));
-        if (per_sm < 1) per_sm = 1;
-        resident.store(per_sm, std::memory_order_relaxed);
-    }
-    const int64_t blocks = std::min<int64_t>(ceil_div(l.args.rows, GROUPS), (int64_t)sm_count() * per_sm);
+    static thread_local Resident resident;
+    TN_TRY(resident_blocks(norm_backward<T, P, VEC, ITEMS, DEPTH, BLOCK, KEEP>, threads, smem, resident));
+    const int64_t blocks = std::min(resident.blocks, ceil_div(a.rows, BLOCK ? 1 : kRowWarps));
     TN_TRY(alloc_partial<S>(l, blocks));
-    norm_backward<T, P, VEC, EPT, TPR><<<(unsigned)blocks, kBlock<TPR>, smem, l.stream>>>(l.args);
+    norm_backward<T, P, VEC, ITEMS, DEPTH, BLOCK, KEEP><<<(unsigned)blocks, threads, smem, l.stream>>>(a);
     tn_status st = after_launch("norm_backward");
     if (st == TN_SUCCESS) st = finish_partial<S, P>(l, blocks);
-    if (l.args.partial) {
-        const tn_status freed = scratch_free(l.args.partial, l.stream);
+    if (a.partial) {
+        const tn_status freed = scratch_free(a.partial, l.stream);
         if (st == TN_SUCCESS) st = freed;
     }
     return st;
@@ -438,19 +592,29 @@ tn_status launch_long(Launch& l) {
     return after_launch("norm_backward_long");
 }
 
+// ITEMS: vectors a thread holds. A warp takes a row of up to 32 (float64: 16) elements a lane.
 template <typename T, typename P, int VEC>
 tn_status launch_sized(Launch& l) {
     const int c = l.args.cols;
-    if (c <= 256) return launch_rows<T, P, VEC, 8, 32>(l);
-    if (c <= 512) return launch_rows<T, P, VEC, 16, 32>(l);
-    if constexpr (std::is_same<T, double>::value) {  // twice the registers an element
-        if (c <= 2048) return launch_rows<T, P, VEC, 16, 128>(l);
+    constexpr bool F64 = std::is_same<T, double>::value;
+    constexpr int Q = F64 ? 16 / VEC : 32 / VEC;  // vectors of a full thread
+    if (!l.backward) {
+        if (c <= 8 * Q * VEC) return launch_forward<T, P, VEC, Q / 4, false>(l);
+        if (c <= 16 * Q * VEC) return launch_forward<T, P, VEC, Q / 2, false>(l);
+        if constexpr (Q % 4 == 0)
+            if (c <= 24 * Q * VEC) return launch_forward<T, P, VEC, Q / 4 * 3, false>(l);
+        if (c <= 32 * Q * VEC) return launch_forward<T, P, VEC, Q, false>(l);
+        if (c <= kMost * Q * VEC) return launch_forward<T, P, VEC, Q, true>(l);
     } else {
-        if (c <= 1024) return launch_rows<T, P, VEC, 32, 32>(l);
-        if (c <= 2048) return launch_rows<T, P, VEC, 16, 128>(l);
-        if (c <= 4096) return launch_rows<T, P, VEC, 16, 256>(l);
-        if (c <= 8192) return launch_rows<T, P, VEC, 16, 512>(l);
-        if (c <= 16384) return launch_rows<T, P, VEC, 32, 512>(l);
+        if (c <= 8 * Q * VEC) return launch_backward<T, P, VEC, Q / 4, false, true>(l);
+        if (c <= 16 * Q * VEC) return launch_backward<T, P, VEC, Q / 2, false, true>(l);
+        if constexpr (!F64) {
+            if (c <= 24 * Q * VEC) return launch_backward<T, P, VEC, Q / 4 * 3, false, true>(l);
+            if (c <= kMost * Q / 2 * VEC) return launch_backward<T, P, VEC, Q / 2, true, true>(l);
+            if (c <= kMost * Q * VEC) return launch_backward<T, P, VEC, Q, true, false>(l);
+        } else {
+            if (c <= kMost * Q / 4 * VEC) return launch_backward<T, P, VEC, Q / 4, true, true>(l);
+        }
     }
     return launch_long<T, P>(l);
 }
