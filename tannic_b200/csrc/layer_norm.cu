@@ -11,8 +11,8 @@
 // A row belongs to a warp while its lanes can hold it (32 elements each, 24 for 768 columns), beyond that to a thread block of
 // up to 512 threads: few threads with many elements each keep the shuffles down. What is in flight must not depend
 // on registers then, so the rows come through a ring in shared memory (cp.async, 16 bytes): a thread copies the
-// vectors that it reads itself, two or three rows ahead, and waits for nobody else's. Rows that are not
-// aligned to 16 bytes go element by element (VEC = 1; 16-bit ones without the ring, whose copies start at four bytes); rows
+// vectors that it reads itself, two rows ahead, and waits for nobody else's. Rows that are not
+// aligned to 16 bytes go element by element (VEC = 1), the next row's elements waiting in registers; rows
 // longer than 16384 elements are read again from L2 by a looping kernel.
 //
 // The parameters' gradients are sums over all rows. The thread blocks of the backward kernel are
@@ -128,17 +128,16 @@ struct Place {
 // N operands' vectors of the next DEPTH - 1 rows, on their way into shared memory: [slot][operand][item][thread].
 template <typename T, int VEC, int ITEMS, int N, int DEPTH>
 struct Ring {
-    static constexpr bool kAsync = sizeof(T) * VEC >= 4;  // cp.async copies 4, 8 or 16 bytes
+    static constexpr bool kAsync = VEC > 1;  // element by element, copies would cost more instructions than loads
     Pack<T, VEC>* mine;   // this thread's place in the first slot
     int pitch;            // threads of the block
     int slot = 0;
     __device__ __forceinline__ Ring(uint8_t* smem) : mine(reinterpret_cast<Pack<T, VEC>*>(smem) + threadIdx.x), pitch(blockDim.x) {}
     __device__ __forceinline__ Pack<T, VEC>* at(int s, int operand, int item) const { return mine + ((s * N + operand) * ITEMS + item) * pitch; }
     __device__ __forceinline__ void copy(int s, int operand, int item, const Pack<T, VEC>* from) const {
-        constexpr int bytes = sizeof(Pack<T, VEC>);
+        static_assert(!kAsync || sizeof(Pack<T, VEC>) == 16, "vectors of 16 bytes");
         const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(at(s, operand, item)));
-        if constexpr (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-        else if constexpr (kAsync) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(bytes) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
     }
     __device__ __forceinline__ static void commit() {
         if constexpr (kAsync) asm volatile("cp.async.commit_group;" ::: "memory");
@@ -161,31 +160,48 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_forwar
     const int vecs = a.cols / VEC;
     const S share = S(1) / static_cast<S>(a.cols);
     auto inside = [&](int i) { return i * at.threads + at.t < vecs; };
-    auto x_at = [&](int64_t r, int i) { return reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.x) + r * a.x_pitch) + (i * at.threads + at.t); };
+    Pack<T, VEC> ahead[In::kAsync ? 1 : ITEMS];
     auto fetch = [&](int64_t r, int slot) {
-        if constexpr (In::kAsync) {
-            if (r < a.rows) {
+        if (r < a.rows) {
+            const Pack<T, VEC>* x = reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.x) + r * a.x_pitch) + at.t;
 #pragma unroll
-                for (int i = 0; i < ITEMS; ++i)
-                    if (inside(i)) ring.copy(slot, 0, i, x_at(r, i));
-            }
-            In::commit();
+            for (int i = 0; i < ITEMS; ++i)
+                if (inside(i)) {
+                    if constexpr (In::kAsync) ring.copy(slot, 0, i, x + i * at.threads);
+                    else ahead[i] = x[i * at.threads];
+                }
         }
+        In::commit();
     };
 #pragma unroll
-    for (int d = 0; d < DEPTH - 1; ++d) fetch(at.first + d * at.step, d);
+    for (int d = 0; d < (In::kAsync ? DEPTH - 1 : 1); ++d) fetch(at.first + d * at.step, d);
+    // the parameters of this thread's columns, read once for all rows
+    Pack<P, VEC> w[ITEMS], b[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            w[i].v[j] = from_compute<P, S>(S(1));
+            b[i].v[j] = from_compute<P, S>(S(0));
+        }
+        if (inside(i) && a.weight) w[i] = static_cast<const Pack<P, VEC>*>(a.weight)[i * at.threads + at.t];
+        if (inside(i) && a.bias) b[i] = static_cast<const Pack<P, VEC>*>(a.bias)[i * at.threads + at.t];
+    }
     for (int64_t row = at.first; row < a.rows; row += at.step) {
-        // the slot before this row's is the one that was read last
-        fetch(row + (DEPTH - 1) * at.step, ring.slot == 0 ? DEPTH - 1 : ring.slot - 1);
-        In::wait();
+        if constexpr (In::kAsync) {
+            // the slot before this row's is the one that was read last
+            fetch(row + (DEPTH - 1) * at.step, ring.slot == 0 ? DEPTH - 1 : ring.slot - 1);
+            In::wait();
+        }
         S v[ITEMS * VEC], sum[1] = {0};
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             Pack<T, VEC> p;
-            if (inside(i)) p = In::kAsync ? *ring.at(ring.slot, 0, i) : *x_at(row, i);
+            if (inside(i)) p = In::kAsync ? *ring.at(ring.slot, 0, i) : ahead[In::kAsync ? 0 : i];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) v[i * VEC + j] = inside(i) ? to_compute<S>(p.v[j]) : S(0);
         }
+        if constexpr (!In::kAsync) fetch(row + at.step, 0);
 #pragma unroll
         for (int e = 0; e < ITEMS * VEC; ++e) sum[0] += v[e];
         row_sums<S, 1, BLOCK>(sum, slots[0]);
@@ -209,24 +225,11 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_forwar
         Pack<T, VEC>* y = reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.y) + row * a.cols);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            const int c = i * at.threads + at.t;
             if (inside(i)) {
                 Pack<T, VEC> out;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) v[i * VEC + j] *= rstd;
-                if (a.weight) {
-                    const Pack<P, VEC> p = static_cast<const Pack<P, VEC>*>(a.weight)[c];
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[i * VEC + j] *= to_compute<S>(p.v[j]);
-                }
-                if (a.bias) {
-                    const Pack<P, VEC> p = static_cast<const Pack<P, VEC>*>(a.bias)[c];
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[i * VEC + j] += to_compute<S>(p.v[j]);
-                }
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) out.v[j] = from_compute<T, S>(v[i * VEC + j]);
-                y[c] = out;
+                for (int j = 0; j < VEC; ++j) out.v[j] = from_compute<T, S>(v[i * VEC + j] * rstd * to_compute<S>(w[i].v[j]) + to_compute<S>(b[i].v[j]));
+                y[i * at.threads + at.t] = out;
             }
         }
         ring.next();
@@ -259,24 +262,37 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_backwa
         }
         return p;
     };
-    auto x_at = [&](int64_t r, int i) { return reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.x) + r * a.x_pitch) + (i * at.threads + at.t); };
-    auto dy_at = [&](int64_t r, int i) { return reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dy) + r * a.dy_pitch) + (i * at.threads + at.t); };
+    constexpr bool AHEAD = !In::kAsync && KEEP;  // the next row waits in registers
+    Pack<T, VEC> ahead_x[AHEAD ? ITEMS : 1], ahead_dy[AHEAD ? ITEMS : 1];
     auto fetch = [&](int64_t r, int slot) {
-        if constexpr (In::kAsync) {
-            if (r < a.rows) {
+        if (r < a.rows) {
+            const Pack<T, VEC>* x = reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.x) + r * a.x_pitch) + at.t;
+            const Pack<T, VEC>* dy = reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dy) + r * a.dy_pitch) + at.t;
 #pragma unroll
-                for (int i = 0; i < ITEMS; ++i)
-                    if (inside(i)) {
-                        ring.copy(slot, 0, i, x_at(r, i));
-                        ring.copy(slot, 1, i, dy_at(r, i));
+            for (int i = 0; i < ITEMS; ++i)
+                if (inside(i)) {
+                    if constexpr (In::kAsync) {
+                        ring.copy(slot, 0, i, x + i * at.threads);
+                        ring.copy(slot, 1, i, dy + i * at.threads);
+                    } else if constexpr (AHEAD) {
+                        ahead_x[i] = x[i * at.threads];
+                        ahead_dy[i] = dy[i * at.threads];
                     }
-            }
-            In::commit();
+                }
         }
+        In::commit();
     };
     auto load = [&](int64_t r, int i, Pack<T, VEC>& px, Pack<T, VEC>& pd) {
-        px = In::kAsync ? *ring.at(ring.slot, 0, i) : *x_at(r, i);
-        pd = In::kAsync ? *ring.at(ring.slot, 1, i) : *dy_at(r, i);
+        if constexpr (In::kAsync) {
+            px = *ring.at(ring.slot, 0, i);
+            pd = *ring.at(ring.slot, 1, i);
+        } else if constexpr (AHEAD) {
+            px = ahead_x[i];
+            pd = ahead_dy[i];
+        } else {
+            px = (reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.x) + r * a.x_pitch) + at.t)[i * at.threads];
+            pd = (reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dy) + r * a.dy_pitch) + at.t)[i * at.threads];
+        }
     };
     Pack<P, VEC> w[KEEP ? ITEMS : 1];
     if constexpr (KEEP) {
@@ -292,11 +308,11 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_backwa
         }
     };
 #pragma unroll
-    for (int d = 0; d < DEPTH - 1; ++d) fetch(at.first + d * at.step, d);
+    for (int d = 0; d < (In::kAsync ? DEPTH - 1 : 1); ++d) fetch(at.first + d * at.step, d);
     statistics(at.first);
     int parity = 0;
     for (int64_t row = at.first; row < a.rows; row += at.step, parity ^= 1) {
-        fetch(row + (DEPTH - 1) * at.step, ring.slot == 0 ? DEPTH - 1 : ring.slot - 1);
+        if constexpr (In::kAsync) fetch(row + (DEPTH - 1) * at.step, ring.slot == 0 ? DEPTH - 1 : ring.slot - 1);
         const S mu = mean, rs = rstd;
         statistics(row + at.step);
         In::wait();
@@ -322,6 +338,7 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_backwa
                     }
                 }
             }
+        if constexpr (AHEAD) fetch(row + at.step, 0);
         row_sums<S, 2, BLOCK>(sums, slots[parity]);
         const S mean_g = sums[0] * share, mean_gz = sums[1] * share;
         Pack<T, VEC>* dx = reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.y) + row * a.cols);
@@ -455,23 +472,26 @@ __global__ void __launch_bounds__(256) norm_columns_long(const NormArgs a) {
     mine[a.cols + c] = db;
 }
 
-// Adds the partial rows, in an order that depends on their number only: 32 columns per block, 32 threads a column.
+// Adds the partial rows, in an order that depends on their number only: eight columns (a sector of 32 bytes) per block and 128 threads
+// a column, so that a few hundred rows are two or three loads a thread, all in flight.
 template <typename S, typename P>
 __global__ void __launch_bounds__(1024) norm_parameters(const S* __restrict__ partial, int blocks, int cols, P* __restrict__ dweight, P* __restrict__ dbias) {
-    __shared__ S part[32][33];
-    const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
+    __shared__ S part[32][8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // columns [0, cols) are the weight's, [cols, 2 cols) the bias's
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
-    const int64_t all = static_cast<int64_t>(cols) * 2;
+    const int64_t all = static_cast<int64_t>(cols) * 2, c = static_cast<int64_t>(blockIdx.x) * 8 + (lane & 7);
     S sum = 0;
     if (c < all) {
 #pragma unroll 4
-        for (int b = k; b < blocks; b += 32) sum += partial[static_cast<int64_t>(b) * all + c];
+        for (int b = threadIdx.x >> 3; b < blocks; b += 128) sum += partial[static_cast<int64_t>(b) * all + c];
     }
-    part[k][lane] = sum;
+    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
+    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
+    if (lane < 8) part[warp][lane] = sum;
     __syncthreads();
-    sum = warp_sum(part[lane][k]);  // thread (lane, k): partial sum `lane` of column k
-    const int64_t out = static_cast<int64_t>(blockIdx.x) * 32 + k;
+    if (warp >= 8) return;
+    sum = warp_sum(part[lane][warp]);  // column `warp`
+    const int64_t out = static_cast<int64_t>(blockIdx.x) * 8 + warp;
     if (lane == 0 && out < all) {
         if (out < cols) {
             if (dweight) dweight[out] = from_compute<P, S>(sum);
@@ -503,7 +523,7 @@ tn_status alloc_partial(Launch& l, int64_t blocks) {
 template <typename S, typename P>
 tn_status finish_partial(Launch& l, int64_t blocks) {
     if (!l.args.partial) return TN_SUCCESS;
-    norm_parameters<S, P><<<(unsigned)ceil_div(2 * (int64_t)l.args.cols, 32), 1024, 0, l.stream>>>(
+    norm_parameters<S, P><<<(unsigned)ceil_div(2 * (int64_t)l.args.cols, 8), 1024, 0, l.stream>>>(
         static_cast<const S*>(l.args.partial), (int)blocks, l.args.cols, static_cast<P*>(l.dweight), static_cast<P*>(l.dbias));
     return after_launch("norm_parameters");
 }
