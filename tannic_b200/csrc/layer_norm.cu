@@ -73,6 +73,45 @@ __device__ __forceinline__ S group_sum(S v, S* slot) {
     return v;
 }
 
+// Two elements at a time: float32 as one packed instruction (the add, mul and fma of f32x2, rounded like the single ones), which
+// halves the arithmetic of kernels that are as near to the issue limit as to HBM's.
+template <typename S> struct Two { S a, b; };
+template <typename S> __device__ __forceinline__ Two<S> both(S v) { return {v, v}; }
+__device__ __forceinline__ uint64_t bits(Two<float> v) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.a), "f"(v.b));
+    return r;
+}
+__device__ __forceinline__ Two<float> pair_of(uint64_t r) {
+    Two<float> v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.a), "=f"(v.b) : "l"(r));
+    return v;
+}
+__device__ __forceinline__ Two<float> add(Two<float> x, Two<float> y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(x)), "l"(bits(y)));
+    return pair_of(r);
+}
+__device__ __forceinline__ Two<float> mul(Two<float> x, Two<float> y) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(x)), "l"(bits(y)));
+    return pair_of(r);
+}
+__device__ __forceinline__ Two<float> fma(Two<float> x, Two<float> y, Two<float> z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(x)), "l"(bits(y)), "l"(bits(z)));
+    return pair_of(r);
+}
+__device__ __forceinline__ Two<double> add(Two<double> x, Two<double> y) { return {x.a + y.a, x.b + y.b}; }
+__device__ __forceinline__ Two<double> mul(Two<double> x, Two<double> y) { return {x.a * y.a, x.b * y.b}; }
+__device__ __forceinline__ Two<double> fma(Two<double> x, Two<double> y, Two<double> z) { return {::fma(x.a, y.a, z.a), ::fma(x.b, y.b, z.b)}; }
+
+// Elements 2k and 2k + 1 of a thread's ITEMS vectors.
+template <typename S, typename T, int VEC, int N>
+__device__ __forceinline__ Two<S> two_of(const Pack<T, VEC> (&p)[N], int k) {
+    return {to_compute<S>(p[2 * k / VEC].v[2 * k % VEC]), to_compute<S>(p[(2 * k + 1) / VEC].v[(2 * k + 1) % VEC])};
+}
+
 constexpr int kMost = 512;       // threads of a block that holds one row
 constexpr int kRowWarps = 4;     // warps of a block whose warps hold a row each
 
@@ -92,12 +131,14 @@ __device__ __forceinline__ void row_sums(S (&v)[NV], S* slots) {
             for (int k = 0; k < NV; ++k) slots[(threadIdx.x >> 5) * NV + k] = v[k];
         }
         __syncthreads();
-        const int warps = blockDim.x >> 5;
+        static_assert(kMost <= 512, "sixteen warps");
+        const int w = threadIdx.x & 15;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) v[k] = slots[k];
-        for (int w = 1; w < warps; ++w) {
+        for (int k = 0; k < NV; ++k) v[k] = w < static_cast<int>(blockDim.x >> 5) ? slots[w * NV + k] : S(0);
 #pragma unroll
-            for (int k = 0; k < NV; ++k) v[k] += slots[w * NV + k];
+        for (int o = 8; o > 0; o >>= 1) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) v[k] += __shfl_xor_sync(0xFFFFFFFFu, v[k], o);
         }
     }
 }
@@ -153,6 +194,7 @@ template <typename T, typename P, int VEC, int ITEMS, int DEPTH, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_forward(const NormArgs a) {
     using S = typename stat_of<T>::type;
     using In = Ring<T, VEC, ITEMS, 1, DEPTH>;
+    constexpr int E = VEC * ITEMS;
     __shared__ S slots[2][BLOCK ? kMost / 32 : 1];
     extern __shared__ __align__(16) uint8_t dynamic[];
     const Place<BLOCK> at;
@@ -193,29 +235,33 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_forwar
             fetch(row + (DEPTH - 1) * at.step, ring.slot == 0 ? DEPTH - 1 : ring.slot - 1);
             In::wait();
         }
-        S v[ITEMS * VEC], sum[1] = {0};
+        Pack<T, VEC> p[ITEMS];
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            Pack<T, VEC> p;
-            if (inside(i)) p = In::kAsync ? *ring.at(ring.slot, 0, i) : ahead[In::kAsync ? 0 : i];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[i * VEC + j] = inside(i) ? to_compute<S>(p.v[j]) : S(0);
+            for (int j = 0; j < VEC; ++j) p[i].v[j] = T(0.0f);
+            if (inside(i)) p[i] = In::kAsync ? *ring.at(ring.slot, 0, i) : ahead[In::kAsync ? 0 : i];
+        }
+        Two<S> v[E / 2], pair = both(S(0));
+#pragma unroll
+        for (int k = 0; k < E / 2; ++k) {
+            v[k] = two_of<S>(p, k);
+            pair = add(pair, v[k]);
         }
         if constexpr (!In::kAsync) fetch(row + at.step, 0);
-#pragma unroll
-        for (int e = 0; e < ITEMS * VEC; ++e) sum[0] += v[e];
+        S sum[1] = {pair.a + pair.b};
         row_sums<S, 1, BLOCK>(sum, slots[0]);
         const S mean = sum[0] * share;
-        sum[0] = 0;
+        pair = both(S(0));
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (inside(i)) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    v[i * VEC + j] -= mean;
-                    sum[0] += v[i * VEC + j] * v[i * VEC + j];
-                }
-            }
+        for (int k = 0; k < E / 2; ++k) {
+            v[k] = add(v[k], both(-mean));
+            // what lies behind the row's end is not mean away from it
+            if (!inside(2 * k / VEC)) v[k].a = S(0);
+            if (!inside((2 * k + 1) / VEC)) v[k].b = S(0);
+            pair = fma(v[k], v[k], pair);
+        }
+        sum[0] = pair.a + pair.b;
         row_sums<S, 1, BLOCK>(sum, slots[1]);
         const S rstd = inverse_root(sum[0] * share + static_cast<S>(a.eps));
         if (at.t == 0) {
@@ -224,14 +270,14 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_forwar
         }
         Pack<T, VEC>* y = reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.y) + row * a.cols);
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            if (inside(i)) {
-                Pack<T, VEC> out;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) out.v[j] = from_compute<T, S>(v[i * VEC + j] * rstd * to_compute<S>(w[i].v[j]) + to_compute<S>(b[i].v[j]));
-                y[i * at.threads + at.t] = out;
-            }
+        for (int k = 0; k < E / 2; ++k) {
+            const Two<S> r = fma(mul(v[k], both(rstd)), two_of<S>(w, k), two_of<S>(b, k));
+            p[2 * k / VEC].v[2 * k % VEC] = from_compute<T, S>(r.a);
+            p[(2 * k + 1) / VEC].v[(2 * k + 1) % VEC] = from_compute<T, S>(r.b);
         }
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (inside(i)) y[i * at.threads + at.t] = p[i];
         ring.next();
     }
 }
@@ -248,9 +294,9 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_backwa
     In ring(dynamic);
     const int vecs = a.cols / VEC;
     const S share = S(1) / static_cast<S>(a.cols);
-    S dw[E], db[E];
+    Two<S> dw[E / 2], db[E / 2];
 #pragma unroll
-    for (int e = 0; e < E; ++e) dw[e] = db[e] = 0;
+    for (int k = 0; k < E / 2; ++k) dw[k] = db[k] = both(S(0));
     auto inside = [&](int i) { return i * at.threads + at.t < vecs; };
     auto weight_at = [&](int i) {
         Pack<P, VEC> p;
@@ -294,11 +340,25 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_backwa
             pd = (reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dy) + r * a.dy_pitch) + at.t)[i * at.threads];
         }
     };
-    Pack<P, VEC> w[KEEP ? ITEMS : 1];
+    // The work goes G vectors at a time, an even number of elements.
+    constexpr int G = VEC > 1 ? 1 : 2, PAIRS = G * VEC / 2;
+    auto weights = [&](int i0, Pack<P, VEC> (&p)[G]) {
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) p[i].v[j] = P(0.0f);
+            if (inside(i0 + i)) p[i] = weight_at(i0 + i);
+        }
+    };
+    Two<S> w[KEEP ? E / 2 : 1];
     if constexpr (KEEP) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (inside(i)) w[i] = weight_at(i);
+        for (int i0 = 0; i0 < ITEMS; i0 += G) {
+            Pack<P, VEC> p[G];
+            weights(i0, p);
+#pragma unroll
+            for (int k = 0; k < PAIRS; ++k) w[i0 * VEC / 2 + k] = two_of<S>(p, k);
+        }
     }
     S mean = 0, rstd = 0;
     auto statistics = [&](int64_t r) {
@@ -316,56 +376,73 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_backwa
         const S mu = mean, rs = rstd;
         statistics(row + at.step);
         In::wait();
-        S z[KEEP ? E : 1], g[KEEP ? E : 1];
-        S sums[2] = {0, 0};
+        auto read = [&](int i0, Pack<T, VEC> (&px)[G], Pack<T, VEC> (&pd)[G]) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (inside(i)) {
-                Pack<T, VEC> px, pd;
-                load(row, i, px, pd);
-                const Pack<P, VEC> pw = KEEP ? w[KEEP ? i : 0] : weight_at(i);
+            for (int i = 0; i < G; ++i) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const int e = i * VEC + j;
-                    const S zz = (to_compute<S>(px.v[j]) - mu) * rs, d = to_compute<S>(pd.v[j]), gg = d * to_compute<S>(pw.v[j]);
-                    sums[0] += gg;
-                    sums[1] += gg * zz;
-                    dw[e] += d * zz;
-                    db[e] += d;
-                    if constexpr (KEEP) {
-                        z[e] = zz;
-                        g[e] = gg;
-                    }
-                }
+                for (int j = 0; j < VEC; ++j) px[i].v[j] = pd[i].v[j] = T(0.0f);  // behind the row's end: no gradient
+                if (inside(i0 + i)) load(row, i0 + i, px[i], pd[i]);
             }
+        };
+        Two<S> c[KEEP ? E / 2 : 1], g[KEEP ? E / 2 : 1];  // x - mean and dy * weight
+        Two<S> sum_g = both(S(0)), sum_gc = both(S(0));
+#pragma unroll
+        for (int i0 = 0; i0 < ITEMS; i0 += G) {
+            Pack<T, VEC> px[G], pd[G];
+            Pack<P, VEC> pw[G];
+            read(i0, px, pd);
+            if constexpr (!KEEP) weights(i0, pw);
+#pragma unroll
+            for (int k = 0; k < PAIRS; ++k) {
+                const int at_k = i0 * VEC / 2 + k;
+                const Two<S> d = two_of<S>(pd, k), cc = add(two_of<S>(px, k), both(-mu));
+                Two<S> gg;
+                if constexpr (KEEP) {
+                    gg = mul(d, w[at_k]);
+                    c[at_k] = cc;
+                    g[at_k] = gg;
+                } else {
+                    gg = mul(d, two_of<S>(pw, k));
+                }
+                sum_g = add(sum_g, gg);
+                sum_gc = fma(gg, cc, sum_gc);
+                dw[at_k] = fma(mul(cc, both(rs)), d, dw[at_k]);
+                db[at_k] = add(db[at_k], d);
+            }
+        }
         if constexpr (AHEAD) fetch(row + at.step, 0);
+        S sums[2] = {sum_g.a + sum_g.b, (sum_gc.a + sum_gc.b) * rs};
         row_sums<S, 2, BLOCK>(sums, slots[parity]);
-        const S mean_g = sums[0] * share, mean_gz = sums[1] * share;
+        // dx = r (g - mean(g)) - (x - mean) r^2 mean(g z)
+        const Two<S> by_g = both(rs), by_c = both(-rs * rs * (sums[1] * share)), shift = both(-rs * (sums[0] * share));
         Pack<T, VEC>* dx = reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.y) + row * a.cols);
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (inside(i)) {
-                Pack<T, VEC> px, pd, out;
-                Pack<P, VEC> pw;
-                if constexpr (!KEEP) {
-                    load(row, i, px, pd);
-                    pw = weight_at(i);
-                }
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const int e = i * VEC + j;
-                    S zz, gg;
-                    if constexpr (KEEP) {
-                        zz = z[e];
-                        gg = g[e];
-                    } else {
-                        zz = (to_compute<S>(px.v[j]) - mu) * rs;
-                        gg = to_compute<S>(pd.v[j]) * to_compute<S>(pw.v[j]);
-                    }
-                    out.v[j] = from_compute<T, S>((gg - mean_g - zz * mean_gz) * rs);
-                }
-                dx[i * at.threads + at.t] = out;
+        for (int i0 = 0; i0 < ITEMS; i0 += G) {
+            Pack<T, VEC> px[G], pd[G];
+            Pack<P, VEC> pw[G];
+            if constexpr (!KEEP) {
+                read(i0, px, pd);
+                weights(i0, pw);
             }
+#pragma unroll
+            for (int k = 0; k < PAIRS; ++k) {
+                const int at_k = i0 * VEC / 2 + k;
+                Two<S> cc, gg;
+                if constexpr (KEEP) {
+                    cc = c[at_k];
+                    gg = g[at_k];
+                } else {
+                    cc = add(two_of<S>(px, k), both(-mu));
+                    gg = mul(two_of<S>(pd, k), two_of<S>(pw, k));
+                }
+                const Two<S> r = fma(cc, by_c, fma(gg, by_g, shift));
+                px[2 * k / VEC].v[2 * k % VEC] = from_compute<T, S>(r.a);
+                px[(2 * k + 1) / VEC].v[(2 * k + 1) % VEC] = from_compute<T, S>(r.b);
+            }
+#pragma unroll
+            for (int i = 0; i < G; ++i)
+                if (inside(i0 + i)) dx[(i0 + i) * at.threads + at.t] = px[i];
+        }
         ring.next();
     }
     if (a.partial == nullptr) return;  // uniform: no parameter gradients wanted
@@ -381,8 +458,9 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_backwa
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) {
                         const int c = (i * at.threads + at.t) * VEC + j, e = i * VEC + j;
-                        all[c] = k ? all[c] + dw[e] : dw[e];
-                        all[a.cols + c] = k ? all[a.cols + c] + db[e] : db[e];
+                        const S one = e % 2 ? dw[e / 2].b : dw[e / 2].a, two = e % 2 ? db[e / 2].b : db[e / 2].a;
+                        all[c] = k ? all[c] + one : one;
+                        all[a.cols + c] = k ? all[a.cols + c] + two : two;
                     }
                 }
         }
@@ -472,26 +550,26 @@ __global__ void __launch_bounds__(256) norm_columns_long(const NormArgs a) {
     mine[a.cols + c] = db;
 }
 
-// Adds the partial rows, in an order that depends on their number only: eight columns (a sector of 32 bytes) per block and 128 threads
-// a column, so that a few hundred rows are two or three loads a thread, all in flight.
-template <typename S, typename P>
+// Adds the partial rows, in an order that depends on their number only. COLS columns per block and 1024 / COLS threads a column: 8 (a
+// sector of 32 bytes, two or three loads a thread for a few hundred rows), 32 where that is blocks enough.
+template <typename S, typename P, int COLS>
 __global__ void __launch_bounds__(1024) norm_parameters(const S* __restrict__ partial, int blocks, int cols, P* __restrict__ dweight, P* __restrict__ dbias) {
-    __shared__ S part[32][8];
+    __shared__ S part[32][COLS + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // columns [0, cols) are the weight's, [cols, 2 cols) the bias's
-    const int64_t all = static_cast<int64_t>(cols) * 2, c = static_cast<int64_t>(blockIdx.x) * 8 + (lane & 7);
+    const int64_t all = static_cast<int64_t>(cols) * 2, c = static_cast<int64_t>(blockIdx.x) * COLS + lane % COLS;
     S sum = 0;
     if (c < all) {
 #pragma unroll 4
-        for (int b = threadIdx.x >> 3; b < blocks; b += 128) sum += partial[static_cast<int64_t>(b) * all + c];
+        for (int b = threadIdx.x / COLS; b < blocks; b += 1024 / COLS) sum += partial[static_cast<int64_t>(b) * all + c];
     }
-    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
-    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
-    if (lane < 8) part[warp][lane] = sum;
+#pragma unroll
+    for (int o = COLS; o < 32; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if (lane < COLS) part[warp][lane] = sum;
     __syncthreads();
-    if (warp >= 8) return;
+    if (warp >= COLS) return;
     sum = warp_sum(part[lane][warp]);  // column `warp`
-    const int64_t out = static_cast<int64_t>(blockIdx.x) * 8 + warp;
+    const int64_t out = static_cast<int64_t>(blockIdx.x) * COLS + warp;
     if (lane == 0 && out < all) {
         if (out < cols) {
             if (dweight) dweight[out] = from_compute<P, S>(sum);
@@ -523,7 +601,9 @@ tn_status alloc_partial(Launch& l, int64_t blocks) {
 template <typename S, typename P>
 tn_status finish_partial(Launch& l, int64_t blocks) {
     if (!l.args.partial) return TN_SUCCESS;
-    norm_parameters<S, P><<<(unsigned)ceil_div(2 * (int64_t)l.args.cols, 8), 1024, 0, l.stream>>>(
+    const int64_t all = 2 * (int64_t)l.args.cols;
+    const bool many = all >= 32 * (int64_t)sm_count();
+    (many ? norm_parameters<S, P, 32> : norm_parameters<S, P, 8>)<<<(unsigned)ceil_div(all, many ? 32 : 8), 1024, 0, l.stream>>>(
         static_cast<const S*>(l.args.partial), (int)blocks, l.args.cols, static_cast<P*>(l.dweight), static_cast<P*>(l.dbias));
     return after_launch("norm_parameters");
 }
