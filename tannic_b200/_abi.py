@@ -85,6 +85,7 @@ class TannicError(RuntimeError):
 
 
 _TP = C.POINTER(TensorT)
+_RP = C.c_void_p  # a record by address: byref(TensorT), or its bytes, which are cheaper to make
 _UNARY = ["neg", "repack", "log", "exp", "sqrt", "abs", "sin", "cos", "tan", "sinh", "cosh", "tanh"]
 _BINARY = ["add", "sub", "mul", "pow", "eq", "ne", "gt", "ge", "lt", "le"]
 _REDUCE = ["argmax", "argmin", "argsum", "argmean", "max"]
@@ -139,10 +140,10 @@ PROTOTYPES = {
     "tn_view_as_polar": [_TP, _TP, _TP, StreamT],
     "tn_reduce_stats": [_TP, _TP, _TP, _TP, StreamT, C.c_uint8],
     "tn_argsum_fixed_scratch": [_TP, _TP, StreamT, C.c_uint8],
-    "tn_layer_norm": [_TP, _TP, _TP, _TP, _TP, _TP, StreamT, C.c_double],
-    "tn_layer_norm_grad": [_TP, _TP, _TP, _TP, _TP, _TP, _TP, _TP, StreamT],
-    "tn_linear_cross_entropy": [_TP, _TP, _TP, _TP, _TP, StreamT, C.c_int64],
-    "tn_linear_cross_entropy_grad": [_TP, _TP, _TP, _TP, _TP, _TP, _TP, StreamT, C.c_int64],
+    "tn_layer_norm": [_RP] * 6 + [StreamT, C.c_double],
+    "tn_layer_norm_grad": [_RP] * 8 + [StreamT],
+    "tn_linear_cross_entropy": [_RP] * 5 + [StreamT, C.c_int64],
+    "tn_linear_cross_entropy_grad": [_RP] * 7 + [StreamT, C.c_int64],
     "tn_cpy": [_TP, _TP, StreamT],
     "tn_allclose": [_TP, _TP, StreamT, C.c_double, C.c_double, C.POINTER(C.c_int)],
     "tn_device_errors": [C.POINTER(C.c_uint)],

@@ -648,7 +648,7 @@ tn_status launch_forward(Launch& l) {
 template <typename T, typename P, int VEC, int ITEMS, bool BLOCK, bool KEEP>
 tn_status launch_backward(Launch& l) {
     using S = typename stat_of<T>::type;
-    constexpr int DEPTH = !KEEP && sizeof(T) == 4 ? 1 : 3;  // one row of 16384 float32 twice is 128 KiB
+    constexpr int DEPTH = !KEEP ? (sizeof(T) == 4 ? 1 : 3) : sizeof(T) * VEC * ITEMS * 2 <= 96 ? 5 : 3;  // one row of 16384 float32 twice is 128 KiB
     NormArgs& a = l.args;
     const int threads = block_threads<T, VEC, ITEMS, BLOCK>(a.cols);
     size_t smem = Ring<T, VEC, ITEMS, 2, DEPTH>::kAsync ? sizeof(T) * VEC * ITEMS * 2 * DEPTH * (size_t)threads : 0;

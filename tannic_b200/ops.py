@@ -39,10 +39,19 @@ def _geometry(shape, strides, dtype, device: int) -> bytes:
     return record[A.TensorT.address.offset + A.TensorT.address.size:]
 
 
+def _record(t: torch.Tensor | None) -> bytes | None:
+    """The bytes of `desc(t)`, for entry points that take records by address; a null pointer for None."""
+    if t is None:
+        return None
+    if t.is_cuda:
+        return t.data_ptr().to_bytes(8, "little") + _geometry(t.shape, t.stride(), t.dtype, t.get_device())
+    return bytes(desc(t))
+
+
 def desc(t: torch.Tensor) -> A.TensorT:
     """tn_tensor_t over a torch tensor's storage (CUDA -> DEVICE environment, CPU -> HOST)."""
     if t.is_cuda:
-        return A.TensorT.from_buffer_copy(t.data_ptr().to_bytes(8, "little") + _geometry(t.shape, t.stride(), t.dtype, t.get_device()))
+        return A.TensorT.from_buffer_copy(_record(t))
     if t.dtype not in TORCH_TO_TN:
         raise A.TannicError(A.UNSUPPORTED_DTYPE, f"torch dtype {t.dtype} has no Tannic equivalent")
     return A.make_tensor(t.data_ptr(), tuple(t.shape), tuple(t.stride()), TORCH_TO_TN[t.dtype], None, pinned=t.is_pinned())
@@ -482,9 +491,9 @@ def reduce_stats(x: torch.Tensor, axis=-1, keepdim=False):
     return mx, sm, am
 
 
-def _ref(t: torch.Tensor | None):
-    """A record to pass by reference, or a null pointer."""
-    return None if t is None else C.byref(desc(t))
+def _dense_like(t: torch.Tensor) -> torch.Tensor:
+    """A dense tensor of t's shape and dtype, by torch's cheapest call for it."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5, stats: bool = False,
@@ -495,12 +504,12 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     if x.dim() == 0:
         raise ValueError("cannot normalise a rank-0 tensor")
     if out is None:
-        out = x.new_empty(x.shape)
+        out = _dense_like(x)
     mean = rstd = None
     if stats:
-        wide = torch.float64 if x.dtype == torch.float64 else torch.float32
-        mean, rstd = x.new_empty(x.shape[:-1], dtype=wide), x.new_empty(x.shape[:-1], dtype=wide)
-    A.check(A.lib().tn_layer_norm(_ref(x), _ref(weight), _ref(bias), _ref(out), _ref(mean), _ref(rstd), current_stream(x), eps))
+        mean = x.new_empty(x.shape[:-1], dtype=torch.float64 if x.dtype == torch.float64 else torch.float32)
+        rstd = torch.empty_like(mean)
+    A.check(A.lib().tn_layer_norm(_record(x), _record(weight), _record(bias), _record(out), _record(mean), _record(rstd), current_stream(x), eps))
     return (out, mean, rstd) if stats else out
 
 
@@ -509,10 +518,11 @@ def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd:
     `weight` the normalisation has no parameters and dweight and dbias are None; `bias=False`: it has no bias."""
     if x.dim() == 0:
         raise ValueError("cannot normalise a rank-0 tensor")
-    dx = x.new_empty(x.shape)
-    dweight = weight.new_empty(weight.shape) if weight is not None else None
-    dbias = weight.new_empty(weight.shape) if weight is not None and bias else None
-    A.check(A.lib().tn_layer_norm_grad(_ref(dy), _ref(x), _ref(mean), _ref(rstd), _ref(weight), _ref(dx), _ref(dweight), _ref(dbias), current_stream(x)))
+    dx = _dense_like(x)
+    dweight = _dense_like(weight) if weight is not None else None
+    dbias = _dense_like(weight) if weight is not None and bias else None
+    A.check(A.lib().tn_layer_norm_grad(_record(dy), _record(x), _record(mean), _record(rstd), _record(weight), _record(dx), _record(dweight),
+                                       _record(dbias), current_stream(x)))
     return dx, dweight, dbias
 
 
@@ -520,8 +530,10 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     """(loss, lse): the softmax cross entropy of the logits hidden . weight^T with `targets`, one float32 per token, and
     the logits' log-sum-exp, which `linear_cross_entropy_grad` reads (tn_linear_cross_entropy). The logits are not
     written. Tokens whose target is `ignore_index` have loss 0."""
-    loss, lse = hidden.new_empty(targets.shape, dtype=torch.float32), hidden.new_empty(targets.shape, dtype=torch.float32)
-    A.check(A.lib().tn_linear_cross_entropy(_ref(hidden), _ref(weight), _ref(targets), _ref(loss), _ref(lse), current_stream(hidden), ignore_index))
+    loss = hidden.new_empty(targets.shape, dtype=torch.float32)
+    lse = torch.empty_like(loss)
+    A.check(A.lib().tn_linear_cross_entropy(_record(hidden), _record(weight), _record(targets), _record(loss), _record(lse), current_stream(hidden),
+                                            ignore_index))
     return loss, lse
 
 
@@ -530,10 +542,10 @@ def linear_cross_entropy_grad(grad: torch.Tensor, hidden: torch.Tensor, weight: 
     """(dhidden, dweight) of `linear_cross_entropy` from `grad`, the gradient of every token's loss (for the mean over the
     tokens that count: 1 / their number, expanded), and its lse (tn_linear_cross_entropy_grad). `dhidden=False` or
     `dweight=False` leaves that one out (None): a frozen trunk, a frozen head."""
-    dh = hidden.new_empty(hidden.shape) if dhidden else None
-    dw = weight.new_empty(weight.shape) if dweight else None
-    A.check(A.lib().tn_linear_cross_entropy_grad(_ref(grad), _ref(hidden), _ref(weight), _ref(targets), _ref(lse), _ref(dh), _ref(dw),
-                                                 current_stream(hidden), ignore_index))
+    dh = _dense_like(hidden) if dhidden else None
+    dw = _dense_like(weight) if dweight else None
+    A.check(A.lib().tn_linear_cross_entropy_grad(_record(grad), _record(hidden), _record(weight), _record(targets), _record(lse), _record(dh),
+                                                 _record(dw), current_stream(hidden), ignore_index))
     return dh, dw
 
 
