@@ -39,6 +39,7 @@
 // The register split that takes is 40 a thread for warps 0..3 and 232 for the others, of 384 x 168 at launch.
 #include <algorithm>
 
+#include "linear_loss.cuh"
 #include "tc_common.cuh"
 
 namespace tnb {
@@ -979,6 +980,31 @@ Problem make_problem(const tn_tensor_t* hidden, const tn_tensor_t* weight, tn_st
     return p;
 }
 
+// Joins `n` groups of logits per row into lse and loss.
+tn_status join(const Problem& p, const float2* halves, int64_t n, const float* target_logit, const void* targets, int wide, int64_t ignore, tn_tensor_t* loss, tn_tensor_t* lse) {
+    const bool few = p.tokens <= 2 * sm_count();  // a block per row fills the GPU at most once
+    (few ? loss_join<1> : loss_join<32>)<<<(unsigned)ceil_div(p.tokens, few ? 1 : 32), 1024, 0, p.stream>>>(
+        halves, n, p.tokens, target_logit, targets, wide, ignore, p.vocab, loss ? static_cast<float*>(loss->address) : nullptr,
+        lse ? static_cast<float*>(lse->address) : nullptr);
+    return after_launch("loss_join");
+}
+
+FewTokens few_tokens(const Problem& p, const RowsIn& h, const RowsIn& w, const void* targets, int wide, int64_t ignore) {
+    FewTokens f;
+    f.dtype = p.dtype;
+    f.tokens = p.tokens;
+    f.hidden = p.hidden;
+    f.vocab = p.vocab;
+    f.h = h.base;
+    f.h_pitch = h.pitch;
+    f.w = w.base;
+    f.w_pitch = w.pitch;
+    f.targets = targets;
+    f.wide = wide;
+    f.ignore = ignore;
+    return f;
+}
+
 tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const tn_tensor_t* targets, tn_tensor_t* loss, tn_tensor_t* lse, tn_stream_t stream,
                    int64_t ignore, Scratch& mem) {
     const Problem p = make_problem(hidden, weight, stream);
@@ -987,6 +1013,18 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
     TN_TRY(rows_in(hidden, &h, mem, stream));
     TN_TRY(rows_in(weight, &w, mem, stream));
     TN_TRY(densely(targets, &t, mem, stream));
+    const int wide = targets->dtype == TN_INT64;
+    float2* halves = nullptr;
+    float* target_logit = nullptr;
+    TN_TRY(mem.take(&target_logit, sizeof(float) * p.tokens));
+    if (few_loss_fits(p.tokens, p.hidden)) {
+        FewTokens f = few_tokens(p, h, w, t, wide, ignore);
+        TN_TRY(mem.take(&halves, sizeof(float2) * (size_t)few_loss_parts() * p.tokens));
+        f.parts = halves;
+        f.target_logit = target_logit;
+        TN_TRY(few_loss(f, p.stream));
+        return join(p, halves, few_loss_parts(), target_logit, t, wide, ignore, loss, lse);
+    }
     Operand a;
     a.parts = p.parts;
     if (in_place(p, h, p.tokens)) {
@@ -1006,10 +1044,7 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
     if (packed) TN_TRY(mem.take(&room, (size_t)p.parts * piece * p.padded * 2));
     int64_t tiles = 0;
     for (int64_t v0 = 0; v0 < p.vocab; v0 += piece) tiles += ceil_div(std::min(piece, p.vocab - v0), BN);
-    float2* halves = nullptr;
-    float* target_logit = nullptr;
     TN_TRY(mem.take(&halves, sizeof(float2) * 2 * (size_t)tiles * p.tokens));
-    TN_TRY(mem.take(&target_logit, sizeof(float) * p.tokens));
     CUtensorMap map_a, map_b;
     TN_TRY(operand_map(&map_a, a, p.bf16, p.hidden, p.tokens, BK, BM));
     int64_t first_half = 0;
@@ -1021,18 +1056,14 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
         LossArgs g = gemm_args(p, p.tokens, n, p.hidden);
         g.vocab0 = v0;
         g.targets = t;
-        g.wide_targets = targets->dtype == TN_INT64;
+        g.wide_targets = wide;
         g.halves = halves;
         g.first_half = first_half;
         g.target_logit = target_logit;
         TN_TRY((launch_one<false, false, EPI_STATS, __half, float, 1, true>(map_a, map_b, map_a, g, p.stream)));
         first_half += 2 * (int64_t)g.n_tiles;
     }
-    const bool few = p.tokens <= 2 * sm_count();  // a block per row fills the GPU at most once
-    (few ? loss_join<1> : loss_join<32>)<<<(unsigned)ceil_div(p.tokens, few ? 1 : 32), 1024, 0, p.stream>>>(
-        halves, first_half, p.tokens, target_logit, t, targets->dtype == TN_INT64, ignore, p.vocab, loss ? static_cast<float*>(loss->address) : nullptr,
-        lse ? static_cast<float*>(lse->address) : nullptr);
-    return after_launch("loss_join");
+    return join(p, halves, first_half, target_logit, t, wide, ignore, loss, lse);
 }
 
 template <typename T, typename OUT, int PARTS>
@@ -1046,6 +1077,18 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
     TN_TRY(densely(targets, &t, mem, stream));
     TN_TRY(densely(grad, &up, mem, stream));
     TN_TRY(densely(lse, &z, mem, stream));
+    const int wide = targets->dtype == TN_INT64;
+    if (few_grad_fits(p.tokens, p.hidden)) {
+        FewTokens f = few_tokens(p, h, w, t, wide, ignore);
+        f.grad = static_cast<const float*>(up);
+        f.lse = static_cast<const float*>(z);
+        if (dhidden) {
+            TN_TRY(mem.take(&f.sums, sizeof(float) * (size_t)few_grad_blocks(p.vocab) * p.tokens * p.hidden));
+            f.dhidden = dhidden->address;
+        }
+        f.dweight = dweight ? dweight->address : nullptr;
+        return few_grad(f, p.stream);
+    }
     RowInfo* info = nullptr;
     int *slot = nullptr, *count = nullptr;
     TN_TRY(mem.take(&info, sizeof(RowInfo) * p.tokens));
@@ -1053,7 +1096,7 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
     TN_TRY(mem.take(&count, 2 * sizeof(int)));
     float* scale = reinterpret_cast<float*>(count + 1);
     const int per_block = (int)std::min<int64_t>(256, std::max<int64_t>(8, ceil_div(p.tokens, 1024)));
-    loss_rows<<<(unsigned)ceil_div(p.tokens, per_block), 256, 0, p.stream>>>(t, targets->dtype == TN_INT64, p.tokens, static_cast<const float*>(up), static_cast<const float*>(z),
+    loss_rows<<<(unsigned)ceil_div(p.tokens, per_block), 256, 0, p.stream>>>(t, wide, p.tokens, static_cast<const float*>(up), static_cast<const float*>(z),
                                                                             ignore, p.vocab, per_block, info, slot, count, scale);
     TN_TRY(after_launch("loss_rows"));
     uint16_t* gathered = nullptr;
