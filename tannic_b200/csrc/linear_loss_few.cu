@@ -146,18 +146,20 @@ constexpr int kGradThreads = 512;
 constexpr int E = 8;  // columns of a thread
 
 template <typename T, int VEC> constexpr int kGradRows = VEC > 1 && sizeof(T) == 2 ? 8 : 4;
-constexpr int kDepth = 3;  // batches of rows in shared memory: one in use, two on their way
+constexpr int kDepth = 3;  // batches of rows in shared memory: two in use, one on its way
 
+// One barrier a batch: between two of them a warp forms its part of the next batch's logits and does everything else of this
+// batch's, so that the chain logits - exponential - products of one batch runs under the other's.
 template <typename T, int VEC, int NT>
 __global__ void __launch_bounds__(kGradThreads, 1) few_grad_kernel(const FewTokens p) {
-    constexpr int ITEMS = E / VEC, R = kGradRows<T, VEC>, V = R * NT, SHIFT = 5 - kLog2<V>;
-    constexpr bool RING = VEC > 1;
+    constexpr int ITEMS = E / VEC, R = kGradRows<T, VEC>, V = R * NT, SHIFT = 5 - kLog2<V>, WARPS = kGradThreads / 32;
+    constexpr bool RING = VEC > 1;  // else the rows are read from memory twice, the second time from L1 or L2
     using P = Pack<T, VEC>;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float part[2][kGradThreads / 32][32];
-    __shared__ __align__(16) float dvals[kGradThreads / 32][32];
-    P* ring = reinterpret_cast<P*>(smem);  // [kDepth][R][ITEMS][threads]
-    const int t = threadIdx.x, threads = blockDim.x, lane = t & 31, warp = t >> 5, warps = threads >> 5;
+    __shared__ float part[2][WARPS][32];
+    __shared__ __align__(16) float dvals[WARPS][32];
+    const int t = threadIdx.x, threads = blockDim.x, lane = t & 31, warp = t >> 5;
+    P* ring = reinterpret_cast<P*>(smem) + t;  // [kDepth][R][ITEMS][threads]
     const int vecs = static_cast<int>(p.hidden / VEC);
     auto inside = [&](int i) { return i * threads + t < vecs; };
 
@@ -185,58 +187,61 @@ __global__ void __launch_bounds__(kGradThreads, 1) few_grad_kernel(const FewToke
     counts = counts && target != p.ignore;
     const float lse = counts ? p.lse[token] : 0.0f;
     const float grad = !counts ? 0.0f : target < 0 || target >= p.vocab ? NAN : p.grad[token];
+    // absent warps add nothing; columns behind the row's end are zero and stay so
+    for (int i = t; i < 2 * WARPS * 32; i += threads) (&part[0][0][0])[i] = 0.0f;
+    if constexpr (RING) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (!inside(i))
+                for (int k = 0; k < kDepth * R; ++k)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) ring[(k * ITEMS + i) * threads].v[j] = T(0.0f);
+    }
+    __syncthreads();
 
     const int64_t step = static_cast<int64_t>(gridDim.x) * R;
-    auto row_at = [&](int64_t v, int i) { return reinterpret_cast<const P*>(static_cast<const T*>(p.w) + v * p.w_pitch) + i * threads + t; };
-    auto slot_at = [&](int s, int r, int i) { return ring + ((s * R + r) * ITEMS + i) * threads + t; };
+    // rows behind the last one are read as the last one; their d is zero and nothing is written for them
+    auto row_at = [&](int64_t v) { return reinterpret_cast<const P*>(static_cast<const T*>(p.w) + min(v, p.vocab - 1) * p.w_pitch) + t; };
     auto fetch = [&](int64_t v0, int s) {
         if constexpr (RING) {
+            if (v0 < p.vocab) {
 #pragma unroll
-            for (int r = 0; r < R; ++r)
+                for (int r = 0; r < R; ++r) {
+                    const P* from = row_at(v0 + r);
 #pragma unroll
-                for (int i = 0; i < ITEMS; ++i)
-                    if (v0 + r < p.vocab && inside(i)) {
-                        const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(slot_at(s, r, i)));
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(row_at(v0 + r, i)) : "memory");
-                    }
+                    for (int i = 0; i < ITEMS; ++i)
+                        if (inside(i)) {
+                            const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(ring + ((s * R + r) * ITEMS + i) * threads));
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from + i * threads) : "memory");
+                        }
+                }
+            }
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
     };
-    int64_t v0 = static_cast<int64_t>(blockIdx.x) * R;
+    // this thread's columns of row r of the batch at v0, in slot s
+    auto row = [&](int64_t v0, int s, int r, float2 (&x)[E / 2]) {
+        P q[ITEMS];
 #pragma unroll
-    for (int d = 0; d < kDepth - 1; ++d) fetch(v0 + d * step, d);
-    int slot = 0, parity = 0;
-    for (; v0 < p.vocab; v0 += step, parity ^= 1) {
-        // a thread reads what it copied itself, and the slot before this one is what it read last
-        fetch(v0 + (kDepth - 1) * step, slot == 0 ? kDepth - 1 : slot - 1);
-        if constexpr (RING) asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
-        P direct[RING ? 1 : R][RING ? 1 : ITEMS];
-        if constexpr (!RING) {
+        for (int i = 0; i < ITEMS; ++i) {
+            if constexpr (RING) {
+                q[i] = ring[((s * R + r) * ITEMS + i) * threads];
+            } else {
 #pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int i = 0; i < ITEMS; ++i)
-                    if (v0 + r < p.vocab && inside(i)) direct[r][i] = *row_at(v0 + r, i);
-        }
-        // this thread's columns of row r, zero where there is none
-        auto row = [&](int r, float2 (&x)[E / 2]) {
-            float y[E];
-#pragma unroll
-            for (int i = 0; i < ITEMS; ++i) {
-                const bool in = v0 + r < p.vocab && inside(i);
-                P q;
-                if (in) q = RING ? *slot_at(slot, r, i) : direct[RING ? 0 : r][RING ? 0 : i];
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) y[i * VEC + j] = in ? to_compute<float>(q.v[j]) : 0.0f;
+                for (int j = 0; j < VEC; ++j) q[i].v[j] = T(0.0f);
+                if (inside(i)) q[i] = row_at(v0 + r)[i * threads];
             }
+        }
 #pragma unroll
-            for (int k = 0; k < E / 2; ++k) x[k] = make_float2(y[2 * k], y[2 * k + 1]);
-        };
+        for (int k = 0; k < E / 2; ++k)
+            x[k] = make_float2(to_compute<float>(q[2 * k / VEC].v[2 * k % VEC]), to_compute<float>(q[(2 * k + 1) / VEC].v[(2 * k + 1) % VEC]));
+    };
+    auto logits = [&](int64_t v0, int s, int to) {
         float dots[V];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             float2 x[E / 2];
-            row(r, x);
+            row(v0, s, r, x);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float2 sum = make_float2(0.0f, 0.0f);
@@ -245,53 +250,72 @@ __global__ void __launch_bounds__(kGradThreads, 1) few_grad_kernel(const FewToke
                 dots[r * NT + n] = sum.x + sum.y;
             }
         }
-        const float mine = lane_sums<V>(dots, lane);
-        part[parity][warp][lane] = mine;
-        __syncthreads();  // the other parity's sums are written only after every thread passed this
-        float logit = 0.0f;
-        for (int k = 0; k < warps; ++k) logit += part[parity][k][lane];
+        part[to][warp][lane] = lane_sums<V>(dots, lane);
+    };
+
+    int64_t v0 = static_cast<int64_t>(blockIdx.x) * R;
+    fetch(v0, 0);
+    fetch(v0 + step, 1);
+    if constexpr (RING) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    if (v0 < p.vocab) logits(v0, 0, 0);
+    __syncthreads();
+    int slot = 0, parity = 0;
+    T* out_row = static_cast<T*>(p.dweight) + v0 * p.hidden;
+    for (; v0 < p.vocab; v0 += step, parity ^= 1, out_row += step * p.hidden) {
+        // a thread reads what it copied itself, and the slot that is filled now is the one that it read last
+        const int next = slot == kDepth - 1 ? 0 : slot + 1, after = next == kDepth - 1 ? 0 : next + 1;
+        fetch(v0 + 2 * step, after);
+        if constexpr (RING) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        // the other parity's sums were read before the last barrier
+        if (v0 + step < p.vocab) logits(v0 + step, next, parity ^ 1);
+        float even = 0.0f, odd = 0.0f;
+#pragma unroll
+        for (int k = 0; k < WARPS; k += 2) {
+            even += part[parity][k][lane];
+            odd += part[parity][k + 1][lane];
+        }
+        const float x_lse = even + odd - lse;
         const int64_t v = v0 + row_in;
         float d = 0.0f;
-        if (counts) d = (v == target ? expm1f(logit - lse) : __expf(logit - lse)) * grad;
+        if (counts && v < p.vocab) d = (v == target ? expm1f(x_lse) : __expf(x_lse)) * grad;
         // every warp keeps the batch's d for itself, in the order (row, token)
+        __syncwarp();
         if ((lane & ((1 << SHIFT) - 1)) == 0) dvals[warp][index] = d;
         __syncwarp();
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (v0 + r < p.vocab) {
-                float dr[NT];
+            float dr[NT];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) dr[n] = dvals[warp][r * NT + n];
-                float2 x[E / 2], out[E / 2];
-                row(r, x);
+            for (int n = 0; n < NT; ++n) dr[n] = dvals[warp][r * NT + n];
+            float2 x[E / 2], out[E / 2];
+            row(v0, slot, r, x);
 #pragma unroll
-                for (int k = 0; k < E / 2; ++k) out[k] = make_float2(0.0f, 0.0f);
+            for (int k = 0; k < E / 2; ++k) out[k] = make_float2(0.0f, 0.0f);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float2 both = make_float2(dr[n], dr[n]);
+            for (int n = 0; n < NT; ++n) {
+                const float2 both = make_float2(dr[n], dr[n]);
 #pragma unroll
-                    for (int k = 0; k < E / 2; ++k) {
-                        dh[n][k] = fma2(both, x[k], dh[n][k]);
-                        out[k] = fma2(both, h[n][k], out[k]);
-                    }
+                for (int k = 0; k < E / 2; ++k) {
+                    dh[n][k] = fma2(both, x[k], dh[n][k]);
+                    out[k] = fma2(both, h[n][k], out[k]);
                 }
-                if (p.dweight) {
-                    P* to = reinterpret_cast<P*>(static_cast<T*>(p.dweight) + (v0 + r) * p.hidden);
+            }
+            if (p.dweight && v0 + r < p.vocab) {
+                P* to = reinterpret_cast<P*>(out_row + r * p.hidden) + t;
 #pragma unroll
-                    for (int i = 0; i < ITEMS; ++i) {
-                        P q;
+                for (int i = 0; i < ITEMS; ++i) {
+                    P q;
 #pragma unroll
-                        for (int j = 0; j < VEC; ++j) {
-                            const int e = i * VEC + j;
-                            q.v[j] = from_compute<T, float>(e % 2 ? out[e / 2].y : out[e / 2].x);
-                        }
-                        if (inside(i)) to[i * threads + t] = q;
+                    for (int j = 0; j < VEC; ++j) {
+                        const int e = i * VEC + j;
+                        q.v[j] = from_compute<T, float>(e % 2 ? out[e / 2].y : out[e / 2].x);
                     }
+                    if (inside(i)) to[i * threads] = q;
                 }
             }
         }
-        __syncwarp();  // before this warp's d of the next batch
-        slot = slot + 1 == kDepth ? 0 : slot + 1;
+        slot = next;
+        __syncthreads();
     }
     if (p.sums) {
 #pragma unroll
@@ -310,27 +334,27 @@ __global__ void __launch_bounds__(kGradThreads, 1) few_grad_kernel(const FewToke
     }
 }
 
-// dh: the blocks' sums added in an order that depends on their number only; eight columns per block, 128 threads a column. Tokens without
-// a target get zero.
-template <typename T>
+// dh: the blocks' sums added in an order that depends on their number only; COLS columns per block, 1024 / COLS threads a column. Tokens
+// without a target get zero.
+template <typename T, int COLS>
 __global__ void __launch_bounds__(1024) few_dhidden_kernel(const FewTokens p, int blocks) {
-    __shared__ float part[32][9];
+    __shared__ float part[32][COLS + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t n_all = p.tokens * p.hidden, c = static_cast<int64_t>(blockIdx.x) * 8 + (lane & 7);
+    const int64_t n_all = p.tokens * p.hidden, c = static_cast<int64_t>(blockIdx.x) * COLS + lane % COLS;
     float sum = 0.0f;
     if (c < n_all) {
-#pragma unroll 2
-        for (int b = threadIdx.x >> 3; b < blocks; b += 128) sum += p.sums[static_cast<int64_t>(b) * n_all + c];
+#pragma unroll 5
+        for (int b = threadIdx.x / COLS; b < blocks; b += 1024 / COLS) sum += p.sums[static_cast<int64_t>(b) * n_all + c];
     }
-    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
-    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
-    if (lane < 8) part[warp][lane] = sum;
+#pragma unroll
+    for (int o = COLS; o < 32; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if (lane < COLS) part[warp][lane] = sum;
     __syncthreads();
-    if (warp >= 8) return;
+    if (warp >= COLS) return;
     sum = part[lane][warp];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    const int64_t out = static_cast<int64_t>(blockIdx.x) * 8 + warp;
+    const int64_t out = static_cast<int64_t>(blockIdx.x) * COLS + warp;
     if (lane == 0 && out < n_all) {
         const bool counts = target_of(p, out / p.hidden) != p.ignore;
         static_cast<T*>(p.dhidden)[out] = from_compute<T, float>(counts ? sum : 0.0f);
@@ -387,7 +411,8 @@ tn_status grad_one(const FewTokens& p, cudaStream_t stream) {
     few_grad_kernel<T, VEC, NT><<<(unsigned)blocks, threads, smem, stream>>>(p);
     TN_TRY(after_launch("few_grad_kernel"));
     if (!p.dhidden) return TN_SUCCESS;
-    few_dhidden_kernel<T><<<(unsigned)ceil_div(p.tokens * p.hidden, 8), 1024, 0, stream>>>(p, (int)blocks);
+    const bool many = p.tokens * p.hidden >= 32 * (int64_t)sm_count();
+    (many ? few_dhidden_kernel<T, 32> : few_dhidden_kernel<T, 8>)<<<(unsigned)ceil_div(p.tokens * p.hidden, many ? 32 : 8), 1024, 0, stream>>>(p, (int)blocks);
     return after_launch("few_dhidden_kernel");
 }
 template <typename T, int VEC>
