@@ -453,9 +453,14 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                             for (int j = 0; j < 32; ++j) d[j] = __expf(__uint_as_float(v[j]) - info.lse) * info.grad;
                             if (at >= c * 32 && at < c * 32 + 32) {
                                 // p - 1 without cancellation: the gradient of a token that is almost certain
+                                float hit = 0.0f;
 #pragma unroll
                                 for (int j = 0; j < 32; ++j)
-                                    if (at == c * 32 + j) d[j] = expm1f(__uint_as_float(v[j]) - info.lse) * info.grad;
+                                    if (at == c * 32 + j) hit = __uint_as_float(v[j]);
+                                hit = expm1f(hit - info.lse) * info.grad;
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (at == c * 32 + j) d[j] = hit;
                             }
                         }
                         uint32_t w[16];
