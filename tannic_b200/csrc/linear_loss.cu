@@ -29,8 +29,14 @@
 // alike). The results are multiplied back in float32.
 //
 // Kernel layout: warp 0 TMA producer, warp 1 MMA issuer, warp 2 tensor memory, warps 4..11 epilogue, persistent
-// thread blocks of a 128 x 256 tile, 64-wide K blocks in four stages, two accumulators so that the
-// epilogue of a tile runs under the products of the next. Bounded waits throughout.
+// thread blocks, 64-wide K blocks, two accumulators so that the epilogue of a tile runs under the products of the
+// next. Bounded waits throughout.
+//
+// A thread block on its own computes 128 x 256: it takes 48 KiB from L2 for every 64 of K, at 64 bytes a cycle
+// more than the 512 cycles its products need, and the tensor pipe was busy 70 % of the time. So two neighbouring SMs work as one
+// (cta_group::2): 256 x 256, each SM holding its 128 rows of A and of the accumulator and half of B, 32 KiB for the
+// same products. The even block of the pair issues the products for both; the loads of both report to its barriers, and its commits
+// report to both. Up to 128 rows leave nothing to the second SM and take the single form.
 //
 // The tensor cores cut off, rather than round, what falls below an accumulator's last place: a sum of K / 16 steps is low by up to
 // K / 16 half units, always towards zero (loss of 8192-wide float32 rows: 2e-6 relative, against 2e-7 of a float32
@@ -53,12 +59,15 @@ tn_status loss_abort_count(unsigned int* count) {
 
 namespace {
 
-constexpr int STAGES = 4;
+// A pair of thread blocks on neighbouring SMs (PAIR) shares a tile of 256 x 256: each loads its 128 rows of A and HALF of B.
+template <bool PAIR> constexpr int kStages = PAIR ? 6 : 4;
+template <bool PAIR> constexpr uint32_t kStageBytes = A_BYTES + (PAIR ? B_BYTES / 2 : B_BYTES);
+static_assert(kStages<true> * kStageBytes<true> == kStages<false> * kStageBytes<false>, "one size of shared memory for both");
 constexpr int kEpilogueWarps = 8;                          // warps 4..11
 constexpr int kThreads = 128 + 32 * kEpilogueWarps;
 constexpr uint32_t kBoxBytes = 2048;                       // 32 rows x 64 bytes
 constexpr uint32_t kWarpBytes = 2 * kBoxBytes;             // two boxes per warp, or 32 rows x 80 bytes
-constexpr uint32_t kSmemBytes = 1024 + STAGES * STAGE_BYTES + kEpilogueWarps * kWarpBytes + 256;
+constexpr uint32_t kSmemBytes = 1024 + kStages<false> * kStageBytes<false> + kEpilogueWarps * kWarpBytes + 256;
 static_assert(kSmemBytes <= 232448, "exceeds the shared memory of an SM");
 
 // A row of the gradient's products: a token with a target, or (target kNoRow) nothing.
@@ -86,7 +95,9 @@ struct LossArgs {
     int n_tiles;
     int m_tiles;
     int k_blocks;            // 64-wide blocks of K, all splits together
-    int splits, split_blocks;
+    int most_splits;         // 1: K in one go
+    int first_k_blocks;      // of the first piece, whose splits the others must not exceed
+    int units;               // thread blocks, or pairs of them, that share the tiles
     int terms;               // 1, or 6 for float32 operands
     int period;              // PROMOTE: passes over a 64-wide block that one accumulator takes
     int is_bf16;
@@ -109,6 +120,76 @@ struct LossArgs {
     const float* scale;
     int tma_store;
 };
+
+// ---- a pair of thread blocks -----------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// Address of the even block's copy of a shared-memory location.
+__device__ __forceinline__ uint32_t in_even_block(uint32_t addr) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(0));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+// A wait that also sees what the other block of the pair did before it arrived.
+__device__ __forceinline__ bool mbar_wait_pair(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    for (uint32_t it = 0; it < kSpinLimit; ++it) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if (it >= kSpinFast) {
+            if (*abort_flag) return false;
+            __nanosleep(64);
+        }
+    }
+    *abort_flag = 1;
+    return false;
+}
+// A load into this block's memory that reports to a barrier of either block.
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t cluster_bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(cluster_bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+__device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Arrives at the barrier of both blocks once the products issued so far are done.
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        ::"r"(bar), "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+
+// Splits of the vocabulary when dh has `tiles` tiles for `units` blocks or pairs: as many as fill the GPU, each with at least four
+// blocks of K. Decided on the device, where the number of tokens that count is known.
+struct SplitPlan { int splits, blocks; };
+__device__ __forceinline__ SplitPlan plan_splits(int tiles, int units, int k_blocks, int most) {
+    int splits = tiles > 0 ? units / tiles : 1;
+    splits = max(1, min(min(splits, most), k_blocks / 4));
+    const int blocks = (k_blocks + splits - 1) / splits;
+    return {(k_blocks + blocks - 1) / blocks, blocks};
+}
 
 __device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
     asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
@@ -212,34 +293,45 @@ __device__ __forceinline__ void online_softmax(const uint32_t (&v)[32], int ncol
 
 // A_M: A is stored [K, M] (M contiguous), else [M, K]. B_N: B is stored [K, N], else [N, K]. T: operand type (bfloat16 parts
 // for float32). OUT: result type of EPI_RESULT. PARTS: parts of d that EPI_D writes.
-template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS, bool PROMOTE>
+template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS, bool PROMOTE, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_d, const LossArgs g) {
+    constexpr int STAGES = kStages<PAIR>, ROWS = PAIR ? 2 * BM : BM;  // rows of a tile
+    constexpr int B_COLS = PAIR ? BN / 2 : BN;                        // columns of B that this block loads
+    constexpr uint32_t STAGE = kStageBytes<PAIR>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;  // swizzled tiles need 1024-byte alignment
     uint8_t* base_ptr = smem_raw + (base - raw);
-    uint8_t* staging_ptr = base_ptr + STAGES * STAGE_BYTES;
-    const uint32_t bars = base + STAGES * STAGE_BYTES + kEpilogueWarps * kWarpBytes;
+    uint8_t* staging_ptr = base_ptr + STAGES * STAGE;
+    const uint32_t bars = base + STAGES * STAGE + kEpilogueWarps * kWarpBytes;
     // barriers of 8 bytes: full[STAGES], empty[STAGES], accumulator full[2], accumulator empty[2]
     const uint32_t full0 = bars, empty0 = bars + 8 * STAGES, accf0 = bars + 16 * STAGES, acce0 = accf0 + 16;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(staging_ptr + kEpilogueWarps * kWarpBytes + 16 * STAGES + 32);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = PAIR ? static_cast<int>(cluster_rank()) : 0;
+    const uint32_t unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, units = PAIR ? gridDim.x >> 1 : gridDim.x;
+    auto wait = [&](uint32_t bar, uint32_t parity) { return PAIR ? mbar_wait_pair(bar, parity, abort_flag) : mbar_wait(bar, parity, abort_flag); };
 
     // the tokens that count bound the rows or the K extent
     int m_tiles = g.m_tiles, k_blocks = g.k_blocks;
     if (g.count_is != COUNT_NONE) {
         const int count = *g.count;
-        if (g.count_is == COUNT_ROWS) m_tiles = (count + BM - 1) / BM;
+        if (g.count_is == COUNT_ROWS) m_tiles = (count + ROWS - 1) / ROWS;
         else k_blocks = (count + BK - 1) / BK;
     }
+    SplitPlan plan = {1, k_blocks};
+    if (g.most_splits > 1) {
+        const int tiles = m_tiles * g.n_tiles;
+        plan = plan_splits(tiles, g.units, k_blocks, plan_splits(tiles, g.units, g.first_k_blocks, g.most_splits).splits);
+    }
     const uint32_t per_split = static_cast<uint32_t>(m_tiles) * static_cast<uint32_t>(g.n_tiles);
-    const uint32_t total = per_split * static_cast<uint32_t>(g.splits);
+    const uint32_t total = per_split * static_cast<uint32_t>(plan.splits);
     // K blocks [first, first + n) of split z
     auto split_range = [&](int z, int& first, int& n) {
-        first = z * g.split_blocks;
-        n = min(k_blocks - first, g.split_blocks);
+        first = z * plan.blocks;
+        n = min(k_blocks - first, plan.blocks);
     };
 
     if (threadIdx.x == 0) {
@@ -249,17 +341,23 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(accf0 + 8 * b, 1);
-            mbar_init(acce0 + 8 * b, kEpilogueWarps);
+            mbar_init(acce0 + 8 * b, PAIR ? 2 * kEpilogueWarps : kEpilogueWarps);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();  // the other block's barriers exist before anything reports to them
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
@@ -271,31 +369,42 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             if (lane == 0) {
                 uint32_t it = 0;
                 bool ok = true;
-                for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
+                for (uint32_t t = unit; ok && t < total; t += units) {
                     int z, mt, nt, first, blocks;
                     tile_coords(t, m_tiles, g.n_tiles, z, mt, nt);
                     split_range(z, first, blocks);
+                    const int row = mt * ROWS + rank * BM, col = nt * BN + rank * B_COLS;  // what this block loads
                     for (int kb = first; ok && kb < first + blocks; ++kb) {
                         for (int term = 0; term < g.terms; ++term, ++it) {
                             const int s = it % STAGES;
-                            if (!mbar_wait(empty0 + 8 * s, ((it / STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
-                            const uint32_t sa = base + s * STAGE_BYTES, sb = sa + A_BYTES, bar = full0 + 8 * s;
+                            if (!wait(empty0 + 8 * s, ((it / STAGES) & 1) ^ 1)) { ok = false; break; }
+                            const uint32_t sa = base + s * STAGE, sb = sa + A_BYTES;
                             const int pa = g.terms > 1 ? kPartA[term] : 0, pb = g.terms > 1 ? kPartB[term] : 0;
-                            mbar_expect_tx(bar, STAGE_BYTES);
+                            uint32_t bar = full0 + 8 * s;
+                            if (rank == 0) mbar_expect_tx(bar, PAIR ? 2 * STAGE : STAGE);
+                            if constexpr (PAIR) bar = in_even_block(bar);
+                            auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
+                                if constexpr (PAIR) tma_load_3d_pair(dst, map, bar, c0, c1, c2);
+                                else tma_load_3d(dst, map, bar, c0, c1, c2);
+                            };
                             if constexpr (A_M) {
 #pragma unroll
-                                for (int c = 0; c < BM / 64; ++c) tma_load_3d(sa + c * (64 * BK * 2), &map_a, bar, mt * BM + c * 64, kb * BK, pa);
+                                for (int c = 0; c < BM / 64; ++c) load(sa + c * (64 * BK * 2), &map_a, row + c * 64, kb * BK, pa);
                             } else {
-                                tma_load_3d(sa, &map_a, bar, kb * BK, mt * BM, pa);
+                                load(sa, &map_a, kb * BK, row, pa);
                             }
                             if constexpr (B_N) {
 #pragma unroll
-                                for (int c = 0; c < BN / 64; ++c) tma_load_3d(sb + c * (64 * BK * 2), &map_b, bar, nt * BN + c * 64, kb * BK, pb);
+                                for (int c = 0; c < B_COLS / 64; ++c) load(sb + c * (64 * BK * 2), &map_b, col + c * 64, kb * BK, pb);
                             } else {
-                                tma_load_3d(sb, &map_b, bar, kb * BK, nt * BN, pb);
+                                load(sb, &map_b, kb * BK, col, pb);
                             }
                         }
                     }
+                }
+                if constexpr (PAIR) {
+                    // the commits that free the last stages have arrived here before this block may go
+                    for (uint32_t i = it > STAGES ? it - STAGES : 0; ok && i < it; ++i) ok = wait(empty0 + 8 * (i % STAGES), (i / STAGES) & 1);
                 }
                 if (!ok) {
                     // transactions that were already issued land before the shared memory goes away
@@ -304,15 +413,15 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             }
         } else if (warp == 1) {
             // ------------------------------------------------------------ MMA issuer ------
-            if (lane == 0) {
+            if (lane == 0 && rank == 0) {
                 // D = F32 (bits 4-5), A and B format (7-9, 10-12: 0 = F16, 1 = BF16), A and B stored with M / N contiguous (15, 16),
                 // N >> 3 (17-22), M >> 4 (24-28)
                 const uint32_t fmt = g.is_bf16 ? 1u : 0u;
                 const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((A_M ? 1u : 0u) << 15) | ((B_N ? 1u : 0u) << 16) |
-                                       (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>(BM >> 4) << 24);
+                                       (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>(ROWS >> 4) << 24);
                 uint32_t it = 0, local = 0;
                 bool ok = true;
-                for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
+                for (uint32_t t = unit; ok && t < total; t += units) {
                     int z, mt, nt, first, blocks;
                     tile_coords(t, m_tiles, g.n_tiles, z, mt, nt);
                     split_range(z, first, blocks);
@@ -320,25 +429,31 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     const int period = PROMOTE ? g.period : steps;
                     for (int i0 = 0; ok && i0 < steps; i0 += period, ++local) {
                         const int buf = local & 1;
-                        if (!mbar_wait(acce0 + 8 * buf, ((local >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                        if (!wait(acce0 + 8 * buf, ((local >> 1) & 1) ^ 1)) { ok = false; break; }
                         tc_fence_after();
                         const uint32_t acc = tmem_base + buf * BN;
                         const int i1 = min(steps, i0 + period);
                         for (int i = i0; i < i1; ++i, ++it) {
                             const int s = it % STAGES;
-                            if (!mbar_wait(full0 + 8 * s, (it / STAGES) & 1, abort_flag)) { ok = false; break; }
+                            if (!wait(full0 + 8 * s, (it / STAGES) & 1)) { ok = false; break; }
                             tc_fence_after();
-                            const uint32_t sa = base + s * STAGE_BYTES, sb = sa + A_BYTES;
+                            const uint32_t sa = base + s * STAGE, sb = sa + A_BYTES;
 #pragma unroll
                             for (int k = 0; k < BK / UMMA_K; ++k) {
                                 // K contiguous: 32 bytes further along the swizzled row; else 16 rows of 128 bytes further, 64-wide boxes 8 KiB apart
                                 const uint64_t da = A_M ? smem_desc(sa + k * UMMA_K * 128, 64 * BK * 2, 1024) : smem_desc(sa + k * UMMA_K * 2, 16, 1024);
                                 const uint64_t db = B_N ? smem_desc(sb + k * UMMA_K * 128, 64 * BK * 2, 1024) : smem_desc(sb + k * UMMA_K * 2, 16, 1024);
-                                umma_f16(acc, da, db, idesc, (i > i0 || k > 0) ? 1u : 0u);
+                                if constexpr (PAIR) umma_f16_pair(acc, da, db, idesc, (i > i0 || k > 0) ? 1u : 0u);
+                                else umma_f16(acc, da, db, idesc, (i > i0 || k > 0) ? 1u : 0u);
                             }
-                            umma_commit(empty0 + 8 * s);  // frees the stage once these MMAs have read it
+                            // frees the stage once these MMAs have read it
+                            if constexpr (PAIR) umma_commit_pair(empty0 + 8 * s);
+                            else umma_commit(empty0 + 8 * s);
                         }
-                        if (ok) umma_commit(accf0 + 8 * buf);
+                        if (ok) {
+                            if constexpr (PAIR) umma_commit_pair(accf0 + 8 * buf);
+                            else umma_commit(accf0 + 8 * buf);
+                        }
                     }
                 }
             }
@@ -353,11 +468,20 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const float scale = EPI == EPI_RESULT ? *g.scale : 1.0f;
         uint32_t local = 0;
         bool ok = true;
-        for (uint32_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
+        // this warp has finished reading an accumulator: tell the block that issues the products
+        auto release = [&](int buf) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_remote(in_even_block(acce0 + 8 * buf));
+                else mbar_arrive(acce0 + 8 * buf);
+            }
+        };
+        for (uint32_t t = unit; ok && t < total; t += units) {
             int z, mt, nt, first, blocks;
             tile_coords(t, m_tiles, g.n_tiles, z, mt, nt);
             split_range(z, first, blocks);
-            const int64_t row0 = static_cast<int64_t>(mt) * BM + quarter * 32, row = row0 + lane;
+            const int64_t row0 = static_cast<int64_t>(mt) * ROWS + rank * BM + quarter * 32, row = row0 + lane;
             const int64_t col0 = static_cast<int64_t>(nt) * BN;
             const int rows = static_cast<int>(max(int64_t(0), min(int64_t(32), g.M - row0)));
             const int cols = static_cast<int>(min(int64_t(BN), g.N - col0)), chunks = (cols + 31) >> 5;
@@ -373,7 +497,7 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 const int steps = blocks * g.terms;
                 for (int i0 = 0; i0 < steps; i0 += g.period, ++local) {
                     const int buf = local & 1;
-                    if (!mbar_wait(accf0 + 8 * buf, (local >> 1) & 1, abort_flag)) { ok = false; break; }
+                    if (!wait(accf0 + 8 * buf, (local >> 1) & 1)) { ok = false; break; }
                     tc_fence_after();
                     if (rows > 0) {  // warp-uniform
 #pragma unroll
@@ -387,14 +511,12 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                             }
                         }
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(acce0 + 8 * buf);
+                    release(buf);
                 }
                 if (!ok) break;
             } else if (!empty) {
                 const int buf = local & 1;
-                if (!mbar_wait(accf0 + 8 * buf, (local >> 1) & 1, abort_flag)) { ok = false; break; }
+                if (!wait(accf0 + 8 * buf, (local >> 1) & 1)) { ok = false; break; }
                 tc_fence_after();
                 taddr = lanes + buf * BN;
             }
@@ -545,10 +667,8 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 }
             }
             if constexpr (!PROMOTE) {
-                if (!empty) {  // this warp has finished reading the accumulator
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(acce0 + 8 * (local & 1));
+                if (!empty) {
+                    release(local & 1);
                     ++local;
                 }
             }
@@ -558,9 +678,11 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();  // neither block goes while the other may still report to it
     if (warp == 2) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
     }
     if (threadIdx.x == 0 && *abort_flag) atomicAdd(&g_loss_aborts, 1u);
 }
@@ -737,11 +859,13 @@ __global__ void __launch_bounds__(256) pack_rows(const T* __restrict__ src, int6
 // dh: the float32 sums of the splits, added in order, scaled back, and put where the tokens stand. VEC: 4 where the rows of the
 // result start on boundaries of four elements, else 1.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) loss_dhidden(const float* __restrict__ sums, int splits, int64_t rows, int64_t cols, int64_t padded, const int* __restrict__ slot,
+__global__ void __launch_bounds__(256) loss_dhidden(const float* __restrict__ sums, const int* __restrict__ count, int tile_rows, int n_tiles, int units, int k_blocks,
+                                                    int most_splits, int64_t rows, int64_t cols, int64_t padded, const int* __restrict__ slot,
                                                     const float* __restrict__ scale, T* __restrict__ out) {
     struct alignas(sizeof(T) * VEC) Result { T v[VEC]; };
     struct alignas(sizeof(float) * VEC) Sums { float v[VEC]; };
     const float by = *scale;
+    const int splits = plan_splits((*count + tile_rows - 1) / tile_rows * n_tiles, units, k_blocks, most_splits).splits;  // of the first piece
     const int64_t groups = cols / VEC;
     for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
         const int at = slot[r];
@@ -891,35 +1015,65 @@ tn_status operand_map(CUtensorMap* map, const Operand& o, bool bf16, int64_t inn
     return make_map(map, o.ptr, bf16, inner, rows, o.parts, o.pitch, o.part_stride, box_inner, box_rows);
 }
 
-template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS, bool PROMOTE>
-tn_status launch_one(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d, const LossArgs& g, cudaStream_t stream) {
+// Thread blocks, or pairs of them, that run at once.
+int unit_count(bool pair) {
+    const int sms = sm_count() - sm_margin();
+    return std::max(1, pair ? sms / 2 : sms);
+}
+// Whether a product with m result rows takes pairs: up to 128 rows the second block would have none.
+bool takes_pairs(int64_t m) { return m > BM; }
+
+template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS, bool PROMOTE, bool PAIR>
+tn_status launch_as(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d, const LossArgs& g, cudaStream_t stream) {
     static thread_local int attr_device = -1;  // the opt-in shared-memory size belongs to kernel and device
+    auto kernel = loss_gemm<A_M, B_N, EPI, T, OUT, PARTS, PROMOTE, PAIR>;
     int dev = 0;
     TN_CUDA(cudaGetDevice(&dev));
     if (attr_device != dev) {
-        TN_CUDA(cudaFuncSetAttribute(loss_gemm<A_M, B_N, EPI, T, OUT, PARTS, PROMOTE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+        TN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
         attr_device = dev;
     }
-    const int64_t total = (int64_t)g.m_tiles * g.n_tiles * g.splits;
+    const int64_t total = (int64_t)g.m_tiles * g.n_tiles * g.most_splits;
     if (total >= (int64_t(1) << 31)) return fail(TN_ERROR, "linear_cross_entropy: %lld tiles are too many", (long long)total);
-    const int64_t sms = sm_count() - sm_margin();
-    loss_gemm<A_M, B_N, EPI, T, OUT, PARTS, PROMOTE><<<(unsigned)std::min(total, sms), kThreads, kSmemBytes, stream>>>(a, b, d, g);
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)std::min<int64_t>(total, g.units) * (PAIR ? 2 : 1));
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = kSmemBytes;
+    config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim = {2, 1, 1};
+    if (PAIR) {
+        config.attrs = &attribute;
+        config.numAttrs = 1;
+    }
+    TN_CUDA(cudaLaunchKernelEx(&config, kernel, a, b, d, g));
     return after_launch("loss_gemm");
+}
+template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS, bool PROMOTE>
+tn_status launch_one(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d, const LossArgs& g, cudaStream_t stream) {
+    return takes_pairs(g.M) ? launch_as<A_M, B_N, EPI, T, OUT, PARTS, PROMOTE, true>(a, b, d, g, stream)
+                            : launch_as<A_M, B_N, EPI, T, OUT, PARTS, PROMOTE, false>(a, b, d, g, stream);
 }
 
 LossArgs gemm_args(const Problem& p, int64_t m, int64_t n, int64_t k) {
     LossArgs g = {};
+    const bool pair = takes_pairs(m);
     g.M = m;
     g.N = n;
-    g.m_tiles = (int)ceil_div(m, BM);
+    g.m_tiles = (int)ceil_div(m, pair ? 2 * BM : BM);
     g.n_tiles = (int)ceil_div(n, BN);
     g.k_blocks = (int)ceil_div(k, BK);
-    g.splits = 1;
-    g.split_blocks = g.k_blocks;
+    g.most_splits = 1;
+    g.units = unit_count(pair);
     g.terms = p.terms;
     g.period = kPeriod;
     g.is_bf16 = p.bf16;
     return g;
+}
+// Map of an operand B stored [N, K] for a product with m result rows: a block of a pair loads half the columns.
+tn_status b_map(CUtensorMap* map, const Operand& o, bool bf16, int64_t k, int64_t n, int64_t m) {
+    return operand_map(map, o, bf16, k, n, BK, takes_pairs(m) ? BN / 2 : BN);
 }
 
 // Vocabulary entries per piece: `bytes_each` is the workspace that one of them takes.
@@ -1057,7 +1211,7 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
         const int64_t n = std::min(piece, p.vocab - v0);
         Operand b;
         TN_TRY(weight_piece(p, w, v0, n, room, &b));
-        TN_TRY(operand_map(&map_b, b, p.bf16, p.hidden, n, BK, BN));
+        TN_TRY(b_map(&map_b, b, p.bf16, p.hidden, n, p.tokens));
         LossArgs g = gemm_args(p, p.tokens, n, p.hidden);
         g.vocab0 = v0;
         g.targets = t;
@@ -1125,14 +1279,14 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
     dd.part_stride = p.tokens * d_pitch;
     dd.parts = p.parts;
 
-    // dh has few tiles when there are few tokens: K (the vocabulary) is split until every SM has a tile, each
-    // split with at least four blocks, and the splits' sums are added in order afterwards
+    // dh has few tiles when there are few tokens: K (the vocabulary) is split until every SM has a tile, and the splits' sums are added
+    // in order afterwards. Room for what the host can know; half of the tokens may turn out not to count.
     float* sums = nullptr;
     int splits = 1;
-    const int64_t sms = sm_count() - sm_margin();
+    const bool pair = takes_pairs(p.tokens);
     if (dhidden) {
-        const int64_t tiles = ceil_div(p.tokens, BM) * ceil_div(p.hidden, BN);
-        splits = (int)std::max<int64_t>(1, std::min(sms / tiles, ceil_div(piece, BK) / 4));
+        const int64_t tiles = ceil_div(p.tokens, pair ? 2 * BM : BM) * ceil_div(p.padded, BN);
+        splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * (unit_count(pair) / tiles), ceil_div(piece, BK) / 4));
         TN_TRY(mem.take(&sums, sizeof(float) * (size_t)splits * p.tokens * p.padded));
     }
 
@@ -1145,7 +1299,7 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
         TN_TRY(weight_piece(p, w, v0, n, room, &b));
         {   // d of this piece
             CUtensorMap map_d;
-            TN_TRY(operand_map(&map, b, p.bf16, p.hidden, n, BK, BN));
+            TN_TRY(b_map(&map, b, p.bf16, p.hidden, n, p.tokens));
             const cuuint64_t dims[3] = {(cuuint64_t)n, (cuuint64_t)p.tokens, (cuuint64_t)p.parts};
             const cuuint64_t strides[2] = {(cuuint64_t)d_pitch * 2, (cuuint64_t)dd.part_stride * 2};
             const cuuint32_t box[3] = {32, 32, 1};
@@ -1165,11 +1319,9 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
             LossArgs g = gemm_args(p, p.tokens, p.padded, n);
             g.count = count;
             g.count_is = COUNT_ROWS;
-            // the last piece may be shorter: every split that has been written keeps at least one block or none
-            g.split_blocks = (int)ceil_div(g.k_blocks, splits);
-            g.splits = (int)ceil_div(g.k_blocks, g.split_blocks);
+            g.most_splits = splits;
+            g.first_k_blocks = (int)ceil_div(piece, BK);
             g.add = v0 > 0;
-            if (v0 == 0) splits = g.splits;
             TN_TRY((launch_one<false, true, EPI_SUM, T, float, 1, true>(map, map_w, map_d, g, p.stream)));
         }
         if (dweight) {
@@ -1193,7 +1345,8 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
         OUT* to = static_cast<OUT*>(dhidden->address);
         const bool wide = p.hidden % 4 == 0 && (reinterpret_cast<uintptr_t>(to) & (4 * sizeof(OUT) - 1)) == 0;
         const dim3 grid((unsigned)std::min<int64_t>(ceil_div(p.hidden, wide ? 1024 : 256), 1024), (unsigned)std::min<int64_t>(p.tokens, 65535));
-        (wide ? loss_dhidden<OUT, 4> : loss_dhidden<OUT, 1>)<<<grid, 256, 0, p.stream>>>(sums, splits, p.tokens, p.hidden, p.padded, slot, scale, to);
+        (wide ? loss_dhidden<OUT, 4> : loss_dhidden<OUT, 1>)<<<grid, 256, 0, p.stream>>>(
+            sums, count, pair ? 2 * BM : BM, (int)ceil_div(p.padded, BN), unit_count(pair), (int)ceil_div(piece, BK), splits, p.tokens, p.hidden, p.padded, slot, scale, to);
         TN_TRY(after_launch("loss_dhidden"));
     }
     return TN_SUCCESS;
