@@ -40,8 +40,10 @@
 //
 // The tensor cores cut off, rather than round, what falls below an accumulator's last place: a sum of K / 16 steps is low by up to
 // K / 16 half units, always towards zero (loss of 8192-wide float32 rows: 2e-6 relative, against 2e-7 of a float32
-// sum). Where the result is float32 or the sum is long (PROMOTE) an accumulator takes only `period` blocks and the epilogue warps
+// sum). Where the result is float32 or the sum is long an accumulator takes only `period` blocks and the epilogue warps
 // add it, in float32, to sums in their registers (128 a thread); its double hides that under the next blocks' products.
+// With the whole tile in registers an accumulator is free as soon as it is read, and the epilogue has 128 independent
+// elements a thread to fill the gaps that two warps to a scheduler leave.
 // The register split that takes is 40 a thread for warps 0..3 and 232 for the others, of 384 x 168 at launch.
 #include <algorithm>
 
@@ -59,16 +61,17 @@ tn_status loss_abort_count(unsigned int* count) {
 
 namespace {
 
+constexpr int kChunks = BN / 64;                           // 32-column chunks of a warp
 // A pair of thread blocks on neighbouring SMs (PAIR) shares a tile of 256 x 256: each loads its 128 rows of A and HALF of B.
-template <bool PAIR> constexpr int kStages = PAIR ? 6 : 4;
+template <bool PAIR> constexpr int kStages = PAIR ? 5 : 3;
 template <bool PAIR> constexpr uint32_t kStageBytes = A_BYTES + (PAIR ? B_BYTES / 2 : B_BYTES);
-static_assert(kStages<true> * kStageBytes<true> == kStages<false> * kStageBytes<false>, "one size of shared memory for both");
 constexpr int kEpilogueWarps = 8;                          // warps 4..11
 constexpr int kThreads = 128 + 32 * kEpilogueWarps;
 constexpr uint32_t kBoxBytes = 2048;                       // 32 rows x 64 bytes
-constexpr uint32_t kWarpBytes = 2 * kBoxBytes;             // two boxes per warp, or 32 rows x 80 bytes
-constexpr uint32_t kSmemBytes = 1024 + kStages<false> * kStageBytes<false> + kEpilogueWarps * kWarpBytes + 256;
-static_assert(kSmemBytes <= 232448, "exceeds the shared memory of an SM");
+constexpr uint32_t kWarpBytes = kChunks * kBoxBytes;       // a box per chunk, or 32 rows x 68 bytes
+template <bool PAIR> constexpr uint32_t kSmemBytes = 1024 + kStages<PAIR> * kStageBytes<PAIR> + kEpilogueWarps * kWarpBytes + 256;
+static_assert(kSmemBytes<true> <= 232448 && kSmemBytes<false> <= 232448, "exceeds the shared memory of an SM");
+constexpr float kLog2e = 1.4426950408889634f;
 
 // A row of the gradient's products: a token with a target, or (target kNoRow) nothing.
 struct alignas(16) RowInfo {
@@ -99,7 +102,7 @@ struct LossArgs {
     int first_k_blocks;      // of the first piece, whose splits the others must not exceed
     int units;               // thread blocks, or pairs of them, that share the tiles
     int terms;               // 1, or 6 for float32 operands
-    int period;              // PROMOTE: passes over a 64-wide block that one accumulator takes
+    int period;              // passes over a 64-wide block that one accumulator takes
     int is_bf16;
     const int* count;        // tokens with a target
     int count_is;
@@ -197,29 +200,39 @@ __device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, uint32_t src,
         : "memory");
 }
 
-// Hands 32 rows x 64 bytes (a lane's row in `w`) to TMA, which clips the box at the tensor's edges.
+// Boxes of 32 rows x 64 bytes (a lane's row in `w`) on their way to TMA, which clips them at the tensor's edges: one per chunk, filled
+// together and sent together, so that the warp waits for the previous tile's boxes only.
 struct BoxStore {
     uint8_t* stage;
     const CUtensorMap* map;
-    int lane, flip;
-    __device__ __forceinline__ void put(const uint32_t (&w)[16], int c0, int c1, int c2, bool add) {
-        uint8_t* buf = stage + (flip & 1) * kBoxBytes;
-        flip ^= 1;
-        if (lane == 0) bulk_wait_read_1();  // the box that used this buffer two boxes ago has left it
+    int lane;
+    __device__ __forceinline__ void begin() const {
+        if (lane == 0) bulk_wait_read_0();  // the boxes sent last have been read
         __syncwarp();
-        const int x = (lane >> 1) & 3;      // 64-byte swizzle
+    }
+    __device__ __forceinline__ void fill(int i, const uint32_t (&w)[16]) const {
+        uint8_t* buf = stage + i * kBoxBytes;
+        const int x = (lane >> 1) & 3;  // 64-byte swizzle
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ x) << 4)) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    }
+    template <typename Send>
+    __device__ __forceinline__ void send(int n, Send&& one) const {
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
-            if (add) tma_add_3d(map, smem_u32(buf), c0, c1, c2);
-            else tma_store_3d(map, smem_u32(buf), c0, c1, c2);
+            for (int i = 0; i < n; ++i) one(i, smem_u32(stage + i * kBoxBytes));
             bulk_commit();
         }
     }
 };
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
@@ -231,69 +244,34 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, f
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// x = p0 + p1 + p2, each part a bfloat16 (whose exponent range is float32's). An infinity or NaN stays in p0.
+// exp(x - base) = power(x) * rest with one multiply-add and one special-function instruction an x: 2^(x log2 e - base log2 e). What
+// rounding base log2 e loses, up to 2^-24 of it and the same for every x, is in `rest`.
+struct Exponent {
+    float shift, rest;
+    __device__ __forceinline__ explicit Exponent(float base) {
+        shift = -base * kLog2e;
+        const float lost = fmaf(base, kLog2e, shift);
+        rest = isfinite(lost) ? exp2_approx(-lost) : 1.0f;
+    }
+    __device__ __forceinline__ float power(float x) const { return exp2_approx(fmaf(x, kLog2e, shift)); }
+};
+
+// x as bfloat16 (whose exponent range is float32's), the largest number where rounding would leave the range.
+__device__ __forceinline__ float first_part(float x) {
+    const float p = __bfloat162float(__float2bfloat16_rn(x));
+    return isinf(p) && !isinf(x) ? copysignf(__uint_as_float(0x7F7F0000u), x) : p;
+}
+// x = p0 + p1 + p2, each part a bfloat16. An infinity or NaN stays in p0.
 __device__ __forceinline__ void three_parts(float x, float& p0, float& p1, float& p2) {
-    p0 = __bfloat162float(__float2bfloat16_rn(x));
-    if (isinf(p0) && !isinf(x)) p0 = copysignf(__uint_as_float(0x7F7F0000u), x);  // rounded up past the largest number
+    p0 = first_part(x);
     const float r = isfinite(x) ? x - p0 : 0.0f;
     p1 = __bfloat162float(__float2bfloat16_rn(r));
     p2 = r - p1;  // at most 8 significand bits are left; rounded when it is packed
 }
 
-// Calls body(values, chunk) for this warp's 32-column chunks of an accumulator; the next chunk's load runs under the body.
-template <typename Body>
-__device__ __forceinline__ void drain(uint32_t taddr, int first, int chunks, Body&& body) {
-    uint32_t va[32], vb[32];
-    int c = first;
-    if (c >= chunks) return;
-    tmem_load_issue(taddr + c * 32, va);
-    while (true) {
-        tmem_load_wait(va);
-        if (c + 2 < chunks) tmem_load_issue(taddr + (c + 2) * 32, vb);
-        body(va, c);
-        c += 2;
-        if (c >= chunks) break;
-        tmem_load_wait(vb);
-        if (c + 2 < chunks) tmem_load_issue(taddr + (c + 2) * 32, va);
-        body(vb, c);
-        c += 2;
-        if (c >= chunks) break;
-    }
-}
-
-// Running maximum and sum of exponentials of the valid ones among 32 logits.
-__device__ __forceinline__ void online_softmax(const uint32_t (&v)[32], int ncols, float& m, float& s) {
-    float top = -INFINITY;
-    if (ncols == 32) {  // warp-uniform
-#pragma unroll
-        for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(v[j]));
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < ncols) top = fmaxf(top, __uint_as_float(v[j]));
-    }
-    const float now = fmaxf(m, top);
-    const float base = now == -INFINITY ? 0.0f : now;  // nothing but -inf so far: the sum stays 0
-    s *= __expf(m - base);
-    float s0 = 0.0f, s1 = 0.0f;
-    if (ncols == 32) {
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-            s0 += __expf(__uint_as_float(v[j]) - base);
-            s1 += __expf(__uint_as_float(v[j + 1]) - base);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < ncols) s0 += __expf(__uint_as_float(v[j]) - base);
-    }
-    s += s0 + s1;
-    m = now;
-}
-
 // A_M: A is stored [K, M] (M contiguous), else [M, K]. B_N: B is stored [K, N], else [N, K]. T: operand type (bfloat16 parts
 // for float32). OUT: result type of EPI_RESULT. PARTS: parts of d that EPI_D writes.
-template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS, bool PROMOTE, bool PAIR>
+template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_d, const LossArgs g) {
     constexpr int STAGES = kStages<PAIR>, ROWS = PAIR ? 2 * BM : BM;  // rows of a tile
@@ -363,7 +341,7 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 
     // all four warps of a group take part, so this comes before the roles
     if (warp < 4) {
-        if constexpr (PROMOTE) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 0) {
             // ------------------------------------------------------------ TMA producer ----
             if (lane == 0) {
@@ -426,13 +404,12 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     tile_coords(t, m_tiles, g.n_tiles, z, mt, nt);
                     split_range(z, first, blocks);
                     const int steps = blocks * g.terms;
-                    const int period = PROMOTE ? g.period : steps;
-                    for (int i0 = 0; ok && i0 < steps; i0 += period, ++local) {
+                    for (int i0 = 0; ok && i0 < steps; i0 += g.period, ++local) {
                         const int buf = local & 1;
                         if (!wait(acce0 + 8 * buf, ((local >> 1) & 1) ^ 1)) { ok = false; break; }
                         tc_fence_after();
                         const uint32_t acc = tmem_base + buf * BN;
-                        const int i1 = min(steps, i0 + period);
+                        const int i1 = min(steps, i0 + g.period);
                         for (int i = i0; i < i1; ++i, ++it) {
                             const int s = it % STAGES;
                             if (!wait(full0 + 8 * s, (it / STAGES) & 1)) { ok = false; break; }
@@ -460,23 +437,14 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
     } else {
         // ------------------------------------------------------------ epilogue --------
-        if constexpr (PROMOTE) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         const int ew = warp - 4;
         const int quarter = warp & 3;  // tensor-memory lanes [32 * quarter, 32 * quarter + 32)
-        const int half = ew >> 2;      // this warp takes the chunks half, half + 2, ...
-        BoxStore box = {staging_ptr + ew * kWarpBytes, &map_d, lane, 0};
+        const int half = ew >> 2;      // this warp takes the 32-column chunks half, half + 2, ...
+        BoxStore box = {staging_ptr + ew * kWarpBytes, &map_d, lane};
         const float scale = EPI == EPI_RESULT ? *g.scale : 1.0f;
         uint32_t local = 0;
         bool ok = true;
-        // this warp has finished reading an accumulator: tell the block that issues the products
-        auto release = [&](int buf) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (PAIR) mbar_arrive_remote(in_even_block(acce0 + 8 * buf));
-                else mbar_arrive(acce0 + 8 * buf);
-            }
-        };
         for (uint32_t t = unit; ok && t < total; t += units) {
             int z, mt, nt, first, blocks;
             tile_coords(t, m_tiles, g.n_tiles, z, mt, nt);
@@ -484,192 +452,212 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             const int64_t row0 = static_cast<int64_t>(mt) * ROWS + rank * BM + quarter * 32, row = row0 + lane;
             const int64_t col0 = static_cast<int64_t>(nt) * BN;
             const int rows = static_cast<int>(max(int64_t(0), min(int64_t(32), g.M - row0)));
-            const int cols = static_cast<int>(min(int64_t(BN), g.N - col0)), chunks = (cols + 31) >> 5;
-            const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-            const bool empty = blocks <= 0;  // no token counts: the product is zero and nothing was accumulated
-            uint32_t taddr = lanes;
-            float sums[PROMOTE ? BN / 64 : 1][32];
-            if constexpr (PROMOTE) {
+            const int cols = static_cast<int>(min(int64_t(BN), g.N - col0));
+            // this warp's chunks that hold anything: chunk i starts at column 64 i + 32 half of the tile
+            const int chunks = rows > 0 ? (cols - 32 * half + 63) >> 6 : 0;  // warp-uniform
+            const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * 32;
+            // The accumulators, added up: v[i][j] is column 64 i + 32 half + j of this lane's row. No steps at all (no token counts) leave zero.
+            float v[kChunks][32];
 #pragma unroll
-                for (int i = 0; i < BN / 64; ++i)
+            for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) sums[i][j] = 0.0f;
-                const int steps = blocks * g.terms;
-                for (int i0 = 0; i0 < steps; i0 += g.period, ++local) {
-                    const int buf = local & 1;
-                    if (!wait(accf0 + 8 * buf, (local >> 1) & 1)) { ok = false; break; }
-                    tc_fence_after();
-                    if (rows > 0) {  // warp-uniform
-#pragma unroll
-                        for (int i = 0; i < BN / 64; ++i) {
-                            if (half + 2 * i < chunks) {
-                                uint32_t v[32];
-                                tmem_load_issue(lanes + buf * BN + (half + 2 * i) * 32, v);
-                                tmem_load_wait(v);
-#pragma unroll
-                                for (int j = 0; j < 32; ++j) sums[i][j] += __uint_as_float(v[j]);
-                            }
-                        }
-                    }
-                    release(buf);
-                }
-                if (!ok) break;
-            } else if (!empty) {
+                for (int j = 0; j < 32; ++j) v[i][j] = 0.0f;
+            const int steps = blocks * g.terms;
+            for (int i0 = 0; i0 < steps; i0 += g.period, ++local) {
                 const int buf = local & 1;
                 if (!wait(accf0 + 8 * buf, (local >> 1) & 1)) { ok = false; break; }
                 tc_fence_after();
-                taddr = lanes + buf * BN;
-            }
-            // body(values, chunk) for every 32-column chunk of this warp
-            auto each = [&](auto&& body) {
-                if constexpr (PROMOTE) {
+                // two chunks at a time, so that one load runs under the other
 #pragma unroll
-                    for (int i = 0; i < BN / 64; ++i) {
-                        if (half + 2 * i < chunks) {
-                            uint32_t v[32];
+                for (int i = 0; i < kChunks; i += 2) {
+                    if (i < chunks) {
+                        uint32_t x[32], y[32];
+                        tmem_load_issue(lanes + buf * BN + i * 64, x);
+                        tmem_load_issue(lanes + buf * BN + (i + 1) * 64, y);
+                        tmem_load_wait(x);
+                        tmem_load_wait(y);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sums[i][j]);
-                            body(v, half + 2 * i);
+                        for (int j = 0; j < 32; ++j) {
+                            v[i][j] += __uint_as_float(x[j]);
+                            v[i + 1][j] += __uint_as_float(y[j]);
                         }
                     }
-                } else {
-                    drain(taddr, half, chunks, body);
                 }
-            };
+                // this warp has finished reading the accumulator: tell the block that issues the products
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (PAIR) mbar_arrive_remote(in_even_block(acce0 + 8 * buf));
+                    else mbar_arrive(acce0 + 8 * buf);
+                }
+            }
+            if (!ok) break;
             if constexpr (EPI == EPI_STATS) {
-                // where this row's target lies within the piece (anywhere outside when it has none here)
+                // where this row's target lies within the tile (anywhere outside when it has none here)
                 int64_t target = -1;
                 if (lane < rows) {
                     target = g.wide_targets ? static_cast<const int64_t*>(g.targets)[row] : static_cast<const int32_t*>(g.targets)[row];
-                    target -= g.vocab0 + col0;
+                    target -= g.vocab0 + col0 + 32 * half;
                 }
-                const int at = target >= 0 && target < cols ? static_cast<int>(target) : -1;
-                float m = -INFINITY, s = 0.0f, hit = 0.0f;
-                if (rows > 0) {  // warp-uniform
-                    each([&](uint32_t (&v)[32], int c) {
-                        online_softmax(v, min(32, cols - c * 32), m, s);
-                        if (at >= c * 32 && at < c * 32 + 32) {
+                const int at = target >= 0 && target < cols - 32 * half && ((target >> 5) & 1) == 0 ? static_cast<int>(target) : -1;
+                if (chunks > 0) {
+                    if (cols < BN) {  // warp-uniform: what lies behind the vocabulary's end has no weight
+#pragma unroll
+                        for (int i = 0; i < kChunks; ++i)
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
-                                if (at == c * 32 + j) hit = __uint_as_float(v[j]);
+                                if (64 * i + 32 * half + j >= cols) v[i][j] = -INFINITY;
+                    }
+                    // independent maxima and sums for every chunk: with two warps to a scheduler, chains are what costs
+                    float top[kChunks], s[kChunks];
+#pragma unroll
+                    for (int i = 0; i < kChunks; ++i) {
+                        top[i] = v[i][0];
+#pragma unroll
+                        for (int j = 1; j < 32; ++j) top[i] = fmaxf(top[i], v[i][j]);
+                        s[i] = 0.0f;
+                    }
+                    const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    const Exponent e(m == -INFINITY ? 0.0f : m);  // nothing but -inf: the sum stays 0
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+#pragma unroll
+                        for (int i = 0; i < kChunks; ++i) s[i] += e.power(v[i][j]);
+                    if (lane < rows) {
+                        g.halves[(g.first_half + 2 * nt + half) * g.M + row] = make_float2(m, ((s[0] + s[1]) + (s[2] + s[3])) * e.rest);
+                        if (at >= 0) {
+                            float hit = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (at == 64 * i + j) hit = v[i][j];
+                            g.target_logit[row] = hit;
                         }
-                    });
-                }
-                if (lane < rows) {
-                    g.halves[(g.first_half + 2 * nt + half) * g.M + row] = make_float2(m, s);
-                    if (at >= 0 && ((at >> 5) & 1) == half) g.target_logit[row] = hit;
+                    }
+                } else if (lane < rows) {
+                    g.halves[(g.first_half + 2 * nt + half) * g.M + row] = make_float2(-INFINITY, 0.0f);
                 }
             } else if constexpr (EPI == EPI_D) {
                 RowInfo info = {0.0f, 0.0f, kNoRow, 0};
                 if (lane < rows) info = g.rows[row];
-                const int64_t rel = info.target >= 0 ? info.target - g.vocab0 - col0 : -1;
-                const int at = rel >= 0 && rel < cols ? static_cast<int>(rel) : -1;
-                if (rows > 0) {
-                    each([&](uint32_t (&v)[32], int c) {
-                        float d[32];
-                        if (info.target == kNoRow) {
+                const int64_t target = info.target >= 0 ? info.target - g.vocab0 - col0 - 32 * half : -1;
+                const int at = target >= 0 && target < cols - 32 * half && ((target >> 5) & 1) == 0 ? static_cast<int>(target) : -1;
+                if (chunks > 0) {
+                    float hit = 0.0f;
+                    if (at >= 0) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) d[j] = 0.0f;  // whatever the logits are
-                        } else {
+                        for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) d[j] = __expf(__uint_as_float(v[j]) - info.lse) * info.grad;
-                            if (at >= c * 32 && at < c * 32 + 32) {
-                                // p - 1 without cancellation: the gradient of a token that is almost certain
-                                float hit = 0.0f;
+                            for (int j = 0; j < 32; ++j)
+                                if (at == 64 * i + j) hit = v[i][j];
+                        // p - 1 without cancellation: the gradient of a token that is almost certain
+                        hit = expm1f(hit - info.lse) * info.grad;
+                    }
+                    const Exponent e(info.lse);
+                    const float by = info.grad * e.rest;
 #pragma unroll
-                                for (int j = 0; j < 32; ++j)
-                                    if (at == c * 32 + j) hit = __uint_as_float(v[j]);
-                                hit = expm1f(hit - info.lse) * info.grad;
+                    for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-                                for (int j = 0; j < 32; ++j)
-                                    if (at == c * 32 + j) d[j] = hit;
-                            }
-                        }
-                        uint32_t w[16];
-                        const int x = static_cast<int>(col0) + c * 32, y = static_cast<int>(row0);
-                        if constexpr (PARTS == 1) {
+                        for (int j = 0; j < 32; ++j) v[i][j] = e.power(v[i][j]) * by;
+                    if (info.target == kNoRow) {
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) w[j] = pack2<T>(d[2 * j], d[2 * j + 1]);
-                            box.put(w, x, y, 0, false);
-                        } else {
-                            // the first part goes out; what it leaves stays in d for the next
+                        for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-                            for (int p = 0; p < PARTS; ++p) {
+                            for (int j = 0; j < 32; ++j) v[i][j] = 0.0f;  // whatever the logits are
+                    }
+                    if (at >= 0) {
 #pragma unroll
-                                for (int j = 0; j < 16; ++j) {
-                                    float lo, hi, unused0, unused1;
-                                    three_parts(d[2 * j], lo, unused0, unused1);
-                                    three_parts(d[2 * j + 1], hi, unused0, unused1);
-                                    w[j] = pack2<T>(lo, hi);
-                                    d[2 * j] = isfinite(d[2 * j]) ? d[2 * j] - lo : 0.0f;
-                                    d[2 * j + 1] = isfinite(d[2 * j + 1]) ? d[2 * j + 1] - hi : 0.0f;
-                                }
-                                box.put(w, x, y, p, false);
-                            }
-                        }
-                    });
-                }
-            } else if constexpr (EPI == EPI_SUM) {
-                if (rows > 0) {
-                    each([&](uint32_t (&v)[32], int c) {
+                        for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            uint32_t w[16];
+                            for (int j = 0; j < 32; ++j)
+                                if (at == 64 * i + j) v[i][j] = hit;
+                    }
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) w[j] = v[q * 16 + j];
-                            const int x = static_cast<int>(col0) + c * 32 + q * 16;
-                            if (x < g.N) box.put(w, x, static_cast<int>(row0), z, g.add != 0);
-                        }
-                    });
-                }
-            } else {
-                auto store = [&](uint32_t (&v)[32], int c) {
-                    constexpr bool F32 = std::is_same<OUT, float>::value;
+                    for (int p = 0; p < PARTS; ++p) {
+                        box.begin();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = empty ? 0u : __float_as_uint(unscale(__uint_as_float(v[j]), scale));
-                    if (g.tma_store) {
-#pragma unroll
-                        for (int q = 0; q < (F32 ? 2 : 1); ++q) {
+                        for (int i = 0; i < kChunks; ++i) {
                             uint32_t w[16];
 #pragma unroll
                             for (int j = 0; j < 16; ++j) {
-                                if constexpr (F32) w[j] = v[q * 16 + j];
-                                else w[j] = pack2<OUT>(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                                float &lo = v[i][2 * j], &hi = v[i][2 * j + 1];
+                                if constexpr (PARTS == 1) {
+                                    w[j] = pack2<T>(lo, hi);
+                                } else {
+                                    // one part goes out, what it leaves stays for the next
+                                    const float a = first_part(lo), b = first_part(hi);
+                                    w[j] = pack2<T>(a, b);
+                                    lo = isfinite(lo) ? lo - a : 0.0f;
+                                    hi = isfinite(hi) ? hi - b : 0.0f;
+                                }
                             }
-                            const int x = static_cast<int>(col0) + c * 32 + q * 16;
-                            if (x < g.N) box.put(w, x, static_cast<int>(row0), 0, false);
+                            box.fill(i, w);
                         }
-                    } else {
-                        // any alignment: through shared memory so that a store instruction runs along a row
-                        float* mine = reinterpret_cast<float*>(box.stage);
+                        box.send(chunks, [&](int i, uint32_t from) { tma_store_3d(&map_d, from, static_cast<int>(col0) + 64 * i + 32 * half, static_cast<int>(row0), p); });
+                    }
+                }
+            } else if constexpr (EPI == EPI_SUM) {
+                if (chunks > 0) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {  // 16 columns of each chunk are 64 bytes
+                        box.begin();
+#pragma unroll
+                        for (int i = 0; i < kChunks; ++i) {
+                            uint32_t w[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[i][16 * q + j]);
+                            box.fill(i, w);
+                        }
+                        box.send(chunks, [&](int i, uint32_t from) {
+                            const int x = static_cast<int>(col0) + 64 * i + 32 * half + 16 * q;
+                            if (x >= g.N) return;
+                            if (g.add) tma_add_3d(&map_d, from, x, static_cast<int>(row0), z);
+                            else tma_store_3d(&map_d, from, x, static_cast<int>(row0), z);
+                        });
+                    }
+                }
+            } else if (chunks > 0) {
+                constexpr bool F32 = std::is_same<OUT, float>::value;
+#pragma unroll
+                for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[i][j] = unscale(v[i][j], scale);
+                if (g.tma_store) {
+#pragma unroll
+                    for (int q = 0; q < (F32 ? 2 : 1); ++q) {
+                        box.begin();
+#pragma unroll
+                        for (int i = 0; i < kChunks; ++i) {
+                            uint32_t w[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                if constexpr (F32) w[j] = __float_as_uint(v[i][16 * q + j]);
+                                else w[j] = pack2<OUT>(v[i][2 * j], v[i][2 * j + 1]);
+                            }
+                            box.fill(i, w);
+                        }
+                        box.send(chunks, [&](int i, uint32_t from) {
+                            const int x = static_cast<int>(col0) + 64 * i + 32 * half + 16 * q;
+                            if (x < g.N) tma_store_3d(&map_d, from, x, static_cast<int>(row0), 0);
+                        });
+                    }
+                } else {
+                    // any alignment: through shared memory so that a store instruction runs along a row
+                    float* mine = reinterpret_cast<float*>(box.stage);
+#pragma unroll
+                    for (int i = 0; i < kChunks; ++i)
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
                             __syncwarp();
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) mine[lane * 17 + j] = __uint_as_float(v[q * 16 + j]);
+                            for (int j = 0; j < 16; ++j) mine[lane * 17 + j] = v[i][16 * q + j];
                             __syncwarp();
-                            const int64_t col = col0 + c * 32 + q * 16 + (lane & 15);
-                            if (col < g.N)
+                            const int64_t col = col0 + 64 * i + 32 * half + 16 * q + (lane & 15);
+                            if (i < chunks && col < g.N)
                                 for (int r = lane >> 4; r < rows; r += 2)
                                     static_cast<OUT*>(g.d)[(row0 + r) * g.ldd + col] = from_compute<OUT, float>(mine[r * 17 + (lane & 15)]);
                         }
-                    }
-                };
-                if (rows > 0) {
-                    if (PROMOTE || !empty) {
-                        each(store);
-                    } else {
-                        uint32_t v[32];
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = 0u;
-                        for (int c = half; c < chunks; c += 2) store(v, c);
-                    }
-                }
-            }
-            if constexpr (!PROMOTE) {
-                if (!empty) {
-                    release(local & 1);
-                    ++local;
                 }
             }
         }
@@ -1023,14 +1011,14 @@ int unit_count(bool pair) {
 // Whether a product with m result rows takes pairs: up to 128 rows the second block would have none.
 bool takes_pairs(int64_t m) { return m > BM; }
 
-template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS, bool PROMOTE, bool PAIR>
+template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS, bool PAIR>
 tn_status launch_as(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d, const LossArgs& g, cudaStream_t stream) {
     static thread_local int attr_device = -1;  // the opt-in shared-memory size belongs to kernel and device
-    auto kernel = loss_gemm<A_M, B_N, EPI, T, OUT, PARTS, PROMOTE, PAIR>;
+    auto kernel = loss_gemm<A_M, B_N, EPI, T, OUT, PARTS, PAIR>;
     int dev = 0;
     TN_CUDA(cudaGetDevice(&dev));
     if (attr_device != dev) {
-        TN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+        TN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<PAIR>));
         attr_device = dev;
     }
     const int64_t total = (int64_t)g.m_tiles * g.n_tiles * g.most_splits;
@@ -1038,7 +1026,7 @@ tn_status launch_as(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMa
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)std::min<int64_t>(total, g.units) * (PAIR ? 2 : 1));
     config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = kSmemBytes;
+    config.dynamicSmemBytes = kSmemBytes<PAIR>;
     config.stream = stream;
     cudaLaunchAttribute attribute = {};
     attribute.id = cudaLaunchAttributeClusterDimension;
@@ -1050,10 +1038,10 @@ tn_status launch_as(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMa
     TN_CUDA(cudaLaunchKernelEx(&config, kernel, a, b, d, g));
     return after_launch("loss_gemm");
 }
-template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS, bool PROMOTE>
+template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS>
 tn_status launch_one(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d, const LossArgs& g, cudaStream_t stream) {
-    return takes_pairs(g.M) ? launch_as<A_M, B_N, EPI, T, OUT, PARTS, PROMOTE, true>(a, b, d, g, stream)
-                            : launch_as<A_M, B_N, EPI, T, OUT, PARTS, PROMOTE, false>(a, b, d, g, stream);
+    return takes_pairs(g.M) ? launch_as<A_M, B_N, EPI, T, OUT, PARTS, true>(a, b, d, g, stream)
+                            : launch_as<A_M, B_N, EPI, T, OUT, PARTS, false>(a, b, d, g, stream);
 }
 
 LossArgs gemm_args(const Problem& p, int64_t m, int64_t n, int64_t k) {
@@ -1067,7 +1055,7 @@ LossArgs gemm_args(const Problem& p, int64_t m, int64_t n, int64_t k) {
     g.most_splits = 1;
     g.units = unit_count(pair);
     g.terms = p.terms;
-    g.period = kPeriod;
+    g.period = p.parts == 3 ? kPeriod : 1 << 20;
     g.is_bf16 = p.bf16;
     return g;
 }
@@ -1213,13 +1201,14 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
         TN_TRY(weight_piece(p, w, v0, n, room, &b));
         TN_TRY(b_map(&map_b, b, p.bf16, p.hidden, n, p.tokens));
         LossArgs g = gemm_args(p, p.tokens, n, p.hidden);
+        g.period = kPeriod;
         g.vocab0 = v0;
         g.targets = t;
         g.wide_targets = wide;
         g.halves = halves;
         g.first_half = first_half;
         g.target_logit = target_logit;
-        TN_TRY((launch_one<false, false, EPI_STATS, __half, float, 1, true>(map_a, map_b, map_a, g, p.stream)));
+        TN_TRY((launch_one<false, false, EPI_STATS, __half, float, 1>(map_a, map_b, map_a, g, p.stream)));
         first_half += 2 * (int64_t)g.n_tiles;
     }
     return join(p, halves, first_half, target_logit, t, wide, ignore, loss, lse);
@@ -1309,7 +1298,7 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
             g.count = count;
             g.count_is = COUNT_ROWS;
             g.rows = info;
-            TN_TRY((launch_one<false, false, EPI_D, T, float, PARTS, PARTS == 3>(rows_a, map, map_d, g, p.stream)));
+            TN_TRY((launch_one<false, false, EPI_D, T, float, PARTS>(rows_a, map, map_d, g, p.stream)));
         }
         if (dhidden) {
             CUtensorMap map_d, map_w;
@@ -1319,10 +1308,11 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
             LossArgs g = gemm_args(p, p.tokens, p.padded, n);
             g.count = count;
             g.count_is = COUNT_ROWS;
+            g.period = kPeriod;
             g.most_splits = splits;
             g.first_k_blocks = (int)ceil_div(piece, BK);
             g.add = v0 > 0;
-            TN_TRY((launch_one<false, true, EPI_SUM, T, float, 1, true>(map, map_w, map_d, g, p.stream)));
+            TN_TRY((launch_one<false, true, EPI_SUM, T, float, 1>(map, map_w, map_d, g, p.stream)));
         }
         if (dweight) {
             CUtensorMap map_d;
@@ -1338,7 +1328,7 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
             g.tma_store = can_tma_store(to, p.hidden, p.hidden * 8, BN, F32);
             map_d = map;  // placeholder when the result does not leave through TMA
             if (g.tma_store) TN_TRY(make_result_map(&map_d, to, F32, p.bf16, p.hidden, n, 1, p.hidden, 0));
-            TN_TRY((launch_one<true, true, EPI_RESULT, T, OUT, 1, PARTS == 3>(map, rows_b, map_d, g, p.stream)));
+            TN_TRY((launch_one<true, true, EPI_RESULT, T, OUT, 1>(map, rows_b, map_d, g, p.stream)));
         }
     }
     if (dhidden) {

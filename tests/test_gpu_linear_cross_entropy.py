@@ -69,6 +69,9 @@ def check_grad(g, h, w, t, lse, got, ignore=IGNORE):
     el = steps(k, h.dtype) * (Hk.abs() @ W.abs().T)
     # p from its logit: the logit's error, the subtraction, the exponential and the product with grad
     ed = p * (el + 2 * U * x.abs() + 12 * U) * 1.01 * G.abs()[:, None]
+    # The power of two is taken with subnormal results flushed: a probability below 2^-126, the smallest normal number, may be zero. That
+    # is at most 2^-126 |grad| for an entry of d, and 2^-126 sum |grad| |h| for one of dweight, of which the tolerance knew nothing.
+    ed += 2.0 ** -126 * G.abs()[:, None]
     at = torch.where(keep, T, torch.zeros_like(T))
     d = p.clone()
     d.scatter_add_(1, at[:, None], -keep.double()[:, None])
