@@ -1164,13 +1164,21 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
     float2* halves = nullptr;
     float* target_logit = nullptr;
     TN_TRY(mem.take(&target_logit, sizeof(float) * p.tokens));
-    if (few_loss_fits(p.tokens, p.hidden)) {
+    const bool few = few_loss_fits(p.dtype, p.tokens, p.hidden);
+    if (few || f32_fits(p.dtype, p.tokens, p.hidden)) {
         FewTokens f = few_tokens(p, h, w, t, wide, ignore);
-        TN_TRY(mem.take(&halves, sizeof(float2) * (size_t)few_loss_parts() * p.tokens));
+        const int64_t parts = few ? few_loss_parts() : f32_loss_parts(p.vocab);
+        TN_TRY(mem.take(&halves, sizeof(float2) * (size_t)parts * p.tokens));
         f.parts = halves;
         f.target_logit = target_logit;
-        TN_TRY(few_loss(f, p.stream));
-        return join(p, halves, few_loss_parts(), target_logit, t, wide, ignore, loss, lse);
+        if (few) {
+            TN_TRY(few_loss(f, p.stream));
+        } else {
+            float* rows = nullptr;
+            TN_TRY(mem.take(&rows, sizeof(float) * f32_row_floats(p.tokens, p.hidden)));
+            TN_TRY(f32_loss(f, rows, p.stream));
+        }
+        return join(p, halves, parts, target_logit, t, wide, ignore, loss, lse);
     }
     Operand a;
     a.parts = p.parts;
@@ -1226,16 +1234,20 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
     TN_TRY(densely(grad, &up, mem, stream));
     TN_TRY(densely(lse, &z, mem, stream));
     const int wide = targets->dtype == TN_INT64;
-    if (few_grad_fits(p.tokens, p.hidden)) {
-        FewTokens f = few_tokens(p, h, w, t, wide, ignore);
-        f.grad = static_cast<const float*>(up);
-        f.lse = static_cast<const float*>(z);
-        if (dhidden) {
-            TN_TRY(mem.take(&f.sums, sizeof(float) * (size_t)few_grad_blocks(p.vocab) * p.tokens * p.hidden));
-            f.dhidden = dhidden->address;
-        }
-        f.dweight = dweight ? dweight->address : nullptr;
-        return few_grad(f, p.stream);
+    FewTokens f = few_tokens(p, h, w, t, wide, ignore);
+    f.grad = static_cast<const float*>(up);
+    f.lse = static_cast<const float*>(z);
+    f.dhidden = dhidden ? dhidden->address : nullptr;
+    f.dweight = dweight ? dweight->address : nullptr;
+    const bool few = few_grad_fits(f);
+    if (few || f32_fits(p.dtype, p.tokens, p.hidden)) {
+        const int64_t blocks = few ? few_grad_blocks(p.vocab) : f32_grad_shares(p.hidden, p.vocab);
+        if (dhidden) TN_TRY(mem.take(&f.sums, sizeof(float) * (size_t)blocks * p.tokens * p.hidden));
+        if (few) return few_grad(f, p.stream);
+        float *rows = nullptr, *d = nullptr;
+        TN_TRY(mem.take(&rows, sizeof(float) * f32_row_floats(p.tokens, p.hidden)));
+        TN_TRY(mem.take(&d, sizeof(float) * f32_d_floats(p.tokens, p.vocab)));
+        return f32_grad(f, rows, d, p.stream);
     }
     RowInfo* info = nullptr;
     int *slot = nullptr, *count = nullptr;

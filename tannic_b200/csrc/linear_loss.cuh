@@ -1,5 +1,5 @@
-// The cross entropy of a linear layer for a few tokens: interface between the dispatcher (linear_loss.cu) and the streaming
-// kernels (linear_loss_few.cu).
+// The cross entropy of a linear layer for a few tokens: interface between the dispatcher (linear_loss.cu), the streaming
+// kernels (linear_loss_few.cu) and the float32 tiles (linear_loss_f32.cu).
 #pragma once
 
 #include "common.cuh"
@@ -16,23 +16,34 @@ struct FewTokens {
     const void* targets = nullptr;         // int64 (wide) or int32
     int wide = 0;
     int64_t ignore = 0;
-    // loss: maximum and sum of exponentials of every group of logits, [few_loss_parts][tokens], and the targets' logits
-    float2* parts = nullptr;
+    // loss: maximum and sum of exponentials of every group of logits, [groups][tokens], and the targets' logits
+    float2* parts = nullptr;               // (few_loss: few_loss_parts() groups, f32_loss: f32_loss_parts())
     float* target_logit = nullptr;
     // gradient
     const float* grad = nullptr;
     const float* lse = nullptr;
-    float* sums = nullptr;                 // [few_grad_blocks][tokens][hidden], may be null (no dhidden wanted)
+    float* sums = nullptr;                 // [blocks or shares][tokens][hidden], null where no dhidden is wanted
     void* dhidden = nullptr;
     void* dweight = nullptr;               // dense, may be null
 };
 
-bool few_loss_fits(int64_t tokens, int64_t hidden);
+bool few_loss_fits(int dtype, int64_t tokens, int64_t hidden);
 int64_t few_loss_parts();
 tn_status few_loss(const FewTokens& p, cudaStream_t stream);
 
-bool few_grad_fits(int64_t tokens, int64_t hidden);
+bool few_grad_fits(const FewTokens& p);
 int64_t few_grad_blocks(int64_t vocab);
 tn_status few_grad(const FewTokens& p, cudaStream_t stream);
+// dhidden from `n` blocks' sums
+tn_status few_dhidden(const FewTokens& p, int64_t n, cudaStream_t stream);
+
+// float32, up to 64 tokens. `h`: workspace of f32_row_floats, `d`: of f32_d_floats.
+bool f32_fits(int dtype, int64_t tokens, int64_t hidden);
+int64_t f32_loss_parts(int64_t vocab);
+size_t f32_row_floats(int64_t tokens, int64_t hidden);
+size_t f32_d_floats(int64_t tokens, int64_t vocab);
+int64_t f32_grad_shares(int64_t hidden, int64_t vocab);
+tn_status f32_loss(const FewTokens& p, float* h, cudaStream_t stream);
+tn_status f32_grad(const FewTokens& p, float* h, float* d, cudaStream_t stream);
 
 }  // namespace tnb

@@ -388,16 +388,23 @@ tn_status loss_one(const FewTokens& p, cudaStream_t stream) {
 }
 template <typename T, int VEC>
 tn_status loss_tokens(const FewTokens& p, cudaStream_t stream) {
-    if (p.tokens <= 1) return loss_one<T, VEC, 1>(p, stream);
-    if (p.tokens <= 2) return loss_one<T, VEC, 2>(p, stream);
-    if (p.tokens <= 4) return loss_one<T, VEC, 4>(p, stream);
-    return loss_one<T, VEC, 8>(p, stream);
+    if constexpr (sizeof(T) == 4) {
+        if (p.tokens > 1) return p.tokens <= 2 ? loss_one<T, VEC, 2>(p, stream) : loss_one<T, VEC, 4>(p, stream);
+    }
+    return loss_one<T, VEC, 1>(p, stream);
 }
 template <typename T>
 tn_status loss_typed(const FewTokens& p, cudaStream_t stream) {
     constexpr int VEC = 16 / sizeof(T);
     const bool wide = p.hidden % VEC == 0 && fits16(p.w, p.w_pitch * (int64_t)sizeof(T));
     return wide ? loss_tokens<T, VEC>(p, stream) : loss_tokens<T, 1>(p, stream);
+}
+
+template <typename T>
+tn_status dhidden_typed(const FewTokens& p, int64_t n, cudaStream_t stream) {
+    const bool many = p.tokens * p.hidden >= 32 * (int64_t)sm_count();
+    (many ? few_dhidden_kernel<T, 32> : few_dhidden_kernel<T, 8>)<<<(unsigned)ceil_div(p.tokens * p.hidden, many ? 32 : 8), 1024, 0, stream>>>(p, (int)n);
+    return after_launch("few_dhidden_kernel");
 }
 
 template <typename T, int VEC, int NT>
@@ -410,10 +417,7 @@ tn_status grad_one(const FewTokens& p, cudaStream_t stream) {
     const int64_t blocks = few_grad_blocks(p.vocab);
     few_grad_kernel<T, VEC, NT><<<(unsigned)blocks, threads, smem, stream>>>(p);
     TN_TRY(after_launch("few_grad_kernel"));
-    if (!p.dhidden) return TN_SUCCESS;
-    const bool many = p.tokens * p.hidden >= 32 * (int64_t)sm_count();
-    (many ? few_dhidden_kernel<T, 32> : few_dhidden_kernel<T, 8>)<<<(unsigned)ceil_div(p.tokens * p.hidden, many ? 32 : 8), 1024, 0, stream>>>(p, (int)blocks);
-    return after_launch("few_dhidden_kernel");
+    return p.dhidden ? few_dhidden(p, blocks, stream) : TN_SUCCESS;
 }
 template <typename T, int VEC>
 tn_status grad_tokens(const FewTokens& p, cudaStream_t stream) {
@@ -430,10 +434,11 @@ tn_status grad_typed(const FewTokens& p, cudaStream_t stream) {
 
 }  // namespace
 
-// Eight tokens and as many columns as shared memory takes beside them.
-bool few_loss_fits(int64_t tokens, int64_t hidden) {
-    const int64_t nt = tokens <= 1 ? 1 : tokens <= 2 ? 2 : tokens <= 4 ? 4 : 8;
-    return tokens <= 8 && nt * (hidden + 8) * 4 <= 200 * 1024;
+// As many columns as shared memory takes beside the tokens. One token of 16 bits: from two on the tensor cores are faster, empty rows and
+// all (four tokens over 32768 x 4096: 57 us against 98); float32 up to four, where its own tiles begin to be (eight: 164 us here).
+bool few_loss_fits(int dtype, int64_t tokens, int64_t hidden) {
+    const int64_t nt = tokens <= 1 ? 1 : tokens <= 2 ? 2 : 4;
+    return tokens <= (dtype == TN_FLOAT32 ? 4 : 1) && nt * (hidden + 8) * 4 <= 200 * 1024;
 }
 int64_t few_loss_parts() { return (int64_t)sm_count() * (kLossThreads / 32); }
 
@@ -445,8 +450,21 @@ tn_status few_loss(const FewTokens& p, cudaStream_t stream) {
     }
 }
 
-// Four tokens with eight columns in each of 512 threads.
-bool few_grad_fits(int64_t tokens, int64_t hidden) { return tokens <= 4 && hidden <= kGradThreads * E; }
+tn_status few_dhidden(const FewTokens& p, int64_t n, cudaStream_t stream) {
+    switch (p.dtype) {
+        case TN_FLOAT16: return dhidden_typed<__half>(p, n, stream);
+        case TN_BFLOAT16: return dhidden_typed<__nv_bfloat16>(p, n, stream);
+        default: return dhidden_typed<float>(p, n, stream);
+    }
+}
+
+// Four tokens with eight columns in each of 512 threads. Rows that are not aligned to 16 bytes are read element by element, twice, which the
+// tensor cores' copy of the weights beats for 16 bits (four tokens over 32000 x 1001: 152 us against 201).
+bool few_grad_fits(const FewTokens& p) {
+    const int size = p.dtype == TN_FLOAT32 ? 4 : 2;
+    const bool wide = p.hidden * size % 16 == 0 && fits16(p.w, p.w_pitch * size) && fits16(p.dweight, 0);
+    return p.tokens <= 4 && p.hidden <= kGradThreads * E && (wide || p.dtype == TN_FLOAT32);
+}
 int64_t few_grad_blocks(int64_t vocab) { return std::min<int64_t>(sm_count(), ceil_div(vocab, 4)); }
 
 tn_status few_grad(const FewTokens& p, cudaStream_t stream) {

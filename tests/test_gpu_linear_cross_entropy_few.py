@@ -1,5 +1,5 @@
-"""The cross entropy of a linear layer for a few tokens, where the products are one pass over the weights (up to eight tokens for the
-loss, four for the gradient): same checks and tolerances as for many."""
+"""The cross entropy of a linear layer for a few tokens, where other kernels run: one pass over the weights (one token, four for the gradient
+and for float32), tiles of the FP32 pipe (float32, up to 64 tokens). Same checks and tolerances as for many."""
 import pytest
 import torch
 
@@ -16,15 +16,23 @@ def test_sizes(tokens, hidden, vocab, dtype):
     both(*data(tokens, hidden, vocab, dtype, tokens + hidden))
 
 
+@pytest.mark.parametrize("tokens", [15, 16, 17, 31, 32, 33, 63, 64, 65])
+@pytest.mark.parametrize("hidden,vocab", [(64, 1000), (72, 129), (71, 128), (33, 127), (1024, 5003), (4, 1), (500, 3)])
+def test_float32_tiles(tokens, hidden, vocab):
+    both(*data(tokens, hidden, vocab, torch.float32, tokens + hidden, ignored=0.2))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("tokens", [1, 4, 8])
 def test_wide_rows_and_large_vocabulary(tokens, dtype):
-    both(*data(tokens, 6000, 500, dtype, 1))   # beyond the gradient's registers and, for eight tokens, the loss's shared memory
+    both(*data(tokens, 6000, 500, dtype, 1))   # beyond the gradient's registers
+    if dtype == torch.float32:
+        both(*data(tokens, 14000, 200, dtype, 1))  # and, for four tokens, the loss's shared memory
     both(*data(tokens, 128, 50257, dtype, 2))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("pattern", [[True, False, False, False], [False, True, True], [True, True, True, True], [True]])
+@pytest.mark.parametrize("pattern", [[True, False, False, False], [False, True, True], [True, True, True, True], [True], [False, True] * 9, [True] * 40])
 def test_ignored_and_undefined_tokens(pattern, dtype):
     n = len(pattern)
     h, w, t, g = data(n, 200, 600, dtype, 3)
@@ -58,15 +66,17 @@ def test_views(view, dtype):
         "transposed": lambda m: m.transpose(-1, -2).contiguous().transpose(-1, -2),
         "expanded rows": lambda m: m[:1].expand(m.shape),
     }[view]
-    h, w, t, g = data(3, 264, 301, dtype, 5)
-    both(make(h), w, t, g)
-    both(h, make(w), t, g)
-    both(h, w, t.int(), g[:1].expand(3))
+    for tokens in (3, 20):
+        h, w, t, g = data(tokens, 264, 301, dtype, 5)
+        both(make(h), w, t, g)
+        both(h, make(w), t, g)
+        both(h, w, t.int(), g[:1].expand(tokens))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_one_of_the_gradients_and_same_bits(dtype):
-    h, w, t, g = data(4, 768, 3000, dtype, 6)
+@pytest.mark.parametrize("tokens", [4, 40])
+def test_one_of_the_gradients_and_same_bits(tokens, dtype):
+    h, w, t, g = data(tokens, 768, 3000, dtype, 6)
     loss, lse = tb.linear_cross_entropy(h, w, t)
     dh, dw = tb.linear_cross_entropy_grad(g, h, w, t, lse)
     assert torch.equal(tb.linear_cross_entropy_grad(g, h, w, t, lse, dweight=False)[0], dh)
@@ -84,8 +94,9 @@ def test_logits_far_apart():
     both(h, w, best, g)
 
 
-def test_captured_and_replayed():
-    h, w, t, g = data(2, 512, 2000, torch.bfloat16, 8)
+@pytest.mark.parametrize("tokens,dtype", [(2, torch.bfloat16), (2, torch.float32), (30, torch.float32)])
+def test_captured_and_replayed(tokens, dtype):
+    h, w, t, g = data(tokens, 512, 2000, dtype, 8)
     loss, lse = tb.linear_cross_entropy(h, w, t)
     want = tb.linear_cross_entropy_grad(g, h, w, t, lse)
     side = torch.cuda.Stream()
@@ -103,13 +114,14 @@ def test_captured_and_replayed():
     check_grad(g, h, w, t, out[1], grads)
 
 
-def test_rows_behind_the_results_are_left_alone():
+@pytest.mark.parametrize("tokens,dtype", [(3, torch.bfloat16), (3, torch.float32), (20, torch.float32), (200, torch.float16)])
+def test_rows_behind_the_results_are_left_alone(tokens, dtype):
     import ctypes as C
     from tannic_b200 import _abi as A
-    h, w, t, g = data(3, 264, 301, torch.bfloat16, 9)
+    h, w, t, g = data(tokens, 264, 301, dtype, 9)
     lse = tb.linear_cross_entropy(h, w, t)[1]
     big_h, big_w = (torch.full((m.shape[0] + 4, m.shape[1]), 7.0, dtype=m.dtype, device="cuda") for m in (h, w))
-    rec = [tb.desc(x) for x in (g, h, w, t, lse, big_h[:3], big_w[:301])]
+    rec = [tb.desc(x) for x in (g, h, w, t, lse, big_h[:tokens], big_w[:301])]
     A.check(A.lib().tn_linear_cross_entropy_grad(*[C.byref(r) for r in rec], tb.current_stream(h), IGNORE))
-    check_grad(g, h, w, t, lse, (big_h[:3], big_w[:301]))
-    assert bool((big_h[3:] == 7.0).all()) and bool((big_w[301:] == 7.0).all())
+    check_grad(g, h, w, t, lse, (big_h[:tokens], big_w[:301]))
+    assert bool((big_h[tokens:] == 7.0).all()) and bool((big_w[301:] == 7.0).all())
