@@ -1167,7 +1167,7 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
     const bool few = few_loss_fits(p.dtype, p.tokens, p.hidden);
     if (few || f32_fits(p.dtype, p.tokens, p.hidden)) {
         FewTokens f = few_tokens(p, h, w, t, wide, ignore);
-        const int64_t parts = few ? few_loss_parts() : f32_loss_parts(p.vocab);
+        const int64_t parts = few ? few_loss_parts() : f32_loss_parts(p.tokens, p.vocab);
         TN_TRY(mem.take(&halves, sizeof(float2) * (size_t)parts * p.tokens));
         f.parts = halves;
         f.target_logit = target_logit;
@@ -1241,7 +1241,7 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
     f.dweight = dweight ? dweight->address : nullptr;
     const bool few = few_grad_fits(f);
     if (few || f32_fits(p.dtype, p.tokens, p.hidden)) {
-        const int64_t blocks = few ? few_grad_blocks(p.vocab) : f32_grad_shares(p.hidden, p.vocab);
+        const int64_t blocks = few ? few_grad_blocks(p.vocab) : f32_grad_shares(p.tokens, p.hidden, p.vocab);
         if (dhidden) TN_TRY(mem.take(&f.sums, sizeof(float) * (size_t)blocks * p.tokens * p.hidden));
         if (few) return few_grad(f, p.stream);
         float *rows = nullptr, *d = nullptr;

@@ -3,11 +3,13 @@
 // The tensor cores take float32 as three bfloat16 parts: W would be read (4 bytes an element), written as parts (6) and read again (6, for
 // each product), and a tile of 128 rows would be mostly empty. With N tokens the products are 2 N operations per element of W and pass, so
 // up to about 64 of them the FP32 pipe keeps up with what the parts would cost (32 tokens, 4096 x 32768: loss 596 us with parts).
-// All three products are tiles in shared memory, filled by cp.async several steps ahead, and 4 x 8 or 8 x 8 sums a thread; two
-// neighbouring elements go through one packed multiply-add.
+// All three products are tiles in shared memory, filled by cp.async several steps ahead; two neighbouring elements go through one
+// packed multiply-add. What a thread reads from shared memory has to serve many of them: in the first two a thread holds 16 tokens
+// and all lanes of a warp the same ones, so that a token's values are one broadcast for the warp (with 1 x 8 sums a thread, neighbouring
+// lanes on neighbouring tokens, shared memory was the bound and 16 tokens over 4096 x 32768 took 330 us).
 //
-//   logits  [tokens] x [128 vocabulary rows], K = hidden. Epilogue: maximum and sum of exponentials per token and tile, or d.
-//   dh      [tokens] x [128 columns], K = a share of the vocabulary; the shares' sums are added in order afterwards.
+//   logits  [tokens] x [128 or 256 vocabulary rows], K = hidden. Epilogue: maximum and sum of exponentials per token and warp, or d.
+//   dh      [tokens] x [256 columns], K = a share of the vocabulary; the shares' sums are added in order afterwards.
 //   dW      [128 vocabulary rows] x [128 columns], K = tokens: bound by writing dW.
 #include <algorithm>
 
@@ -17,7 +19,8 @@ namespace tnb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kCols = 128;       // of a tile
+constexpr int kCols = 128;       // of a tile of dW
+constexpr int kTokens = 16;      // of a thread
 constexpr int kStep = 32;        // of K
 constexpr int kPitch = kStep + 4;   // floats of a tile's row along K: 16-byte aligned, eight neighbouring rows in different banks
 constexpr int kWide = kCols + 4;    // floats of a tile's row along the columns
@@ -64,17 +67,40 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const FewTokens p, int ro
     }
 }
 
-// TM: tokens of the tile (16, 32 or 64). h: [TM][padded]. D: write d into `d` ([TM][d_pitch]), else the tile's statistics.
+// Lane i ends up with the sum (or maximum) of value i >> 1 over all lanes.
+template <bool MAX>
+__device__ __forceinline__ float lane_reduce(float (&v)[kTokens], int lane) {
+    auto two = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };
+    int o = 16;
+#pragma unroll
+    for (int n = kTokens / 2; n >= 1; n /= 2, o /= 2) {
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const bool up = lane & o;
+            const float give = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+            v[i] = two(keep, __shfl_xor_sync(0xFFFFFFFFu, give, o));
+        }
+    }
+    return two(v[0], __shfl_xor_sync(0xFFFFFFFFu, v[0], 1));
+}
+
+// TM: tokens of the tile (16, 32 or 64), sixteen to a group of warps; a warp has WIDTH vocabulary rows a lane, 32 apart.
+template <int TM> constexpr int kGroupWarps = 8 / (TM / kTokens);
+template <int TM> constexpr int kWidth = TM == 16 ? 1 : 2;
+template <int TM> constexpr int kLogitCols = kGroupWarps<TM> * 32 * kWidth<TM>;
+
+// h: [TM][padded]. D: write d into `d` ([TM][d_pitch]), else the warps' statistics.
 template <int TM, bool ALIGNED, bool D>
 __global__ void __launch_bounds__(kThreads) logits_kernel(const FewTokens p, const float* __restrict__ h, int64_t padded, float* __restrict__ d, int64_t d_pitch) {
-    constexpr int R = TM / 16;
-    extern __shared__ __align__(16) float smem[];  // [kStages][(TM + kCols)][kPitch]
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t v0 = static_cast<int64_t>(blockIdx.x) * kCols;
+    constexpr int COLS = kLogitCols<TM>, W = kWidth<TM>;
+    extern __shared__ __align__(16) float smem[];  // [kStages][(TM + COLS)][kPitch]
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int n0 = warp / kGroupWarps<TM> * kTokens, part = warp % kGroupWarps<TM>;
+    const int64_t v0 = static_cast<int64_t>(blockIdx.x) * COLS;
     const int steps = static_cast<int>((p.hidden + kStep - 1) / kStep);
     auto fill = [&](int step) {
         if (step < steps) {
-            float* a = smem + (step % kStages) * (TM + kCols) * kPitch;
+            float* a = smem + (step % kStages) * (TM + COLS) * kPitch;
             float* b = a + TM * kPitch;
             const int64_t k0 = static_cast<int64_t>(step) * kStep;
             for (int i = threadIdx.x; i < TM * (kStep / 4); i += kThreads) {
@@ -83,7 +109,7 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const FewTokens p, con
                 copy4<true>(a + r * kPitch + c, h + r * padded + (valid > 0 ? k0 + c : 0), valid);
             }
 #pragma unroll
-            for (int i = threadIdx.x; i < kCols * (kStep / 4); i += kThreads) {
+            for (int i = threadIdx.x; i < COLS * (kStep / 4); i += kThreads) {
                 const int r = i / (kStep / 4), c = i % (kStep / 4) * 4;
                 const int valid = v0 + r < p.vocab ? static_cast<int>(min(int64_t(4), p.hidden - k0 - c)) : 0;
                 copy4<ALIGNED>(b + r * kPitch + c, static_cast<const float*>(p.w) + (valid > 0 ? (v0 + r) * p.w_pitch + k0 + c : 0), valid);
@@ -93,80 +119,94 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const FewTokens p, con
     };
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) fill(s);
-    float2 acc[R][8];  // even and odd elements of K
+    float2 acc[kTokens][W];  // even and odd elements of K
 #pragma unroll
-    for (int i = 0; i < R; ++i)
+    for (int i = 0; i < kTokens; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = make_float2(0.0f, 0.0f);
+        for (int j = 0; j < W; ++j) acc[i][j] = make_float2(0.0f, 0.0f);
     for (int step = 0; step < steps; ++step) {
         wait_oldest();
         __syncthreads();  // this step's tile is there for everyone, and the last step's is read
         fill(step + kStages - 1);
-        const float* a = smem + (step % kStages) * (TM + kCols) * kPitch;
-        const float* b = a + TM * kPitch;
+        const float* a = smem + (step % kStages) * (TM + COLS) * kPitch;
+        const float* b = a + TM * kPitch + (part * 32 * W + lane) * kPitch;
+        a += n0 * kPitch;
 #pragma unroll
         for (int k = 0; k < kStep; k += 4) {
-            float4 x[R];
+            float4 y[W];
 #pragma unroll
-            for (int i = 0; i < R; ++i) x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * kPitch + k);
+            for (int j = 0; j < W; ++j) y[j] = *reinterpret_cast<const float4*>(b + 32 * j * kPitch + k);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float4 y = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * kPitch + k);
+            for (int i = 0; i < kTokens; ++i) {
+                const float4 x = *reinterpret_cast<const float4*>(a + i * kPitch + k);
 #pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    acc[i][j] = fma2(make_float2(x[i].x, x[i].y), make_float2(y.x, y.y), acc[i][j]);
-                    acc[i][j] = fma2(make_float2(x[i].z, x[i].w), make_float2(y.z, y.w), acc[i][j]);
+                for (int j = 0; j < W; ++j) {
+                    acc[i][j] = fma2(make_float2(x.x, x.y), make_float2(y[j].x, y[j].y), acc[i][j]);
+                    acc[i][j] = fma2(make_float2(x.z, x.w), make_float2(y[j].z, y[j].w), acc[i][j]);
                 }
             }
         }
     }
+    const int64_t v = v0 + part * 32 * W + lane;  // and 32 further
+    if constexpr (D) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int n = ty + 16 * i;  // the sixteen threads of a token are half a warp
-        const int64_t target = n < p.tokens ? target_of(p, n) : -1;
-        if constexpr (D) {
+        for (int i = 0; i < kTokens; ++i) {
+            const int n = n0 + i;
+            const int64_t target = n < p.tokens ? target_of(p, n) : -1;
             const bool counts = n < p.tokens && target != p.ignore;
             const float lse = counts ? p.lse[n] : 0.0f;
             const float grad = !counts ? 0.0f : target < 0 || target >= p.vocab ? NAN : p.grad[n];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int64_t v = v0 + tx + 16 * j;
+            for (int j = 0; j < W; ++j) {
                 const float x = acc[i][j].x + acc[i][j].y - lse;
-                if (v < d_pitch) d[n * d_pitch + v] = counts && v < p.vocab ? (v == target ? expm1f(x) : __expf(x)) * grad : 0.0f;
+                if (v + 32 * j < d_pitch) d[n * d_pitch + v + 32 * j] = counts && v + 32 * j < p.vocab ? (v + 32 * j == target ? expm1f(x) : __expf(x)) * grad : 0.0f;
             }
-        } else {
-            float m = -INFINITY, s = 0.0f, x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int64_t v = v0 + tx + 16 * j;
-                x[j] = v < p.vocab ? acc[i][j].x + acc[i][j].y : -INFINITY;
-                m = fmaxf(m, x[j]);
-                if (v == target && v < p.vocab) p.target_logit[n] = x[j];
-            }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-            const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s += __expf(x[j] - base);
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-            if (tx == 0 && n < p.tokens) p.parts[static_cast<int64_t>(blockIdx.x) * p.tokens + n] = make_float2(m, s);
         }
+    } else {
+        float top[kTokens], sum[kTokens];
+#pragma unroll
+        for (int i = 0; i < kTokens; ++i) {
+            const int n = n0 + i;
+            const int64_t target = n < p.tokens ? target_of(p, n) : -1;
+            top[i] = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const bool in = v + 32 * j < p.vocab;
+                acc[i][j].x = in ? acc[i][j].x + acc[i][j].y : -INFINITY;
+                top[i] = fmaxf(top[i], acc[i][j].x);
+                if (in && v + 32 * j == target) p.target_logit[n] = acc[i][j].x;
+            }
+        }
+        const float m = lane_reduce<true>(top, lane);  // of token lane / 2
+#pragma unroll
+        for (int i = 0; i < kTokens; ++i) {
+            const float mi = __shfl_sync(0xFFFFFFFFu, m, 2 * i), base = mi == -INFINITY ? 0.0f : mi;
+            sum[i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < W; ++j) sum[i] += __expf(acc[i][j].x - base);
+        }
+        const float s = lane_reduce<false>(sum, lane);
+        const int n = n0 + (lane >> 1);
+        if ((lane & 1) == 0 && n < p.tokens) p.parts[(static_cast<int64_t>(blockIdx.x) * kGroupWarps<TM> + part) * p.tokens + n] = make_float2(m, s);
     }
 }
 
-// dh's sums over the vocabulary rows [blockIdx.y * share, + share).
+// dh's sums over the vocabulary rows [blockIdx.y * share, + share): sixteen tokens and 4 columns a thread, 256 columns a block. With fewer than 64
+// tokens the warps that are left share K (kShares of them), each with sums of its own.
+constexpr int kHiddenCols = 256, kHiddenWide = kHiddenCols + 4, kHiddenStages = 3;
+template <int TM> constexpr int kShares = 4 / (TM / kTokens);
+
 template <int TM, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) dhidden_kernel(const FewTokens p, const float* __restrict__ d, int64_t d_pitch, int64_t share) {
-    constexpr int R = TM / 16;
-    extern __shared__ __align__(16) float smem[];  // [kStages][TM][kPitch] and [kStages][kStep][kWide]
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kCols, first = blockIdx.y * share, last = min(p.vocab, first + share);
+    extern __shared__ __align__(16) float smem[];  // [kHiddenStages] of [TM][kPitch] and [kStep][kHiddenWide]
+    constexpr int TILE = TM * kPitch + kStep * kHiddenWide, S = kShares<TM>, MINE = kStep / S;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int half = warp & 1, turn = (warp >> 1) % S, n0 = (warp >> 1) / S * kTokens;
+    const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kHiddenCols, first = blockIdx.y * share, last = min(p.vocab, first + share);
     const int steps = last > first ? static_cast<int>((last - first + kStep - 1) / kStep) : 0;
-    constexpr int TILE = TM * kPitch + kStep * kWide;
     auto fill = [&](int step) {
         if (step < steps) {
-            float* a = smem + (step % kStages) * TILE;
+            float* a = smem + (step % kHiddenStages) * TILE;
             float* b = a + TM * kPitch;
             const int64_t k0 = first + static_cast<int64_t>(step) * kStep;
             for (int i = threadIdx.x; i < TM * (kStep / 4); i += kThreads) {
@@ -175,58 +215,52 @@ __global__ void __launch_bounds__(kThreads) dhidden_kernel(const FewTokens p, co
                 copy4<true>(a + r * kPitch + c, d + r * d_pitch + (valid > 0 ? k0 + c : 0), valid);
             }
 #pragma unroll
-            for (int i = threadIdx.x; i < kStep * (kCols / 4); i += kThreads) {
-                const int r = i / (kCols / 4), c = i % (kCols / 4) * 4;
+            for (int i = threadIdx.x; i < kStep * (kHiddenCols / 4); i += kThreads) {
+                const int r = i / (kHiddenCols / 4), c = i % (kHiddenCols / 4) * 4;
                 const int valid = k0 + r < last ? static_cast<int>(min(int64_t(4), p.hidden - c0 - c)) : 0;
-                copy4<ALIGNED>(b + r * kWide + c, static_cast<const float*>(p.w) + (valid > 0 ? (k0 + r) * p.w_pitch + c0 + c : 0), valid);
+                copy4<ALIGNED>(b + r * kHiddenWide + c, static_cast<const float*>(p.w) + (valid > 0 ? (k0 + r) * p.w_pitch + c0 + c : 0), valid);
             }
         }
         commit();
     };
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) fill(s);
-    float2 acc[R][4];  // columns 4 tx + {0, 1}, {2, 3}, and 64 further
+    for (int s = 0; s < kHiddenStages - 1; ++s) fill(s);
+    float2 acc[kTokens][2];
 #pragma unroll
-    for (int i = 0; i < R; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = make_float2(0.0f, 0.0f);
+    for (int i = 0; i < kTokens; ++i) acc[i][0] = acc[i][1] = make_float2(0.0f, 0.0f);
     for (int step = 0; step < steps; ++step) {
-        wait_oldest();
+        asm volatile("cp.async.wait_group %0;" ::"n"(kHiddenStages - 2) : "memory");
         __syncthreads();
-        fill(step + kStages - 1);
-        const float* a = smem + (step % kStages) * TILE;
-        const float* b = a + TM * kPitch;
+        fill(step + kHiddenStages - 1);
+        const float* a = smem + (step % kHiddenStages) * TILE + n0 * kPitch + turn * MINE;
+        const float* b = smem + (step % kHiddenStages) * TILE + TM * kPitch + turn * MINE * kHiddenWide + half * 128 + 4 * lane;
+#pragma unroll 2
+        for (int k = 0; k < MINE; k += 4) {
+            float4 y[4];
 #pragma unroll
-        for (int k = 0; k < kStep; k += 4) {
-            float4 x[R];
+            for (int q = 0; q < 4; ++q) y[q] = *reinterpret_cast<const float4*>(b + (k + q) * kHiddenWide);
 #pragma unroll
-            for (int i = 0; i < R; ++i) x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * kPitch + k);
+            for (int i = 0; i < kTokens; ++i) {
+                const float4 x = *reinterpret_cast<const float4*>(a + i * kPitch + k);
+                const float s[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float4 y0 = *reinterpret_cast<const float4*>(b + (k + q) * kWide + 4 * tx), y1 = *reinterpret_cast<const float4*>(b + (k + q) * kWide + 4 * tx + 64);
-#pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    const float s = q == 0 ? x[i].x : q == 1 ? x[i].y : q == 2 ? x[i].z : x[i].w;
-                    const float2 both = make_float2(s, s);
-                    acc[i][0] = fma2(both, make_float2(y0.x, y0.y), acc[i][0]);
-                    acc[i][1] = fma2(both, make_float2(y0.z, y0.w), acc[i][1]);
-                    acc[i][2] = fma2(both, make_float2(y1.x, y1.y), acc[i][2]);
-                    acc[i][3] = fma2(both, make_float2(y1.z, y1.w), acc[i][3]);
+                for (int q = 0; q < 4; ++q) {
+                    acc[i][0] = fma2(make_float2(s[q], s[q]), make_float2(y[q].x, y[q].y), acc[i][0]);
+                    acc[i][1] = fma2(make_float2(s[q], s[q]), make_float2(y[q].z, y[q].w), acc[i][1]);
                 }
             }
         }
     }
+    const int64_t c = c0 + half * 128 + 4 * lane;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int64_t n = ty + 16 * i;
+    for (int i = 0; i < kTokens; ++i) {
+        const int64_t n = n0 + i;
         if (n < p.tokens) {
-            float* to = p.sums + (blockIdx.y * p.tokens + n) * p.hidden;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t c = c0 + 4 * tx + 64 * (j / 2) + 2 * (j % 2);
-                if (c < p.hidden) to[c] = acc[i][j].x;
-                if (c + 1 < p.hidden) to[c + 1] = acc[i][j].y;
-            }
+            float* to = p.sums + ((blockIdx.y * S + turn) * p.tokens + n) * p.hidden + c;
+            if (c < p.hidden) to[0] = acc[i][0].x;
+            if (c + 1 < p.hidden) to[1] = acc[i][0].y;
+            if (c + 2 < p.hidden) to[2] = acc[i][1].x;
+            if (c + 3 < p.hidden) to[3] = acc[i][1].y;
         }
     }
 }
@@ -304,6 +338,12 @@ bool aligned(const FewTokens& p) {
     return p.hidden % 4 == 0 && p.w_pitch % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.w) | reinterpret_cast<uintptr_t>(p.dweight)) & 15) == 0;
 }
 
+// Vocabulary rows of a block of dh: about two blocks to every SM, each with at least eight steps.
+int64_t vocabulary_share(int64_t hidden, int64_t vocab) {
+    const int64_t blocks = std::max<int64_t>(1, std::min((int64_t)sm_count() * 2 / ceil_div(hidden, kHiddenCols), vocab / (8 * kStep)));
+    return ceil_div(ceil_div(vocab, blocks), kStep) * kStep;
+}
+
 template <typename K>
 tn_status allow(K kernel, size_t smem, int& last) {
     int dev = 0;
@@ -324,9 +364,9 @@ tn_status prepare_rows(const FewTokens& p, float* h, bool drop_ignored, cudaStre
 template <int TM, bool ALIGNED, bool D>
 tn_status logits(const FewTokens& p, const float* h, float* d, int64_t d_pitch, cudaStream_t stream) {
     static thread_local int device = -1;
-    const size_t smem = sizeof(float) * kStages * (TM + kCols) * kPitch;
+    const size_t smem = sizeof(float) * kStages * (TM + kLogitCols<TM>) * kPitch;
     TN_TRY(allow(logits_kernel<TM, ALIGNED, D>, smem, device));
-    logits_kernel<TM, ALIGNED, D><<<(unsigned)ceil_div(p.vocab, kCols), kThreads, smem, stream>>>(p, h, padded_of(p.hidden), d, d_pitch);
+    logits_kernel<TM, ALIGNED, D><<<(unsigned)ceil_div(p.vocab, kLogitCols<TM>), kThreads, smem, stream>>>(p, h, padded_of(p.hidden), d, d_pitch);
     return after_launch("logits_kernel");
 }
 
@@ -336,12 +376,12 @@ tn_status gradient(const FewTokens& p, const float* h, float* d, int64_t d_pitch
     const int64_t across = ceil_div(p.hidden, kCols);
     if (p.sums) {
         static thread_local int device = -1;
-        const size_t smem = sizeof(float) * kStages * (TM * kPitch + kStep * kWide);
+        const size_t smem = sizeof(float) * kHiddenStages * (TM * kPitch + kStep * kHiddenWide);
         TN_TRY(allow(dhidden_kernel<TM, ALIGNED>, smem, device));
-        const int64_t shares = f32_grad_shares(p.hidden, p.vocab), share = ceil_div(ceil_div(p.vocab, shares), kStep) * kStep;
-        dhidden_kernel<TM, ALIGNED><<<dim3((unsigned)across, (unsigned)shares), kThreads, smem, stream>>>(p, d, d_pitch, share);
+        const int64_t share = vocabulary_share(p.hidden, p.vocab);
+        dhidden_kernel<TM, ALIGNED><<<dim3((unsigned)ceil_div(p.hidden, kHiddenCols), (unsigned)ceil_div(p.vocab, share)), kThreads, smem, stream>>>(p, d, d_pitch, share);
         TN_TRY(after_launch("dhidden_kernel"));
-        TN_TRY(few_dhidden(p, shares, stream));
+        TN_TRY(few_dhidden(p, f32_grad_shares(p.tokens, p.hidden, p.vocab), stream));
     }
     if (p.dweight) {
         static thread_local int device = -1;
@@ -358,13 +398,17 @@ tn_status gradient(const FewTokens& p, const float* h, float* d, int64_t d_pitch
 
 // Up to 64 tokens; grid extents within their limits.
 bool f32_fits(int dtype, int64_t tokens, int64_t hidden) { return dtype == TN_FLOAT32 && tokens <= 64 && hidden <= int64_t(1) << 20; }
-int64_t f32_loss_parts(int64_t vocab) { return ceil_div(vocab, kCols); }
+int64_t f32_loss_parts(int64_t tokens, int64_t vocab) {
+    switch (token_rows(tokens)) {
+        case 16: return ceil_div(vocab, kLogitCols<16>) * kGroupWarps<16>;
+        case 32: return ceil_div(vocab, kLogitCols<32>) * kGroupWarps<32>;
+        default: return ceil_div(vocab, kLogitCols<64>) * kGroupWarps<64>;
+    }
+}
 size_t f32_row_floats(int64_t tokens, int64_t hidden) { return (size_t)token_rows(tokens) * padded_of(hidden); }
 size_t f32_d_floats(int64_t tokens, int64_t vocab) { return (size_t)token_rows(tokens) * padded_of(vocab); }
-// Shares of the vocabulary for dh: two blocks to every SM, each with at least eight steps.
-int64_t f32_grad_shares(int64_t hidden, int64_t vocab) {
-    const int64_t shares = std::max<int64_t>(1, std::min((int64_t)sm_count() * 2 / ceil_div(hidden, kCols), vocab / (8 * kStep)));
-    return ceil_div(vocab, ceil_div(ceil_div(vocab, shares), kStep) * kStep);
+int64_t f32_grad_shares(int64_t tokens, int64_t hidden, int64_t vocab) {
+    return ceil_div(vocab, vocabulary_share(hidden, vocab)) * (64 / token_rows(tokens));
 }
 
 tn_status f32_loss(const FewTokens& p, float* h, cudaStream_t stream) {
