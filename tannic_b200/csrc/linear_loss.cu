@@ -1165,7 +1165,7 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
     float* target_logit = nullptr;
     TN_TRY(mem.take(&target_logit, sizeof(float) * p.tokens));
     const bool few = few_loss_fits(p.dtype, p.tokens, p.hidden);
-    if (few || f32_fits(p.dtype, p.tokens, p.hidden)) {
+    if (few || f32_fits(p.dtype, p.tokens, p.hidden, false)) {
         FewTokens f = few_tokens(p, h, w, t, wide, ignore);
         const int64_t parts = few ? few_loss_parts() : f32_loss_parts(p.tokens, p.vocab);
         TN_TRY(mem.take(&halves, sizeof(float2) * (size_t)parts * p.tokens));
@@ -1240,8 +1240,8 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
     f.dhidden = dhidden ? dhidden->address : nullptr;
     f.dweight = dweight ? dweight->address : nullptr;
     const bool few = few_grad_fits(f);
-    if (few || f32_fits(p.dtype, p.tokens, p.hidden)) {
-        const int64_t blocks = few ? few_grad_blocks(p.vocab) : f32_grad_shares(p.tokens, p.hidden, p.vocab);
+    if (few || f32_fits(p.dtype, p.tokens, p.hidden, true)) {
+        const int64_t blocks = few ? few_grad_blocks(p.vocab) : f32_grad_shares(p.hidden, p.vocab);
         if (dhidden) TN_TRY(mem.take(&f.sums, sizeof(float) * (size_t)blocks * p.tokens * p.hidden));
         if (few) return few_grad(f, p.stream);
         float *rows = nullptr, *d = nullptr;

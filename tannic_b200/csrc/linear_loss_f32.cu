@@ -1,12 +1,12 @@
-// The cross entropy of a linear layer and its gradient for up to 64 tokens of float32, on the FP32 pipe.
+// The cross entropy of a linear layer and its gradient for up to 64 tokens of float32.
 //
-// The tensor cores take float32 as three bfloat16 parts: W would be read (4 bytes an element), written as parts (6) and read again (6, for
-// each product), and a tile of 128 rows would be mostly empty. With N tokens the products are 2 N operations per element of W and pass, so
-// up to about 64 of them the FP32 pipe keeps up with what the parts would cost (32 tokens, 4096 x 32768: loss 596 us with parts).
-// All three products are tiles in shared memory, filled by cp.async several steps ahead; two neighbouring elements go through one
-// packed multiply-add. What a thread reads from shared memory has to serve many of them: in the first two a thread holds 16 tokens
-// and all lanes of a warp the same ones, so that a token's values are one broadcast for the warp (with 1 x 8 sums a thread, neighbouring
-// lanes on neighbouring tokens, shared memory was the bound and 16 tokens over 4096 x 32768 took 330 us).
+// The large path writes float32 weights out as three bfloat16 parts first: 4 bytes an element read, 6 written, and 6 read again for each
+// product, which for a few tokens is most of the time (16 tokens over 4096 x 32768: loss 594 us, the FP32 pipe 198 us).
+// Here W stays as it is. Its tiles come into shared memory by cp.async, several steps ahead, and a warp splits its fragments in registers:
+// x = hi + lo, both tf32 (11 significand bits each, rounded to nearest), a b = hi hi + hi lo + lo hi; what is left out is below
+// 2^-22 of the product and of either sign. The products run as mma.sync m16n8k8: tcgen05 takes its operands from shared memory, where
+// the parts would have to be written back, and its 128-row tile would be mostly empty; the bound is W's way through shared memory.
+// The tensor cores cut off below an accumulator's last place, so every step of 32 starts from zero and is added in float32.
 //
 //   logits  [tokens] x [128 or 256 vocabulary rows], K = hidden. Epilogue: maximum and sum of exponentials per token and warp, or d.
 //   dh      [tokens] x [256 columns], K = a share of the vocabulary; the shares' sums are added in order afterwards.
@@ -19,22 +19,57 @@ namespace tnb {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
 constexpr int kCols = 128;       // of a tile of dW
-constexpr int kTokens = 16;      // of a thread
 constexpr int kStep = 32;        // of K
-constexpr int kPitch = kStep + 4;   // floats of a tile's row along K: 16-byte aligned, eight neighbouring rows in different banks
-constexpr int kWide = kCols + 4;    // floats of a tile's row along the columns
-constexpr int kStages = 4;
+constexpr int kPitch = kStep + 4;   // floats of a tile's row along K: rows g and columns t of a fragment lie in banks 4 g + t
+constexpr int kWide = kCols + 8;    // floats of a tile's row along the columns: rows t and columns g in banks 8 t + g
+constexpr int kStages = 3;
 
-__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
-    uint64_t a, b, c, r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(x.x), "f"(x.y));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(y.x), "f"(y.y));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(c) : "f"(z.x), "f"(z.y));
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    float2 v;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
-    return v;
+// A fragment's element as two tf32.
+struct Split { uint32_t hi, lo; };
+__device__ __forceinline__ Split split(float x) {
+    Split s;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(s.hi) : "f"(x));
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(s.lo) : "f"(x - __uint_as_float(s.hi)));
+    return s;
+}
+// c += a b for 16 x 8 x 8: lane (g = lane / 4, t = lane % 4) holds a at rows g, g + 8 and columns t, t + 4 (row first), b at rows t, t + 4 of
+// column g, c at rows g, g + 8 (row last) and columns 2 t, 2 t + 1.
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+struct FragmentA { uint32_t hi[4], lo[4]; };
+struct FragmentB { uint32_t hi[2], lo[2]; };
+// element(row, k) and element(k, column)
+template <typename F>
+__device__ __forceinline__ FragmentA fragment_a(F&& element, int g, int t) {
+    FragmentA f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const Split s = split(element(g + 8 * (q & 1), t + 4 * (q >> 1)));
+        f.hi[q] = s.hi;
+        f.lo[q] = s.lo;
+    }
+    return f;
+}
+template <typename F>
+__device__ __forceinline__ FragmentB fragment_b(F&& element, int g, int t) {
+    FragmentB f;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const Split s = split(element(t + 4 * q, g));
+        f.hi[q] = s.hi;
+        f.lo[q] = s.lo;
+    }
+    return f;
+}
+__device__ __forceinline__ void mma3(float (&c)[4], const FragmentA& a, const FragmentB& b) {
+    mma(c, a.lo, b.hi);
+    mma(c, a.hi, b.lo);
+    mma(c, a.hi, b.hi);
 }
 
 __device__ __forceinline__ int64_t target_of(const FewTokens& p, int64_t n) {
@@ -58,52 +93,38 @@ __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;"
 // until the oldest of kStages - 1 groups has arrived
 __device__ __forceinline__ void wait_oldest() { asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory"); }
 
-// The tokens as the products read them: [rows][padded], zero where there is no token, no target (that is for the gradient) or no column.
+// The tokens as the products read them: [rows][padded], zero where there is no token, no target (that is for the gradient) or no column; behind
+// them their hi and lo, which every warp of the logits would otherwise work out for itself.
 __global__ void __launch_bounds__(256) few_rows_kernel(const FewTokens p, int rows, int64_t padded, int drop_ignored, float* __restrict__ out) {
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < rows * padded; i += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t n = i / padded, c = i - n * padded;
         const bool in = n < p.tokens && c < p.hidden && !(drop_ignored && target_of(p, n) == p.ignore);
-        out[i] = in ? static_cast<const float*>(p.h)[n * p.h_pitch + c] : 0.0f;
+        const float x = in ? static_cast<const float*>(p.h)[n * p.h_pitch + c] : 0.0f;
+        const Split s = split(x);
+        out[i] = x;
+        out[i + rows * padded] = __uint_as_float(s.hi);
+        out[i + 2 * rows * padded] = __uint_as_float(s.lo);
     }
 }
 
-// Lane i ends up with the sum (or maximum) of value i >> 1 over all lanes.
-template <bool MAX>
-__device__ __forceinline__ float lane_reduce(float (&v)[kTokens], int lane) {
-    auto two = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };
-    int o = 16;
-#pragma unroll
-    for (int n = kTokens / 2; n >= 1; n /= 2, o /= 2) {
-#pragma unroll
-        for (int i = 0; i < n; ++i) {
-            const bool up = lane & o;
-            const float give = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
-            v[i] = two(keep, __shfl_xor_sync(0xFFFFFFFFu, give, o));
-        }
-    }
-    return two(v[0], __shfl_xor_sync(0xFFFFFFFFu, v[0], 1));
-}
+// TM: tokens of the tile (16, 32 or 64). A warp has all of them and NT fragments of eight vocabulary rows.
+template <int TM> constexpr int kFragments = TM == 64 ? 2 : 4;
+template <int TM> constexpr int kLogitCols = kWarps * 8 * kFragments<TM>;
 
-// TM: tokens of the tile (16, 32 or 64), sixteen to a group of warps; a warp has WIDTH vocabulary rows a lane, 32 apart.
-template <int TM> constexpr int kGroupWarps = 8 / (TM / kTokens);
-template <int TM> constexpr int kWidth = TM == 16 ? 1 : 2;
-template <int TM> constexpr int kLogitCols = kGroupWarps<TM> * 32 * kWidth<TM>;
-
-// h: [TM][padded]. D: write d into `d` ([TM][d_pitch]), else the warps' statistics.
+// h: hi and lo of the tokens, [2][TM][padded]. D: write d into `d` ([TM][d_pitch]), else the warps' statistics.
 template <int TM, bool ALIGNED, bool D>
 __global__ void __launch_bounds__(kThreads) logits_kernel(const FewTokens p, const float* __restrict__ h, int64_t padded, float* __restrict__ d, int64_t d_pitch) {
-    constexpr int COLS = kLogitCols<TM>, W = kWidth<TM>;
-    extern __shared__ __align__(16) float smem[];  // [kStages][(TM + COLS)][kPitch]
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int n0 = warp / kGroupWarps<TM> * kTokens, part = warp % kGroupWarps<TM>;
+    constexpr int COLS = kLogitCols<TM>, MT = TM / 16, NT = kFragments<TM>;
+    extern __shared__ __align__(16) float smem[];  // [kStages][2 TM + COLS][kPitch]
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int64_t v0 = static_cast<int64_t>(blockIdx.x) * COLS;
     const int steps = static_cast<int>((p.hidden + kStep - 1) / kStep);
     auto fill = [&](int step) {
         if (step < steps) {
-            float* a = smem + (step % kStages) * (TM + COLS) * kPitch;
-            float* b = a + TM * kPitch;
+            float* a = smem + (step % kStages) * (2 * TM + COLS) * kPitch;
+            float* b = a + 2 * TM * kPitch;
             const int64_t k0 = static_cast<int64_t>(step) * kStep;
-            for (int i = threadIdx.x; i < TM * (kStep / 4); i += kThreads) {
+            for (int i = threadIdx.x; i < 2 * TM * (kStep / 4); i += kThreads) {
                 const int r = i / (kStep / 4), c = i % (kStep / 4) * 4;
                 const int valid = static_cast<int>(min(int64_t(4), padded - k0 - c));
                 copy4<true>(a + r * kPitch + c, h + r * padded + (valid > 0 ? k0 + c : 0), valid);
@@ -119,89 +140,102 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const FewTokens p, con
     };
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) fill(s);
-    float2 acc[kTokens][W];  // even and odd elements of K
+    float sum[MT][NT][4];
 #pragma unroll
-    for (int i = 0; i < kTokens; ++i)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < W; ++j) acc[i][j] = make_float2(0.0f, 0.0f);
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) sum[i][j][q] = 0.0f;
     for (int step = 0; step < steps; ++step) {
         wait_oldest();
         __syncthreads();  // this step's tile is there for everyone, and the last step's is read
         fill(step + kStages - 1);
-        const float* a = smem + (step % kStages) * (TM + COLS) * kPitch;
-        const float* b = a + TM * kPitch + (part * 32 * W + lane) * kPitch;
-        a += n0 * kPitch;
+        const float* a = smem + (step % kStages) * (2 * TM + COLS) * kPitch;
+        const float* b = a + (2 * TM + warp * 8 * NT) * kPitch;
+        float part[MT][NT][4];
 #pragma unroll
-        for (int k = 0; k < kStep; k += 4) {
-            float4 y[W];
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < W; ++j) y[j] = *reinterpret_cast<const float4*>(b + 32 * j * kPitch + k);
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int i = 0; i < kTokens; ++i) {
-                const float4 x = *reinterpret_cast<const float4*>(a + i * kPitch + k);
+                for (int q = 0; q < 4; ++q) part[i][j][q] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < W; ++j) {
-                    acc[i][j] = fma2(make_float2(x.x, x.y), make_float2(y[j].x, y[j].y), acc[i][j]);
-                    acc[i][j] = fma2(make_float2(x.z, x.w), make_float2(y[j].z, y[j].w), acc[i][j]);
+        for (int k = 0; k < kStep; k += 8) {
+            FragmentB y[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) y[j] = fragment_b([&](int kk, int c) { return b[(8 * j + c) * kPitch + k + kk]; }, g, t);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                FragmentA x;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float* at = a + (16 * i + g + 8 * (q & 1)) * kPitch + k + t + 4 * (q >> 1);
+                    x.hi[q] = __float_as_uint(at[0]);
+                    x.lo[q] = __float_as_uint(at[TM * kPitch]);
                 }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) mma3(part[i][j], x, y[j]);
             }
         }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) sum[i][j][q] += part[i][j][q];
     }
-    const int64_t v = v0 + part * 32 * W + lane;  // and 32 further
-    if constexpr (D) {
+    // lane (g, t) holds tokens 16 i + g and + 8, vocabulary rows 8 j + 2 t and + 1 of its warp's
+    const int64_t first = v0 + warp * 8 * NT + 2 * t;
 #pragma unroll
-        for (int i = 0; i < kTokens; ++i) {
-            const int n = n0 + i;
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int up = 0; up < 2; ++up) {
+            const int n = 16 * i + g + 8 * up;
             const int64_t target = n < p.tokens ? target_of(p, n) : -1;
-            const bool counts = n < p.tokens && target != p.ignore;
-            const float lse = counts ? p.lse[n] : 0.0f;
-            const float grad = !counts ? 0.0f : target < 0 || target >= p.vocab ? NAN : p.grad[n];
+            if constexpr (D) {
+                const bool counts = n < p.tokens && target != p.ignore;
+                const float lse = counts ? p.lse[n] : 0.0f;
+                const float grad = !counts ? 0.0f : target < 0 || target >= p.vocab ? NAN : p.grad[n];
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-                const float x = acc[i][j].x + acc[i][j].y - lse;
-                if (v + 32 * j < d_pitch) d[n * d_pitch + v + 32 * j] = counts && v + 32 * j < p.vocab ? (v + 32 * j == target ? expm1f(x) : __expf(x)) * grad : 0.0f;
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int64_t v = first + 8 * j + q;
+                        const float x = sum[i][j][2 * up + q] - lse;
+                        if (v < d_pitch) d[n * d_pitch + v] = counts && v < p.vocab ? (v == target ? expm1f(x) : __expf(x)) * grad : 0.0f;
+                    }
+            } else {
+                float m = -INFINITY, s = 0.0f, x[NT][2];
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int64_t v = first + 8 * j + q;
+                        x[j][q] = v < p.vocab ? sum[i][j][2 * up + q] : -INFINITY;
+                        m = fmaxf(m, x[j][q]);
+                        if (v == target && v < p.vocab) p.target_logit[n] = x[j][q];
+                    }
+                m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+                m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+                const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) s += __expf(x[j][0] - base) + __expf(x[j][1] - base);
+                s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
+                s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
+                if (t == 0 && n < p.tokens) p.parts[(static_cast<int64_t>(blockIdx.x) * kWarps + warp) * p.tokens + n] = make_float2(m, s);
             }
         }
-    } else {
-        float top[kTokens], sum[kTokens];
-#pragma unroll
-        for (int i = 0; i < kTokens; ++i) {
-            const int n = n0 + i;
-            const int64_t target = n < p.tokens ? target_of(p, n) : -1;
-            top[i] = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < W; ++j) {
-                const bool in = v + 32 * j < p.vocab;
-                acc[i][j].x = in ? acc[i][j].x + acc[i][j].y : -INFINITY;
-                top[i] = fmaxf(top[i], acc[i][j].x);
-                if (in && v + 32 * j == target) p.target_logit[n] = acc[i][j].x;
-            }
-        }
-        const float m = lane_reduce<true>(top, lane);  // of token lane / 2
-#pragma unroll
-        for (int i = 0; i < kTokens; ++i) {
-            const float mi = __shfl_sync(0xFFFFFFFFu, m, 2 * i), base = mi == -INFINITY ? 0.0f : mi;
-            sum[i] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < W; ++j) sum[i] += __expf(acc[i][j].x - base);
-        }
-        const float s = lane_reduce<false>(sum, lane);
-        const int n = n0 + (lane >> 1);
-        if ((lane & 1) == 0 && n < p.tokens) p.parts[(static_cast<int64_t>(blockIdx.x) * kGroupWarps<TM> + part) * p.tokens + n] = make_float2(m, s);
-    }
 }
 
-// dh's sums over the vocabulary rows [blockIdx.y * share, + share): sixteen tokens and 4 columns a thread, 256 columns a block. With fewer than 64
-// tokens the warps that are left share K (kShares of them), each with sums of its own.
-constexpr int kHiddenCols = 256, kHiddenWide = kHiddenCols + 4, kHiddenStages = 3;
-template <int TM> constexpr int kShares = 4 / (TM / kTokens);
+// dh's sums over the vocabulary rows [blockIdx.y * share, + share): 256 columns a block, 32 a warp.
+constexpr int kHiddenCols = 256, kHiddenWide = kHiddenCols + 8, kHiddenStages = 3;
 
 template <int TM, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) dhidden_kernel(const FewTokens p, const float* __restrict__ d, int64_t d_pitch, int64_t share) {
     extern __shared__ __align__(16) float smem[];  // [kHiddenStages] of [TM][kPitch] and [kStep][kHiddenWide]
-    constexpr int TILE = TM * kPitch + kStep * kHiddenWide, S = kShares<TM>, MINE = kStep / S;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int half = warp & 1, turn = (warp >> 1) % S, n0 = (warp >> 1) / S * kTokens;
+    constexpr int TILE = TM * kPitch + kStep * kHiddenWide, MT = TM / 16, NT = kHiddenCols / kWarps / 8;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kHiddenCols, first = blockIdx.y * share, last = min(p.vocab, first + share);
     const int steps = last > first ? static_cast<int>((last - first + kStep - 1) / kStep) : 0;
     auto fill = [&](int step) {
@@ -225,51 +259,61 @@ __global__ void __launch_bounds__(kThreads) dhidden_kernel(const FewTokens p, co
     };
 #pragma unroll
     for (int s = 0; s < kHiddenStages - 1; ++s) fill(s);
-    float2 acc[kTokens][2];
+    float sum[MT][NT][4];
 #pragma unroll
-    for (int i = 0; i < kTokens; ++i) acc[i][0] = acc[i][1] = make_float2(0.0f, 0.0f);
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) sum[i][j][q] = 0.0f;
     for (int step = 0; step < steps; ++step) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kHiddenStages - 2) : "memory");
         __syncthreads();
         fill(step + kHiddenStages - 1);
-        const float* a = smem + (step % kHiddenStages) * TILE + n0 * kPitch + turn * MINE;
-        const float* b = smem + (step % kHiddenStages) * TILE + TM * kPitch + turn * MINE * kHiddenWide + half * 128 + 4 * lane;
-#pragma unroll 2
-        for (int k = 0; k < MINE; k += 4) {
-            float4 y[4];
+        const float* a = smem + (step % kHiddenStages) * TILE;
+        const float* b = a + TM * kPitch + warp * 8 * NT;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) y[q] = *reinterpret_cast<const float4*>(b + (k + q) * kHiddenWide);
+        for (int i = 0; i < MT; ++i) {  // sixteen tokens at a time: their step from zero takes 16 registers
+            float part[NT][4];
 #pragma unroll
-            for (int i = 0; i < kTokens; ++i) {
-                const float4 x = *reinterpret_cast<const float4*>(a + i * kPitch + k);
-                const float s[4] = {x.x, x.y, x.z, x.w};
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    acc[i][0] = fma2(make_float2(s[q], s[q]), make_float2(y[q].x, y[q].y), acc[i][0]);
-                    acc[i][1] = fma2(make_float2(s[q], s[q]), make_float2(y[q].z, y[q].w), acc[i][1]);
+                for (int q = 0; q < 4; ++q) part[j][q] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kStep; k += 8) {
+                const FragmentA x = fragment_a([&](int r, int kk) { return a[(16 * i + r) * kPitch + k + kk]; }, g, t);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) mma3(part[j], x, fragment_b([&](int kk, int c) { return b[(k + kk) * kHiddenWide + 8 * j + c]; }, g, t));
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) sum[i][j][q] += part[j][q];
+        }
+    }
+    const int64_t column = c0 + warp * 8 * NT + 2 * t;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int64_t n = 16 * i + g + 8 * (q >> 1);
+            if (n < p.tokens) {
+                float* to = p.sums + (blockIdx.y * p.tokens + n) * p.hidden;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const int64_t c = column + 8 * j + (q & 1);
+                    if (c < p.hidden) to[c] = sum[i][j][q];
                 }
             }
         }
-    }
-    const int64_t c = c0 + half * 128 + 4 * lane;
-#pragma unroll
-    for (int i = 0; i < kTokens; ++i) {
-        const int64_t n = n0 + i;
-        if (n < p.tokens) {
-            float* to = p.sums + ((blockIdx.y * S + turn) * p.tokens + n) * p.hidden + c;
-            if (c < p.hidden) to[0] = acc[i][0].x;
-            if (c + 1 < p.hidden) to[1] = acc[i][0].y;
-            if (c + 2 < p.hidden) to[2] = acc[i][1].x;
-            if (c + 3 < p.hidden) to[3] = acc[i][1].y;
-        }
-    }
 }
 
-// dW: a tile of 128 x 128, K = the tokens, all of them in shared memory at once.
+// dW: a tile of 128 x 128, K = the tokens, all of them in shared memory at once; a warp has 32 vocabulary rows and 64 columns.
 template <int TM, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) dweight_kernel(const FewTokens p, const float* __restrict__ h, int64_t padded, const float* __restrict__ d, int64_t d_pitch) {
     extern __shared__ __align__(16) float smem[];  // [TM][kWide] of d and of h
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int row = warp / 2 * 32, column = warp % 2 * 64;
     const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kCols;
     float* a = smem;
     float* b = smem + TM * kWide;
@@ -289,45 +333,44 @@ __global__ void __launch_bounds__(kThreads) dweight_kernel(const FewTokens p, co
         commit();
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();
-        float2 acc[8][4];
+        float sum[2][8][4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = make_float2(0.0f, 0.0f);
-#pragma unroll 4
-        for (int k = 0; k < TM; ++k) {
-            const float4 x0 = *reinterpret_cast<const float4*>(a + k * kWide + 4 * ty), x1 = *reinterpret_cast<const float4*>(a + k * kWide + 4 * ty + 64);
-            const float4 y0 = *reinterpret_cast<const float4*>(b + k * kWide + 4 * tx), y1 = *reinterpret_cast<const float4*>(b + k * kWide + 4 * tx + 64);
-            const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+            for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float2 both = make_float2(x[i], x[i]);
-                acc[i][0] = fma2(both, make_float2(y0.x, y0.y), acc[i][0]);
-                acc[i][1] = fma2(both, make_float2(y0.z, y0.w), acc[i][1]);
-                acc[i][2] = fma2(both, make_float2(y1.x, y1.y), acc[i][2]);
-                acc[i][3] = fma2(both, make_float2(y1.z, y1.w), acc[i][3]);
+                for (int q = 0; q < 4; ++q) sum[i][j][q] = 0.0f;
+#pragma unroll 2
+        for (int k = 0; k < TM; k += 8) {
+            FragmentA x[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) x[i] = fragment_a([&](int r, int kk) { return a[(k + kk) * kWide + row + 16 * i + r]; }, g, t);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const FragmentB y = fragment_b([&](int kk, int c) { return b[(k + kk) * kWide + column + 8 * j + c]; }, g, t);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) mma3(sum[i][j], x[i], y);
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int64_t v = v0 + 4 * ty + 64 * (i / 4) + i % 4;
-            if (v < p.vocab) {
-                float* to = static_cast<float*>(p.dweight) + v * p.hidden;
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const int64_t c = c0 + 4 * tx + 64 * q;
-                    const float4 out = make_float4(acc[i][2 * q].x, acc[i][2 * q].y, acc[i][2 * q + 1].x, acc[i][2 * q + 1].y);
-                    if (ALIGNED) {
-                        if (c < p.hidden) *reinterpret_cast<float4*>(to + c) = out;
-                    } else {
-                        if (c < p.hidden) to[c] = out.x;
-                        if (c + 1 < p.hidden) to[c + 1] = out.y;
-                        if (c + 2 < p.hidden) to[c + 2] = out.z;
-                        if (c + 3 < p.hidden) to[c + 3] = out.w;
+            for (int up = 0; up < 2; ++up) {
+                const int64_t v = v0 + row + 16 * i + g + 8 * up;
+                if (v < p.vocab) {
+                    float* to = static_cast<float*>(p.dweight) + v * p.hidden;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int64_t c = c0 + column + 8 * j + 2 * t;
+                        if (ALIGNED) {
+                            if (c < p.hidden) *reinterpret_cast<float2*>(to + c) = make_float2(sum[i][j][2 * up], sum[i][j][2 * up + 1]);
+                        } else {
+                            if (c < p.hidden) to[c] = sum[i][j][2 * up];
+                            if (c + 1 < p.hidden) to[c + 1] = sum[i][j][2 * up + 1];
+                        }
                     }
                 }
             }
-        }
     }
 }
 
@@ -364,9 +407,9 @@ tn_status prepare_rows(const FewTokens& p, float* h, bool drop_ignored, cudaStre
 template <int TM, bool ALIGNED, bool D>
 tn_status logits(const FewTokens& p, const float* h, float* d, int64_t d_pitch, cudaStream_t stream) {
     static thread_local int device = -1;
-    const size_t smem = sizeof(float) * kStages * (TM + kLogitCols<TM>) * kPitch;
+    const size_t smem = sizeof(float) * kStages * (2 * TM + kLogitCols<TM>) * kPitch;
     TN_TRY(allow(logits_kernel<TM, ALIGNED, D>, smem, device));
-    logits_kernel<TM, ALIGNED, D><<<(unsigned)ceil_div(p.vocab, kLogitCols<TM>), kThreads, smem, stream>>>(p, h, padded_of(p.hidden), d, d_pitch);
+    logits_kernel<TM, ALIGNED, D><<<(unsigned)ceil_div(p.vocab, kLogitCols<TM>), kThreads, smem, stream>>>(p, h + TM * padded_of(p.hidden), padded_of(p.hidden), d, d_pitch);
     return after_launch("logits_kernel");
 }
 
@@ -381,7 +424,7 @@ tn_status gradient(const FewTokens& p, const float* h, float* d, int64_t d_pitch
         const int64_t share = vocabulary_share(p.hidden, p.vocab);
         dhidden_kernel<TM, ALIGNED><<<dim3((unsigned)ceil_div(p.hidden, kHiddenCols), (unsigned)ceil_div(p.vocab, share)), kThreads, smem, stream>>>(p, d, d_pitch, share);
         TN_TRY(after_launch("dhidden_kernel"));
-        TN_TRY(few_dhidden(p, f32_grad_shares(p.tokens, p.hidden, p.vocab), stream));
+        TN_TRY(few_dhidden(p, f32_grad_shares(p.hidden, p.vocab), stream));
     }
     if (p.dweight) {
         static thread_local int device = -1;
@@ -396,20 +439,21 @@ tn_status gradient(const FewTokens& p, const float* h, float* d, int64_t d_pitch
 
 }  // namespace
 
-// Up to 64 tokens; grid extents within their limits.
-bool f32_fits(int dtype, int64_t tokens, int64_t hidden) { return dtype == TN_FLOAT32 && tokens <= 64 && hidden <= int64_t(1) << 20; }
+// The loss up to 64 tokens and the gradient up to 32, where the bfloat16 parts of the large path have paid (4096 x 32768, 64 tokens: see the
+// figures at the top); grid extents within their limits.
+bool f32_fits(int dtype, int64_t tokens, int64_t hidden, bool gradient) {
+    return dtype == TN_FLOAT32 && tokens <= (gradient ? 32 : 64) && hidden <= int64_t(1) << 20;
+}
 int64_t f32_loss_parts(int64_t tokens, int64_t vocab) {
     switch (token_rows(tokens)) {
-        case 16: return ceil_div(vocab, kLogitCols<16>) * kGroupWarps<16>;
-        case 32: return ceil_div(vocab, kLogitCols<32>) * kGroupWarps<32>;
-        default: return ceil_div(vocab, kLogitCols<64>) * kGroupWarps<64>;
+        case 16: return ceil_div(vocab, kLogitCols<16>) * kWarps;
+        case 32: return ceil_div(vocab, kLogitCols<32>) * kWarps;
+        default: return ceil_div(vocab, kLogitCols<64>) * kWarps;
     }
 }
-size_t f32_row_floats(int64_t tokens, int64_t hidden) { return (size_t)token_rows(tokens) * padded_of(hidden); }
+size_t f32_row_floats(int64_t tokens, int64_t hidden) { return 3 * (size_t)token_rows(tokens) * padded_of(hidden); }
 size_t f32_d_floats(int64_t tokens, int64_t vocab) { return (size_t)token_rows(tokens) * padded_of(vocab); }
-int64_t f32_grad_shares(int64_t tokens, int64_t hidden, int64_t vocab) {
-    return ceil_div(vocab, vocabulary_share(hidden, vocab)) * (64 / token_rows(tokens));
-}
+int64_t f32_grad_shares(int64_t hidden, int64_t vocab) { return ceil_div(vocab, vocabulary_share(hidden, vocab)); }
 
 tn_status f32_loss(const FewTokens& p, float* h, cudaStream_t stream) {
     TN_TRY(prepare_rows(p, h, false, stream));
@@ -427,8 +471,7 @@ tn_status f32_grad(const FewTokens& p, float* h, float* d, cudaStream_t stream) 
     const int64_t pitch = padded_of(p.vocab);
     switch (token_rows(p.tokens)) {
         case 16: return a ? gradient<16, true>(p, h, d, pitch, stream) : gradient<16, false>(p, h, d, pitch, stream);
-        case 32: return a ? gradient<32, true>(p, h, d, pitch, stream) : gradient<32, false>(p, h, d, pitch, stream);
-        default: return a ? gradient<64, true>(p, h, d, pitch, stream) : gradient<64, false>(p, h, d, pitch, stream);
+        default: return a ? gradient<32, true>(p, h, d, pitch, stream) : gradient<32, false>(p, h, d, pitch, stream);
     }
 }
 
