@@ -324,11 +324,13 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_forwar
     }
 }
 
-// KEEP: x - mean and g stay in registers between the two halves of the work; else (32 elements in each of 512 threads) they are formed again.
-// A vector that is read again is the thread's own, so that needs no barrier.
+// KEEP: x - mean and g stay in registers between the two halves of the work; else they are formed again (32 elements in each of 512 threads leave
+// no room; 24 of 16 bits in a lane leave room for half as many warps, 57 us against 55 at 50432 x 768). A vector that is
+// read again is the thread's own, so that needs no barrier.
 template <typename T, typename P, int VEC, int ITEMS, int DEPTH, bool BLOCK, bool KEEP>
 __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_backward(const NormArgs a) {
     using S = typename stat_of<T>::type;
+    static_assert(KEEP || VEC > 1, "a window is not read again after the sums without a barrier");
     constexpr int E = VEC * ITEMS;
     __shared__ S slots[2][BLOCK ? kMost / 32 * 2 : 1];
     extern __shared__ __align__(16) uint8_t dynamic[];
@@ -370,8 +372,9 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_backwa
             if (inside(i0 + i)) p[i] = weight_at(i0 + i);
         }
     };
-    Two<S> w[KEEP ? E / 2 : 1];
-    if constexpr (KEEP) {
+    constexpr bool WEIGHTS = E <= 24;  // the weight stays in registers, as float32
+    Two<S> w[WEIGHTS ? E / 2 : 1];
+    if constexpr (WEIGHTS) {
 #pragma unroll
         for (int i0 = 0; i0 < ITEMS; i0 += G) {
             Pack<P, VEC> p[G];
@@ -414,18 +417,15 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_backwa
             Pack<T, VEC> px[G], pd[G];
             Pack<P, VEC> pw[G];
             read(i0, px, pd);
-            if constexpr (!KEEP) weights(i0, pw);
+            if constexpr (!WEIGHTS) weights(i0, pw);
 #pragma unroll
             for (int k = 0; k < PAIRS; ++k) {
                 const int at_k = i0 * VEC / 2 + k;
                 const Two<S> d = two_of<S>(pd, k), cc = add(two_of<S>(px, k), both(-mu));
-                Two<S> gg;
+                const Two<S> gg = mul(d, WEIGHTS ? w[WEIGHTS ? at_k : 0] : two_of<S>(pw, k));
                 if constexpr (KEEP) {
-                    gg = mul(d, w[at_k]);
                     c[at_k] = cc;
                     g[at_k] = gg;
-                } else {
-                    gg = mul(d, two_of<S>(pw, k));
                 }
                 sum_g = add(sum_g, gg);
                 sum_gc = fma(gg, cc, sum_gc);
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_backwa
             Pack<P, VEC> pw[G];
             if constexpr (!KEEP) {
                 read(i0, px, pd);
-                weights(i0, pw);
+                if constexpr (!WEIGHTS) weights(i0, pw);
             }
 #pragma unroll
             for (int k = 0; k < PAIRS; ++k) {
@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_backwa
                     gg = g[at_k];
                 } else {
                     cc = add(two_of<S>(px, k), both(-mu));
-                    gg = mul(two_of<S>(pd, k), two_of<S>(pw, k));
+                    gg = mul(two_of<S>(pd, k), WEIGHTS ? w[WEIGHTS ? at_k : 0] : two_of<S>(pw, k));
                 }
                 const Two<S> r = fma(cc, by_c, fma(gg, by_g, shift));
                 px[2 * k / VEC].v[2 * k % VEC] = from_compute<T, S>(r.a);
@@ -670,7 +670,8 @@ tn_status launch_forward(Launch& l) {
 template <typename T, typename P, int VEC, int ITEMS, bool BLOCK, bool KEEP>
 tn_status launch_backward(Launch& l) {
     using S = typename stat_of<T>::type;
-    constexpr int DEPTH = !KEEP ? (sizeof(T) == 4 ? 1 : 3) : sizeof(T) * VEC * ITEMS * 2 <= 96 ? 5 : 3;  // one row of 16384 float32 twice is 128 KiB
+    // what shared memory holds beside the blocks that the registers allow; one row of 16384 float32 twice is 128 KiB
+    constexpr int DEPTH = VEC * ITEMS > 24 ? (sizeof(T) == 4 ? 1 : 3) : KEEP && sizeof(T) * VEC * ITEMS * 2 <= 96 ? 5 : 3;
     NormArgs& a = l.args;
     const int threads = block_threads<T, VEC, ITEMS, BLOCK>(a.cols);
     size_t smem = Ring<T, VEC, ITEMS, 2, DEPTH, BLOCK>::bytes(a.cols, threads);
@@ -744,7 +745,7 @@ tn_status launch_sized(Launch& l) {
         if (c <= 8 * Q * VEC) return launch_backward<T, P, VEC, Q / 4, false, true>(l);
         if (c <= 16 * Q * VEC) return launch_backward<T, P, VEC, Q / 2, false, true>(l);
         if constexpr (!F64) {
-            if (c <= 24 * Q * VEC) return launch_backward<T, P, VEC, Q / 4 * 3, false, true>(l);
+            if (c <= 24 * Q * VEC) return launch_backward<T, P, VEC, Q / 4 * 3, false, VEC == 1 || sizeof(T) == 4>(l);
             if (c <= kMost * Q / 2 * VEC) return launch_backward<T, P, VEC, Q / 2, true, true>(l);
             if constexpr (VEC > 1)  // element by element the looping kernels are faster: 13531 columns of bfloat16, 5000 rows: 280 us against 640
                 if (c <= kMost * Q * VEC) return launch_backward<T, P, VEC, Q, true, false>(l);
