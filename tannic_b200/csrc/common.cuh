@@ -39,6 +39,29 @@ tn_status fail(tn_status code, const char* fmt, ...);
 extern std::atomic<uint64_t> g_launches;
 inline void count_launch(uint64_t n = 1) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 
+// Launch of a kernel, as clusters of `cluster` blocks. `behind`: another kernel of the same call is the last work on the stream, and
+// this one may be set up under its end (see chain_wait). The first kernel of a call is launched plainly: nothing is known of the
+// kernel before it.
+template <typename... P, typename... A>
+cudaError_t launch_chained(bool behind, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, int cluster, const A&... args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = block;
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2] = {};
+    config.attrs = attributes;
+    if (behind) {
+        attributes[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attributes[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attributes[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attributes[config.numAttrs++].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+    }
+    return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
+}
+
 // Checks the launch that was just issued (pattern of src/cuda/argred.cu:138) and counts it.
 tn_status after_launch(const char* what);
 
@@ -112,6 +135,13 @@ __device__ __forceinline__ void store_as(void* base, int dt, int64_t idx, C v) {
 // name is looked up once per process; later calls return the remembered value. `name` must be a
 // string literal (the cache is keyed by its address). Values <= 0 or unset give `fallback`.
 int env_knob(const char* name, int fallback);
+
+// ---------------------------------------------------------------- chains -------------
+// Kernels that follow one another in one call are launched so that the next one's blocks start (barriers, tensor memory, tensor
+// maps) while the last blocks of the one before still run. Such a kernel calls chain_wait() before it touches memory, and so
+// waits for everything before it, and chain_go() once it may itself be followed.
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void chain_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---------------------------------------------------------------- geometry -----------
 // Number of SMs of the current device (148 on B200); grids of the streaming kernels are sized

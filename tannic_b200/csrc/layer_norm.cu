@@ -468,6 +468,7 @@ __global__ void __launch_bounds__(BLOCK ? kMost : 32 * kRowWarps, 1) norm_backwa
         ring.next();
     }
     if (a.partial == nullptr) return;  // uniform: no parameter gradients wanted
+    chain_go();
     S* mine = static_cast<S*>(a.partial) + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
     S* all = BLOCK ? mine : reinterpret_cast<S*>(dynamic);
     // a block that holds one row has its sums; the warps of the others add theirs up one after the other, where the ring was
@@ -575,8 +576,9 @@ __global__ void __launch_bounds__(256) norm_columns_long(const NormArgs a) {
 // Adds the partial rows, in an order that depends on their number only. COLS columns per block and 1024 / COLS threads a column: 8 (a
 // sector of 32 bytes, two or three loads a thread for a few hundred rows), 32 where that is blocks enough.
 template <typename S, typename P, int COLS>
-__global__ void __launch_bounds__(1024) norm_parameters(const S* __restrict__ partial, int blocks, int cols, P* __restrict__ dweight, P* __restrict__ dbias) {
+__global__ void __launch_bounds__(1024) norm_parameters(const S* partial, int blocks, int cols, P* __restrict__ dweight, P* __restrict__ dbias) {
     __shared__ S part[32][COLS + 1];
+    chain_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // columns [0, cols) are the weight's, [cols, 2 cols) the bias's
     const int64_t all = static_cast<int64_t>(cols) * 2, c = static_cast<int64_t>(blockIdx.x) * COLS + lane % COLS;
@@ -625,8 +627,8 @@ tn_status finish_partial(Launch& l, int64_t blocks) {
     if (!l.args.partial) return TN_SUCCESS;
     const int64_t all = 2 * (int64_t)l.args.cols;
     const bool many = all >= 32 * (int64_t)sm_count();
-    (many ? norm_parameters<S, P, 32> : norm_parameters<S, P, 8>)<<<(unsigned)ceil_div(all, many ? 32 : 8), 1024, 0, l.stream>>>(
-        static_cast<const S*>(l.args.partial), (int)blocks, l.args.cols, static_cast<P*>(l.dweight), static_cast<P*>(l.dbias));
+    TN_CUDA(launch_chained(true, many ? norm_parameters<S, P, 32> : norm_parameters<S, P, 8>, (unsigned)ceil_div(all, many ? 32 : 8), 1024, 0, l.stream, 1,
+                           static_cast<const S*>(l.args.partial), (int)blocks, l.args.cols, static_cast<P*>(l.dweight), static_cast<P*>(l.dbias)));
     return after_launch("norm_parameters");
 }
 

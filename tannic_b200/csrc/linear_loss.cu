@@ -292,26 +292,6 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     const uint32_t unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, units = PAIR ? gridDim.x >> 1 : gridDim.x;
     auto wait = [&](uint32_t bar, uint32_t parity) { return PAIR ? mbar_wait_pair(bar, parity, abort_flag) : mbar_wait(bar, parity, abort_flag); };
 
-    // the tokens that count bound the rows or the K extent
-    int m_tiles = g.m_tiles, k_blocks = g.k_blocks;
-    if (g.count_is != COUNT_NONE) {
-        const int count = *g.count;
-        if (g.count_is == COUNT_ROWS) m_tiles = (count + ROWS - 1) / ROWS;
-        else k_blocks = (count + BK - 1) / BK;
-    }
-    SplitPlan plan = {1, k_blocks};
-    if (g.most_splits > 1) {
-        const int tiles = m_tiles * g.n_tiles;
-        plan = plan_splits(tiles, g.units, k_blocks, plan_splits(tiles, g.units, g.first_k_blocks, g.most_splits).splits);
-    }
-    const uint32_t per_split = static_cast<uint32_t>(m_tiles) * static_cast<uint32_t>(g.n_tiles);
-    const uint32_t total = per_split * static_cast<uint32_t>(plan.splits);
-    // K blocks [first, first + n) of split z
-    auto split_range = [&](int z, int& first, int& n) {
-        first = z * plan.blocks;
-        n = min(k_blocks - first, plan.blocks);
-    };
-
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(full0 + 8 * s, 1);
@@ -338,6 +318,29 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     if constexpr (PAIR) cluster_sync();  // the other block's barriers exist before anything reports to them
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+
+    // everything above ran under the kernel before this one; from here on its results are there
+    chain_wait();
+    chain_go();
+    // the tokens that count bound the rows or the K extent
+    int m_tiles = g.m_tiles, k_blocks = g.k_blocks;
+    if (g.count_is != COUNT_NONE) {
+        const int count = *g.count;
+        if (g.count_is == COUNT_ROWS) m_tiles = (count + ROWS - 1) / ROWS;
+        else k_blocks = (count + BK - 1) / BK;
+    }
+    SplitPlan plan = {1, k_blocks};
+    if (g.most_splits > 1) {
+        const int tiles = m_tiles * g.n_tiles;
+        plan = plan_splits(tiles, g.units, k_blocks, plan_splits(tiles, g.units, g.first_k_blocks, g.most_splits).splits);
+    }
+    const uint32_t per_split = static_cast<uint32_t>(m_tiles) * static_cast<uint32_t>(g.n_tiles);
+    const uint32_t total = per_split * static_cast<uint32_t>(plan.splits);
+    // K blocks [first, first + n) of split z
+    auto split_range = [&](int z, int& first, int& n) {
+        first = z * plan.blocks;
+        n = min(k_blocks - first, plan.blocks);
+    };
 
     // all four warps of a group take part, so this comes before the roles
     if (warp < 4) {
@@ -678,9 +681,11 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 // Joins the halves of a row: R rows per block (32, or 1 when there are few), the halves of a row spread over 1024 / R threads. A
 // thread takes eight at a time, so that eight loads are in flight and one maximum serves eight exponentials.
 template <int R>
-__global__ void __launch_bounds__(1024) loss_join(const float2* __restrict__ halves, int64_t n_halves, int64_t rows, const float* __restrict__ target_logit,
+__global__ void __launch_bounds__(1024) loss_join(const float2* halves, int64_t n_halves, int64_t rows, const float* target_logit,
                                                   const void* targets, int wide, int64_t ignore, int64_t vocab, float* __restrict__ loss, float* __restrict__ lse) {
     __shared__ float2 part[32][33];
+    chain_wait();
+    chain_go();
     constexpr int STEP = 1024 / R;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * R + threadIdx.x % R;
@@ -744,17 +749,20 @@ __global__ void __launch_bounds__(256) loss_rows(const void* targets, int wide, 
                                                  float* __restrict__ scale) {
     __shared__ int ints[3][8];
     __shared__ float tops[8];
+    chain_wait();
+    chain_go();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t n0 = static_cast<int64_t>(blockIdx.x) * per_block;
     auto target_of = [&](int64_t i) { return wide ? static_cast<const int64_t*>(targets)[i] : static_cast<int64_t>(static_cast<const int32_t*>(targets)[i]); };
     int before = 0, all = 0;
     float top = 0.0f;
+#pragma unroll 4
     for (int64_t i = tid; i < n; i += 256) {
-        if (target_of(i) == ignore) continue;
-        ++all;
-        before += i < n0;
+        const bool one = target_of(i) != ignore;
         const float a = fabsf(grad[i]);
-        if (isfinite(a)) top = fmaxf(top, a);
+        all += one;
+        before += one && i < n0;
+        if (one && isfinite(a)) top = fmaxf(top, a);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -806,7 +814,9 @@ __global__ void __launch_bounds__(256) loss_rows(const void* targets, int wide, 
 // order, or row r at slot[r] (zeros where that is negative: row -1 - slot[r]); float32 as three parts of bfloat16.
 template <typename T>
 __global__ void __launch_bounds__(256) pack_rows(const T* __restrict__ src, int64_t pitch, int64_t rows, int64_t cols, int64_t padded, uint16_t* __restrict__ dst,
-                                                 int64_t part_stride, const int* __restrict__ slot, int vectors) {
+                                                 int64_t part_stride, const int* slot, int vectors) {
+    chain_wait();
+    chain_go();
     const int64_t groups = padded / 8, n = rows * groups;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t r = i / groups, c = (i - r * groups) * 8;
@@ -847,32 +857,46 @@ __global__ void __launch_bounds__(256) pack_rows(const T* __restrict__ src, int6
 // dh: the float32 sums of the splits, added in order, scaled back, and put where the tokens stand. VEC: 4 where the rows of the
 // result start on boundaries of four elements, else 1.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) loss_dhidden(const float* __restrict__ sums, const int* __restrict__ count, int tile_rows, int n_tiles, int units, int k_blocks,
-                                                    int most_splits, int64_t rows, int64_t cols, int64_t padded, const int* __restrict__ slot,
-                                                    const float* __restrict__ scale, T* __restrict__ out) {
+__global__ void __launch_bounds__(256) loss_dhidden(const float* sums, const int* count, int tile_rows, int n_tiles, int units, int k_blocks,
+                                                    int most_splits, int64_t rows, int64_t cols, int64_t padded, const int* slot, const float* scale, T* out) {
     struct alignas(sizeof(T) * VEC) Result { T v[VEC]; };
     struct alignas(sizeof(float) * VEC) Sums { float v[VEC]; };
+    constexpr int ROWS = 4;  // a thread's rows, their loads in flight together
+    chain_wait();
+    chain_go();
     const float by = *scale;
     const int splits = plan_splits((*count + tile_rows - 1) / tile_rows * n_tiles, units, k_blocks, most_splits).splits;  // of the first piece
-    const int64_t groups = cols / VEC;
-    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-        const int at = slot[r];
-        for (int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; c < groups; c += static_cast<int64_t>(gridDim.x) * 256) {
-            Sums total;
+    const int64_t c = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * VEC;
+    if (c >= cols) return;
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.y) * ROWS; r0 < rows; r0 += static_cast<int64_t>(gridDim.y) * ROWS) {
+        int at[ROWS];
+        Sums total[ROWS];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) total.v[j] = 0.0f;
-            if (at >= 0) {
-#pragma unroll 4
-                for (int z = 0; z < splits; ++z) {
-                    const Sums one = *reinterpret_cast<const Sums*>(sums + (z * rows + at) * padded + c * VEC);
+        for (int k = 0; k < ROWS; ++k) {
+            at[k] = r0 + k < rows ? slot[r0 + k] : -1;
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) total.v[j] += one.v[j];
+            for (int j = 0; j < VEC; ++j) total[k].v[j] = 0.0f;
+        }
+        for (int z = 0; z < splits; ++z) {
+            Sums one[ROWS];
+#pragma unroll
+            for (int k = 0; k < ROWS; ++k)
+                if (at[k] >= 0) one[k] = *reinterpret_cast<const Sums*>(sums + (z * rows + at[k]) * padded + c);
+#pragma unroll
+            for (int k = 0; k < ROWS; ++k)
+                if (at[k] >= 0) {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) total[k].v[j] += one[k].v[j];
                 }
-            }
-            Result res;
+        }
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) res.v[j] = from_compute<T, float>(at >= 0 ? unscale(total.v[j], by) : 0.0f);
-            *reinterpret_cast<Result*>(out + r * cols + c * VEC) = res;
+        for (int k = 0; k < ROWS; ++k) {
+            if (r0 + k < rows) {
+                Result res;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) res.v[j] = from_compute<T, float>(at[k] >= 0 ? unscale(total[k].v[j], by) : 0.0f);
+                *reinterpret_cast<Result*>(out + (r0 + k) * cols + c) = res;
+            }
         }
     }
 }
@@ -964,6 +988,13 @@ struct Problem {
     int parts, terms;
     int64_t tokens, hidden, vocab, padded;
     cudaStream_t stream;
+    // Asked at each launch: whether a kernel of this call came before it.
+    bool behind() const {
+        const bool had = begun;
+        begun = true;
+        return had;
+    }
+    mutable bool begun = false;
 };
 
 bool in_place(const Problem& p, const RowsIn& r, int64_t rows) {
@@ -978,9 +1009,9 @@ tn_status pack(const Problem& p, const RowsIn& r, int64_t first, int64_t rows, u
     const int64_t work = rows * (p.padded / 8);
     const int grid = (int)std::min<int64_t>(ceil_div(work, 256), (int64_t)sm_count() * 16);
     if (p.parts == 1)
-        pack_rows<uint16_t><<<grid, 256, 0, p.stream>>>(reinterpret_cast<const uint16_t*>(src), r.pitch, rows, p.hidden, p.padded, to, 0, slot, vectors);
+        TN_CUDA(launch_chained(p.behind(), pack_rows<uint16_t>, grid, 256, 0, p.stream, 1, reinterpret_cast<const uint16_t*>(src), r.pitch, rows, p.hidden, p.padded, to, 0, slot, vectors));
     else
-        pack_rows<float><<<grid, 256, 0, p.stream>>>(reinterpret_cast<const float*>(src), r.pitch, rows, p.hidden, p.padded, to, rows * p.padded, slot, vectors);
+        TN_CUDA(launch_chained(p.behind(), pack_rows<float>, grid, 256, 0, p.stream, 1, reinterpret_cast<const float*>(src), r.pitch, rows, p.hidden, p.padded, to, rows * p.padded, slot, vectors));
     return after_launch("pack_rows");
 }
 
@@ -1012,7 +1043,7 @@ int unit_count(bool pair) {
 bool takes_pairs(int64_t m) { return m > BM; }
 
 template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS, bool PAIR>
-tn_status launch_as(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d, const LossArgs& g, cudaStream_t stream) {
+tn_status launch_as(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d, const LossArgs& g, const Problem& p) {
     static thread_local int attr_device = -1;  // the opt-in shared-memory size belongs to kernel and device
     auto kernel = loss_gemm<A_M, B_N, EPI, T, OUT, PARTS, PAIR>;
     int dev = 0;
@@ -1023,25 +1054,14 @@ tn_status launch_as(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMa
     }
     const int64_t total = (int64_t)g.m_tiles * g.n_tiles * g.most_splits;
     if (total >= (int64_t(1) << 31)) return fail(TN_ERROR, "linear_cross_entropy: %lld tiles are too many", (long long)total);
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)std::min<int64_t>(total, g.units) * (PAIR ? 2 : 1));
-    config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = kSmemBytes<PAIR>;
-    config.stream = stream;
-    cudaLaunchAttribute attribute = {};
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim = {2, 1, 1};
-    if (PAIR) {
-        config.attrs = &attribute;
-        config.numAttrs = 1;
-    }
-    TN_CUDA(cudaLaunchKernelEx(&config, kernel, a, b, d, g));
+    const unsigned grid = (unsigned)std::min<int64_t>(total, g.units) * (PAIR ? 2 : 1);
+    TN_CUDA(launch_chained(p.behind(), kernel, grid, kThreads, kSmemBytes<PAIR>, p.stream, PAIR ? 2 : 1, a, b, d, g));
     return after_launch("loss_gemm");
 }
 template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS>
-tn_status launch_one(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d, const LossArgs& g, cudaStream_t stream) {
-    return takes_pairs(g.M) ? launch_as<A_M, B_N, EPI, T, OUT, PARTS, true>(a, b, d, g, stream)
-                            : launch_as<A_M, B_N, EPI, T, OUT, PARTS, false>(a, b, d, g, stream);
+tn_status launch_one(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d, const LossArgs& g, const Problem& p) {
+    return takes_pairs(g.M) ? launch_as<A_M, B_N, EPI, T, OUT, PARTS, true>(a, b, d, g, p)
+                            : launch_as<A_M, B_N, EPI, T, OUT, PARTS, false>(a, b, d, g, p);
 }
 
 LossArgs gemm_args(const Problem& p, int64_t m, int64_t n, int64_t k) {
@@ -1130,9 +1150,8 @@ Problem make_problem(const tn_tensor_t* hidden, const tn_tensor_t* weight, tn_st
 // Joins `n` groups of logits per row into lse and loss.
 tn_status join(const Problem& p, const float2* halves, int64_t n, const float* target_logit, const void* targets, int wide, int64_t ignore, tn_tensor_t* loss, tn_tensor_t* lse) {
     const bool few = p.tokens <= 2 * sm_count();  // a block per row fills the GPU at most once
-    (few ? loss_join<1> : loss_join<32>)<<<(unsigned)ceil_div(p.tokens, few ? 1 : 32), 1024, 0, p.stream>>>(
-        halves, n, p.tokens, target_logit, targets, wide, ignore, p.vocab, loss ? static_cast<float*>(loss->address) : nullptr,
-        lse ? static_cast<float*>(lse->address) : nullptr);
+    TN_CUDA(launch_chained(true, few ? loss_join<1> : loss_join<32>, (unsigned)ceil_div(p.tokens, few ? 1 : 32), 1024, 0, p.stream, 1, halves, n, p.tokens, target_logit, targets, wide,
+                           ignore, p.vocab, loss ? static_cast<float*>(loss->address) : nullptr, lse ? static_cast<float*>(lse->address) : nullptr));
     return after_launch("loss_join");
 }
 
@@ -1182,14 +1201,13 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
     }
     Operand a;
     a.parts = p.parts;
+    uint16_t* tokens = nullptr;
     if (in_place(p, h, p.tokens)) {
         a.ptr = h.base;
         a.pitch = h.pitch;
     } else {
-        uint16_t* room = nullptr;
-        TN_TRY(mem.take(&room, (size_t)p.parts * p.tokens * p.padded * 2));
-        TN_TRY(pack(p, h, 0, p.tokens, room, nullptr));
-        a.ptr = room;
+        TN_TRY(mem.take(&tokens, (size_t)p.parts * p.tokens * p.padded * 2));
+        a.ptr = tokens;
         a.pitch = p.padded;
         a.part_stride = p.tokens * p.padded;
     }
@@ -1200,6 +1218,7 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
     int64_t tiles = 0;
     for (int64_t v0 = 0; v0 < p.vocab; v0 += piece) tiles += ceil_div(std::min(piece, p.vocab - v0), BN);
     TN_TRY(mem.take(&halves, sizeof(float2) * 2 * (size_t)tiles * p.tokens));
+    if (tokens) TN_TRY(pack(p, h, 0, p.tokens, tokens, nullptr));
     CUtensorMap map_a, map_b;
     TN_TRY(operand_map(&map_a, a, p.bf16, p.hidden, p.tokens, BK, BM));
     int64_t first_half = 0;
@@ -1216,7 +1235,7 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
         g.halves = halves;
         g.first_half = first_half;
         g.target_logit = target_logit;
-        TN_TRY((launch_one<false, false, EPI_STATS, __half, float, 1>(map_a, map_b, map_a, g, p.stream)));
+        TN_TRY((launch_one<false, false, EPI_STATS, __half, float, 1>(map_a, map_b, map_a, g, p)));
         first_half += 2 * (int64_t)g.n_tiles;
     }
     return join(p, halves, first_half, target_logit, t, wide, ignore, loss, lse);
@@ -1255,13 +1274,8 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
     TN_TRY(mem.take(&slot, sizeof(int) * p.tokens));
     TN_TRY(mem.take(&count, 2 * sizeof(int)));
     float* scale = reinterpret_cast<float*>(count + 1);
-    const int per_block = (int)std::min<int64_t>(256, std::max<int64_t>(8, ceil_div(p.tokens, 1024)));
-    loss_rows<<<(unsigned)ceil_div(p.tokens, per_block), 256, 0, p.stream>>>(t, wide, p.tokens, static_cast<const float*>(up), static_cast<const float*>(z),
-                                                                            ignore, p.vocab, per_block, info, slot, count, scale);
-    TN_TRY(after_launch("loss_rows"));
     uint16_t* gathered = nullptr;
     TN_TRY(mem.take(&gathered, (size_t)p.parts * p.tokens * p.padded * 2));
-    TN_TRY(pack(p, h, 0, p.tokens, gathered, slot));
     Operand a;
     a.ptr = gathered;
     a.pitch = p.padded;
@@ -1291,6 +1305,14 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
         TN_TRY(mem.take(&sums, sizeof(float) * (size_t)splits * p.tokens * p.padded));
     }
 
+    // the scratch memory is all taken: what follows are kernels, one behind the other
+    // every block reads all targets, so there are not too many of them
+    const int per_block = (int)std::min<int64_t>(256, std::max<int64_t>(32, ceil_div(p.tokens, 256)));
+    TN_CUDA(launch_chained(p.behind(), loss_rows, (unsigned)ceil_div(p.tokens, per_block), 256, 0, p.stream, 1, t, wide, p.tokens, f.grad, f.lse, ignore, p.vocab, per_block,
+                           info, slot, count, scale));
+    TN_TRY(after_launch("loss_rows"));
+    TN_TRY(pack(p, h, 0, p.tokens, gathered, slot));
+
     CUtensorMap rows_a, rows_b, map;
     TN_TRY(operand_map(&rows_a, a, p.bf16, p.hidden, p.tokens, BK, BM));   // h as [tokens, hidden], K = hidden
     TN_TRY(operand_map(&rows_b, a, p.bf16, p.hidden, p.tokens, 64, BK));   // h as B of dW, K = tokens
@@ -1310,7 +1332,7 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
             g.count = count;
             g.count_is = COUNT_ROWS;
             g.rows = info;
-            TN_TRY((launch_one<false, false, EPI_D, T, float, PARTS>(rows_a, map, map_d, g, p.stream)));
+            TN_TRY((launch_one<false, false, EPI_D, T, float, PARTS>(rows_a, map, map_d, g, p)));
         }
         if (dhidden) {
             CUtensorMap map_d, map_w;
@@ -1324,7 +1346,7 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
             g.most_splits = splits;
             g.first_k_blocks = (int)ceil_div(piece, BK);
             g.add = v0 > 0;
-            TN_TRY((launch_one<false, true, EPI_SUM, T, float, 1>(map, map_w, map_d, g, p.stream)));
+            TN_TRY((launch_one<false, true, EPI_SUM, T, float, 1>(map, map_w, map_d, g, p)));
         }
         if (dweight) {
             CUtensorMap map_d;
@@ -1340,15 +1362,15 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
             g.tma_store = can_tma_store(to, p.hidden, p.hidden * 8, BN, F32);
             map_d = map;  // placeholder when the result does not leave through TMA
             if (g.tma_store) TN_TRY(make_result_map(&map_d, to, F32, p.bf16, p.hidden, n, 1, p.hidden, 0));
-            TN_TRY((launch_one<true, true, EPI_RESULT, T, OUT, 1>(map, rows_b, map_d, g, p.stream)));
+            TN_TRY((launch_one<true, true, EPI_RESULT, T, OUT, 1>(map, rows_b, map_d, g, p)));
         }
     }
     if (dhidden) {
         OUT* to = static_cast<OUT*>(dhidden->address);
         const bool wide = p.hidden % 4 == 0 && (reinterpret_cast<uintptr_t>(to) & (4 * sizeof(OUT) - 1)) == 0;
-        const dim3 grid((unsigned)std::min<int64_t>(ceil_div(p.hidden, wide ? 1024 : 256), 1024), (unsigned)std::min<int64_t>(p.tokens, 65535));
-        (wide ? loss_dhidden<OUT, 4> : loss_dhidden<OUT, 1>)<<<grid, 256, 0, p.stream>>>(
-            sums, count, pair ? 2 * BM : BM, (int)ceil_div(p.padded, BN), unit_count(pair), (int)ceil_div(piece, BK), splits, p.tokens, p.hidden, p.padded, slot, scale, to);
+        const dim3 grid((unsigned)ceil_div(p.hidden, wide ? 1024 : 256), (unsigned)std::min<int64_t>(ceil_div(p.tokens, 4), 65535));
+        TN_CUDA(launch_chained(true, wide ? loss_dhidden<OUT, 4> : loss_dhidden<OUT, 1>, grid, 256, 0, p.stream, 1, sums, count, pair ? 2 * BM : BM, (int)ceil_div(p.padded, BN),
+                               unit_count(pair), (int)ceil_div(piece, BK), splits, p.tokens, p.hidden, p.padded, slot, scale, to));
         TN_TRY(after_launch("loss_dhidden"));
     }
     return TN_SUCCESS;

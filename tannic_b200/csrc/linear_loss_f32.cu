@@ -96,6 +96,7 @@ __device__ __forceinline__ void wait_oldest() { asm volatile("cp.async.wait_grou
 // The tokens as the products read them: [rows][padded], zero where there is no token, no target (that is for the gradient) or no column; behind
 // them their hi and lo, which every warp of the logits would otherwise work out for itself.
 __global__ void __launch_bounds__(256) few_rows_kernel(const FewTokens p, int rows, int64_t padded, int drop_ignored, float* __restrict__ out) {
+    chain_go();
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < rows * padded; i += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t n = i / padded, c = i - n * padded;
         const bool in = n < p.tokens && c < p.hidden && !(drop_ignored && target_of(p, n) == p.ignore);
@@ -113,7 +114,7 @@ template <int TM> constexpr int kLogitCols = kWarps * 8 * kFragments<TM>;
 
 // h: hi and lo of the tokens, [2][TM][padded]. D: write d into `d` ([TM][d_pitch]), else the warps' statistics.
 template <int TM, bool ALIGNED, bool D>
-__global__ void __launch_bounds__(kThreads) logits_kernel(const FewTokens p, const float* __restrict__ h, int64_t padded, float* __restrict__ d, int64_t d_pitch) {
+__global__ void __launch_bounds__(kThreads) logits_kernel(const FewTokens p, const float* h, int64_t padded, float* d, int64_t d_pitch) {
     constexpr int COLS = kLogitCols<TM>, MT = TM / 16, NT = kFragments<TM>;
     extern __shared__ __align__(16) float smem[];  // [kStages][2 TM + COLS][kPitch]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -138,6 +139,8 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const FewTokens p, con
         }
         commit();
     };
+    chain_wait();
+    chain_go();
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) fill(s);
     float sum[MT][NT][4];
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const FewTokens p, con
 constexpr int kHiddenCols = 256, kHiddenWide = kHiddenCols + 8, kHiddenStages = 3;
 
 template <int TM, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) dhidden_kernel(const FewTokens p, const float* __restrict__ d, int64_t d_pitch, int64_t share) {
+__global__ void __launch_bounds__(kThreads) dhidden_kernel(const FewTokens p, const float* d, int64_t d_pitch, int64_t share) {
     extern __shared__ __align__(16) float smem[];  // [kHiddenStages] of [TM][kPitch] and [kStep][kHiddenWide]
     constexpr int TILE = TM * kPitch + kStep * kHiddenWide, MT = TM / 16, NT = kHiddenCols / kWarps / 8;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -257,6 +260,8 @@ __global__ void __launch_bounds__(kThreads) dhidden_kernel(const FewTokens p, co
         }
         commit();
     };
+    chain_wait();
+    chain_go();
 #pragma unroll
     for (int s = 0; s < kHiddenStages - 1; ++s) fill(s);
     float sum[MT][NT][4];
@@ -310,13 +315,15 @@ __global__ void __launch_bounds__(kThreads) dhidden_kernel(const FewTokens p, co
 
 // dW: a tile of 128 x 128, K = the tokens, all of them in shared memory at once; a warp has 32 vocabulary rows and 64 columns.
 template <int TM, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) dweight_kernel(const FewTokens p, const float* __restrict__ h, int64_t padded, const float* __restrict__ d, int64_t d_pitch) {
+__global__ void __launch_bounds__(kThreads) dweight_kernel(const FewTokens p, const float* h, int64_t padded, const float* d, int64_t d_pitch) {
     extern __shared__ __align__(16) float smem[];  // [TM][kWide] of d and of h
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int row = warp / 2 * 32, column = warp % 2 * 64;
     const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kCols;
     float* a = smem;
     float* b = smem + TM * kWide;
+    chain_wait();
+    chain_go();
     for (int i = threadIdx.x; i < TM * (kCols / 4); i += kThreads) {
         const int r = i / (kCols / 4), c = i % (kCols / 4) * 4;
         const int valid = static_cast<int>(min(int64_t(4), padded - c0 - c));
@@ -400,7 +407,8 @@ tn_status allow(K kernel, size_t smem, int& last) {
 tn_status prepare_rows(const FewTokens& p, float* h, bool drop_ignored, cudaStream_t stream) {
     const int rows = token_rows(p.tokens);
     const int64_t padded = padded_of(p.hidden);
-    few_rows_kernel<<<(unsigned)std::min<int64_t>(ceil_div(rows * padded, 256), (int64_t)sm_count() * 4), 256, 0, stream>>>(p, rows, padded, drop_ignored, h);
+    TN_CUDA(launch_chained(false, few_rows_kernel, (unsigned)std::min<int64_t>(ceil_div(rows * padded, 256), (int64_t)sm_count() * 4), 256, 0, stream, 1, p, rows,
+                           padded, drop_ignored, h));
     return after_launch("few_rows_kernel");
 }
 
@@ -409,7 +417,8 @@ tn_status logits(const FewTokens& p, const float* h, float* d, int64_t d_pitch, 
     static thread_local int device = -1;
     const size_t smem = sizeof(float) * kStages * (2 * TM + kLogitCols<TM>) * kPitch;
     TN_TRY(allow(logits_kernel<TM, ALIGNED, D>, smem, device));
-    logits_kernel<TM, ALIGNED, D><<<(unsigned)ceil_div(p.vocab, kLogitCols<TM>), kThreads, smem, stream>>>(p, h + TM * padded_of(p.hidden), padded_of(p.hidden), d, d_pitch);
+    TN_CUDA(launch_chained(true, logits_kernel<TM, ALIGNED, D>, (unsigned)ceil_div(p.vocab, kLogitCols<TM>), kThreads, smem, stream, 1, p, h + TM * padded_of(p.hidden),
+                           padded_of(p.hidden), d, d_pitch));
     return after_launch("logits_kernel");
 }
 
@@ -422,7 +431,8 @@ tn_status gradient(const FewTokens& p, const float* h, float* d, int64_t d_pitch
         const size_t smem = sizeof(float) * kHiddenStages * (TM * kPitch + kStep * kHiddenWide);
         TN_TRY(allow(dhidden_kernel<TM, ALIGNED>, smem, device));
         const int64_t share = vocabulary_share(p.hidden, p.vocab);
-        dhidden_kernel<TM, ALIGNED><<<dim3((unsigned)ceil_div(p.hidden, kHiddenCols), (unsigned)ceil_div(p.vocab, share)), kThreads, smem, stream>>>(p, d, d_pitch, share);
+        TN_CUDA(launch_chained(true, dhidden_kernel<TM, ALIGNED>, dim3((unsigned)ceil_div(p.hidden, kHiddenCols), (unsigned)ceil_div(p.vocab, share)), kThreads, smem, stream,
+                               1, p, d, d_pitch, share));
         TN_TRY(after_launch("dhidden_kernel"));
         TN_TRY(few_dhidden(p, f32_grad_shares(p.hidden, p.vocab), stream));
     }
@@ -431,7 +441,7 @@ tn_status gradient(const FewTokens& p, const float* h, float* d, int64_t d_pitch
         const size_t smem = sizeof(float) * 2 * TM * kWide;
         TN_TRY(allow(dweight_kernel<TM, ALIGNED>, smem, device));
         const int64_t rows = std::min(ceil_div(p.vocab, kCols), std::max<int64_t>(1, (int64_t)sm_count() * 4 / across));
-        dweight_kernel<TM, ALIGNED><<<dim3((unsigned)across, (unsigned)rows), kThreads, smem, stream>>>(p, h, padded_of(p.hidden), d, d_pitch);
+        TN_CUDA(launch_chained(true, dweight_kernel<TM, ALIGNED>, dim3((unsigned)across, (unsigned)rows), kThreads, smem, stream, 1, p, h, padded_of(p.hidden), d, d_pitch));
         TN_TRY(after_launch("dweight_kernel"));
     }
     return TN_SUCCESS;

@@ -65,6 +65,7 @@ template <typename T, int VEC, int NT>
 __global__ void __launch_bounds__(kLossThreads, 1) few_loss_kernel(const FewTokens p, int64_t padded) {
     extern __shared__ __align__(16) float hid[];  // [NT][padded], zeros behind a row's end and in the rows without a token
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    chain_go();
     for (int64_t i = threadIdx.x; i < NT * padded; i += kLossThreads) {
         const int64_t n = i / padded, c = i - n * padded;
         hid[i] = n < p.tokens && c < p.hidden ? to_compute<float>(static_cast<const T*>(p.h)[n * p.h_pitch + c]) : 0.0f;
@@ -162,6 +163,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) few_grad_kernel(const FewToke
     P* ring = reinterpret_cast<P*>(smem) + t;  // [kDepth][R][ITEMS][threads]
     const int vecs = static_cast<int>(p.hidden / VEC);
     auto inside = [&](int i) { return i * threads + t < vecs; };
+    chain_go();
 
     // the tokens' columns of this thread; a token without a target is nothing, whatever it holds
     float2 h[NT][E / 2], dh[NT][E / 2];
@@ -339,6 +341,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) few_grad_kernel(const FewToke
 template <typename T, int COLS>
 __global__ void __launch_bounds__(1024) few_dhidden_kernel(const FewTokens p, int blocks) {
     __shared__ float part[32][COLS + 1];
+    chain_wait();
+    chain_go();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t n_all = p.tokens * p.hidden, c = static_cast<int64_t>(blockIdx.x) * COLS + lane % COLS;
     float sum = 0.0f;
@@ -383,7 +387,7 @@ tn_status loss_one(const FewTokens& p, cudaStream_t stream) {
     const int64_t padded = (p.hidden + 7) & ~int64_t(7);
     const size_t smem = sizeof(float) * NT * (size_t)padded;
     TN_TRY(allow_smem(few_loss_kernel<T, VEC, NT>, smem, device, allowed));
-    few_loss_kernel<T, VEC, NT><<<(unsigned)(few_loss_parts() / (kLossThreads / 32)), kLossThreads, smem, stream>>>(p, padded);
+    TN_CUDA(launch_chained(false, few_loss_kernel<T, VEC, NT>, (unsigned)(few_loss_parts() / (kLossThreads / 32)), kLossThreads, smem, stream, 1, p, padded));
     return after_launch("few_loss_kernel");
 }
 template <typename T, int VEC>
@@ -403,7 +407,8 @@ tn_status loss_typed(const FewTokens& p, cudaStream_t stream) {
 template <typename T>
 tn_status dhidden_typed(const FewTokens& p, int64_t n, cudaStream_t stream) {
     const bool many = p.tokens * p.hidden >= 32 * (int64_t)sm_count();
-    (many ? few_dhidden_kernel<T, 32> : few_dhidden_kernel<T, 8>)<<<(unsigned)ceil_div(p.tokens * p.hidden, many ? 32 : 8), 1024, 0, stream>>>(p, (int)n);
+    TN_CUDA(launch_chained(true, many ? few_dhidden_kernel<T, 32> : few_dhidden_kernel<T, 8>, (unsigned)ceil_div(p.tokens * p.hidden, many ? 32 : 8), 1024, 0,
+                           stream, 1, p, (int)n));
     return after_launch("few_dhidden_kernel");
 }
 
@@ -415,7 +420,7 @@ tn_status grad_one(const FewTokens& p, cudaStream_t stream) {
     const size_t smem = VEC > 1 ? sizeof(T) * E * kGradRows<T, VEC> * kDepth * (size_t)threads : 0;
     TN_TRY(allow_smem(few_grad_kernel<T, VEC, NT>, smem, device, allowed));
     const int64_t blocks = few_grad_blocks(p.vocab);
-    few_grad_kernel<T, VEC, NT><<<(unsigned)blocks, threads, smem, stream>>>(p);
+    TN_CUDA(launch_chained(false, few_grad_kernel<T, VEC, NT>, (unsigned)blocks, threads, smem, stream, 1, p));
     TN_TRY(after_launch("few_grad_kernel"));
     return p.dhidden ? few_dhidden(p, blocks, stream) : TN_SUCCESS;
 }
