@@ -82,8 +82,6 @@ struct alignas(16) RowInfo {
 };
 constexpr int kNoRow = -1;
 constexpr int kPeriod = 16;       // 64-wide blocks an accumulator takes before it is added up in registers
-constexpr float kTop = 16384.0f;  // where the largest |grad| lands in d: float16 ends at 65504
-__device__ __forceinline__ float unscale(float v, float largest) { return v * (1.0f / kTop) * largest; }
 
 // Passes over the parts of a float32 operand pair, largest product first.
 __constant__ int kPartA[6] = {0, 0, 1, 0, 1, 2};
@@ -1258,10 +1256,11 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
     f.lse = static_cast<const float*>(z);
     f.dhidden = dhidden ? dhidden->address : nullptr;
     f.dweight = dweight ? dweight->address : nullptr;
-    const bool few = few_grad_fits(f);
-    if (few || f32_fits(p.dtype, p.tokens, p.hidden, true)) {
-        const int64_t blocks = few ? few_grad_blocks(p.vocab) : f32_grad_shares(p.hidden, p.vocab);
+    const bool half = half_grad_fits(f), few = few_grad_fits(f);
+    if (half || few || f32_fits(p.dtype, p.tokens, p.hidden, true)) {
+        const int64_t blocks = half ? half_grad_blocks(p.hidden, p.vocab) : few ? few_grad_blocks(p.vocab) : f32_grad_shares(p.hidden, p.vocab);
         if (dhidden) TN_TRY(mem.take(&f.sums, sizeof(float) * (size_t)blocks * p.tokens * p.hidden));
+        if (half) return half_grad(f, p.stream);
         if (few) return few_grad(f, p.stream);
         float *rows = nullptr, *d = nullptr;
         TN_TRY(mem.take(&rows, sizeof(float) * f32_row_floats(p.tokens, p.hidden)));

@@ -1,5 +1,5 @@
 // The cross entropy of a linear layer for a few tokens: interface between the dispatcher (linear_loss.cu), the streaming
-// kernels (linear_loss_few.cu) and the float32 tiles (linear_loss_f32.cu).
+// kernels (linear_loss_few.cu), the gradient of a few tokens of 16 bits (linear_loss_half.cu) and the float32 tiles (linear_loss_f32.cu).
 #pragma once
 
 #include "common.cuh"
@@ -31,6 +31,16 @@ bool few_loss_fits(int dtype, int64_t tokens, int64_t hidden);
 int64_t few_loss_parts();
 tn_status few_loss(const FewTokens& p, cudaStream_t stream);
 
+// d is scaled by kTop over the largest |grad|, and what is formed from it scaled back.
+constexpr float kTop = 16384.0f;  // float16 ends at 65504
+__device__ __forceinline__ float unscale(float v, float largest) { return v * (1.0f / kTop) * largest; }
+
+// 16 bits, up to eight tokens
+bool half_grad_fits(const FewTokens& p);
+int64_t half_grad_blocks(int64_t hidden, int64_t vocab);
+tn_status half_grad(const FewTokens& p, cudaStream_t stream);
+
+// float32, up to four tokens
 bool few_grad_fits(const FewTokens& p);
 int64_t few_grad_blocks(int64_t vocab);
 tn_status few_grad(const FewTokens& p, cudaStream_t stream);

@@ -146,16 +146,16 @@ __global__ void __launch_bounds__(kLossThreads, 1) few_loss_kernel(const FewToke
 constexpr int kGradThreads = 512;
 constexpr int E = 8;  // columns of a thread
 
-template <typename T, int VEC> constexpr int kGradRows = VEC > 1 && sizeof(T) == 2 ? 8 : 4;
+constexpr int kGradRows = 4;
 constexpr int kDepth = 3;  // batches of rows in shared memory: two in use, one on its way
 
 // One barrier a batch: between two of them a warp forms its part of the next batch's logits and does everything else of this
 // batch's, so that the chain logits - exponential - products of one batch runs under the other's.
-template <typename T, int VEC, int NT>
+template <int VEC, int NT>
 __global__ void __launch_bounds__(kGradThreads, 1) few_grad_kernel(const FewTokens p) {
-    constexpr int ITEMS = E / VEC, R = kGradRows<T, VEC>, V = R * NT, SHIFT = 5 - kLog2<V>, WARPS = kGradThreads / 32;
+    constexpr int ITEMS = E / VEC, R = kGradRows, V = R * NT, SHIFT = 5 - kLog2<V>, WARPS = kGradThreads / 32;
     constexpr bool RING = VEC > 1;  // else the rows are read from memory twice, the second time from L1 or L2
-    using P = Pack<T, VEC>;
+    using P = Pack<float, VEC>;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float part[2][WARPS][32];
     __shared__ __align__(16) float dvals[WARPS][32];
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) few_grad_kernel(const FewToke
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
-                x[i * VEC + j] = counts && inside(i) ? to_compute<float>(static_cast<const T*>(p.h)[n * p.h_pitch + static_cast<int64_t>(i * threads + t) * VEC + j]) : 0.0f;
+                x[i * VEC + j] = counts && inside(i) ? static_cast<const float*>(p.h)[n * p.h_pitch + static_cast<int64_t>(i * threads + t) * VEC + j] : 0.0f;
 #pragma unroll
         for (int k = 0; k < E / 2; ++k) {
             h[n][k] = make_float2(x[2 * k], x[2 * k + 1]);
@@ -197,13 +197,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) few_grad_kernel(const FewToke
             if (!inside(i))
                 for (int k = 0; k < kDepth * R; ++k)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) ring[(k * ITEMS + i) * threads].v[j] = T(0.0f);
+                    for (int j = 0; j < VEC; ++j) ring[(k * ITEMS + i) * threads].v[j] = 0.0f;
     }
     __syncthreads();
 
     const int64_t step = static_cast<int64_t>(gridDim.x) * R;
     // rows behind the last one are read as the last one; their d is zero and nothing is written for them
-    auto row_at = [&](int64_t v) { return reinterpret_cast<const P*>(static_cast<const T*>(p.w) + min(v, p.vocab - 1) * p.w_pitch) + t; };
+    auto row_at = [&](int64_t v) { return reinterpret_cast<const P*>(static_cast<const float*>(p.w) + min(v, p.vocab - 1) * p.w_pitch) + t; };
     auto fetch = [&](int64_t v0, int s) {
         if constexpr (RING) {
             if (v0 < p.vocab) {
@@ -230,13 +230,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) few_grad_kernel(const FewToke
                 q[i] = ring[((s * R + r) * ITEMS + i) * threads];
             } else {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) q[i].v[j] = T(0.0f);
+                for (int j = 0; j < VEC; ++j) q[i].v[j] = 0.0f;
                 if (inside(i)) q[i] = row_at(v0 + r)[i * threads];
             }
         }
 #pragma unroll
         for (int k = 0; k < E / 2; ++k)
-            x[k] = make_float2(to_compute<float>(q[2 * k / VEC].v[2 * k % VEC]), to_compute<float>(q[(2 * k + 1) / VEC].v[(2 * k + 1) % VEC]));
+            x[k] = make_float2(q[2 * k / VEC].v[2 * k % VEC], q[(2 * k + 1) / VEC].v[(2 * k + 1) % VEC]);
     };
     auto logits = [&](int64_t v0, int s, int to) {
         float dots[V];
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) few_grad_kernel(const FewToke
     if (v0 < p.vocab) logits(v0, 0, 0);
     __syncthreads();
     int slot = 0, parity = 0;
-    T* out_row = static_cast<T*>(p.dweight) + v0 * p.hidden;
+    float* out_row = static_cast<float*>(p.dweight) + v0 * p.hidden;
     for (; v0 < p.vocab; v0 += step, parity ^= 1, out_row += step * p.hidden) {
         // a thread reads what it copied itself, and the slot that is filled now is the one that it read last
         const int next = slot == kDepth - 1 ? 0 : slot + 1, after = next == kDepth - 1 ? 0 : next + 1;
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) few_grad_kernel(const FewToke
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) {
                         const int e = i * VEC + j;
-                        q.v[j] = from_compute<T, float>(e % 2 ? out[e / 2].y : out[e / 2].x);
+                        q.v[j] = e % 2 ? out[e / 2].y : out[e / 2].x;
                     }
                     if (inside(i)) to[i * threads] = q;
                 }
@@ -412,31 +412,24 @@ tn_status dhidden_typed(const FewTokens& p, int64_t n, cudaStream_t stream) {
     return after_launch("few_dhidden_kernel");
 }
 
-template <typename T, int VEC, int NT>
+template <int VEC, int NT>
 tn_status grad_one(const FewTokens& p, cudaStream_t stream) {
     static thread_local int device = -1;
     static thread_local size_t allowed = 0;
     const int threads = (int)(ceil_div(ceil_div(p.hidden / VEC, E / VEC), 32) * 32);
-    const size_t smem = VEC > 1 ? sizeof(T) * E * kGradRows<T, VEC> * kDepth * (size_t)threads : 0;
-    TN_TRY(allow_smem(few_grad_kernel<T, VEC, NT>, smem, device, allowed));
+    const size_t smem = VEC > 1 ? sizeof(float) * E * kGradRows * kDepth * (size_t)threads : 0;
+    TN_TRY(allow_smem(few_grad_kernel<VEC, NT>, smem, device, allowed));
     const int64_t blocks = few_grad_blocks(p.vocab);
-    TN_CUDA(launch_chained(false, few_grad_kernel<T, VEC, NT>, (unsigned)blocks, threads, smem, stream, 1, p));
+    TN_CUDA(launch_chained(false, few_grad_kernel<VEC, NT>, (unsigned)blocks, threads, smem, stream, 1, p));
     TN_TRY(after_launch("few_grad_kernel"));
     return p.dhidden ? few_dhidden(p, blocks, stream) : TN_SUCCESS;
 }
-template <typename T, int VEC>
+template <int VEC>
 tn_status grad_tokens(const FewTokens& p, cudaStream_t stream) {
-    if (p.tokens <= 1) return grad_one<T, VEC, 1>(p, stream);
-    if (p.tokens <= 2) return grad_one<T, VEC, 2>(p, stream);
-    return grad_one<T, VEC, 4>(p, stream);
+    if (p.tokens <= 1) return grad_one<VEC, 1>(p, stream);
+    if (p.tokens <= 2) return grad_one<VEC, 2>(p, stream);
+    return grad_one<VEC, 4>(p, stream);
 }
-template <typename T>
-tn_status grad_typed(const FewTokens& p, cudaStream_t stream) {
-    constexpr int VEC = 16 / sizeof(T);
-    const bool wide = p.hidden % VEC == 0 && fits16(p.w, p.w_pitch * (int64_t)sizeof(T)) && fits16(p.dweight, 0);
-    return wide ? grad_tokens<T, VEC>(p, stream) : grad_tokens<T, 1>(p, stream);
-}
-
 }  // namespace
 
 // As many columns as shared memory takes beside the tokens. One token of 16 bits: from two on the tensor cores are faster, empty rows and
@@ -463,21 +456,13 @@ tn_status few_dhidden(const FewTokens& p, int64_t n, cudaStream_t stream) {
     }
 }
 
-// Four tokens with eight columns in each of 512 threads. Rows that are not aligned to 16 bytes are read element by element, twice, which the
-// tensor cores' copy of the weights beats for 16 bits (four tokens over 32000 x 1001: 152 us against 201).
-bool few_grad_fits(const FewTokens& p) {
-    const int size = p.dtype == TN_FLOAT32 ? 4 : 2;
-    const bool wide = p.hidden * size % 16 == 0 && fits16(p.w, p.w_pitch * size) && fits16(p.dweight, 0);
-    return p.tokens <= 4 && p.hidden <= kGradThreads * E && (wide || p.dtype == TN_FLOAT32);
-}
-int64_t few_grad_blocks(int64_t vocab) { return std::min<int64_t>(sm_count(), ceil_div(vocab, 4)); }
+// Four tokens with eight columns in each of 512 threads.
+bool few_grad_fits(const FewTokens& p) { return p.dtype == TN_FLOAT32 && p.tokens <= 4 && p.hidden <= kGradThreads * E; }
+int64_t few_grad_blocks(int64_t vocab) { return std::min<int64_t>(sm_count(), ceil_div(vocab, kGradRows)); }
 
 tn_status few_grad(const FewTokens& p, cudaStream_t stream) {
-    switch (p.dtype) {
-        case TN_FLOAT16: return grad_typed<__half>(p, stream);
-        case TN_BFLOAT16: return grad_typed<__nv_bfloat16>(p, stream);
-        default: return grad_typed<float>(p, stream);
-    }
+    const bool wide = p.hidden % 4 == 0 && fits16(p.w, p.w_pitch * 4) && fits16(p.dweight, 0);
+    return wide ? grad_tokens<4>(p, stream) : grad_tokens<1>(p, stream);
 }
 
 }  // namespace tnb

@@ -1,0 +1,287 @@
+// The gradient of a linear layer's cross entropy for up to eight tokens of 16 bits.
+//
+// With lse known one pass over W does everything: for eight vocabulary rows at a time the logits, d = (exp(logit - lse) - [target]) grad
+// from them, then dW = d^T h and dh += d W before the next rows take their place. The bound is memory: W is read once and dW written once.
+// The products run as mma.sync with the eight tokens on one side: tcgen05's smallest tile has 64 rows, reads both operands from shared
+// memory, where d would have to be written first, and returns through TMEM, where dW would wait; here d stays in registers from one
+// product's result to the next one's operand. (On the FP32 pipe the same pass took 127 us for four tokens over 32000 x 4096.)
+//
+// A warp owns groups of 32 columns of all rows, fetches them with cp.async, reads each eight rows twice from shared memory (as they lie for
+// the logits, transposed for dh) and fetches the next ones in their place, so the only barrier is the one over the warps' parts of the logits.
+//   logits [8 rows of W, 8 tokens]  k = columns. A lane takes 16 bytes of a row of W, columns 8 t .. 8 t + 7 (t = lane % 4); h lies in
+//                                   shared memory in the order that makes this the fragment of two steps.
+//   dh [columns, 8 tokens]          k = the eight rows, once with d's upper part and once with its lower one.
+//   dW [8 rows, columns]            k = the tokens; rows 0 to 7 of the tile take d's upper part, rows 8 to 15 its lower one, and the two
+//                                   are added. h's order puts eight neighbouring columns into a lane: one store of 16 bytes.
+// d is the sum of two values of the operands' type (2^-17 of it for bfloat16, 2^-22 for float16), scaled like the larger products' d so that
+// float16 does not lose small gradients.
+#include <algorithm>
+
+#include "linear_loss.cuh"
+
+namespace tnb {
+namespace {
+
+constexpr int kTokens = 8, kBatch = 8;  // tokens, and vocabulary rows at a time
+constexpr int kGroup = 32;              // columns
+constexpr int kMostGroups = 8;          // of a warp: 64 registers of dh's sums
+
+template <typename T> struct Pair;
+template <> struct Pair<__half> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 v = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&v); }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+};
+template <> struct Pair<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { const __nv_bfloat162 v = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&v); }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v)); }
+};
+
+template <typename T>
+__device__ __forceinline__ void mma_k16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <typename T>
+__device__ __forceinline__ void mma_k8(float* c, uint32_t a0, uint32_t a1, uint32_t b) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(b));
+    else
+        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(b));
+}
+__device__ __forceinline__ void load4(uint32_t (&m)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(m[0]), "=r"(m[1]), "=r"(m[2]), "=r"(m[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void load4_transposed(uint32_t (&m)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(m[0]), "=r"(m[1]), "=r"(m[2]), "=r"(m[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+__host__ __device__ __forceinline__ int groups_of(int64_t hidden) { return static_cast<int>((hidden + kGroup - 1) / kGroup); }
+// Bytes between the tokens in shared memory (16 more than a multiple of 64: eight rows fall on different banks) and between W's rows.
+__host__ __device__ __forceinline__ uint32_t h_bytes(int groups) { return groups * 64 + 16; }
+__host__ __device__ __forceinline__ uint32_t w_bytes(int groups) { return (groups + 1) / 2 * 128; }
+__host__ __device__ __forceinline__ size_t smem_bytes(int groups, int slots, int warps) {
+    return static_cast<size_t>(slots) * kBatch * w_bytes(groups) + kTokens * h_bytes(groups) + 2 * warps * 32 * sizeof(float2);
+}
+
+// SLOTS batches of W lie in shared memory or are on their way there.
+template <typename T, int WARPS, int SLOTS>
+__global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) half_grad_kernel(const FewTokens p) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int groups = groups_of(p.hidden), each = (groups + WARPS - 1) / WARPS, group0 = warp * each;
+    const int mine = min(each, groups - group0);  // may be negative
+    const uint32_t h_row = h_bytes(groups), w_row = w_bytes(groups), slot_bytes = kBatch * w_row;
+    uint8_t* tokens = smem + SLOTS * slot_bytes;
+    float2* parts = reinterpret_cast<float2*>(tokens + kTokens * h_row);  // [2][WARPS][32]
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)), hs = ring + SLOTS * slot_bytes;
+    chain_go();
+
+    // Where the 16 bytes `chunk` (0 to 3) of a group of row r lie. The exchange of chunks by the row's bits, in reverse order, puts both the
+    // eight rows of one chunk and two rows of four chunks on different banks.
+    auto w_at = [&](int r, int chunk, int group) {
+        const int turn = (r & 1) << 2 | (r & 2) | (r >> 2 & 1);
+        return static_cast<uint32_t>(r) * w_row + (group >> 1) * 128 + ((((group & 1) << 2) + chunk) ^ turn) * 16;
+    };
+    // rows behind the last one and columns behind the row's end are zeros
+    auto fetch = [&](int64_t v0, int slot) {
+        if (v0 < p.vocab) {
+            const bool row = v0 + g < p.vocab;
+            const T* from = static_cast<const T*>(p.w) + (row ? v0 + g : 0) * p.w_pitch;
+#pragma unroll
+            for (int i = 0; i < kMostGroups; ++i) {
+                if (i < mine) {
+                    const int64_t c = static_cast<int64_t>(group0 + i) * kGroup + t * 8;
+                    const bool in = row && c < p.hidden;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ring + slot * slot_bytes + w_at(g, t, group0 + i)), "l"(from + (in ? c : 0)), "r"(in ? 16 : 0)
+                                 : "memory");
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kBatch;
+    int64_t v0 = static_cast<int64_t>(blockIdx.x) * kBatch;
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) fetch(v0 + s * step, s);
+
+    auto target_of = [&](int64_t n) { return p.wide ? static_cast<const int64_t*>(p.targets)[n] : static_cast<int64_t>(static_cast<const int32_t*>(p.targets)[n]); };
+    // the largest finite gradient, which lands at kTop
+    const bool live = lane < p.tokens && target_of(lane) != p.ignore;
+    const unsigned lives = __ballot_sync(0xFFFFFFFFu, live);
+    float top = live ? fabsf(p.grad[lane]) : 0.0f;
+    if (!isfinite(top)) top = 0.0f;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    top = __shfl_sync(0xFFFFFFFFu, top, 0);
+    if (top == 0.0f) top = 1.0f;
+    // this lane's token
+    const bool counts = lives >> g & 1;
+    const int64_t target = counts ? target_of(g) : 0;
+    const float lse = counts ? p.lse[g] : 0.0f;
+    const float grad = !counts ? 0.0f : target < 0 || target >= p.vocab ? NAN : p.grad[g] / top * kTop;
+
+    // The tokens, zeros where there is none or it does not count: column 8 a + 2 b + c of a group (a, b in 0..3, c in 0..1) at 8 b + 2 a + c.
+    {
+        struct alignas(16) Eight { uint16_t v[8]; };
+        const uint16_t* from = static_cast<const uint16_t*>(p.h);
+        const bool vectors = ((reinterpret_cast<uintptr_t>(from) | static_cast<uintptr_t>(p.h_pitch * 2)) & 15) == 0;
+        const int chunks = groups * 4;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < kTokens * chunks; i += WARPS * 32) {
+            const int n = i / chunks, k = i - n * chunks;
+            Eight e = {};
+            if ((lives >> n & 1) && k * 8 < p.hidden) {
+                const uint16_t* at = from + n * p.h_pitch + k * 8;
+                if (vectors) {
+                    e = *reinterpret_cast<const Eight*>(at);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) e.v[j] = at[j];
+                }
+            }
+            uint8_t* to = tokens + n * h_row + (k >> 2) * 64 + (k & 3) * 4;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) *reinterpret_cast<uint32_t*>(to + b * 16) = e.v[2 * b] | static_cast<uint32_t>(e.v[2 * b + 1]) << 16;
+        }
+    }
+    __syncthreads();
+
+    float dh[kMostGroups][8];
+#pragma unroll
+    for (int i = 0; i < kMostGroups; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dh[i][j] = 0.0f;
+    const uint32_t h_at = hs + (lane & 7) * h_row + (lane >> 3) * 16;  // this lane's row of the four matrices of a group
+    int slot = 0, parity = 0;
+    for (; v0 < p.vocab; v0 += step, parity ^= 1) {
+        const uint32_t w = ring + slot * slot_bytes;
+        asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 1) : "memory");
+        __syncwarp();  // the other lanes' copies
+        float sums[2][4] = {};
+#pragma unroll
+        for (int i = 0; i < kMostGroups; ++i) {
+            if (i < mine) {
+                uint32_t a[4], x, y, z, u;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x), "=r"(y), "=r"(z), "=r"(u) : "r"(w + w_at(g, t, group0 + i)) : "memory");
+                load4(a, h_at + (group0 + i) * 64);
+                mma_k16<T>(sums[0], a[0], 0, a[1], 0, x, y);
+                mma_k16<T>(sums[1], a[2], 0, a[3], 0, z, u);
+            }
+        }
+        // token g, rows 2 t and 2 t + 1; the other parity's were read before the last barrier
+        parts[(parity * WARPS + warp) * 32 + lane] = make_float2(sums[0][0] + sums[1][0], sums[0][1] + sums[1][1]);
+        __syncthreads();
+        float2 x = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < WARPS; ++k) {
+            const float2 one = parts[(parity * WARPS + k) * 32 + lane];
+            x.x += one.x;
+            x.y += one.y;
+        }
+        auto d_of = [&](float logit, int64_t v) {
+            if (!counts || v >= p.vocab) return 0.0f;
+            return (v == target ? expm1f(logit - lse) : __expf(logit - lse)) * grad;
+        };
+        const float d0 = d_of(x.x, v0 + 2 * t), d1 = d_of(x.y, v0 + 2 * t + 1);
+        const uint32_t hi = Pair<T>::pack(d0, d1);
+        const float2 back = Pair<T>::unpack(hi);
+        // an infinity has no rest
+        const uint32_t lo = Pair<T>::pack(isinf(back.x) ? 0.0f : d0 - back.x, isinf(back.y) ? 0.0f : d1 - back.y);
+        const uint32_t hi_rows = transposed(hi), lo_rows = transposed(lo);  // row g, tokens 2 t and 2 t + 1
+        T* out = static_cast<T*>(p.dweight) + (v0 + g) * p.hidden + t * 8;
+        const bool writes = p.dweight && v0 + g < p.vocab;
+#pragma unroll
+        for (int i = 0; i < kMostGroups; ++i) {
+            if (i < mine) {
+                const int group = group0 + i;
+                if (p.sums) {
+                    uint32_t m[4];
+                    load4_transposed(m, w + w_at(lane & 7, lane >> 3, group));
+                    mma_k16<T>(dh[i], m[0], m[1], m[0], m[1], hi, lo);
+                    mma_k16<T>(dh[i] + 4, m[2], m[3], m[2], m[3], hi, lo);
+                }
+                if (p.dweight) {
+                    uint32_t b[4], r[4];
+                    load4_transposed(b, h_at + group * 64);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float c[4] = {};
+                        mma_k8<T>(c, hi_rows, lo_rows, b[k]);
+                        r[k] = Pair<T>::pack(unscale(c[0] + c[2], top), unscale(c[1] + c[3], top));
+                    }
+                    if (writes && group * kGroup + t * 8 < p.hidden) *reinterpret_cast<uint4*>(out + group * kGroup) = make_uint4(r[0], r[1], r[2], r[3]);
+                }
+            }
+        }
+        __syncwarp();  // all lanes have read the slot
+        fetch(v0 + SLOTS * step, slot);
+        slot = slot == SLOTS - 1 ? 0 : slot + 1;
+    }
+    if (p.sums) {
+#pragma unroll
+        for (int i = 0; i < kMostGroups; ++i) {
+            if (i < mine) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int64_t c = (group0 + i) * kGroup + (j >> 2) * 16 + (j >> 1 & 1) * 8 + g;
+                    const int n = 2 * t + (j & 1);
+                    if (n < p.tokens && c < p.hidden) p.sums[(static_cast<int64_t>(blockIdx.x) * p.tokens + n) * p.hidden + c] = unscale(dh[i][j], top);
+                }
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host ---------------
+// Rows of up to 64 groups leave room for two blocks of eight warps on an SM, whose barriers cover for one another.
+int warps_for(int64_t hidden) { return groups_of(hidden) <= 8 * kMostGroups ? 8 : 16; }
+
+template <typename T, int WARPS, int SLOTS>
+tn_status launch(const FewTokens& p, cudaStream_t stream) {
+    static thread_local int device = -1;  // the opt-in shared-memory size belongs to kernel and device
+    const size_t smem = smem_bytes(groups_of(p.hidden), SLOTS, WARPS);
+    int dev = 0;
+    TN_CUDA(cudaGetDevice(&dev));
+    if (device != dev) {
+        TN_CUDA(cudaFuncSetAttribute(half_grad_kernel<T, WARPS, SLOTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        device = dev;
+    }
+    half_grad_kernel<T, WARPS, SLOTS><<<(unsigned)half_grad_blocks(p.hidden, p.vocab), WARPS * 32, smem, stream>>>(p);
+    return after_launch("half_grad_kernel");
+}
+template <typename T, int WARPS>
+tn_status launch_slots(const FewTokens& p, cudaStream_t stream) {
+    // a third batch where it fits
+    return smem_bytes(groups_of(p.hidden), 3, WARPS) <= 226 * 1024 / (16 / WARPS) ? launch<T, WARPS, 3>(p, stream) : launch<T, WARPS, 2>(p, stream);
+}
+template <typename T>
+tn_status launch_typed(const FewTokens& p, cudaStream_t stream) {
+    return warps_for(p.hidden) == 8 ? launch_slots<T, 8>(p, stream) : launch_slots<T, 16>(p, stream);
+}
+
+}  // namespace
+
+// Sixteen warps hold dh's sums of 4096 columns. Rows that are not aligned to 16 bytes take the larger products, which copy the weights.
+bool half_grad_fits(const FewTokens& p) {
+    const bool wide = p.hidden % 8 == 0 && p.w_pitch % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.w) | reinterpret_cast<uintptr_t>(p.dweight)) & 15) == 0;
+    return (p.dtype == TN_FLOAT16 || p.dtype == TN_BFLOAT16) && p.tokens <= kTokens && p.hidden <= 16 * kMostGroups * kGroup && wide;
+}
+int64_t half_grad_blocks(int64_t hidden, int64_t vocab) { return std::min<int64_t>((int64_t)sm_count() * (16 / warps_for(hidden)), ceil_div(vocab, kBatch)); }
+
+tn_status half_grad(const FewTokens& p, cudaStream_t stream) {
+    TN_TRY(p.dtype == TN_FLOAT16 ? launch_typed<__half>(p, stream) : launch_typed<__nv_bfloat16>(p, stream));
+    return p.dhidden ? few_dhidden(p, half_grad_blocks(p.hidden, p.vocab), stream) : TN_SUCCESS;
+}
+
+}  // namespace tnb

@@ -125,3 +125,26 @@ def test_rows_behind_the_results_are_left_alone(tokens, dtype):
     A.check(A.lib().tn_linear_cross_entropy_grad(*[C.byref(r) for r in rec], tb.current_stream(h), IGNORE))
     check_grad(g, h, w, t, lse, (big_h[:tokens], big_w[:301]))
     assert bool((big_h[tokens:] == 7.0).all()) and bool((big_w[301:] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hidden,vocab", [(8, 1), (40, 7), (264, 10007), (768, 9), (1696, 4801), (2048, 2000), (2056, 3001), (3456, 2500), (4096, 5003)])
+@pytest.mark.parametrize("tokens", [1, 5, 8, 9])
+def test_one_pass_of_sixteen_bits(tokens, hidden, vocab, dtype):
+    both(*data(tokens, hidden, vocab, dtype, 10))
+
+
+def test_small_and_infinite_gradients():
+    """float16's d would be lost unscaled; one infinite gradient leaves the other tokens' rows as they are."""
+    h, w, t, g = data(6, 264, 3000, torch.float16, 11)
+    both(h, w, t, g * 2.0**-20)
+    lse = tb.linear_cross_entropy(h, w, t)[1]
+    want = tb.linear_cross_entropy_grad(g, h, w, t, lse)[0]
+    keep = [0, 1, 2, 4, 5]
+    rest = g.clone()
+    rest[3] = 0.0
+    same = tb.linear_cross_entropy_grad(rest, h, w, t, lse)[0]
+    g[3] = float("inf")
+    got, dw = tb.linear_cross_entropy_grad(g, h, w, t, lse)
+    assert torch.equal(got[keep], same[keep]) and not bool(torch.isfinite(got[3]).any()) and not bool(torch.isfinite(dw).any())
+    assert bool(torch.isfinite(want).all())
