@@ -45,14 +45,17 @@ __device__ __forceinline__ void mma_k16(float* c, uint32_t a0, uint32_t a1, uint
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// Rows 0 to 7 and rows 8 to 15 of the product, added.
 template <typename T>
-__device__ __forceinline__ void mma_k8(float* c, uint32_t a0, uint32_t a1, uint32_t b) {
+__device__ __forceinline__ float2 mma_k8(uint32_t a0, uint32_t a1, uint32_t b) {
+    float c[4];
     if constexpr (std::is_same<T, __half>::value)
-        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(b));
+        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%7, %7, %7, %7};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(b), "f"(0.0f));
     else
-        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(b));
+        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%7, %7, %7, %7};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(b), "f"(0.0f));
+    return make_float2(c[0] + c[2], c[1] + c[3]);
 }
 __device__ __forceinline__ void load4(uint32_t (&m)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(m[0]), "=r"(m[1]), "=r"(m[2]), "=r"(m[3]) : "r"(at) : "memory");
@@ -77,46 +80,51 @@ __host__ __device__ __forceinline__ size_t smem_bytes(int groups, int slots, int
 // SLOTS batches of W lie in shared memory or are on their way there.
 template <typename T, int WARPS, int SLOTS>
 __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) half_grad_kernel(const FewTokens p) {
+    constexpr bool SCALED = std::is_same<T, __half>::value;
     extern __shared__ __align__(128) uint8_t smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int groups = groups_of(p.hidden), each = (groups + WARPS - 1) / WARPS, group0 = warp * each;
+    const int groups = groups_of(p.hidden), each = (groups + 2 * WARPS - 1) / (2 * WARPS) * 2, group0 = warp * each;  // an even number
     const int mine = min(each, groups - group0);  // may be negative
+    const int left = min(static_cast<int>(p.hidden) - group0 * kGroup, each * kGroup) - t * 8;  // columns from this lane's first on
     const uint32_t h_row = h_bytes(groups), w_row = w_bytes(groups), slot_bytes = kBatch * w_row;
     uint8_t* tokens = smem + SLOTS * slot_bytes;
     float2* parts = reinterpret_cast<float2*>(tokens + kTokens * h_row);  // [2][WARPS][32]
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)), hs = ring + SLOTS * slot_bytes;
     chain_go();
 
-    // Where the 16 bytes `chunk` (0 to 3) of a group of row r lie. The exchange of chunks by the row's bits, in reverse order, puts both the
-    // eight rows of one chunk and two rows of four chunks on different banks.
-    auto w_at = [&](int r, int chunk, int group) {
+    // Where the 16 bytes `chunk` (0 to 3) of this warp's group i of row r lie. The exchange of chunks by the row's bits, in reverse order, puts
+    // both the eight rows of one chunk and two rows of four chunks on different banks.
+    auto w_at = [&](int r, int chunk) {
         const int turn = (r & 1) << 2 | (r & 2) | (r >> 2 & 1);
-        return static_cast<uint32_t>(r) * w_row + (group >> 1) * 128 + ((((group & 1) << 2) + chunk) ^ turn) * 16;
+        return ring + static_cast<uint32_t>(r) * w_row + group0 * 64 + (chunk ^ turn) * 16;
     };
-    // rows behind the last one and columns behind the row's end are zeros
-    auto fetch = [&](int64_t v0, int slot) {
-        if (v0 < p.vocab) {
-            const bool row = v0 + g < p.vocab;
-            const T* from = static_cast<const T*>(p.w) + (row ? v0 + g : 0) * p.w_pitch;
-#pragma unroll
-            for (int i = 0; i < kMostGroups; ++i) {
-                if (i < mine) {
-                    const int64_t c = static_cast<int64_t>(group0 + i) * kGroup + t * 8;
-                    const bool in = row && c < p.hidden;
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ring + slot * slot_bytes + w_at(g, t, group0 + i)), "l"(from + (in ? c : 0)), "r"(in ? 16 : 0)
-                                 : "memory");
-                }
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+    const uint32_t copied = w_at(g, t), matrix = w_at(lane & 7, lane >> 3);
+    auto of_group = [](uint32_t at, int i) { return (i & 1 ? at ^ 64 : at) + (i >> 1) * 128; };
+    const T* const w_first = static_cast<const T*>(p.w) + group0 * kGroup + t * 8;
+    // rows behind the last one are zeros
+    auto fetch = [&](const T* from, int bytes, uint32_t to, int i) {
+        if (i * kGroup < left) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + of_group(copied, i)), "l"(from + i * kGroup), "r"(bytes) : "memory");
     };
+    auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
     const int64_t step = static_cast<int64_t>(gridDim.x) * kBatch;
     int64_t v0 = static_cast<int64_t>(blockIdx.x) * kBatch;
 #pragma unroll
-    for (int s = 0; s < SLOTS; ++s) fetch(v0 + s * step, s);
+    for (int s = 0; s < SLOTS; ++s) {
+        const int64_t v = v0 + s * step;
+        const bool row = v + g < p.vocab;
+        if (v < p.vocab) {
+#pragma unroll
+            for (int i = 0; i < kMostGroups; ++i) fetch(w_first + (row ? v + g : 0) * p.w_pitch, row ? 16 : 0, s * slot_bytes, i);
+        }
+        commit();
+        // columns behind the row's end are zeros and stay so
+#pragma unroll
+        for (int i = 0; i < kMostGroups; ++i)
+            if (i < mine && i * kGroup >= left) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(of_group(copied, i) + s * slot_bytes), "r"(0) : "memory");
+    }
 
     auto target_of = [&](int64_t n) { return p.wide ? static_cast<const int64_t*>(p.targets)[n] : static_cast<int64_t>(static_cast<const int32_t*>(p.targets)[n]); };
-    // the largest finite gradient, which lands at kTop
+    // float16: the largest finite gradient lands at kTop (what is lost where top / kTop is no normal number, float16 cannot hold)
     const bool live = lane < p.tokens && target_of(lane) != p.ignore;
     const unsigned lives = __ballot_sync(0xFFFFFFFFu, live);
     float top = live ? fabsf(p.grad[lane]) : 0.0f;
@@ -125,11 +133,12 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) half_grad_kernel(const
     for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     top = __shfl_sync(0xFFFFFFFFu, top, 0);
     if (top == 0.0f) top = 1.0f;
+    const float back = top / kTop;
     // this lane's token
     const bool counts = lives >> g & 1;
     const int64_t target = counts ? target_of(g) : 0;
     const float lse = counts ? p.lse[g] : 0.0f;
-    const float grad = !counts ? 0.0f : target < 0 || target >= p.vocab ? NAN : p.grad[g] / top * kTop;
+    const float grad = !counts ? 0.0f : target < 0 || target >= p.vocab ? NAN : SCALED ? p.grad[g] / top * kTop : p.grad[g];
 
     // The tokens, zeros where there is none or it does not count: column 8 a + 2 b + c of a group (a, b in 0..3, c in 0..1) at 8 b + 2 a + c.
     {
@@ -162,10 +171,10 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) half_grad_kernel(const
     for (int i = 0; i < kMostGroups; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) dh[i][j] = 0.0f;
-    const uint32_t h_at = hs + (lane & 7) * h_row + (lane >> 3) * 16;  // this lane's row of the four matrices of a group
-    int slot = 0, parity = 0;
+    const uint32_t h_at = hs + (lane & 7) * h_row + (lane >> 3) * 16 + group0 * 64;  // this lane's row of the four matrices of a group
+    uint32_t slot = 0;
+    int parity = 0;
     for (; v0 < p.vocab; v0 += step, parity ^= 1) {
-        const uint32_t w = ring + slot * slot_bytes;
         asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 1) : "memory");
         __syncwarp();  // the other lanes' copies
         float sums[2][4] = {};
@@ -173,8 +182,8 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) half_grad_kernel(const
         for (int i = 0; i < kMostGroups; ++i) {
             if (i < mine) {
                 uint32_t a[4], x, y, z, u;
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x), "=r"(y), "=r"(z), "=r"(u) : "r"(w + w_at(g, t, group0 + i)) : "memory");
-                load4(a, h_at + (group0 + i) * 64);
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x), "=r"(y), "=r"(z), "=r"(u) : "r"(of_group(copied, i) + slot) : "memory");
+                load4(a, h_at + i * 64);
                 mma_k16<T>(sums[0], a[0], 0, a[1], 0, x, y);
                 mma_k16<T>(sums[1], a[2], 0, a[3], 0, z, u);
             }
@@ -195,39 +204,42 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) half_grad_kernel(const
         };
         const float d0 = d_of(x.x, v0 + 2 * t), d1 = d_of(x.y, v0 + 2 * t + 1);
         const uint32_t hi = Pair<T>::pack(d0, d1);
-        const float2 back = Pair<T>::unpack(hi);
+        const float2 upper = Pair<T>::unpack(hi);
         // an infinity has no rest
-        const uint32_t lo = Pair<T>::pack(isinf(back.x) ? 0.0f : d0 - back.x, isinf(back.y) ? 0.0f : d1 - back.y);
+        const uint32_t lo = Pair<T>::pack(isinf(upper.x) ? 0.0f : d0 - upper.x, isinf(upper.y) ? 0.0f : d1 - upper.y);
         const uint32_t hi_rows = transposed(hi), lo_rows = transposed(lo);  // row g, tokens 2 t and 2 t + 1
-        T* out = static_cast<T*>(p.dweight) + (v0 + g) * p.hidden + t * 8;
-        const bool writes = p.dweight && v0 + g < p.vocab;
+        T* out = static_cast<T*>(p.dweight) + (v0 + g) * p.hidden + group0 * kGroup + t * 8;
+        const int stores = p.dweight && v0 + g < p.vocab ? left : 0;
+        const int64_t after = v0 + SLOTS * step;
+        const bool row = after + g < p.vocab;
+        const T* next = w_first + (row ? after + g : 0) * p.w_pitch;
 #pragma unroll
         for (int i = 0; i < kMostGroups; ++i) {
             if (i < mine) {
-                const int group = group0 + i;
+                uint32_t m[4];
+                load4_transposed(m, of_group(matrix, i) + slot);
+                __syncwarp();  // all lanes have read the group: the next rows may take its place
+                fetch(next, row ? 16 : 0, slot, i);
                 if (p.sums) {
-                    uint32_t m[4];
-                    load4_transposed(m, w + w_at(lane & 7, lane >> 3, group));
                     mma_k16<T>(dh[i], m[0], m[1], m[0], m[1], hi, lo);
                     mma_k16<T>(dh[i] + 4, m[2], m[3], m[2], m[3], hi, lo);
                 }
                 if (p.dweight) {
                     uint32_t b[4], r[4];
-                    load4_transposed(b, h_at + group * 64);
+                    load4_transposed(b, h_at + i * 64);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        float c[4] = {};
-                        mma_k8<T>(c, hi_rows, lo_rows, b[k]);
-                        r[k] = Pair<T>::pack(unscale(c[0] + c[2], top), unscale(c[1] + c[3], top));
+                        const float2 c = mma_k8<T>(hi_rows, lo_rows, b[k]);
+                        r[k] = SCALED ? Pair<T>::pack(c.x * back, c.y * back) : Pair<T>::pack(c.x, c.y);
                     }
-                    if (writes && group * kGroup + t * 8 < p.hidden) *reinterpret_cast<uint4*>(out + group * kGroup) = make_uint4(r[0], r[1], r[2], r[3]);
+                    if (i * kGroup < stores) *reinterpret_cast<uint4*>(out + i * kGroup) = make_uint4(r[0], r[1], r[2], r[3]);
                 }
             }
         }
-        __syncwarp();  // all lanes have read the slot
-        fetch(v0 + SLOTS * step, slot);
-        slot = slot == SLOTS - 1 ? 0 : slot + 1;
+        commit();
+        slot = slot == (SLOTS - 1) * slot_bytes ? 0 : slot + slot_bytes;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (p.sums) {
 #pragma unroll
         for (int i = 0; i < kMostGroups; ++i) {
@@ -236,7 +248,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) half_grad_kernel(const
                 for (int j = 0; j < 8; ++j) {
                     const int64_t c = (group0 + i) * kGroup + (j >> 2) * 16 + (j >> 1 & 1) * 8 + g;
                     const int n = 2 * t + (j & 1);
-                    if (n < p.tokens && c < p.hidden) p.sums[(static_cast<int64_t>(blockIdx.x) * p.tokens + n) * p.hidden + c] = unscale(dh[i][j], top);
+                    if (n < p.tokens && c < p.hidden) p.sums[(static_cast<int64_t>(blockIdx.x) * p.tokens + n) * p.hidden + c] = SCALED ? dh[i][j] * back : dh[i][j];
                 }
             }
         }
