@@ -4,7 +4,10 @@
 // from them, then dW = d^T h and dh += d W before the next rows take their place. The bound is memory: W is read once and dW written once.
 // The products run as mma.sync with the eight tokens on one side: tcgen05's smallest tile has 64 rows, reads both operands from shared
 // memory, where d would have to be written first, and returns through TMEM, where dW would wait; here d stays in registers from one
-// product's result to the next one's operand. (On the FP32 pipe the same pass took 127 us for four tokens over 32000 x 4096.)
+// product's result to the next one's operand. Four tokens over 32000 x 4096 bfloat16: 107 us with dh's second kernel, 81 at copy speed (on the
+// FP32 pipe the same pass took 136, the products for many tokens take 230); 8 over 131072 x 4096: 366 us, 90 % of copy speed. What is left is
+// shared memory's: its pipe is busy 80 % of the time, with W and the tokens read twice a batch; a batch of 16 rows would read the tokens
+// half as often, but two such batches of 4096 columns do not fit.
 //
 // A warp owns groups of 32 columns of all rows, fetches them with cp.async, reads each eight rows twice from shared memory (as they lie for
 // the logits, transposed for dh) and fetches the next ones in their place, so the only barrier is the one over the warps' parts of the logits.
@@ -25,6 +28,7 @@ namespace {
 constexpr int kTokens = 8, kBatch = 8;  // tokens, and vocabulary rows at a time
 constexpr int kGroup = 32;              // columns
 constexpr int kMostGroups = 8;          // of a warp: 64 registers of dh's sums
+template <int EACH> constexpr int kSlots = EACH == kMostGroups ? 2 : 3;  // what fits beside the tokens
 
 template <typename T> struct Pair;
 template <> struct Pair<__half> {
@@ -69,24 +73,21 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     return r;
 }
 
-__host__ __device__ __forceinline__ int groups_of(int64_t hidden) { return static_cast<int>((hidden + kGroup - 1) / kGroup); }
 // Bytes between the tokens in shared memory (16 more than a multiple of 64: eight rows fall on different banks) and between W's rows.
-__host__ __device__ __forceinline__ uint32_t h_bytes(int groups) { return groups * 64 + 16; }
-__host__ __device__ __forceinline__ uint32_t w_bytes(int groups) { return (groups + 1) / 2 * 128; }
-__host__ __device__ __forceinline__ size_t smem_bytes(int groups, int slots, int warps) {
-    return static_cast<size_t>(slots) * kBatch * w_bytes(groups) + kTokens * h_bytes(groups) + 2 * warps * 32 * sizeof(float2);
-}
+constexpr uint32_t h_bytes(int groups) { return groups * 64 + 16; }
+constexpr uint32_t w_bytes(int groups) { return groups * 64; }
 
-// SLOTS batches of W lie in shared memory or are on their way there.
-template <typename T, int WARPS, int SLOTS>
+// EACH groups per warp; a row is taken to have WARPS * EACH of them, zeros behind its end, so that no branch keeps one group's loads from
+// running under another's products. DW: with the weights' gradient. SLOTS batches of W lie in shared memory or are on their way there.
+template <typename T, int WARPS, int EACH, bool DW>
 __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) half_grad_kernel(const FewTokens p) {
     constexpr bool SCALED = std::is_same<T, __half>::value;
     extern __shared__ __align__(128) uint8_t smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int groups = groups_of(p.hidden), each = (groups + 2 * WARPS - 1) / (2 * WARPS) * 2, group0 = warp * each;  // an even number
-    const int mine = min(each, groups - group0);  // may be negative
-    const int left = min(static_cast<int>(p.hidden) - group0 * kGroup, each * kGroup) - t * 8;  // columns from this lane's first on
-    const uint32_t h_row = h_bytes(groups), w_row = w_bytes(groups), slot_bytes = kBatch * w_row;
+    constexpr int GROUPS = WARPS * EACH, SLOTS = kSlots<EACH>;
+    constexpr uint32_t h_row = h_bytes(GROUPS), w_row = w_bytes(GROUPS), slot_bytes = kBatch * w_row;
+    const int group0 = warp * EACH;
+    const int left = static_cast<int>(p.hidden) - group0 * kGroup - t * 8;  // columns from this lane's first on; may be negative
     uint8_t* tokens = smem + SLOTS * slot_bytes;
     float2* parts = reinterpret_cast<float2*>(tokens + kTokens * h_row);  // [2][WARPS][32]
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)), hs = ring + SLOTS * slot_bytes;
@@ -98,29 +99,47 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) half_grad_kernel(const
         const int turn = (r & 1) << 2 | (r & 2) | (r >> 2 & 1);
         return ring + static_cast<uint32_t>(r) * w_row + group0 * 64 + (chunk ^ turn) * 16;
     };
-    const uint32_t copied = w_at(g, t), matrix = w_at(lane & 7, lane >> 3);
+    const uint32_t mine = w_at(g, t), matrix = w_at(lane & 7, lane >> 3);
     auto of_group = [](uint32_t at, int i) { return (i & 1 ? at ^ 64 : at) + (i >> 1) * 128; };
-    const T* const w_first = static_cast<const T*>(p.w) + group0 * kGroup + t * 8;
-    // rows behind the last one are zeros
-    auto fetch = [&](const T* from, int bytes, uint32_t to, int i) {
-        if (i * kGroup < left) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + of_group(copied, i)), "l"(from + i * kGroup), "r"(bytes) : "memory");
+    // A copy takes 128 bytes, two groups, of four rows: 64 bytes of eight rows are twice as many transactions (113 us against 106 at 32000 x 4096).
+    const int copy_row = lane >> 3, copy_left = static_cast<int>(p.hidden) - group0 * kGroup - (lane & 7) * 8;
+    uint32_t copied[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) copied[k] = w_at(copy_row + 4 * k, lane & 7);
+    const T* const w_first = static_cast<const T*>(p.w) + group0 * kGroup + (lane & 7) * 8;
+    struct Rows { const T* from[2]; int bytes[2]; };
+    // rows copy_row and copy_row + 4 of the batch at v; rows behind the last one are zeros
+    auto rows_at = [&](int64_t v) {
+        Rows r;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const bool row = v + copy_row + 4 * k < p.vocab;
+            r.from[k] = w_first + (row ? v + copy_row + 4 * k : 0) * p.w_pitch;
+            r.bytes[k] = row ? 16 : 0;
+        }
+        return r;
+    };
+    auto fetch = [&](const Rows& r, uint32_t slot, int i) {  // groups 2 i and 2 i + 1
+        if (i * 2 * kGroup < copy_left)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(copied[k] + slot + i * 128), "l"(r.from[k] + i * 2 * kGroup), "r"(r.bytes[k]) : "memory");
     };
     auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
     const int64_t step = static_cast<int64_t>(gridDim.x) * kBatch;
     int64_t v0 = static_cast<int64_t>(blockIdx.x) * kBatch;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-        const int64_t v = v0 + s * step;
-        const bool row = v + g < p.vocab;
-        if (v < p.vocab) {
-#pragma unroll
-            for (int i = 0; i < kMostGroups; ++i) fetch(w_first + (row ? v + g : 0) * p.w_pitch, row ? 16 : 0, s * slot_bytes, i);
-        }
-        commit();
+        const Rows rows = rows_at(v0 + s * step);
         // columns behind the row's end are zeros and stay so
 #pragma unroll
-        for (int i = 0; i < kMostGroups; ++i)
-            if (i < mine && i * kGroup >= left) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(of_group(copied, i) + s * slot_bytes), "r"(0) : "memory");
+        for (int i = 0; i < EACH / 2; ++i) {
+            fetch(rows, s * slot_bytes, i);
+            if (i * 2 * kGroup >= copy_left)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(copied[k] + s * slot_bytes + i * 128), "r"(0) : "memory");
+        }
+        commit();
     }
 
     auto target_of = [&](int64_t n) { return p.wide ? static_cast<const int64_t*>(p.targets)[n] : static_cast<int64_t>(static_cast<const int32_t*>(p.targets)[n]); };
@@ -145,7 +164,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) half_grad_kernel(const
         struct alignas(16) Eight { uint16_t v[8]; };
         const uint16_t* from = static_cast<const uint16_t*>(p.h);
         const bool vectors = ((reinterpret_cast<uintptr_t>(from) | static_cast<uintptr_t>(p.h_pitch * 2)) & 15) == 0;
-        const int chunks = groups * 4;
+        constexpr int chunks = GROUPS * 4;
 #pragma unroll 4
         for (int i = threadIdx.x; i < kTokens * chunks; i += WARPS * 32) {
             const int n = i / chunks, k = i - n * chunks;
@@ -166,9 +185,9 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) half_grad_kernel(const
     }
     __syncthreads();
 
-    float dh[kMostGroups][8];
+    float dh[EACH][8];
 #pragma unroll
-    for (int i = 0; i < kMostGroups; ++i)
+    for (int i = 0; i < EACH; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) dh[i][j] = 0.0f;
     const uint32_t h_at = hs + (lane & 7) * h_row + (lane >> 3) * 16 + group0 * 64;  // this lane's row of the four matrices of a group
@@ -179,14 +198,12 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) half_grad_kernel(const
         __syncwarp();  // the other lanes' copies
         float sums[2][4] = {};
 #pragma unroll
-        for (int i = 0; i < kMostGroups; ++i) {
-            if (i < mine) {
-                uint32_t a[4], x, y, z, u;
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x), "=r"(y), "=r"(z), "=r"(u) : "r"(of_group(copied, i) + slot) : "memory");
-                load4(a, h_at + i * 64);
-                mma_k16<T>(sums[0], a[0], 0, a[1], 0, x, y);
-                mma_k16<T>(sums[1], a[2], 0, a[3], 0, z, u);
-            }
+        for (int i = 0; i < EACH; ++i) {
+            uint32_t a[4], x, y, z, u;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x), "=r"(y), "=r"(z), "=r"(u) : "r"(of_group(mine, i) + slot) : "memory");
+            load4(a, h_at + i * 64);
+            mma_k16<T>(sums[0], a[0], 0, a[1], 0, x, y);
+            mma_k16<T>(sums[1], a[2], 0, a[3], 0, z, u);
         }
         // token g, rows 2 t and 2 t + 1; the other parity's were read before the last barrier
         parts[(parity * WARPS + warp) * 32 + lane] = make_float2(sums[0][0] + sums[1][0], sums[0][1] + sums[1][1]);
@@ -209,31 +226,27 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) half_grad_kernel(const
         const uint32_t lo = Pair<T>::pack(isinf(upper.x) ? 0.0f : d0 - upper.x, isinf(upper.y) ? 0.0f : d1 - upper.y);
         const uint32_t hi_rows = transposed(hi), lo_rows = transposed(lo);  // row g, tokens 2 t and 2 t + 1
         T* out = static_cast<T*>(p.dweight) + (v0 + g) * p.hidden + group0 * kGroup + t * 8;
-        const int stores = p.dweight && v0 + g < p.vocab ? left : 0;
-        const int64_t after = v0 + SLOTS * step;
-        const bool row = after + g < p.vocab;
-        const T* next = w_first + (row ? after + g : 0) * p.w_pitch;
+        const int stores = v0 + g < p.vocab ? left : 0;
+        const Rows next = rows_at(v0 + SLOTS * step);
 #pragma unroll
-        for (int i = 0; i < kMostGroups; ++i) {
-            if (i < mine) {
-                uint32_t m[4];
-                load4_transposed(m, of_group(matrix, i) + slot);
-                __syncwarp();  // all lanes have read the group: the next rows may take its place
-                fetch(next, row ? 16 : 0, slot, i);
-                if (p.sums) {
-                    mma_k16<T>(dh[i], m[0], m[1], m[0], m[1], hi, lo);
-                    mma_k16<T>(dh[i] + 4, m[2], m[3], m[2], m[3], hi, lo);
-                }
-                if (p.dweight) {
-                    uint32_t b[4], r[4];
-                    load4_transposed(b, h_at + i * 64);
+        for (int i = 0; i < EACH; ++i) {
+            uint32_t m[4];
+            load4_transposed(m, of_group(matrix, i) + slot);
+            if (i & 1) {
+                __syncwarp();  // all lanes have read the two groups: the next rows may take their place
+                fetch(next, slot, i / 2);
+            }
+            mma_k16<T>(dh[i], m[0], m[1], m[0], m[1], hi, lo);
+            mma_k16<T>(dh[i] + 4, m[2], m[3], m[2], m[3], hi, lo);
+            if constexpr (DW) {
+                uint32_t b[4], r[4];
+                load4_transposed(b, h_at + i * 64);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float2 c = mma_k8<T>(hi_rows, lo_rows, b[k]);
-                        r[k] = SCALED ? Pair<T>::pack(c.x * back, c.y * back) : Pair<T>::pack(c.x, c.y);
-                    }
-                    if (i * kGroup < stores) *reinterpret_cast<uint4*>(out + i * kGroup) = make_uint4(r[0], r[1], r[2], r[3]);
+                for (int k = 0; k < 4; ++k) {
+                    const float2 c = mma_k8<T>(hi_rows, lo_rows, b[k]);
+                    r[k] = SCALED ? Pair<T>::pack(c.x * back, c.y * back) : Pair<T>::pack(c.x, c.y);
                 }
+                if (i * kGroup < stores) *reinterpret_cast<uint4*>(out + i * kGroup) = make_uint4(r[0], r[1], r[2], r[3]);
             }
         }
         commit();
@@ -242,44 +255,48 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) half_grad_kernel(const
     asm volatile("cp.async.wait_all;" ::: "memory");
     if (p.sums) {
 #pragma unroll
-        for (int i = 0; i < kMostGroups; ++i) {
-            if (i < mine) {
+        for (int i = 0; i < EACH; ++i) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int64_t c = (group0 + i) * kGroup + (j >> 2) * 16 + (j >> 1 & 1) * 8 + g;
-                    const int n = 2 * t + (j & 1);
-                    if (n < p.tokens && c < p.hidden) p.sums[(static_cast<int64_t>(blockIdx.x) * p.tokens + n) * p.hidden + c] = SCALED ? dh[i][j] * back : dh[i][j];
-                }
+            for (int j = 0; j < 8; ++j) {
+                const int64_t c = (group0 + i) * kGroup + (j >> 2) * 16 + (j >> 1 & 1) * 8 + g;
+                const int n = 2 * t + (j & 1);
+                if (n < p.tokens && c < p.hidden) p.sums[(static_cast<int64_t>(blockIdx.x) * p.tokens + n) * p.hidden + c] = SCALED ? dh[i][j] * back : dh[i][j];
             }
         }
     }
 }
 
 // ------------------------------------------------------------------ host ---------------
+int groups_of(int64_t hidden) { return (int)((hidden + kGroup - 1) / kGroup); }
 // Rows of up to 64 groups leave room for two blocks of eight warps on an SM, whose barriers cover for one another.
 int warps_for(int64_t hidden) { return groups_of(hidden) <= 8 * kMostGroups ? 8 : 16; }
 
-template <typename T, int WARPS, int SLOTS>
+template <typename T, int WARPS, int EACH, bool DW>
 tn_status launch(const FewTokens& p, cudaStream_t stream) {
     static thread_local int device = -1;  // the opt-in shared-memory size belongs to kernel and device
-    const size_t smem = smem_bytes(groups_of(p.hidden), SLOTS, WARPS);
+    constexpr int GROUPS = WARPS * EACH;
+    constexpr size_t smem = kSlots<EACH> * kBatch * w_bytes(GROUPS) + kTokens * h_bytes(GROUPS) + 2 * WARPS * 32 * sizeof(float2);
+    static_assert(smem <= 227 * 1024 / (16 / WARPS) - (WARPS == 8 ? 1024 : 0), "does not fit");
     int dev = 0;
     TN_CUDA(cudaGetDevice(&dev));
     if (device != dev) {
-        TN_CUDA(cudaFuncSetAttribute(half_grad_kernel<T, WARPS, SLOTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        TN_CUDA(cudaFuncSetAttribute(half_grad_kernel<T, WARPS, EACH, DW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         device = dev;
     }
-    half_grad_kernel<T, WARPS, SLOTS><<<(unsigned)half_grad_blocks(p.hidden, p.vocab), WARPS * 32, smem, stream>>>(p);
+    half_grad_kernel<T, WARPS, EACH, DW><<<(unsigned)half_grad_blocks(p.hidden, p.vocab), WARPS * 32, smem, stream>>>(p);
     return after_launch("half_grad_kernel");
 }
-template <typename T, int WARPS>
-tn_status launch_slots(const FewTokens& p, cudaStream_t stream) {
-    // a third batch where it fits
-    return smem_bytes(groups_of(p.hidden), 3, WARPS) <= 226 * 1024 / (16 / WARPS) ? launch<T, WARPS, 3>(p, stream) : launch<T, WARPS, 2>(p, stream);
+template <typename T, bool DW>
+tn_status launch_sized(const FewTokens& p, cudaStream_t stream) {
+    const int groups = groups_of(p.hidden);
+    if (warps_for(p.hidden) == 16) return groups <= 16 * 6 ? launch<T, 16, 6, DW>(p, stream) : launch<T, 16, 8, DW>(p, stream);
+    if (groups <= 8 * 2) return launch<T, 8, 2, DW>(p, stream);
+    if (groups <= 8 * 4) return launch<T, 8, 4, DW>(p, stream);
+    return groups <= 8 * 6 ? launch<T, 8, 6, DW>(p, stream) : launch<T, 8, 8, DW>(p, stream);
 }
 template <typename T>
 tn_status launch_typed(const FewTokens& p, cudaStream_t stream) {
-    return warps_for(p.hidden) == 8 ? launch_slots<T, 8>(p, stream) : launch_slots<T, 16>(p, stream);
+    return p.dweight ? launch_sized<T, true>(p, stream) : launch_sized<T, false>(p, stream);
 }
 
 }  // namespace
