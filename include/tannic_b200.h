@@ -425,7 +425,8 @@ tn_status tn_layer_norm_grad(const tn_tensor_t* dy, const tn_tensor_t* x, const 
  * hidden: [..., H], weight: [V, H], both float16, bfloat16 or float32, any strides; targets: int32 or int64 of hidden's
  * leading shape. loss and lse: float32, dense, of the targets' shape; either may be NULL (lse is what the gradient reads;
  * it is computed for ignored tokens too). Products accumulate in float32; float32 operands
- * enter as three bfloat16 parts, which keeps 24 significand bits (a token whose operands hold an infinity has NaN). A target outside the vocabulary that is
+ * enter as three bfloat16 parts or, for a few tokens, as two tf32 parts or as they are, which leaves float32's accuracy (a token
+ * whose operands hold an infinity may have NaN). A target outside the vocabulary that is
  * not ignore_index gives NaN for that token; nothing outside the tensors is read. Without tokens nothing is written. */
 tn_status tn_linear_cross_entropy(const tn_tensor_t* hidden, const tn_tensor_t* weight, const tn_tensor_t* targets,
                                   tn_tensor_t* loss, tn_tensor_t* lse, tn_stream_t stream, int64_t ignore_index);
@@ -434,8 +435,8 @@ tn_status tn_linear_cross_entropy(const tn_tensor_t* hidden, const tn_tensor_t* 
  *   dhidden = d . weight,  dweight = d^T . hidden
  * dense, of the operands' dtypes and shapes; either may be NULL. The logits are formed again in pieces of the vocabulary, so
  * the workspace is d for one piece (about half a GiB) and float32 sums of dhidden's size. d is rounded to the operands'
- * type (float32: three bfloat16 parts) after scaling by a power of two that keeps float16 clear of underflow; everything else is
- * float32 until the result's one rounding. Ignored tokens take no part, whatever their hidden states hold, and
+ * type (up to eight tokens: two parts of it; float32: three bfloat16 parts), relative to the largest |grad|, which keeps float16
+ * clear of underflow; everything else is float32 until the result's one rounding. Ignored tokens take no part, whatever their hidden states hold, and
  * cost nothing. A target outside the vocabulary makes that row of dhidden, and dweight, NaN. The same call gives the same bits. */
 tn_status tn_linear_cross_entropy_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_tensor_t* weight,
                                        const tn_tensor_t* targets, const tn_tensor_t* lse, tn_tensor_t* dhidden,

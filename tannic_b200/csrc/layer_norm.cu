@@ -718,7 +718,7 @@ tn_status launch_long(Launch& l) {
 }
 
 // ITEMS: vectors a thread holds. A warp takes a row of up to 32 (float64: 16) elements a lane. Element by element the steps are finer: every
-// element beyond the row's end costs as much as one within (271 columns of float16 in 16 elements a lane: 33 us for 62447 rows, in 12: 25).
+// element beyond the row's end costs as much as one within (271 columns of float16 in 16 elements a lane: 33 us for 62447 rows, in 12: 29).
 template <typename T, typename P, int VEC>
 tn_status launch_sized(Launch& l) {
     const int c = l.args.cols;

@@ -449,8 +449,8 @@ tn_status gradient(const FewTokens& p, const float* h, float* d, int64_t d_pitch
 
 }  // namespace
 
-// The loss up to 64 tokens and the gradient up to 32, where the bfloat16 parts of the large path have paid (4096 x 32768, 64 tokens: see the
-// figures at the top); grid extents within their limits.
+// The loss up to 64 tokens and the gradient up to 32, where the large path's bfloat16 parts, written out first, have cost more than they gain;
+// grid extents within their limits.
 bool f32_fits(int dtype, int64_t tokens, int64_t hidden, bool gradient) {
     return dtype == TN_FLOAT32 && tokens <= (gradient ? 32 : 64) && hidden <= int64_t(1) << 20;
 }

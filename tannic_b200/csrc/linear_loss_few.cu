@@ -1,7 +1,8 @@
-// The cross entropy of a linear layer and its gradient for a few tokens (scoring or adapting to one token at a time).
+// The cross entropy of a linear layer for one token (float32: up to four) and its gradient for up to four of float32.
 //
 // With so few rows the products are all weights: the bound is reading W once (and writing dW once), and a tensor-core tile of 128
 // rows would be empty. float32 operands gain most, which would otherwise be written out as three bfloat16 parts first.
+// One token over 131072 x 4096 bfloat16: 171 us, 6.3 TB/s.
 //
 //   loss       A warp takes four vocabulary rows at a time and forms their products with all tokens in float32; the tokens lie in
 //              shared memory and every value read from there serves four rows.
