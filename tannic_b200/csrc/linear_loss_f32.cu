@@ -8,7 +8,7 @@
 // the parts would have to be written back, and its 128-row tile would be mostly empty; the bound is W's way through shared memory.
 // The tensor cores cut off below an accumulator's last place, so every step of 32 starts from zero and is added in float32.
 //
-//   logits  [tokens] x [128 or 256 vocabulary rows], K = hidden. Epilogue: maximum and sum of exponentials per token and warp, or d.
+//   logits  [tokens] x [128 vocabulary rows], K = hidden. Epilogue: maximum and sum of exponentials per token and warp, or d.
 //   dh      [tokens] x [256 columns], K = a share of the vocabulary; the shares' sums are added in order afterwards.
 //   dW      [128 vocabulary rows] x [128 columns], K = tokens: bound by writing dW.
 #include <algorithm>
@@ -108,30 +108,35 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const FewTokens p, int ro
     }
 }
 
-// TM: tokens of the tile (16, 32 or 64). A warp has all of them and NT fragments of eight vocabulary rows.
-template <int TM> constexpr int kFragments = TM == 64 ? 2 : 4;
-template <int TM> constexpr int kLogitCols = kWarps * 8 * kFragments<TM>;
+// TM: tokens of the tile (16, 32 or 64). A warp has all of them and NT fragments of eight vocabulary rows. The thread block's two halves
+// take the two halves of K, each with its own stages: with one block to an SM, and few blocks where the vocabulary is small, the time is that
+// of the steps one after the other (64 tokens over 16903 x 2104 with eight warps a block: 210 us).
+constexpr int kFragments = 2;
+constexpr int kLogitCols = kWarps * 8 * kFragments;
+constexpr int kLogitThreads = 2 * kThreads;
 
 // h: hi and lo of the tokens, [2][TM][padded]. D: write d into `d` ([TM][d_pitch]), else the warps' statistics.
 template <int TM, bool ALIGNED, bool D>
-__global__ void __launch_bounds__(kThreads) logits_kernel(const FewTokens p, const float* h, int64_t padded, float* d, int64_t d_pitch) {
-    constexpr int COLS = kLogitCols<TM>, MT = TM / 16, NT = kFragments<TM>;
-    extern __shared__ __align__(16) float smem[];  // [kStages][2 TM + COLS][kPitch]
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+__global__ void __launch_bounds__(kLogitThreads) logits_kernel(const FewTokens p, const float* h, int64_t padded, float* d, int64_t d_pitch) {
+    constexpr int COLS = kLogitCols, MT = TM / 16, NT = kFragments, STAGE = (2 * TM + COLS) * kPitch;
+    extern __shared__ __align__(16) float smem[];  // [2][kStages][2 TM + COLS][kPitch]
+    const int half = threadIdx.x / kThreads, tid = threadIdx.x % kThreads;
+    const int lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int64_t v0 = static_cast<int64_t>(blockIdx.x) * COLS;
-    const int steps = static_cast<int>((p.hidden + kStep - 1) / kStep);
+    const int all = static_cast<int>((p.hidden + kStep - 1) / kStep), first_step = half * ((all + 1) / 2), steps = half ? all - first_step : (all + 1) / 2;
+    float* const stages = smem + half * kStages * STAGE;
     auto fill = [&](int step) {
         if (step < steps) {
-            float* a = smem + (step % kStages) * (2 * TM + COLS) * kPitch;
+            float* a = stages + (step % kStages) * STAGE;
             float* b = a + 2 * TM * kPitch;
-            const int64_t k0 = static_cast<int64_t>(step) * kStep;
-            for (int i = threadIdx.x; i < 2 * TM * (kStep / 4); i += kThreads) {
+            const int64_t k0 = static_cast<int64_t>(first_step + step) * kStep;
+            for (int i = tid; i < 2 * TM * (kStep / 4); i += kThreads) {
                 const int r = i / (kStep / 4), c = i % (kStep / 4) * 4;
                 const int valid = static_cast<int>(min(int64_t(4), padded - k0 - c));
                 copy4<true>(a + r * kPitch + c, h + r * padded + (valid > 0 ? k0 + c : 0), valid);
             }
 #pragma unroll
-            for (int i = threadIdx.x; i < COLS * (kStep / 4); i += kThreads) {
+            for (int i = tid; i < COLS * (kStep / 4); i += kThreads) {
                 const int r = i / (kStep / 4), c = i % (kStep / 4) * 4;
                 const int valid = v0 + r < p.vocab ? static_cast<int>(min(int64_t(4), p.hidden - k0 - c)) : 0;
                 copy4<ALIGNED>(b + r * kPitch + c, static_cast<const float*>(p.w) + (valid > 0 ? (v0 + r) * p.w_pitch + k0 + c : 0), valid);
@@ -139,6 +144,7 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const FewTokens p, con
         }
         commit();
     };
+    auto half_barrier = [&] { asm volatile("bar.sync %0, %1;" ::"r"(half + 1), "n"(kThreads) : "memory"); };
     chain_wait();
     chain_go();
 #pragma unroll
@@ -152,9 +158,9 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const FewTokens p, con
             for (int q = 0; q < 4; ++q) sum[i][j][q] = 0.0f;
     for (int step = 0; step < steps; ++step) {
         wait_oldest();
-        __syncthreads();  // this step's tile is there for everyone, and the last step's is read
+        half_barrier();  // this step's tile is there for everyone, and the last step's is read
         fill(step + kStages - 1);
-        const float* a = smem + (step % kStages) * (2 * TM + COLS) * kPitch;
+        const float* a = stages + (step % kStages) * STAGE;
         const float* b = a + (2 * TM + warp * 8 * NT) * kPitch;
         float part[MT][NT][4];
 #pragma unroll
@@ -188,6 +194,18 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const FewTokens p, con
 #pragma unroll
                 for (int q = 0; q < 4; ++q) sum[i][j][q] += part[i][j][q];
     }
+    // the second half's sums, through its own stages
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    half_barrier();
+    float* const other = smem + kStages * STAGE + tid;
+    if (half == 1) {
+#pragma unroll
+        for (int i = 0; i < MT * NT * 4; ++i) other[i * kThreads] = sum[i / (NT * 4)][i / 4 % NT][i % 4];
+    }
+    __syncthreads();
+    if (half == 1) return;
+#pragma unroll
+    for (int i = 0; i < MT * NT * 4; ++i) sum[i / (NT * 4)][i / 4 % NT][i % 4] += other[i * kThreads];
     // lane (g, t) holds tokens 16 i + g and + 8, vocabulary rows 8 j + 2 t and + 1 of its warp's
     const int64_t first = v0 + warp * 8 * NT + 2 * t;
 #pragma unroll
@@ -415,9 +433,10 @@ tn_status prepare_rows(const FewTokens& p, float* h, bool drop_ignored, cudaStre
 template <int TM, bool ALIGNED, bool D>
 tn_status logits(const FewTokens& p, const float* h, float* d, int64_t d_pitch, cudaStream_t stream) {
     static thread_local int device = -1;
-    const size_t smem = sizeof(float) * kStages * (2 * TM + kLogitCols<TM>) * kPitch;
+    constexpr size_t smem = sizeof(float) * 2 * kStages * (2 * TM + kLogitCols) * kPitch;
+    static_assert(smem <= 227 * 1024, "does not fit");
     TN_TRY(allow(logits_kernel<TM, ALIGNED, D>, smem, device));
-    TN_CUDA(launch_chained(true, logits_kernel<TM, ALIGNED, D>, (unsigned)ceil_div(p.vocab, kLogitCols<TM>), kThreads, smem, stream, 1, p, h + TM * padded_of(p.hidden),
+    TN_CUDA(launch_chained(true, logits_kernel<TM, ALIGNED, D>, (unsigned)ceil_div(p.vocab, kLogitCols), kLogitThreads, smem, stream, 1, p, h + TM * padded_of(p.hidden),
                            padded_of(p.hidden), d, d_pitch));
     return after_launch("logits_kernel");
 }
@@ -454,13 +473,7 @@ tn_status gradient(const FewTokens& p, const float* h, float* d, int64_t d_pitch
 bool f32_fits(int dtype, int64_t tokens, int64_t hidden, bool gradient) {
     return dtype == TN_FLOAT32 && tokens <= (gradient ? 32 : 64) && hidden <= int64_t(1) << 20;
 }
-int64_t f32_loss_parts(int64_t tokens, int64_t vocab) {
-    switch (token_rows(tokens)) {
-        case 16: return ceil_div(vocab, kLogitCols<16>) * kWarps;
-        case 32: return ceil_div(vocab, kLogitCols<32>) * kWarps;
-        default: return ceil_div(vocab, kLogitCols<64>) * kWarps;
-    }
-}
+int64_t f32_loss_parts(int64_t vocab) { return ceil_div(vocab, kLogitCols) * kWarps; }
 size_t f32_row_floats(int64_t tokens, int64_t hidden) { return 3 * (size_t)token_rows(tokens) * padded_of(hidden); }
 size_t f32_d_floats(int64_t tokens, int64_t vocab) { return (size_t)token_rows(tokens) * padded_of(vocab); }
 int64_t f32_grad_shares(int64_t hidden, int64_t vocab) { return ceil_div(vocab, vocabulary_share(hidden, vocab)); }
