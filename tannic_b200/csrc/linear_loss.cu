@@ -1190,7 +1190,7 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
     const bool few = few_loss_fits(p.dtype, p.tokens, p.hidden);
     if (few || f32_fits(p.dtype, p.tokens, p.hidden, false)) {
         FewTokens f = few_tokens(p, h, w, t, wide, ignore);
-        const int64_t parts = few ? few_loss_parts() : f32_loss_parts(p.vocab);
+        const int64_t parts = few ? few_loss_parts() : f32_loss_parts(p.tokens, p.vocab);
         TN_TRY(mem.take(&halves, sizeof(float2) * (size_t)parts * p.tokens));
         f.parts = halves;
         f.target_logit = target_logit;

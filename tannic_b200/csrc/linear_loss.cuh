@@ -49,7 +49,7 @@ tn_status few_dhidden(const FewTokens& p, int64_t n, cudaStream_t stream);
 
 // float32, up to 64 tokens (gradient: 32). `h`: workspace of f32_row_floats, `d`: of f32_d_floats.
 bool f32_fits(int dtype, int64_t tokens, int64_t hidden, bool gradient);
-int64_t f32_loss_parts(int64_t vocab);
+int64_t f32_loss_parts(int64_t tokens, int64_t vocab);
 size_t f32_row_floats(int64_t tokens, int64_t hidden);
 size_t f32_d_floats(int64_t tokens, int64_t vocab);
 int64_t f32_grad_shares(int64_t hidden, int64_t vocab);

@@ -8,7 +8,7 @@
 // the parts would have to be written back, and its 128-row tile would be mostly empty; the bound is W's way through shared memory.
 // The tensor cores cut off below an accumulator's last place, so every step of 32 starts from zero and is added in float32.
 //
-//   logits  [tokens] x [128 vocabulary rows], K = hidden. Epilogue: maximum and sum of exponentials per token and warp, or d.
+//   logits  [tokens] x [64 or 128 vocabulary rows], K = hidden. Epilogue: maximum and sum of exponentials per token and warp, or d.
 //   dh      [tokens] x [256 columns], K = a share of the vocabulary; the shares' sums are added in order afterwards.
 //   dW      [128 vocabulary rows] x [128 columns], K = tokens: bound by writing dW.
 #include <algorithm>
@@ -110,15 +110,15 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const FewTokens p, int ro
 
 // TM: tokens of the tile (16, 32 or 64). A warp has all of them and NT fragments of eight vocabulary rows. The thread block's two halves
 // take the two halves of K, each with its own stages: with one block to an SM, and few blocks where the vocabulary is small, the time is that
-// of the steps one after the other (64 tokens over 16903 x 2104 with eight warps a block: 210 us).
-constexpr int kFragments = 2;
-constexpr int kLogitCols = kWarps * 8 * kFragments;
+// of the steps one after the other (64 tokens over 16903 x 2104: 116 us, with eight warps a block and all of K 210).
+constexpr int kMostFragments = 2;
+constexpr int columns_of(int fragments) { return kWarps * 8 * fragments; }
 constexpr int kLogitThreads = 2 * kThreads;
 
 // h: hi and lo of the tokens, [2][TM][padded]. D: write d into `d` ([TM][d_pitch]), else the warps' statistics.
-template <int TM, bool ALIGNED, bool D>
+template <int TM, int NT, bool ALIGNED, bool D>
 __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const FewTokens p, const float* h, int64_t padded, float* d, int64_t d_pitch) {
-    constexpr int COLS = kLogitCols, MT = TM / 16, NT = kFragments, STAGE = (2 * TM + COLS) * kPitch;
+    constexpr int COLS = columns_of(NT), MT = TM / 16, STAGE = (2 * TM + COLS) * kPitch;
     extern __shared__ __align__(16) float smem[];  // [2][kStages][2 TM + COLS][kPitch]
     const int half = threadIdx.x / kThreads, tid = threadIdx.x % kThreads;
     const int lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -430,15 +430,26 @@ tn_status prepare_rows(const FewTokens& p, float* h, bool drop_ignored, cudaStre
     return after_launch("few_rows_kernel");
 }
 
+// One fragment a warp where two would leave half of the SMs idle: 64 tokens over 8192 x 4096 140 us, with two 195. The smaller tiles have too
+// little to do for their loads of the tokens then (32 tokens there: 150 us against 135).
+int fragments(int tile, int64_t vocab) { return tile == 64 && 2 * ceil_div(vocab, columns_of(kMostFragments)) <= sm_count() ? 1 : kMostFragments; }
+
+template <int TM, int NT, bool ALIGNED, bool D>
+tn_status logits_of(const FewTokens& p, const float* h, float* d, int64_t d_pitch, cudaStream_t stream) {
+    static thread_local int device = -1;
+    constexpr size_t smem = sizeof(float) * 2 * kStages * (2 * TM + columns_of(NT)) * kPitch;
+    static_assert(smem <= 227 * 1024, "does not fit");
+    TN_TRY(allow(logits_kernel<TM, NT, ALIGNED, D>, smem, device));
+    TN_CUDA(launch_chained(true, logits_kernel<TM, NT, ALIGNED, D>, (unsigned)ceil_div(p.vocab, columns_of(NT)), kLogitThreads, smem, stream, 1, p,
+                           h + TM * padded_of(p.hidden), padded_of(p.hidden), d, d_pitch));
+    return after_launch("logits_kernel");
+}
 template <int TM, bool ALIGNED, bool D>
 tn_status logits(const FewTokens& p, const float* h, float* d, int64_t d_pitch, cudaStream_t stream) {
-    static thread_local int device = -1;
-    constexpr size_t smem = sizeof(float) * 2 * kStages * (2 * TM + kLogitCols) * kPitch;
-    static_assert(smem <= 227 * 1024, "does not fit");
-    TN_TRY(allow(logits_kernel<TM, ALIGNED, D>, smem, device));
-    TN_CUDA(launch_chained(true, logits_kernel<TM, ALIGNED, D>, (unsigned)ceil_div(p.vocab, kLogitCols), kLogitThreads, smem, stream, 1, p, h + TM * padded_of(p.hidden),
-                           padded_of(p.hidden), d, d_pitch));
-    return after_launch("logits_kernel");
+    if constexpr (TM == 64) {
+        if (fragments(TM, p.vocab) == 1) return logits_of<TM, 1, ALIGNED, D>(p, h, d, d_pitch, stream);
+    }
+    return logits_of<TM, kMostFragments, ALIGNED, D>(p, h, d, d_pitch, stream);
 }
 
 template <int TM, bool ALIGNED>
@@ -473,7 +484,7 @@ tn_status gradient(const FewTokens& p, const float* h, float* d, int64_t d_pitch
 bool f32_fits(int dtype, int64_t tokens, int64_t hidden, bool gradient) {
     return dtype == TN_FLOAT32 && tokens <= (gradient ? 32 : 64) && hidden <= int64_t(1) << 20;
 }
-int64_t f32_loss_parts(int64_t vocab) { return ceil_div(vocab, kLogitCols) * kWarps; }
+int64_t f32_loss_parts(int64_t tokens, int64_t vocab) { return ceil_div(vocab, columns_of(fragments(token_rows(tokens), vocab))) * kWarps; }
 size_t f32_row_floats(int64_t tokens, int64_t hidden) { return 3 * (size_t)token_rows(tokens) * padded_of(hidden); }
 size_t f32_d_floats(int64_t tokens, int64_t vocab) { return (size_t)token_rows(tokens) * padded_of(vocab); }
 int64_t f32_grad_shares(int64_t hidden, int64_t vocab) { return ceil_div(vocab, vocabulary_share(hidden, vocab)); }
