@@ -435,7 +435,7 @@ tn_status tn_linear_cross_entropy(const tn_tensor_t* hidden, const tn_tensor_t* 
  *   dhidden = d . weight,  dweight = d^T . hidden
  * dense, of the operands' dtypes and shapes; either may be NULL. The logits are formed again in pieces of the vocabulary, so
  * the workspace is d for one piece (about half a GiB) and float32 sums of dhidden's size. d is rounded to the operands'
- * type (up to eight tokens: two parts of it; float32: three bfloat16 parts), relative to the largest |grad|, which keeps float16
+ * type (a few tokens: two parts of it; float32: three bfloat16 parts), relative to the largest |grad|, which keeps float16
  * clear of underflow; everything else is float32 until the result's one rounding. Ignored tokens take no part, whatever their hidden states hold, and
  * cost nothing. A target outside the vocabulary makes that row of dhidden, and dweight, NaN. The same call gives the same bits. */
 tn_status tn_linear_cross_entropy_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_tensor_t* weight,

@@ -1264,7 +1264,7 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
     f.dweight = dweight ? dweight->address : nullptr;
     const bool half = half_grad_fits(f), few = few_grad_fits(f);
     if (half || few || f32_fits(p.dtype, p.tokens, p.hidden, true)) {
-        const int64_t blocks = half ? half_grad_blocks(p.hidden, p.vocab) : few ? few_grad_blocks(p.vocab) : f32_grad_shares(p.hidden, p.vocab);
+        const int64_t blocks = half ? half_grad_blocks(p.tokens, p.hidden, p.vocab) : few ? few_grad_blocks(p.vocab) : f32_grad_shares(p.hidden, p.vocab);
         if (dhidden) TN_TRY(mem.take(&f.sums, sizeof(float) * (size_t)blocks * p.tokens * p.hidden));
         if (half) return half_grad(f, p.stream);
         if (few) return few_grad(f, p.stream);

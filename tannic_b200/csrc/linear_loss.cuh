@@ -35,9 +35,9 @@ tn_status few_loss(const FewTokens& p, cudaStream_t stream);
 constexpr float kTop = 16384.0f;  // float16 ends at 65504
 __device__ __forceinline__ float unscale(float v, float largest) { return v * (1.0f / kTop) * largest; }
 
-// 16 bits, up to eight tokens
+// 16 bits, up to sixteen tokens
 bool half_grad_fits(const FewTokens& p);
-int64_t half_grad_blocks(int64_t hidden, int64_t vocab);
+int64_t half_grad_blocks(int64_t tokens, int64_t hidden, int64_t vocab);
 tn_status half_grad(const FewTokens& p, cudaStream_t stream);
 
 // float32, up to four tokens

@@ -134,6 +134,18 @@ def test_one_pass_of_sixteen_bits(tokens, hidden, vocab, dtype):
     both(*data(tokens, hidden, vocab, dtype, 10))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hidden,vocab", [(8, 3), (512, 10007), (520, 41), (1024, 7001), (1032, 999), (2048, 5003), (2056, 300)])
+@pytest.mark.parametrize("tokens", [9, 12, 16, 17])
+def test_one_pass_of_two_tiles(tokens, hidden, vocab, dtype):
+    h, w, t, g = data(tokens, hidden, vocab, dtype, 12, ignored=0.2)
+    both(h, w, t, g)
+    lse = tb.linear_cross_entropy(h, w, t)[1]
+    dh, dw = tb.linear_cross_entropy_grad(g, h, w, t, lse)
+    assert torch.equal(tb.linear_cross_entropy_grad(g, h, w, t, lse, dweight=False)[0], dh)
+    assert torch.equal(tb.linear_cross_entropy_grad(g, h, w, t, lse, dhidden=False)[1], dw)
+
+
 def test_small_and_infinite_gradients():
     """float16's d would be lost unscaled; one infinite gradient leaves the other tokens' rows as they are."""
     h, w, t, g = data(6, 264, 3000, torch.float16, 11)
