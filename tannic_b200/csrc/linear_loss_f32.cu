@@ -1,7 +1,7 @@
 // The cross entropy of a linear layer and its gradient for up to 64 tokens of float32.
 //
 // The large path writes float32 weights out as three bfloat16 parts first: 4 bytes an element read, 6 written, and 6 read again for each
-// product, which for a few tokens is most of the time (16 tokens over 4096 x 32768: loss 594 us, the FP32 pipe 198 us).
+// product, which for a few tokens is most of the time (16 tokens over 4096 x 32768: loss 594 us, here 177).
 // Here W stays as it is. Its tiles come into shared memory by cp.async, several steps ahead, and a warp splits its fragments in registers:
 // x = hi + lo, both tf32 (11 significand bits each, rounded to nearest), a b = hi hi + hi lo + lo hi; what is left out is below
 // 2^-22 of the product and of either sign. The products run as mma.sync m16n8k8: tcgen05 takes its operands from shared memory, where
@@ -24,7 +24,6 @@ constexpr int kCols = 128;       // of a tile of dW
 constexpr int kStep = 32;        // of K
 constexpr int kPitch = kStep + 4;   // floats of a tile's row along K: rows g and columns t of a fragment lie in banks 4 g + t
 constexpr int kWide = kCols + 8;    // floats of a tile's row along the columns: rows t and columns g in banks 8 t + g
-constexpr int kStages = 3;
 
 // A fragment's element as two tf32.
 struct Split { uint32_t hi, lo; };
@@ -90,9 +89,6 @@ __device__ __forceinline__ void copy4(float* to, const float* from, int valid) {
     }
 }
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// until the oldest of kStages - 1 groups has arrived
-__device__ __forceinline__ void wait_oldest() { asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory"); }
-
 // The tokens as the products read them: [rows][padded], zero where there is no token, no target (that is for the gradient) or no column; behind
 // them their hi and lo, which every warp of the logits would otherwise work out for itself.
 __global__ void __launch_bounds__(256) few_rows_kernel(const FewTokens p, int rows, int64_t padded, int drop_ignored, float* __restrict__ out) {
@@ -114,20 +110,24 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const FewTokens p, int ro
 constexpr int kMostFragments = 2;
 constexpr int columns_of(int fragments) { return kWarps * 8 * fragments; }
 constexpr int kLogitThreads = 2 * kThreads;
+// Steps in shared memory. Five fit for the smallest tile and serve whole copies (16 tokens over 8192 x 4096: 93 us, with three 105); element by
+// element the way to the first step is longer than they save (4005 x 1033: 46 us against 55), and the larger tiles, of which four would fit,
+// do not gain.
+template <int TM, bool ALIGNED> constexpr int kLogitStages = TM == 16 && ALIGNED ? 5 : 3;
 
 // h: hi and lo of the tokens, [2][TM][padded]. D: write d into `d` ([TM][d_pitch]), else the warps' statistics.
 template <int TM, int NT, bool ALIGNED, bool D>
 __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const FewTokens p, const float* h, int64_t padded, float* d, int64_t d_pitch) {
-    constexpr int COLS = columns_of(NT), MT = TM / 16, STAGE = (2 * TM + COLS) * kPitch;
-    extern __shared__ __align__(16) float smem[];  // [2][kStages][2 TM + COLS][kPitch]
+    constexpr int COLS = columns_of(NT), MT = TM / 16, STAGE = (2 * TM + COLS) * kPitch, STAGES = kLogitStages<TM, ALIGNED>;
+    extern __shared__ __align__(16) float smem[];  // [2][STAGES][2 TM + COLS][kPitch]
     const int half = threadIdx.x / kThreads, tid = threadIdx.x % kThreads;
     const int lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int64_t v0 = static_cast<int64_t>(blockIdx.x) * COLS;
     const int all = static_cast<int>((p.hidden + kStep - 1) / kStep), first_step = half * ((all + 1) / 2), steps = half ? all - first_step : (all + 1) / 2;
-    float* const stages = smem + half * kStages * STAGE;
+    float* const stages = smem + half * STAGES * STAGE;
     auto fill = [&](int step) {
         if (step < steps) {
-            float* a = stages + (step % kStages) * STAGE;
+            float* a = stages + (step % STAGES) * STAGE;
             float* b = a + 2 * TM * kPitch;
             const int64_t k0 = static_cast<int64_t>(first_step + step) * kStep;
             for (int i = tid; i < 2 * TM * (kStep / 4); i += kThreads) {
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const FewTokens p
     chain_wait();
     chain_go();
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) fill(s);
+    for (int s = 0; s < STAGES - 1; ++s) fill(s);
     float sum[MT][NT][4];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -157,10 +157,10 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const FewTokens p
 #pragma unroll
             for (int q = 0; q < 4; ++q) sum[i][j][q] = 0.0f;
     for (int step = 0; step < steps; ++step) {
-        wait_oldest();
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         half_barrier();  // this step's tile is there for everyone, and the last step's is read
-        fill(step + kStages - 1);
-        const float* a = stages + (step % kStages) * STAGE;
+        fill(step + STAGES - 1);
+        const float* a = stages + (step % STAGES) * STAGE;
         const float* b = a + (2 * TM + warp * 8 * NT) * kPitch;
         float part[MT][NT][4];
 #pragma unroll
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const FewTokens p
     // the second half's sums, through its own stages
     asm volatile("cp.async.wait_all;" ::: "memory");
     half_barrier();
-    float* const other = smem + kStages * STAGE + tid;
+    float* const other = smem + STAGES * STAGE + tid;
     if (half == 1) {
 #pragma unroll
         for (int i = 0; i < MT * NT * 4; ++i) other[i * kThreads] = sum[i / (NT * 4)][i / 4 % NT][i % 4];
@@ -437,7 +437,7 @@ int fragments(int tile, int64_t vocab) { return tile == 64 && 2 * ceil_div(vocab
 template <int TM, int NT, bool ALIGNED, bool D>
 tn_status logits_of(const FewTokens& p, const float* h, float* d, int64_t d_pitch, cudaStream_t stream) {
     static thread_local int device = -1;
-    constexpr size_t smem = sizeof(float) * 2 * kStages * (2 * TM + columns_of(NT)) * kPitch;
+    constexpr size_t smem = sizeof(float) * 2 * kLogitStages<TM, ALIGNED> * (2 * TM + columns_of(NT)) * kPitch;
     static_assert(smem <= 227 * 1024, "does not fit");
     TN_TRY(allow(logits_kernel<TM, NT, ALIGNED, D>, smem, device));
     TN_CUDA(launch_chained(true, logits_kernel<TM, NT, ALIGNED, D>, (unsigned)ceil_div(p.vocab, columns_of(NT)), kLogitThreads, smem, stream, 1, p,

@@ -17,8 +17,8 @@
 //   dh [columns, 8 tokens]          k = the eight rows, once with d's upper part and once with its lower one.
 //   dW [8 rows, columns]            k = the tokens; rows 0 to 7 of the product take d's upper part, rows 8 to 15 its lower one, and the two
 //                                   are added. h's order puts eight neighbouring columns into a lane: one store of 16 bytes.
-// d is the sum of two values of the operands' type (2^-17 of it for bfloat16, 2^-22 for float16), scaled like the larger products' d so that
-// float16 does not lose small gradients.
+// d is the sum of two values of the operands' type (good to 2^-17 of it for bfloat16, 2^-22 for float16); float16's is relative to the largest
+// gradient, like the larger products', and does not lose small ones.
 #include <algorithm>
 
 #include "linear_loss.cuh"

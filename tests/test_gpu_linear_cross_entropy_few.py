@@ -1,5 +1,5 @@
-"""The cross entropy of a linear layer for a few tokens, where other kernels run: one pass over the weights (one token, four for the gradient
-and for float32), tiles of the FP32 pipe (float32, up to 64 tokens). Same checks and tolerances as for many."""
+"""The cross entropy of a linear layer for a few tokens, where other kernels run: one pass over the weights (one token, float32 up to
+four; the gradient of 16 bits up to sixteen), tiles of mma.sync (float32, up to 64 tokens). Same checks and tolerances as for many."""
 import pytest
 import torch
 
