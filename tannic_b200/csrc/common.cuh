@@ -139,7 +139,8 @@ int env_knob(const char* name, int fallback);
 // ---------------------------------------------------------------- chains -------------
 // Kernels that follow one another in one call are launched so that the next one's blocks start (barriers, tensor memory, tensor
 // maps) while the last blocks of the one before still run. Such a kernel calls chain_wait() before it touches memory, and so
-// waits for everything before it, and chain_go() once it may itself be followed.
+// waits for everything before it, and chain_go() once it may itself be followed. The last kernel of a call does not: what comes after a call
+// finds its results written when it starts, however it was launched.
 __device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void chain_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -324,7 +324,7 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 
     // everything above ran under the kernel before this one; from here on its results are there
     chain_wait();
-    chain_go();
+    if constexpr (EPI != EPI_RESULT) chain_go();  // that one may be the last of its call
     // the tokens that count bound the rows or the K extent
     int m_tiles = g.m_tiles, k_blocks = g.k_blocks;
     if (g.count_is != COUNT_NONE) {
@@ -688,7 +688,6 @@ __global__ void __launch_bounds__(1024) loss_join(const float2* halves, int64_t 
                                                   const void* targets, int wide, int64_t ignore, int64_t vocab, float* __restrict__ loss, float* __restrict__ lse) {
     __shared__ float2 part[32][33];
     chain_wait();
-    chain_go();
     constexpr int STEP = 1024 / R;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * R + threadIdx.x % R;
@@ -866,7 +865,6 @@ __global__ void __launch_bounds__(256) loss_dhidden(const float* sums, const int
     struct alignas(sizeof(float) * VEC) Sums { float v[VEC]; };
     constexpr int ROWS = 4;  // a thread's rows, their loads in flight together
     chain_wait();
-    chain_go();
     const float by = *scale;
     const int splits = plan_splits((*count + tile_rows - 1) / tile_rows * n_tiles, units, k_blocks, most_splits).splits;  // of the first piece
     const int64_t c = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * VEC;

@@ -341,7 +341,6 @@ __global__ void __launch_bounds__(kThreads) dweight_kernel(const FewTokens p, co
     float* a = smem;
     float* b = smem + TM * kWide;
     chain_wait();
-    chain_go();
     for (int i = threadIdx.x; i < TM * (kCols / 4); i += kThreads) {
         const int r = i / (kCols / 4), c = i % (kCols / 4) * 4;
         const int valid = static_cast<int>(min(int64_t(4), padded - c0 - c));

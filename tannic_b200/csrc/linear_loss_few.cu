@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) few_grad_kernel(const FewToke
     P* ring = reinterpret_cast<P*>(smem) + t;  // [kDepth][R][ITEMS][threads]
     const int vecs = static_cast<int>(p.hidden / VEC);
     auto inside = [&](int i) { return i * threads + t < vecs; };
-    chain_go();
+    if (p.sums) chain_go();
 
     // the tokens' columns of this thread; a token without a target is nothing, whatever it holds
     float2 h[NT][E / 2], dh[NT][E / 2];
@@ -343,7 +343,6 @@ template <typename T, int COLS>
 __global__ void __launch_bounds__(1024) few_dhidden_kernel(const FewTokens p, int blocks) {
     __shared__ float part[32][COLS + 1];
     chain_wait();
-    chain_go();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t n_all = p.tokens * p.hidden, c = static_cast<int64_t>(blockIdx.x) * COLS + lane % COLS;
     float sum = 0.0f;

@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) half_grad_kernel(const
     uint8_t* tokens = smem + SLOTS * slot_bytes;
     float2* parts = reinterpret_cast<float2*>(tokens + TILES * kTile * h_row);  // [2][WARPS][TILES][32]
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)), hs = ring + SLOTS * slot_bytes;
-    chain_go();
+    if (p.sums) chain_go();
 
     // Where the 16 bytes `chunk` (0 to 3) of this warp's group i of row r lie. The exchange of chunks by the row's bits, in reverse order, puts
     // both the eight rows of one chunk and two rows of four chunks on different banks.
