@@ -62,6 +62,21 @@ cudaError_t launch_chained(bool behind, void (*kernel)(P...), dim3 grid, dim3 bl
     return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
 }
 
+// Lets a kernel have all the dynamic shared memory that a block can have beside its static one. The permission belongs to kernel and
+// device, not to a call: every call gives the same, so that none takes back what a call of another thread is about to use.
+// `last`: the device this thread gave it on last, one per kernel and thread.
+template <typename... P>
+tn_status allow_shared_memory(void (*kernel)(P...), int device, int& last) {
+    if (last == device) return TN_SUCCESS;
+    cudaFuncAttributes attributes;
+    int most = 0;
+    TN_CUDA(cudaFuncGetAttributes(&attributes, kernel));
+    TN_CUDA(cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device));
+    TN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - static_cast<int>(attributes.sharedSizeBytes)));
+    last = device;
+    return TN_SUCCESS;
+}
+
 // Checks the launch that was just issued (pattern of src/cuda/argred.cu:138) and counts it.
 tn_status after_launch(const char* what);
 

@@ -632,10 +632,10 @@ tn_status finish_partial(Launch& l, int64_t blocks) {
     return after_launch("norm_parameters");
 }
 
-// Thread blocks of a kernel that are on the GPU at once; lets the kernel have that much shared memory. The answer to the last
-// question (device, threads, shared memory) is kept in `last`, one per kernel and thread.
+// Thread blocks of a kernel that are on the GPU at once. The answer to the last question (device, threads, shared memory) is kept
+// in `last`, one per kernel and thread.
 struct Resident {
-    int device = -1, threads = 0;
+    int device = -1, allowed = -1, threads = 0;
     size_t smem = 0;
     int64_t blocks = 0;
 };
@@ -644,10 +644,12 @@ tn_status resident_blocks(K kernel, int threads, size_t smem, Resident& last) {
     int device = 0, per_sm = 0;
     TN_CUDA(cudaGetDevice(&device));
     if (last.device == device && last.threads == threads && last.smem == smem) return TN_SUCCESS;
-    // 48 KiB need no permission, but the kernels' static shared memory counts as well
-    if (smem > 40 * 1024) TN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    TN_TRY(allow_shared_memory(kernel, device, last.allowed));
     TN_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
-    last = {device, threads, smem, (int64_t)sm_count() * std::max(per_sm, 1)};
+    last.device = device;
+    last.threads = threads;
+    last.smem = smem;
+    last.blocks = (int64_t)sm_count() * std::max(per_sm, 1);
     return TN_SUCCESS;
 }
 

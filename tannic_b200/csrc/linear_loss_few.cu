@@ -368,25 +368,19 @@ __global__ void __launch_bounds__(1024) few_dhidden_kernel(const FewTokens p, in
 // ------------------------------------------------------------------ host ---------------
 bool fits16(const void* p, int64_t pitch_bytes) { return ((reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(pitch_bytes)) & 15) == 0; }
 
-// Opt-in shared memory of a kernel, once per device and size.
 template <typename K>
-tn_status allow_smem(K kernel, size_t smem, int& last_device, size_t& last_smem) {
-    int dev = 0;
-    TN_CUDA(cudaGetDevice(&dev));
-    if (last_device == dev && last_smem >= smem) return TN_SUCCESS;
-    if (smem > 24 * 1024) TN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    last_device = dev;
-    last_smem = smem;
-    return TN_SUCCESS;
+tn_status allow(K kernel, int& last) {
+    int device = 0;
+    TN_CUDA(cudaGetDevice(&device));
+    return allow_shared_memory(kernel, device, last);
 }
 
 template <typename T, int VEC, int NT>
 tn_status loss_one(const FewTokens& p, cudaStream_t stream) {
     static thread_local int device = -1;
-    static thread_local size_t allowed = 0;
     const int64_t padded = (p.hidden + 7) & ~int64_t(7);
     const size_t smem = sizeof(float) * NT * (size_t)padded;
-    TN_TRY(allow_smem(few_loss_kernel<T, VEC, NT>, smem, device, allowed));
+    TN_TRY(allow(few_loss_kernel<T, VEC, NT>, device));
     TN_CUDA(launch_chained(false, few_loss_kernel<T, VEC, NT>, (unsigned)(few_loss_parts() / (kLossThreads / 32)), kLossThreads, smem, stream, 1, p, padded));
     return after_launch("few_loss_kernel");
 }
@@ -415,10 +409,9 @@ tn_status dhidden_typed(const FewTokens& p, int64_t n, cudaStream_t stream) {
 template <int VEC, int NT>
 tn_status grad_one(const FewTokens& p, cudaStream_t stream) {
     static thread_local int device = -1;
-    static thread_local size_t allowed = 0;
     const int threads = (int)(ceil_div(ceil_div(p.hidden / VEC, E / VEC), 32) * 32);
     const size_t smem = VEC > 1 ? sizeof(float) * E * kGradRows * kDepth * (size_t)threads : 0;
-    TN_TRY(allow_smem(few_grad_kernel<VEC, NT>, smem, device, allowed));
+    TN_TRY(allow(few_grad_kernel<VEC, NT>, device));
     const int64_t blocks = few_grad_blocks(p.vocab);
     TN_CUDA(launch_chained(false, few_grad_kernel<VEC, NT>, (unsigned)blocks, threads, smem, stream, 1, p));
     TN_TRY(after_launch("few_grad_kernel"));
