@@ -988,6 +988,7 @@ struct Problem {
     bool bf16;
     int parts, terms;
     int64_t tokens, hidden, vocab, padded;
+    int sms;  // that the call may use. The margin is read once: what one kernel plans by it another one adds up by
     cudaStream_t stream;
     // Asked at each launch: whether a kernel of this call came before it.
     bool behind() const {
@@ -1036,10 +1037,7 @@ tn_status operand_map(CUtensorMap* map, const Operand& o, bool bf16, int64_t inn
 }
 
 // Thread blocks, or pairs of them, that run at once.
-int unit_count(bool pair) {
-    const int sms = sm_count() - sm_margin();
-    return std::max(1, pair ? sms / 2 : sms);
-}
+int unit_count(const Problem& p, bool pair) { return std::max(1, pair ? p.sms / 2 : p.sms); }
 // Whether a product with m result rows takes pairs: up to 128 rows the second block would have none.
 bool takes_pairs(int64_t m) { return m > BM; }
 
@@ -1074,7 +1072,7 @@ LossArgs gemm_args(const Problem& p, int64_t m, int64_t n, int64_t k) {
     g.n_tiles = (int)ceil_div(n, BN);
     g.k_blocks = (int)ceil_div(k, BK);
     g.most_splits = 1;
-    g.units = unit_count(pair);
+    g.units = unit_count(p, pair);
     g.terms = p.terms;
     g.period = p.parts == 3 ? kPeriod : 1 << 20;
     g.is_bf16 = p.bf16;
@@ -1145,6 +1143,7 @@ Problem make_problem(const tn_tensor_t* hidden, const tn_tensor_t* weight, tn_st
     p.tokens = (int64_t)hidden->size / p.hidden;
     p.vocab = (int64_t)weight->shape.sizes[0];
     p.padded = (p.hidden + 7) & ~int64_t(7);
+    p.sms = std::max(1, sm_count() - sm_margin());
     p.stream = as_cuda(stream);
     return p;
 }
@@ -1304,7 +1303,7 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
     const bool pair = takes_pairs(p.tokens);
     if (dhidden) {
         const int64_t tiles = ceil_div(p.tokens, pair ? 2 * BM : BM) * ceil_div(p.padded, BN);
-        splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * (unit_count(pair) / tiles), ceil_div(piece, BK) / 4));
+        splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * (unit_count(p, pair) / tiles), ceil_div(piece, BK) / 4));
         TN_TRY(mem.take(&sums, sizeof(float) * (size_t)splits * p.tokens * p.padded));
     }
 
@@ -1373,7 +1372,7 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
         const bool wide = p.hidden % 4 == 0 && (reinterpret_cast<uintptr_t>(to) & (4 * sizeof(OUT) - 1)) == 0;
         const dim3 grid((unsigned)ceil_div(p.hidden, wide ? 1024 : 256), (unsigned)std::min<int64_t>(ceil_div(p.tokens, 4), 65535));
         TN_CUDA(launch_chained(true, wide ? loss_dhidden<OUT, 4> : loss_dhidden<OUT, 1>, grid, 256, 0, p.stream, 1, sums, count, pair ? 2 * BM : BM, (int)ceil_div(p.padded, BN),
-                               unit_count(pair), (int)ceil_div(piece, BK), splits, p.tokens, p.hidden, p.padded, slot, scale, to));
+                               unit_count(p, pair), (int)ceil_div(piece, BK), splits, p.tokens, p.hidden, p.padded, slot, scale, to));
         TN_TRY(after_launch("loss_dhidden"));
     }
     return TN_SUCCESS;
