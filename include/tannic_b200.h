@@ -479,10 +479,11 @@ tn_status tn_gemm_mirrored(const tn_tensor_t* a, const tn_tensor_t* b, tn_tensor
                            int n_mirrors, tn_stream_t stream);
 
 /* The tensor-core GEMM and convolution kernels are persistent, one thread block per SM, and a block fills
- * its SM's shared memory: while one runs, no kernel of another stream gets an SM. A caller that wants a
+ * its SM's shared memory: while one runs, no kernel of another stream gets an SM. The same goes for the cross entropy of a
+ * linear layer and its gradient (not for float32 of 5 to 64 tokens, gradient 32, whose blocks come and go). A caller that wants a
  * communication kernel (an NCCL send/receive of the rows just produced) to run UNDER the next GEMM sets a
- * margin: these kernels then launch on (SM count - margin) SMs. Process-wide, 0..64, default 0. No reference
- * counterpart. */
+ * margin: these kernels then launch on (SM count - margin) SMs. A call keeps to the margin that it finds when it is made. The loss and
+ * dhidden are summed in an order that depends on it. Process-wide, 0..64, default 0. No reference counterpart. */
 tn_status tn_set_sm_margin(int sms);
 
 /* Diagnostics, no reference counterpart: launches of the tensor-core GEMM since load, by variant:

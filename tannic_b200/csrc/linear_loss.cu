@@ -1162,6 +1162,7 @@ FewTokens few_tokens(const Problem& p, const RowsIn& h, const RowsIn& w, const v
     f.tokens = p.tokens;
     f.hidden = p.hidden;
     f.vocab = p.vocab;
+    f.sms = p.sms;
     f.h = h.base;
     f.h_pitch = h.pitch;
     f.w = w.base;
@@ -1187,7 +1188,7 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
     const bool few = few_loss_fits(p.dtype, p.tokens, p.hidden);
     if (few || f32_fits(p.dtype, p.tokens, p.hidden, false)) {
         FewTokens f = few_tokens(p, h, w, t, wide, ignore);
-        const int64_t parts = few ? few_loss_parts() : f32_loss_parts(p.tokens, p.vocab);
+        const int64_t parts = few ? few_loss_parts(f) : f32_loss_parts(p.tokens, p.vocab);
         TN_TRY(mem.take(&halves, sizeof(float2) * (size_t)parts * p.tokens));
         f.parts = halves;
         f.target_logit = target_logit;
@@ -1261,7 +1262,7 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
     f.dweight = dweight ? dweight->address : nullptr;
     const bool half = half_grad_fits(f), few = few_grad_fits(f);
     if (half || few || f32_fits(p.dtype, p.tokens, p.hidden, true)) {
-        const int64_t blocks = half ? half_grad_blocks(p.tokens, p.hidden, p.vocab) : few ? few_grad_blocks(p.vocab) : f32_grad_shares(p.hidden, p.vocab);
+        const int64_t blocks = half ? half_grad_blocks(f) : few ? few_grad_blocks(f) : f32_grad_shares(p.hidden, p.vocab);
         if (dhidden) TN_TRY(mem.take(&f.sums, sizeof(float) * (size_t)blocks * p.tokens * p.hidden));
         if (half) return half_grad(f, p.stream);
         if (few) return few_grad(f, p.stream);

@@ -9,6 +9,7 @@ namespace tnb {
 struct FewTokens {
     int dtype = 0;                         // TN_FLOAT16, TN_BFLOAT16 or TN_FLOAT32
     int64_t tokens = 0, hidden = 0, vocab = 0;
+    int sms = 1;                           // that the persistent kernels may use
     const void* h = nullptr;               // [tokens, hidden], rows h_pitch elements apart
     int64_t h_pitch = 0;
     const void* w = nullptr;               // [vocab, hidden], rows w_pitch elements apart
@@ -28,7 +29,7 @@ struct FewTokens {
 };
 
 bool few_loss_fits(int dtype, int64_t tokens, int64_t hidden);
-int64_t few_loss_parts();
+int64_t few_loss_parts(const FewTokens& p);
 tn_status few_loss(const FewTokens& p, cudaStream_t stream);
 
 // d is scaled by kTop over the largest |grad|, and what is formed from it scaled back.
@@ -37,12 +38,12 @@ __device__ __forceinline__ float unscale(float v, float largest) { return v * (1
 
 // 16 bits, up to sixteen tokens
 bool half_grad_fits(const FewTokens& p);
-int64_t half_grad_blocks(int64_t tokens, int64_t hidden, int64_t vocab);
+int64_t half_grad_blocks(const FewTokens& p);
 tn_status half_grad(const FewTokens& p, cudaStream_t stream);
 
 // float32, up to four tokens
 bool few_grad_fits(const FewTokens& p);
-int64_t few_grad_blocks(int64_t vocab);
+int64_t few_grad_blocks(const FewTokens& p);
 tn_status few_grad(const FewTokens& p, cudaStream_t stream);
 // dhidden from `n` blocks' sums
 tn_status few_dhidden(const FewTokens& p, int64_t n, cudaStream_t stream);

@@ -381,7 +381,7 @@ tn_status loss_one(const FewTokens& p, cudaStream_t stream) {
     const int64_t padded = (p.hidden + 7) & ~int64_t(7);
     const size_t smem = sizeof(float) * NT * (size_t)padded;
     TN_TRY(allow(few_loss_kernel<T, VEC, NT>, device));
-    TN_CUDA(launch_chained(false, few_loss_kernel<T, VEC, NT>, (unsigned)(few_loss_parts() / (kLossThreads / 32)), kLossThreads, smem, stream, 1, p, padded));
+    TN_CUDA(launch_chained(false, few_loss_kernel<T, VEC, NT>, (unsigned)p.sms, kLossThreads, smem, stream, 1, p, padded));
     return after_launch("few_loss_kernel");
 }
 template <typename T, int VEC>
@@ -412,7 +412,7 @@ tn_status grad_one(const FewTokens& p, cudaStream_t stream) {
     const int threads = (int)(ceil_div(ceil_div(p.hidden / VEC, E / VEC), 32) * 32);
     const size_t smem = VEC > 1 ? sizeof(float) * E * kGradRows * kDepth * (size_t)threads : 0;
     TN_TRY(allow(few_grad_kernel<VEC, NT>, device));
-    const int64_t blocks = few_grad_blocks(p.vocab);
+    const int64_t blocks = few_grad_blocks(p);
     TN_CUDA(launch_chained(false, few_grad_kernel<VEC, NT>, (unsigned)blocks, threads, smem, stream, 1, p));
     TN_TRY(after_launch("few_grad_kernel"));
     return p.dhidden ? few_dhidden(p, blocks, stream) : TN_SUCCESS;
@@ -431,7 +431,7 @@ bool few_loss_fits(int dtype, int64_t tokens, int64_t hidden) {
     const int64_t nt = tokens <= 1 ? 1 : tokens <= 2 ? 2 : 4;
     return tokens <= (dtype == TN_FLOAT32 ? 4 : 1) && nt * (hidden + 8) * 4 <= 200 * 1024;
 }
-int64_t few_loss_parts() { return (int64_t)sm_count() * (kLossThreads / 32); }
+int64_t few_loss_parts(const FewTokens& p) { return (int64_t)p.sms * (kLossThreads / 32); }
 
 tn_status few_loss(const FewTokens& p, cudaStream_t stream) {
     switch (p.dtype) {
@@ -451,7 +451,7 @@ tn_status few_dhidden(const FewTokens& p, int64_t n, cudaStream_t stream) {
 
 // Four tokens with eight columns in each of 512 threads.
 bool few_grad_fits(const FewTokens& p) { return p.dtype == TN_FLOAT32 && p.tokens <= 4 && p.hidden <= kGradThreads * E; }
-int64_t few_grad_blocks(int64_t vocab) { return std::min<int64_t>(sm_count(), ceil_div(vocab, kGradRows)); }
+int64_t few_grad_blocks(const FewTokens& p) { return std::min<int64_t>(p.sms, ceil_div(p.vocab, kGradRows)); }
 
 tn_status few_grad(const FewTokens& p, cudaStream_t stream) {
     const bool wide = p.hidden % 4 == 0 && fits16(p.w, p.w_pitch * 4) && fits16(p.dweight, 0);

@@ -320,7 +320,7 @@ tn_status launch(const FewTokens& p, cudaStream_t stream) {
         TN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         device = dev;
     }
-    kernel<<<(unsigned)half_grad_blocks(p.tokens, p.hidden, p.vocab), WARPS * 32, smem, stream>>>(p);
+    kernel<<<(unsigned)half_grad_blocks(p), WARPS * 32, smem, stream>>>(p);
     return after_launch("half_grad_kernel");
 }
 template <typename T, bool DW>
@@ -349,13 +349,13 @@ bool half_grad_fits(const FewTokens& p) {
     const bool wide = p.hidden % 8 == 0 && p.w_pitch % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.w) | reinterpret_cast<uintptr_t>(p.dweight)) & 15) == 0;
     return (p.dtype == TN_FLOAT16 || p.dtype == TN_BFLOAT16) && p.tokens <= 2 * kTile && p.hidden * tiles_for(p.tokens) <= 16 * kMostGroups * kGroup && wide;
 }
-int64_t half_grad_blocks(int64_t tokens, int64_t hidden, int64_t vocab) {
-    return std::min<int64_t>((int64_t)sm_count() * (16 / warps_for(tokens, hidden)), ceil_div(vocab, kBatch));
+int64_t half_grad_blocks(const FewTokens& p) {
+    return std::min<int64_t>((int64_t)p.sms * (16 / warps_for(p.tokens, p.hidden)), ceil_div(p.vocab, kBatch));
 }
 
 tn_status half_grad(const FewTokens& p, cudaStream_t stream) {
     TN_TRY(p.dtype == TN_FLOAT16 ? launch_typed<__half>(p, stream) : launch_typed<__nv_bfloat16>(p, stream));
-    return p.dhidden ? few_dhidden(p, half_grad_blocks(p.tokens, p.hidden, p.vocab), stream) : TN_SUCCESS;
+    return p.dhidden ? few_dhidden(p, half_grad_blocks(p), stream) : TN_SUCCESS;
 }
 
 }  // namespace tnb
