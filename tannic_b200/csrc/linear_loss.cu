@@ -43,10 +43,13 @@
 // alone, on the same three products, makes 1340; 16-bit loss of 4095 x 768 by 50257: 245 us for 316 GFLOP. The main loop without its
 // epilogue reaches 1500 TFLOP/s at burst clocks; the epilogue's exponentials share the SM's power and issue slots with it.
 //
-// The tensor cores cut off, rather than round, what falls below an accumulator's last place: a sum of K / 16 steps is low by up to
-// K / 16 half units, always towards zero (float32 loss of 512 x 1024 by 14336: off by up to 1.8e-6 relative, 3.1e-7 with the sums
-// below). Where the result is float32 or the sum is long an accumulator takes only `period` blocks and the epilogue warps
+// The tensor cores cut off, rather than round, what falls below an accumulator's last place: the more steps of 16 an accumulator takes, the
+// further it is off, always towards zero. Where the result is float32 or the sum is long an accumulator takes only `group` blocks and the epilogue warps
 // add it, in float32, to sums in their registers (128 a thread); its double hides that under the next blocks' products.
+// Logits of 4096 products of either sign, rms in units of 2^-24 of theirs: float32 2.8, where the six passes of two blocks go smallest products
+// first, so that only the last eight steps find anything to lose (20 with the largest first and 16 passes to an accumulator; the
+// same loop on the FP32 pipe, one sum to a thread, 4.8). A group of one: 2.7, but 365 us for the gradient of 512 x 1024 by 14336 against 343
+// (groups of three 337 us and 3.2). 16 bits: 17 (bfloat16) and 21 (float16).
 // With the whole tile in registers an accumulator is free as soon as it is read, and the epilogue has 128 independent
 // elements a thread to fill the gaps that two warps to a scheduler leave.
 // The register split that takes is 40 a thread for warps 0..3 and 232 for the others, of 384 x 168 at launch.
@@ -86,11 +89,12 @@ struct alignas(16) RowInfo {
     int unused;
 };
 constexpr int kNoRow = -1;
-constexpr int kPeriod = 16;       // 64-wide blocks an accumulator takes before it is added up in registers
+// 64-wide blocks an accumulator takes before it is added up in registers, and as many where the operands are float32 in parts.
+constexpr int kGroup = 16, kGroupParts = 2;
 
-// Passes over the parts of a float32 operand pair, largest product first.
-__constant__ int kPartA[6] = {0, 0, 1, 0, 1, 2};
-__constant__ int kPartB[6] = {0, 1, 0, 2, 1, 0};
+// Passes over the parts of a float32 operand pair, smallest product first: an accumulator that holds little loses little.
+__constant__ int kPartA[6] = {2, 1, 0, 1, 0, 0};
+__constant__ int kPartB[6] = {0, 1, 2, 0, 1, 0};
 
 enum { EPI_STATS = 0, EPI_D = 1, EPI_SUM = 2, EPI_RESULT = 3 };
 // How the number of tokens that count bounds a product: not at all, its rows, or its K extent.
@@ -105,7 +109,7 @@ struct LossArgs {
     int first_k_blocks;      // of the first piece, whose splits the others must not exceed
     int units;               // thread blocks, or pairs of them, that share the tiles
     int terms;               // 1, or 6 for float32 operands
-    int period;              // passes over a 64-wide block that one accumulator takes
+    int group;               // 64-wide blocks of K that one accumulator takes
     int is_bf16;
     const int* count;        // tokens with a target
     int count_is;
@@ -358,30 +362,35 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     tile_coords(t, m_tiles, g.n_tiles, z, mt, nt);
                     split_range(z, first, blocks);
                     const int row = mt * ROWS + rank * BM, col = nt * BN + rank * B_COLS;  // what this block loads
-                    for (int kb = first; ok && kb < first + blocks; ++kb) {
-                        for (int term = 0; term < g.terms; ++term, ++it) {
-                            const int s = it % STAGES;
-                            if (!wait(empty0 + 8 * s, ((it / STAGES) & 1) ^ 1)) { ok = false; break; }
-                            const uint32_t sa = base + s * STAGE, sb = sa + A_BYTES;
+                    // the blocks of one accumulator, once for every term
+                    const int last = first + blocks;
+                    for (int kb0 = first; ok && kb0 < last; kb0 += g.group) {
+                        const int kb1 = min(kb0 + g.group, last);
+                        for (int term = 0; ok && term < g.terms; ++term) {
                             const int pa = g.terms > 1 ? kPartA[term] : 0, pb = g.terms > 1 ? kPartB[term] : 0;
-                            uint32_t bar = full0 + 8 * s;
-                            if (rank == 0) mbar_expect_tx(bar, PAIR ? 2 * STAGE : STAGE);
-                            if constexpr (PAIR) bar = in_even_block(bar);
-                            auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
-                                if constexpr (PAIR) tma_load_3d_pair(dst, map, bar, c0, c1, c2);
-                                else tma_load_3d(dst, map, bar, c0, c1, c2);
-                            };
-                            if constexpr (A_M) {
+                            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                                const int s = it % STAGES;
+                                if (!wait(empty0 + 8 * s, ((it / STAGES) & 1) ^ 1)) { ok = false; break; }
+                                const uint32_t sa = base + s * STAGE, sb = sa + A_BYTES;
+                                uint32_t bar = full0 + 8 * s;
+                                if (rank == 0) mbar_expect_tx(bar, PAIR ? 2 * STAGE : STAGE);
+                                if constexpr (PAIR) bar = in_even_block(bar);
+                                auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
+                                    if constexpr (PAIR) tma_load_3d_pair(dst, map, bar, c0, c1, c2);
+                                    else tma_load_3d(dst, map, bar, c0, c1, c2);
+                                };
+                                if constexpr (A_M) {
 #pragma unroll
-                                for (int c = 0; c < BM / 64; ++c) load(sa + c * (64 * BK * 2), &map_a, row + c * 64, kb * BK, pa);
-                            } else {
-                                load(sa, &map_a, kb * BK, row, pa);
-                            }
-                            if constexpr (B_N) {
+                                    for (int c = 0; c < BM / 64; ++c) load(sa + c * (64 * BK * 2), &map_a, row + c * 64, kb * BK, pa);
+                                } else {
+                                    load(sa, &map_a, kb * BK, row, pa);
+                                }
+                                if constexpr (B_N) {
 #pragma unroll
-                                for (int c = 0; c < B_COLS / 64; ++c) load(sb + c * (64 * BK * 2), &map_b, col + c * 64, kb * BK, pb);
-                            } else {
-                                load(sb, &map_b, kb * BK, col, pb);
+                                    for (int c = 0; c < B_COLS / 64; ++c) load(sb + c * (64 * BK * 2), &map_b, col + c * 64, kb * BK, pb);
+                                } else {
+                                    load(sb, &map_b, kb * BK, col, pb);
+                                }
                             }
                         }
                     }
@@ -409,13 +418,13 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     int z, mt, nt, first, blocks;
                     tile_coords(t, m_tiles, g.n_tiles, z, mt, nt);
                     split_range(z, first, blocks);
-                    const int steps = blocks * g.terms;
-                    for (int i0 = 0; ok && i0 < steps; i0 += g.period, ++local) {
+                    const int steps = blocks * g.terms, period = g.group * g.terms;
+                    for (int i0 = 0; ok && i0 < steps; i0 += period, ++local) {
                         const int buf = local & 1;
                         if (!wait(acce0 + 8 * buf, ((local >> 1) & 1) ^ 1)) { ok = false; break; }
                         tc_fence_after();
                         const uint32_t acc = tmem_base + buf * BN;
-                        const int i1 = min(steps, i0 + g.period);
+                        const int i1 = min(steps, i0 + period);
                         for (int i = i0; i < i1; ++i, ++it) {
                             const int s = it % STAGES;
                             if (!wait(full0 + 8 * s, (it / STAGES) & 1)) { ok = false; break; }
@@ -468,8 +477,7 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             for (int i = 0; i < kChunks; ++i)
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[i][j] = 0.0f;
-            const int steps = blocks * g.terms;
-            for (int i0 = 0; i0 < steps; i0 += g.period, ++local) {
+            for (int i0 = 0; i0 < blocks; i0 += g.group, ++local) {
                 const int buf = local & 1;
                 if (!wait(accf0 + 8 * buf, (local >> 1) & 1)) { ok = false; break; }
                 tc_fence_after();
@@ -1074,7 +1082,7 @@ LossArgs gemm_args(const Problem& p, int64_t m, int64_t n, int64_t k) {
     g.most_splits = 1;
     g.units = unit_count(p, pair);
     g.terms = p.terms;
-    g.period = p.parts == 3 ? kPeriod : 1 << 20;
+    g.group = p.parts == 3 ? kGroupParts : 1 << 20;
     g.is_bf16 = p.bf16;
     return g;
 }
@@ -1230,7 +1238,7 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
         TN_TRY(weight_piece(p, w, v0, n, room, &b));
         TN_TRY(b_map(&map_b, b, p.bf16, p.hidden, n, p.tokens));
         LossArgs g = gemm_args(p, p.tokens, n, p.hidden);
-        g.period = kPeriod;
+        if (p.parts == 1) g.group = kGroup;
         g.vocab0 = v0;
         g.targets = t;
         g.wide_targets = wide;
@@ -1345,7 +1353,7 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
             LossArgs g = gemm_args(p, p.tokens, p.padded, n);
             g.count = count;
             g.count_is = COUNT_ROWS;
-            g.period = kPeriod;
+            if (p.parts == 1) g.group = kGroup;
             g.most_splits = splits;
             g.first_k_blocks = (int)ceil_div(piece, BK);
             g.add = v0 > 0;

@@ -1,0 +1,61 @@
+"""What the gradient of a linear layer's cross entropy makes of the forward pass's log-sum-exp, where small differences count."""
+import pytest
+import torch
+
+from tannic_b200 import ops as tb
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [torch.float32])
+@pytest.mark.parametrize("tokens", [1, 2, 4, 8, 9, 16, 17, 40, 64, 100, 128, 129, 300])
+@pytest.mark.parametrize("hidden", [1024, 2048, 4096])
+def test_nearly_certain_tokens(hidden, tokens, dtype):
+    """Logits of 20 made of products of one sign, where a sum that is cut off drifts most, and about 1e-3 left for the other entries:
+    d = p - 1 of the target is the difference of two numbers near 20. The forward pass's lse has to belong to the logits that the
+    gradient forms."""
+    vocab = 512
+    gen = torch.Generator(device="cuda").manual_seed(tokens + hidden)
+    u = torch.randn(hidden, generator=gen, device="cuda").abs()
+    u /= u.sum() * (2 / torch.pi) ** 0.5
+    h = torch.randn(tokens, hidden, generator=gen, device="cuda").abs().to(dtype)
+    size = torch.rand(vocab, 1, generator=gen, device="cuda") + 6.2
+    size[0] = 20.0
+    w = (size * u).to(dtype)
+    t = torch.zeros(tokens, dtype=torch.int64, device="cuda")
+    g = torch.ones(tokens, device="cuda")
+    _, lse = tb.linear_cross_entropy(h, w, t)
+    dh, dw = tb.linear_cross_entropy_grad(g, h, w, t, lse)
+    H, W = h.double(), w.double()
+    logits = H @ W.T
+    exact = torch.logsumexp(logits, -1)
+    others = (logits[:, 1:] - exact[:, None]).exp()
+    d = torch.cat([-others.sum(-1, keepdim=True), others], 1)
+    # Along u, dh is d . (W u); the target's part is 20 d_0, the others' about -7 d_0 in all, so a relative error of d_0 becomes 20 / 13 of it.
+    # lse is rounded to float32, at most half a unit of numbers from 16 to 32, which is 2^-19, and so are its logarithm and the
+    # difference: three units. Where one kernel forms the logits of both passes they are the same, whatever their error. Where two do,
+    # each adds up at most K / 32 partial sums in float32: a running sum that grows evenly to 20 rounds to units of 2^-19 for
+    # a fifth of the additions, half of that for two fifths, a quarter for one fifth, and so on: a variance of 0.3125 / 12 units^2 each. Six standard
+    # deviations of the two together. d and dh are rounded to the type.
+    same = 5 <= tokens <= 32 or tokens > 64 if dtype == torch.float32 else tokens > 16
+    units = 3 if same else 3 + 6 * (2 * (hidden / 32) * 0.3125 / 12) ** 0.5
+    along = dh.double() @ u.double()
+    want = (d @ W) @ u.double()
+    slack = units * 2.0 ** -19 * 20 / 13 / d[:, 0].abs()
+    step = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 8 * U
+    tol = (slack + 3 * step) * want.abs() * (1 + 1e-3)
+    if dtype == torch.float16:
+        tol = tol + 2.0 ** -25 * u.double().sum()
+    err = (along - want).abs()
+    assert bool((err <= tol).all()), (float((err / want.abs()).max()), float((tol / want.abs()).min()))
+    # the same for the target's row of dweight: the sum of d_0 h over the tokens
+    v = H.mean(0)
+    want = (d[:, 0] @ H) @ v
+    slack = units * 2.0 ** -19 / float(d[:, 0].abs().min())
+    err = (dw[0].double() @ v - want).abs()
+    tol = (slack + 3 * step) * want.abs() * (1 + 1e-3)
+    if dtype == torch.float16:
+        tol = tol + 2.0 ** -25 * v.abs().sum()
+    assert bool(err <= tol), (float(err / want.abs()), float(tol / want.abs()))
