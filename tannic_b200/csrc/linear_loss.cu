@@ -10,8 +10,8 @@
 //   loss       The epilogue of the product keeps, per row and per half of a tile, the running maximum m and
 //              s = sum exp(l - m), and picks the target's logit out of its registers. A small kernel joins the halves
 //              of a row: lse = M + log sum s exp(m - M).
-//   gradient   The vocabulary is cut into pieces. For each piece the product is formed again (the same
-//              instructions in the same order, so the same logits) and its epilogue writes d, rounded to the operands' type, into a
+//   gradient   The vocabulary is cut into pieces. For each piece the product is formed again (by the same
+//              kernel in the same order, so the same logits) and its epilogue writes d, rounded to the operands' type, into a
 //              workspace of at most about half a GiB; two more products read it, dW's piece = d^T h and
 //              dh += d W's piece, the latter in float32 in memory. Forming the logits again costs
 //              2 N H V operations and saves writing, keeping and reading 4 N V bytes.
@@ -89,8 +89,9 @@ struct alignas(16) RowInfo {
     int unused;
 };
 constexpr int kNoRow = -1;
-// 64-wide blocks an accumulator takes before it is added up in registers, and as many where the operands are float32 in parts.
-constexpr int kGroup = 16, kGroupParts = 2;
+// 64-wide blocks an accumulator takes before it is added up in registers; as many where the operands are float32 in parts; and for the logits
+// of up to 128 tokens of 16 bits, where reading W is the time and the additions run under it.
+constexpr int kGroup = 16, kGroupParts = 2, kGroupFew = 1;
 
 // Passes over the parts of a float32 operand pair, smallest product first: an accumulator that holds little loses little.
 __constant__ int kPartA[6] = {2, 1, 0, 1, 0, 0};
@@ -1086,6 +1087,11 @@ LossArgs gemm_args(const Problem& p, int64_t m, int64_t n, int64_t k) {
     g.is_bf16 = p.bf16;
     return g;
 }
+// Loss and gradient form the logits of 16-bit operands alike: d = exp(l - lse) - 1 of a nearly certain token is the difference of two
+// large numbers, and lse has to belong to the same l. Up to sixteen tokens half_grad_kernel forms the gradient's, in short sums of its own; what the
+// loss cuts off has to be small then: logits of 20 over 4096 columns are low by 4e-5 to 1.1e-4 with sixteen blocks to an accumulator, by less
+// than 4e-6 with one. Four tokens over 32768 x 4096: 95 us from memory against 93.
+int logit_group(const Problem& p) { return takes_pairs(p.tokens) ? kGroup : kGroupFew; }
 // Map of an operand B stored [N, K] for a product with m result rows: a block of a pair loads half the columns.
 tn_status b_map(CUtensorMap* map, const Operand& o, bool bf16, int64_t k, int64_t n, int64_t m) {
     return operand_map(map, o, bf16, k, n, BK, takes_pairs(m) ? BN / 2 : BN);
@@ -1238,7 +1244,7 @@ tn_status run_loss(const tn_tensor_t* hidden, const tn_tensor_t* weight, const t
         TN_TRY(weight_piece(p, w, v0, n, room, &b));
         TN_TRY(b_map(&map_b, b, p.bf16, p.hidden, n, p.tokens));
         LossArgs g = gemm_args(p, p.tokens, n, p.hidden);
-        if (p.parts == 1) g.group = kGroup;
+        if (p.parts == 1) g.group = logit_group(p);
         g.vocab0 = v0;
         g.targets = t;
         g.wide_targets = wide;
@@ -1339,6 +1345,7 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
             const cuuint32_t box[3] = {32, 32, 1};
             TN_TRY(encode_as(&map_d, d, p.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_SWIZZLE_64B, 3, dims, strides, box));
             LossArgs g = gemm_args(p, p.tokens, n, p.hidden);
+            if (p.parts == 1) g.group = logit_group(p);
             g.vocab0 = v0;
             g.count = count;
             g.count_is = COUNT_ROWS;

@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 
 
-@pytest.mark.parametrize("dtype", [torch.float32])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("tokens", [1, 2, 4, 8, 9, 16, 17, 40, 64, 100, 128, 129, 300])
 @pytest.mark.parametrize("hidden", [1024, 2048, 4096])
 def test_nearly_certain_tokens(hidden, tokens, dtype):
