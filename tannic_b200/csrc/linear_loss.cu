@@ -44,7 +44,7 @@
 // epilogue reaches 1500 TFLOP/s at burst clocks; the epilogue's exponentials share the SM's power and issue slots with it.
 //
 // The tensor cores cut off, rather than round, what falls below an accumulator's last place: the more steps of 16 an accumulator takes, the
-// further it is off, always towards zero. Where the result is float32 or the sum is long an accumulator takes only `group` blocks and the epilogue warps
+// further it is off, always towards zero. So one takes only `group` blocks, and the epilogue warps
 // add it, in float32, to sums in their registers (128 a thread); its double hides that under the next blocks' products.
 // Logits of 4096 products of either sign, rms in units of 2^-24 of theirs: float32 2.8, where the six passes of two blocks go smallest products
 // first, so that only the last eight steps find anything to lose (20 with the largest first and 16 passes to an accumulator; the
@@ -1083,7 +1083,7 @@ LossArgs gemm_args(const Problem& p, int64_t m, int64_t n, int64_t k) {
     g.most_splits = 1;
     g.units = unit_count(p, pair);
     g.terms = p.terms;
-    g.group = p.parts == 3 ? kGroupParts : 1 << 20;
+    g.group = p.parts == 3 ? kGroupParts : kGroup;
     g.is_bf16 = p.bf16;
     return g;
 }
@@ -1360,7 +1360,6 @@ tn_status run_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_
             LossArgs g = gemm_args(p, p.tokens, p.padded, n);
             g.count = count;
             g.count_is = COUNT_ROWS;
-            if (p.parts == 1) g.group = kGroup;
             g.most_splits = splits;
             g.first_k_blocks = (int)ceil_div(piece, BK);
             g.add = v0 > 0;

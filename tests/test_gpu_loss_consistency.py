@@ -1,4 +1,5 @@
-"""What the gradient of a linear layer's cross entropy makes of the forward pass's log-sum-exp, where small differences count."""
+"""What the gradient of a linear layer's cross entropy makes of the forward pass's log-sum-exp, where small differences count: nearly
+certain tokens, and sums over very many tokens."""
 import pytest
 import torch
 
@@ -59,3 +60,30 @@ def test_nearly_certain_tokens(hidden, tokens, dtype):
     if dtype == torch.float16:
         tol = tol + 2.0 ** -25 * v.abs().sum()
     assert bool(err <= tol), (float(err / want.abs()), float(tol / want.abs()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_sums_over_very_many_tokens(dtype):
+    """A million positive terms to an element of dweight: an accumulator that cuts off what falls below its last place would lose
+    about a thousandth, more than the result's rounding."""
+    tokens, hidden, vocab = 1 << 20, 16, 64
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    h = (torch.rand(tokens, hidden, generator=gen, device="cuda") + 0.5).to(dtype)
+    w = (torch.randn(vocab, hidden, generator=gen, device="cuda") * 0.1).to(dtype)
+    t = torch.full((tokens,), vocab - 1, device="cuda")
+    g = torch.full((tokens,), 0.01, device="cuda")
+    _, lse = tb.linear_cross_entropy(h, w, t)
+    _, dw = tb.linear_cross_entropy_grad(g, h, w, t, lse, dhidden=False)
+    want = torch.zeros(vocab, hidden, dtype=torch.float64, device="cuda")
+    for i in range(0, tokens, 1 << 17):
+        H = h[i:i + (1 << 17)].double()
+        p = (H @ w.double().T).softmax(-1)
+        p[:, -1] -= 1.0
+        want += (p * 0.01).T @ H
+    rel = (dw.double() - want) / want
+    # every result is rounded by at most half a step, d's roundings are evened out over the tokens; the logits are right to a few 2^-24
+    assert float(rel.abs().max()) <= torch.finfo(dtype).eps / 2 * (1 + 1e-2) + 40 * U, float(rel.abs().max())
+    # and on the whole nothing is lost: the roundings of 1024 results, uniform within half a step, have a mean of a thirtieth of its third
+    # root; five times that
+    spread = torch.finfo(dtype).eps / 2 / 3 ** 0.5 / (vocab * hidden) ** 0.5
+    assert abs(float(rel.mean())) <= 5 * spread + 40 * U, float(rel.mean())
