@@ -264,6 +264,22 @@ struct Exponent {
     __device__ __forceinline__ float power(float x) const { return exp2_approx(fmaf(x, kLog2e, shift)); }
 };
 
+// exp(x - base) of two x, with the rounding of the difference like any float32 form and three more: t log2 e as the sum of two float32, log2 e
+// itself as two, exp(t) = 2^hi 2^lo = 2^hi (1 + lo ln 2). In pairs this costs about half of what expf does: the
+// gradient of 2000 x 512 by 30000, 1.32 ms, is 6 % longer than with Exponent, with expf 11 %; from 1024 columns on neither shows.
+// Below -200 everything is zero; NaN stays.
+__device__ __forceinline__ float2 exp_of_difference(float2 x, float base) {
+    constexpr float kLog2eRest = static_cast<float>(1.4426950408889634 - static_cast<double>(kLog2e)), kLn2 = 0.6931471805599453f;
+    float2 t = add2(x, make_float2(-base, -base));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(t.x) : "f"(-200.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(t.y) : "f"(-200.0f));
+    const float2 hi = mul2(t, make_float2(kLog2e, kLog2e));
+    float2 lo = fma2(t, make_float2(kLog2e, kLog2e), make_float2(-hi.x, -hi.y));
+    lo = fma2(t, make_float2(kLog2eRest, kLog2eRest), lo);
+    const float2 p = make_float2(exp2_approx(hi.x), exp2_approx(hi.y));
+    return fma2(mul2(p, make_float2(kLn2, kLn2)), lo, p);
+}
+
 // x as bfloat16 (whose exponent range is float32's), the largest number where rounding would leave the range.
 __device__ __forceinline__ float first_part(float x) {
     const float p = __bfloat162float(__float2bfloat16_rn(x));
@@ -574,7 +590,17 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 #pragma unroll
                     for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[i][j] = e.power(v[i][j]) * by;
+                        for (int j = 0; j < 32; j += 2) {
+                            // 16 bits hide what the short form leaves, a unit of 2^-24 for every one of |l - lse|; float32 does not
+                            if constexpr (PARTS == 1) {
+                                v[i][j] = e.power(v[i][j]) * by;
+                                v[i][j + 1] = e.power(v[i][j + 1]) * by;
+                            } else {
+                                const float2 p = mul2(exp_of_difference(make_float2(v[i][j], v[i][j + 1]), info.lse), make_float2(info.grad, info.grad));
+                                v[i][j] = p.x;
+                                v[i][j + 1] = p.y;
+                            }
+                        }
                     if (info.target == kNoRow) {
 #pragma unroll
                         for (int i = 0; i < kChunks; ++i)

@@ -6,6 +6,33 @@
 
 namespace tnb {
 
+// Two elements as one packed instruction each, rounded like the single ones.
+__device__ __forceinline__ uint64_t pair_bits(float2 v) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+    return r;
+}
+__device__ __forceinline__ float2 pair_of(uint64_t r) {
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+    return v;
+}
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(x)), "l"(pair_bits(y)));
+    return pair_of(r);
+}
+__device__ __forceinline__ float2 mul2(float2 x, float2 y) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(x)), "l"(pair_bits(y)));
+    return pair_of(r);
+}
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_bits(x)), "l"(pair_bits(y)), "l"(pair_bits(z)));
+    return pair_of(r);
+}
+
 struct FewTokens {
     int dtype = 0;                         // TN_FLOAT16, TN_BFLOAT16 or TN_FLOAT32
     int64_t tokens = 0, hidden = 0, vocab = 0;

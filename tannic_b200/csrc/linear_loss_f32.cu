@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const FewTokens p
                     for (int q = 0; q < 2; ++q) {
                         const int64_t v = first + 8 * j + q;
                         const float x = sum[i][j][2 * up + q] - lse;
-                        if (v < d_pitch) d[n * d_pitch + v] = counts && v < p.vocab ? (v == target ? expm1f(x) : __expf(x)) * grad : 0.0f;
+                        if (v < d_pitch) d[n * d_pitch + v] = counts && v < p.vocab ? (v == target ? expm1f(x) : expf(x)) * grad : 0.0f;
                     }
             } else {
                 float m = -INFINITY, s = 0.0f, x[NT][2];

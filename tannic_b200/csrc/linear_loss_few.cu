@@ -22,18 +22,6 @@ struct alignas(sizeof(T) * VEC < 16 ? sizeof(T) * VEC : 16) Pack {
     T v[VEC];
 };
 
-// Two elements as one packed instruction.
-__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
-    uint64_t a, b, c, r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(x.x), "f"(x.y));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(y.x), "f"(y.y));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(c) : "f"(z.x), "f"(z.y));
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    float2 v;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
-    return v;
-}
-
 // V sums over the 32 lanes at once (V a power of two up to 32): afterwards lane i holds the sum number i >> (5 - log2 V). Each step
 // halves the values a lane carries instead of passing all of them on.
 template <int V>
@@ -280,7 +268,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) few_grad_kernel(const FewToke
         const float x_lse = even + odd - lse;
         const int64_t v = v0 + row_in;
         float d = 0.0f;
-        if (counts && v < p.vocab) d = (v == target ? expm1f(x_lse) : __expf(x_lse)) * grad;
+        if (counts && v < p.vocab) d = (v == target ? expm1f(x_lse) : expf(x_lse)) * grad;
         // every warp keeps the batch's d for itself, in the order (row, token)
         __syncwarp();
         if ((lane & ((1 << SHIFT) - 1)) == 0) dvals[warp][index] = d;

@@ -1,5 +1,5 @@
 """What the gradient of a linear layer's cross entropy makes of the forward pass's log-sum-exp, where small differences count: nearly
-certain tokens, and sums over very many tokens."""
+certain tokens, small probabilities, and sums over very many tokens."""
 import pytest
 import torch
 
@@ -60,6 +60,63 @@ def test_nearly_certain_tokens(hidden, tokens, dtype):
     if dtype == torch.float16:
         tol = tol + 2.0 ** -25 * v.abs().sum()
     assert bool(err <= tol), (float(err / want.abs()), float(tol / want.abs()))
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 5, 16, 17, 32, 33, 64, 65, 200])
+def test_small_probabilities_of_float32(tokens):
+    """One token counts, its hidden state is 1 and the weights are the logits themselves: a row of dweight is exp(logit - lse) grad and
+    nothing else. lse = 0 and grad = 1 make it the exponential of a float32 that is known exactly."""
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    w = (-60 * torch.rand(20000, 1, generator=gen, device="cuda")).contiguous()
+    h = torch.ones(tokens, 1, device="cuda")
+    t = torch.full((tokens,), -100, device="cuda", dtype=torch.int64)
+    t[tokens // 2] = 0
+    zero, one = torch.zeros(tokens, device="cuda"), torch.ones(tokens, device="cuda")
+    _, dw = tb.linear_cross_entropy_grad(one, h, w, t, zero)
+    want = w.double().exp()
+    want[0] -= 1
+    # exp of float32 within two units of 2^-23; d scaled and back, its three parts (or two tf32) and the result's rounding: three more of 2^-24,
+    # and the two tf32 leave 2^-22
+    tol = torch.full_like(want, 11 * U)
+    if 5 <= tokens <= 32:
+        # The logit is a product of two tf32 parts: a part is rounded to eleven bits, 2^-11 relative at most, so what the second one leaves
+        # of w is 2^-22 |w|, which exp passes on.
+        tol += 2.0 ** -22 * w.double().abs()
+    err = ((dw.double() - want) / want).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 5, 16, 17, 32, 33, 64, 65, 200])
+def test_small_probabilities_of_short_weights(tokens):
+    """The same over weights of ten bits, which every split of float32 leaves as they are."""
+    w = (-torch.arange(960, device="cuda").float() / 16)[:, None].contiguous()
+    h = torch.ones(tokens, 1, device="cuda")
+    t = torch.full((tokens,), -100, device="cuda", dtype=torch.int64)
+    t[tokens // 2] = 0
+    zero, one = torch.zeros(tokens, device="cuda"), torch.ones(tokens, device="cuda")
+    _, dw = tb.linear_cross_entropy_grad(one, h, w, t, zero)
+    want = w.double().exp()
+    want[0] -= 1
+    assert float(dw[0]) == 0.0
+    err = ((dw.double() - want) / want)[1:].abs()
+    assert float(err.max()) <= 11 * U, float(err.max() / U)  # as above
+
+
+@pytest.mark.parametrize("tokens", [3, 16, 40, 200])
+def test_logits_at_the_ends_of_float32(tokens):
+    """Entries that lie as far below the log-sum-exp as float32 goes have no probability, and an undefined logit stays undefined."""
+    w = torch.tensor([0.0, -1.0, -80.0, -150.0, -1e4, -1e30, -3.0e38], device="cuda")[:, None].contiguous()
+    h = torch.ones(tokens, 1, device="cuda")
+    t = torch.zeros(tokens, device="cuda", dtype=torch.int64)
+    g = torch.ones(tokens, device="cuda")
+    loss, lse = tb.linear_cross_entropy(h, w, t)
+    want = torch.logsumexp(w.double()[:, 0], 0)
+    assert bool(((lse.double() - want).abs() <= 8 * U).all()) and torch.equal(loss, lse)
+    dh, dw = tb.linear_cross_entropy_grad(g, h, w, t, lse, dhidden=False)
+    assert bool(torch.isfinite(dw).all()) and bool((dw[3:].abs() <= 1e-40 * tokens).all())
+    assert abs(float(dw[2]) / (tokens * float((w.double()[2, 0] - want).exp())) - 1) <= 64 * U
+    w[1] = float("nan")
+    assert bool(torch.isnan(tb.linear_cross_entropy_grad(g, h, w, t, lse)[1][1]).all())
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
