@@ -7,7 +7,6 @@ namespace tnb {
 
 bool read_host_scalar(const tn_scalar_t* sc, double* f, int64_t* i);
 tn_status tc_abort_count(unsigned int* count);
-tn_status loss_abort_count(unsigned int* count);
 void tc_path_launches(uint64_t (&out)[4]);
 tn_status reduce_abort_count(unsigned int* count);
 tn_status tc_wait_probe(cudaStream_t stream, unsigned int polls);
@@ -17,11 +16,10 @@ tn_status surface_device_aborts() {
     int dev = 0;
     TN_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) return TN_SUCCESS;
-    unsigned int tc = 0, red = 0, loss = 0;
+    unsigned int tc = 0, red = 0;
     TN_TRY(tc_abort_count(&tc));
     TN_TRY(reduce_abort_count(&red));
-    TN_TRY(loss_abort_count(&loss));
-    const unsigned int total = tc + red + loss, before = seen[dev].exchange(total);
+    const unsigned int total = tc + red, before = seen[dev].exchange(total);
     if (total > before)
         return fail(TN_ERROR, "%u thread block(s) on device %d gave up on a bounded device-side wait since the last synchronising call; "
                               "results written by those launches are incomplete", total - before, dev);
@@ -590,11 +588,10 @@ tn_status tn_gemm_scaled_stats(const tn_tensor_t* a, const tn_tensor_t* b, const
 
 tn_status tn_device_errors(unsigned int* count) {
     if (!count) return fail(TN_ERROR, "null count");
-    unsigned int tc = 0, red = 0, loss = 0;
+    unsigned int tc = 0, red = 0;
     TN_TRY(tc_abort_count(&tc));
     TN_TRY(reduce_abort_count(&red));
-    TN_TRY(loss_abort_count(&loss));
-    *count = tc + red + loss;
+    *count = tc + red;
     return TN_SUCCESS;
 }
 

@@ -1294,6 +1294,12 @@ void tc_path_launches(uint64_t (&out)[4]) {
     for (int i = 0; i < 4; ++i) out[i] = g_path_launches[i].load(std::memory_order_relaxed);
 }
 
+// Where kernels of other files count as well: a synchronising call reads one number back for all of them.
+tn_status tc_abort_counter(unsigned int** counter) {
+    TN_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(counter), g_tc_aborts));
+    return TN_SUCCESS;
+}
+
 tn_status tc_abort_count(unsigned int* count) {
     TN_CUDA(cudaMemcpyFromSymbol(count, g_tc_aborts, sizeof(unsigned int)));
     return TN_SUCCESS;

@@ -60,12 +60,7 @@
 
 namespace tnb {
 
-static __device__ unsigned int g_loss_aborts = 0;
-
-tn_status loss_abort_count(unsigned int* count) {
-    TN_CUDA(cudaMemcpyFromSymbol(count, g_loss_aborts, sizeof(unsigned int)));
-    return TN_SUCCESS;
-}
+tn_status tc_abort_counter(unsigned int** counter);  // of the current device
 
 namespace {
 
@@ -130,6 +125,7 @@ struct LossArgs {
     int64_t ldd;
     const float* scale;
     int tma_store;
+    unsigned int* aborts;    // thread blocks that gave up on a bounded wait
 };
 
 // ---- a pair of thread blocks -----------------------------------------------------------------
@@ -713,7 +709,7 @@ loss_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
         else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
     }
-    if (threadIdx.x == 0 && *abort_flag) atomicAdd(&g_loss_aborts, 1u);
+    if (threadIdx.x == 0 && *abort_flag) atomicAdd(g.aborts, 1u);
 }
 
 // Joins the halves of a row: R rows per block (32, or 1 when there are few), the halves of a row spread over 1024 / R threads. A
@@ -1077,15 +1073,18 @@ int unit_count(const Problem& p, bool pair) { return std::max(1, pair ? p.sms / 
 bool takes_pairs(int64_t m) { return m > BM; }
 
 template <bool A_M, bool B_N, int EPI, typename T, typename OUT, int PARTS, bool PAIR>
-tn_status launch_as(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d, const LossArgs& g, const Problem& p) {
-    static thread_local int attr_device = -1;  // the opt-in shared-memory size belongs to kernel and device
+tn_status launch_as(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d, LossArgs g, const Problem& p) {
+    static thread_local int attr_device = -1;  // the opt-in shared-memory size belongs to kernel and device, the counter to the device
+    static thread_local unsigned int* aborts = nullptr;
     auto kernel = loss_gemm<A_M, B_N, EPI, T, OUT, PARTS, PAIR>;
     int dev = 0;
     TN_CUDA(cudaGetDevice(&dev));
     if (attr_device != dev) {
         TN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<PAIR>));
+        TN_TRY(tc_abort_counter(&aborts));
         attr_device = dev;
     }
+    g.aborts = aborts;
     const int64_t total = (int64_t)g.m_tiles * g.n_tiles * g.most_splits;
     if (total >= (int64_t(1) << 31)) return fail(TN_ERROR, "linear_cross_entropy: %lld tiles are too many", (long long)total);
     const unsigned grid = (unsigned)std::min<int64_t>(total, g.units) * (PAIR ? 2 : 1);
