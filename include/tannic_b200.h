@@ -411,7 +411,7 @@ tn_status tn_layer_norm(const tn_tensor_t* x, const tn_tensor_t* weight, const t
  *   dx = rstd * (g - sum(g) / C - z * sum(g * z) / C),  dweight = sum over rows of dy * z,  dbias = sum over rows of dy
  * dx is dense and may be dy or x where that one is dense. dweight and dbias have the parameters' dtype and
  * may be NULL; weight is NULL where the forward pass had none. The sums over rows are added in an
- * order that depends on the sizes only, so the same call gives the same bits. Without rows the
+ * order that depends on the sizes, the operands' alignment and the GPU only, so the same call gives the same bits. Without rows the
  * parameters' gradients are zero. */
 tn_status tn_layer_norm_grad(const tn_tensor_t* dy, const tn_tensor_t* x, const tn_tensor_t* mean, const tn_tensor_t* rstd,
                              const tn_tensor_t* weight, tn_tensor_t* dx, tn_tensor_t* dweight, tn_tensor_t* dbias,
@@ -425,8 +425,10 @@ tn_status tn_layer_norm_grad(const tn_tensor_t* dy, const tn_tensor_t* x, const 
  * hidden: [..., H], weight: [V, H], both float16, bfloat16 or float32, any strides; targets: int32 or int64 of hidden's
  * leading shape. loss and lse: float32, dense, of the targets' shape; either may be NULL (lse is what the gradient reads;
  * it is computed for ignored tokens too). Products accumulate in float32; float32 operands
- * enter as three bfloat16 parts or, for a few tokens, as two tf32 parts or as they are, which leaves float32's accuracy (a token
- * whose operands hold an infinity may have NaN). A target outside the vocabulary that is
+ * enter as three bfloat16 parts (from 65 tokens on, gradient 33), as two tf32 parts (from 5) or as they are, and logits of random operands are off by
+ * 2 to 5 units of 2^-24, rms; 16-bit operands of more than 128 tokens by up to 21, and by up to 93 where all products of a long row have one sign,
+ * the same in the loss and its gradient. An infinite logit of a positive sign makes the token's lse NaN; float32 operands that hold an infinity
+ * of either sign may. A target outside the vocabulary that is
  * not ignore_index gives NaN for that token; nothing outside the tensors is read. Without tokens nothing is written. */
 tn_status tn_linear_cross_entropy(const tn_tensor_t* hidden, const tn_tensor_t* weight, const tn_tensor_t* targets,
                                   tn_tensor_t* loss, tn_tensor_t* lse, tn_stream_t stream, int64_t ignore_index);
@@ -434,10 +436,13 @@ tn_status tn_linear_cross_entropy(const tn_tensor_t* hidden, const tn_tensor_t* 
  * expanded number will do), lse the forward pass's. With d = (exp(l - lse) - onehot(target)) * grad, d = 0 for ignored tokens:
  *   dhidden = d . weight,  dweight = d^T . hidden
  * dense, of the operands' dtypes and shapes; either may be NULL. The logits are formed again in pieces of the vocabulary, so
- * the workspace is d for one piece (about half a GiB) and float32 sums of dhidden's size. d is rounded to the operands'
- * type (a few tokens: two parts of it; float32: three bfloat16 parts), relative to the largest |grad|, which keeps float16
+ * the workspace is d for one piece, with the weights of the piece where they are not aligned or float32 (half a GiB, or 4096 entries where that is
+ * more: 8192 bytes for every token of 16 bits, 24576 of float32), the hidden states once more (float32: one and a half times) and float32 sums of
+ * dhidden's size, or copies of them up to 39 MB together where that is small; a few tokens need less. d is rounded to the operands'
+ * type (a few tokens: two parts of it; float32: 22 bits or more), relative to the largest |grad|, which keeps float16
  * clear of underflow; everything else is float32 until the result's one rounding. Ignored tokens take no part, whatever their hidden states hold, and
- * cost nothing. A target outside the vocabulary makes that row of dhidden, and dweight, NaN. The same call gives the same bits. */
+ * cost nothing. A target outside the vocabulary makes that row of dhidden, and dweight, NaN. The same call under
+ * the same SM margin gives the same bits. */
 tn_status tn_linear_cross_entropy_grad(const tn_tensor_t* grad, const tn_tensor_t* hidden, const tn_tensor_t* weight,
                                        const tn_tensor_t* targets, const tn_tensor_t* lse, tn_tensor_t* dhidden,
                                        tn_tensor_t* dweight, tn_stream_t stream, int64_t ignore_index);

@@ -12,7 +12,7 @@
 //              of a row: lse = M + log sum s exp(m - M).
 //   gradient   The vocabulary is cut into pieces. For each piece the product is formed again (by the same
 //              kernel in the same order, so the same logits) and its epilogue writes d, rounded to the operands' type, into a
-//              workspace of at most about half a GiB; two more products read it, dW's piece = d^T h and
+//              workspace (half a GiB, or 4096 entries of every token where that is more); two more products read it, dW's piece = d^T h and
 //              dh += d W's piece, the latter in float32 in memory. Forming the logits again costs
 //              2 N H V operations and saves writing, keeping and reading 4 N V bytes.
 //
@@ -39,8 +39,8 @@
 // its barriers, and its commits report to both. At full clocks it is the same time (8192 x 4096 by 32768: 1.50 ms against 1.51),
 // with a third less traffic under the power cap that long runs meet. Up to 128 rows leave nothing to the second SM and take the single form.
 //
-// Measured (bfloat16, 8192 tokens, 4096 wide, 131072 entries): loss and gradient at 1160 TFLOP/s over 23 ms under the power cap, where cuBLAS
-// alone, on the same three products, makes 1340; 16-bit loss of 4095 x 768 by 50257: 245 us for 316 GFLOP. The main loop without its
+// Measured (bfloat16, 8192 tokens, 4096 wide, 131072 entries): the gradient at 1190 TFLOP/s over 22 ms under the power cap, where cuBLAS
+// alone, on the same three products, makes 1340; 16-bit loss of 4095 x 768 by 50257: 247 us for 316 GFLOP. The main loop without its
 // epilogue reaches 1500 TFLOP/s at burst clocks; the epilogue's exponentials share the SM's power and issue slots with it.
 //
 // The tensor cores cut off, rather than round, what falls below an accumulator's last place: the more steps of 16 an accumulator takes, the
@@ -49,7 +49,8 @@
 // Logits of 4096 products of either sign, rms in units of 2^-24 of theirs: float32 2.8, where the six passes of two blocks go smallest products
 // first, so that only the last eight steps find anything to lose (20 with the largest first and 16 passes to an accumulator; the
 // same loop on the FP32 pipe, one sum to a thread, 4.8). A group of one: 2.7, but 365 us for the gradient of 512 x 1024 by 14336 against 343
-// (groups of three 337 us and 3.2). 16 bits: 17 (bfloat16) and 21 (float16).
+// (groups of three 337 us and 3.2). 16 bits, sixteen blocks: 17 (bfloat16) and 21 (float16), for products of one sign 33 and 93; eight blocks
+// halve that and cost 3 to 12 % (8192 x 4096 by 16384: 822 us, 918), four 27 %.
 // With the whole tile in registers an accumulator is free as soon as it is read, and the epilogue has 128 independent
 // elements a thread to fill the gaps that two warps to a scheduler leave.
 // The register split that takes is 40 a thread for warps 0..3 and 232 for the others, of 384 x 168 at launch.

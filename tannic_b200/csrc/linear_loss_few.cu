@@ -414,7 +414,7 @@ tn_status grad_tokens(const FewTokens& p, cudaStream_t stream) {
 }  // namespace
 
 // As many columns as shared memory takes beside the tokens. One token of 16 bits: from two on the tensor cores are faster, empty rows and
-// all (four tokens over 32768 x 4096: 57 us against 98); float32 up to four, where its own tiles begin to be (eight: 164 us here).
+// all (four tokens over 32768 x 4096: 59 us against 98); float32 up to four, where its own tiles begin to be (eight: 164 us here).
 bool few_loss_fits(int dtype, int64_t tokens, int64_t hidden) {
     const int64_t nt = tokens <= 1 ? 1 : tokens <= 2 ? 2 : 4;
     return tokens <= (dtype == TN_FLOAT32 ? 4 : 1) && nt * (hidden + 8) * 4 <= 200 * 1024;
